@@ -159,6 +159,58 @@ def argmax_dev(out_d, v_d, n):
     check(runtime.lib().qwen3_hip_argmax_dev(VP(out_d), VP(v_d), n), "qwen3_hip_argmax_dev")
 
 
+# ---- serving operators (include/qwen3_hip_serve.h); pointers are device addresses ----
+KV8_FORMATS = {"e4m3": 0, "int8": 1}
+
+
+def kv8_cache(format, kv_heads, head_dim, block, n_page, n_seq, max_blocks, k, v, k_scale, v_scale, k_tail, v_tail,
+              table):
+    """A description of one layer's 8-bit KV cache (qwen3_hip_kv8) for the calls below."""
+    return runtime.Kv8(KV8_FORMATS[format], kv_heads, head_dim, block, n_page, n_seq, max_blocks, k, v, k_scale, v_scale,
+                       k_tail, v_tail, table)
+
+
+def kv8_bytes(cache):
+    return int(runtime.lib().qwen3_hip_kv8_bytes(ctypes.byref(cache)))
+
+
+def kv8_append_dev(cache, k_d, v_d, ldk, ldv, bf16, row_d, pos_d, n, rows, max_rows):
+    """New K and V rows of n sequences into the cache; row_d None: one row each."""
+    check(runtime.lib().qwen3_hip_kv8_append_dev(ctypes.byref(cache), k_d, v_d, ldk, ldv, bf16, row_d, pos_d, n, rows,
+                                                 max_rows), "qwen3_hip_kv8_append_dev")
+
+
+def kv8_attention_work(cache, q_heads, n, max_rows, max_ctx):
+    """Bytes of work_d that kv8_attention_dev needs for these sizes."""
+    return int(runtime.lib().qwen3_hip_kv8_attention_work(ctypes.byref(cache), q_heads, n, max_rows, max_ctx))
+
+
+def kv8_attention_dev(cache, out_d, q_d, ldo, ldq, bf16, q_heads, row_d, pos_d, n, rows, max_rows, max_ctx, scale, work_d,
+                      work_bytes):
+    """Causal attention of the rows just appended over the cache."""
+    check(runtime.lib().qwen3_hip_kv8_attention_dev(ctypes.byref(cache), out_d, q_d, ldo, ldq, bf16, q_heads, row_d, pos_d,
+                                                    n, rows, max_rows, max_ctx, scale, work_d, work_bytes),
+          "qwen3_hip_kv8_attention_dev")
+
+
+def beam_select_work(vocab, n_group, width):
+    return int(runtime.lib().qwen3_hip_beam_select_work(vocab, n_group, width))
+
+
+def beam_select_dev(logits_d, ld, vocab, n_group, width, score_d, done_d, end0, end1, score_out_d, done_out_d, token_out_d,
+                    parent_out_d, work_d, work_bytes):
+    """The best `width` continuations of each group of beams."""
+    check(runtime.lib().qwen3_hip_beam_select_dev(logits_d, ld, vocab, n_group, width, score_d, done_d, end0, end1,
+                                                  score_out_d, done_out_d, token_out_d, parent_out_d, work_d, work_bytes),
+          "qwen3_hip_beam_select_dev")
+
+
+def beam_reorder_dev(dst_d, src_d, parent_d, n_group, width, slabs, slab_stride, seq_stride, runs, run_stride, run_bytes):
+    """The beams' states after their parents (dst_d may be src_d)."""
+    check(runtime.lib().qwen3_hip_beam_reorder_dev(dst_d, src_d, parent_d, n_group, width, slabs, slab_stride, seq_stride,
+                                                   runs, run_stride, run_bytes), "qwen3_hip_beam_reorder_dev")
+
+
 def sync():
     check(runtime.lib().qwen3_hip_sync(), "qwen3_hip_sync")
 

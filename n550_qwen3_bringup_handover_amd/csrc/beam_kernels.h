@@ -1,0 +1,350 @@
+// Beam search: the choice of each group's continuations and the reordering of
+// the beams' states.  Compiled into hip_model.hip.
+
+// ---------------------------------------------------------------------------
+// choice
+// ---------------------------------------------------------------------------
+// Group g holds W beams (rows g W ..).  Beam w continues with token v at
+//   score_w + x_wv - log sum_u e^(x_wu)
+// (a finished beam with one candidate, the end token at score_w); the best W
+// of them all, in order, ties to the lowest w V + v.
+//
+// Within a row the scores are ordered as the logits are, so one pass over the
+// logits finds each piece's maximum, sum of e^(x - max) and W best logits; a
+// second launch joins the pieces' sums and lists.  Scores are compared in
+// 64 bits: the logits' differences are of the order of their last bits only
+// where fp32 sums would lose them.
+#define BEAM_MAX QM_BEAM_MAX_WIDTH     // beams of a group
+#define BEAM_PIECE 2048                // logits of a wave: 32 a lane
+#define BEAM_V (BEAM_PIECE / WAVE)
+#define BEAM_NONE 0x7FFFFFFF           // the index of no candidate
+
+struct beam_cand { float v; int i; };
+struct beam_sum { float m, s; };
+
+// workspace: sums [row][piece], lists [row][piece][W]
+static size_t beam_pieces(int vocab) { return ((size_t)vocab + BEAM_PIECE - 1) / BEAM_PIECE; }
+
+template <int CTRL>
+__device__ __forceinline__ int dpp_int(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, false); }
+__device__ __forceinline__ int wave_min_int(int v) {
+    v = min(v, dpp_int<0xB1>(v));
+    v = min(v, dpp_int<0x4E>(v));
+    v = min(v, dpp_int<0x141>(v));
+    v = min(v, dpp_int<0x140>(v));
+    auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = min((int)p[0], (int)p[1]);
+    p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return min((int)p[0], (int)p[1]);
+}
+
+// a comes before b: larger, or equal with the lower index
+__device__ __forceinline__ bool beam_before(float av, int ai, float bv, int bi) {
+    return av > bv || (av == bv && ai < bi);
+}
+
+// Wave: one piece of one row.  Each lane keeps its best and second best;
+// W times the wave's best is taken and its lane moves up, scanning its values
+// again only after its second was used.
+template <bool VEC>
+__global__ __launch_bounds__(NTH) void k_beam_pieces(const float *__restrict__ logits, size_t ld, int vocab, int rows,
+                                                    int W, int pieces, const float *__restrict__ score,
+                                                    const int *__restrict__ done, beam_sum *__restrict__ sums,
+                                                    beam_cand *__restrict__ lists) {
+    const int lane = threadIdx.x & 63;
+    const int piece = blockIdx.x * (NTH / WAVE) + (threadIdx.x >> 6), r = blockIdx.y;
+    if (piece >= pieces) return;
+    beam_cand *out = lists + ((size_t)r * pieces + piece) * W;
+    // a finished beam's row is not read; a beam that cannot be chosen for its
+    // score offers its first tokens, in case nothing else is left
+    const bool over = done && done[r] != 0;
+    if (over || score[r] == -INFINITY) {
+        if (lane < W) out[lane] = beam_cand{-INFINITY, !over && piece == 0 && lane < vocab ? lane : BEAM_NONE};
+        if (lane == 0) sums[(size_t)r * pieces + piece] = beam_sum{-INFINITY, 0.0f};
+        return;
+    }
+    const float *x = logits + (size_t)r * ld;
+    const int base = piece * BEAM_PIECE;
+    float v[BEAM_V];
+    auto at = [&](int k) { return VEC ? base + (k >> 2) * (4 * WAVE) + 4 * lane + (k & 3) : base + k * WAVE + lane; };
+    if constexpr (VEC) {
+#pragma unroll
+        for (int k = 0; k < BEAM_V; k += 4) {
+            const int i = at(k);
+            f32x4 t = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (i + 3 < vocab) t = __builtin_nontemporal_load((const f32x4 *)(x + i));
+            else {
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (i + u < vocab) t[u] = x[i + u];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) v[k + u] = t[u];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < BEAM_V; k++) v[k] = at(k) < vocab ? x[at(k)] : -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < BEAM_V; k++) {
+        v[k] = v[k] == v[k] ? v[k] : -INFINITY;           // a NaN is never chosen
+        mx = fmaxf(mx, v[k]);
+    }
+    mx = wave_max(mx);
+    float sum = 0.0f;
+    if (mx > -INFINITY) {
+#pragma unroll
+        for (int k = 0; k < BEAM_V; k++) sum += expf(v[k] - mx);
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) sums[(size_t)r * pieces + piece] = beam_sum{mx, sum};
+
+    float v1 = -INFINITY, v2 = -INFINITY;
+    int i1 = BEAM_NONE, i2 = BEAM_NONE;
+    // the best two that come behind (pv, pi)
+    auto scan = [&](float pv, int pi) {
+        v1 = v2 = -INFINITY;
+        i1 = i2 = BEAM_NONE;
+#pragma unroll
+        for (int k = 0; k < BEAM_V; k++) {
+            const int i = at(k);
+            if (i < vocab && beam_before(pv, pi, v[k], i)) {
+                if (beam_before(v[k], i, v1, i1)) {
+                    v2 = v1; i2 = i1;
+                    v1 = v[k]; i1 = i;
+                } else if (beam_before(v[k], i, v2, i2)) {
+                    v2 = v[k]; i2 = i;
+                }
+            }
+        }
+    };
+    scan(INFINITY, -1);
+    for (int w = 0; w < W; w++) {
+        const float bv = wave_max(v1);
+        const int bi = wave_min_int(v1 == bv ? i1 : BEAM_NONE);
+        if (lane == 0) out[w] = beam_cand{bv, bi};
+        const bool mine = i1 == bi && bi != BEAM_NONE;
+        if (mine) { v1 = v2; i1 = i2; v2 = -INFINITY; i2 = BEAM_NONE; }
+        // i2 used up and i1 as well: look again behind what was taken
+        if (__any(mine && i1 == BEAM_NONE)) {
+            if (mine && i1 == BEAM_NONE) scan(bv, bi);
+        }
+    }
+}
+
+__device__ __forceinline__ bool beam_before(double av, int ai, double bv, int bi) {
+    return av > bv || (av == bv && ai < bi);
+}
+// the wave's best (score, index), in every lane
+__device__ __forceinline__ void beam_wave_best(double &v, int &i) {
+#pragma unroll
+    for (int s = 32; s >= 1; s >>= 1) {
+        const double ov = __shfl_xor(v, s);
+        const int oi = __shfl_xor(i, s);
+        if (beam_before(ov, oi, v, i)) { v = ov; i = oi; }
+    }
+}
+
+// Block: one group.  Wave w joins row w's sums and merges its pieces' lists
+// (each lane walks its own lists' heads); then wave 0 picks W of the W x W
+// rows' best.
+__global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, int pieces, const float *score,
+                                                             const int *done, int end0, int end1,
+                                                             const beam_sum *__restrict__ sums,
+                                                             const beam_cand *__restrict__ lists, float *score_out,
+                                                             int *done_out, int *__restrict__ token_out,
+                                                             int *__restrict__ parent_out) {
+    const int g = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    __shared__ double cv[BEAM_MAX * BEAM_MAX];
+    __shared__ int ci[BEAM_MAX * BEAM_MAX];              // token
+    __shared__ unsigned char head[BEAM_MAX][QM_BEAM_MAX_PIECES];
+    __shared__ int sdone[BEAM_MAX];
+    const int r = g * W + w;                              // grid: W waves a block
+    const bool over = done && done[r] != 0;
+    const double base = score[r];
+    if (lane == 0) sdone[w] = over;
+    if (over) {
+        if (lane < W) {
+            cv[w * W + lane] = lane == 0 ? base : -INFINITY;
+            ci[w * W + lane] = lane == 0 ? end0 : BEAM_NONE;
+        }
+    } else {
+        // log of the sum of e^x over the row
+        const beam_sum *ps = sums + (size_t)r * pieces;
+        float mx = -INFINITY;
+        for (int p = lane; p < pieces; p += WAVE) mx = fmaxf(mx, ps[p].m);
+        mx = wave_max(mx);
+        double sum = 0.0;
+        for (int p = lane; p < pieces; p += WAVE)
+            if (ps[p].m > -INFINITY) sum += (double)ps[p].s * exp((double)ps[p].m - (double)mx);
+#pragma unroll
+        for (int s = 32; s >= 1; s >>= 1) sum += __shfl_xor(sum, s);
+        const double lse = (double)mx + log(sum);
+        const beam_cand *pl = lists + (size_t)r * pieces * W;
+        for (int p = lane; p < pieces; p += WAVE) head[w][p] = 0;
+        for (int k = 0; k < W; k++) {
+            float bv = -INFINITY;
+            int bi = BEAM_NONE, bp = -1;
+            for (int p = lane; p < pieces; p += WAVE) {
+                const int hd = head[w][p];
+                if (hd >= W) continue;
+                const beam_cand t = pl[(size_t)p * W + hd];
+                if (beam_before(t.v, t.i, bv, bi)) { bv = t.v; bi = t.i; bp = p; }
+            }
+            const float wv = wave_max(bv);
+            const int wi = wave_min_int(bv == wv ? bi : BEAM_NONE);
+            if (bp >= 0 && bi == wi) head[w][bp]++;
+            if (lane == 0) {
+                const double t = base + ((double)wv - lse);
+                cv[w * W + k] = t == t ? t : -INFINITY;   // no probabilities, no score
+                ci[w * W + k] = wi;
+            }
+        }
+    }
+    __syncthreads();
+    if (w > 0) return;
+    // BEAM_MAX^2 / 64 candidates a lane, by place w' W + k; a tie goes to the
+    // lowest w' V + token
+    constexpr int PER = BEAM_MAX * BEAM_MAX / WAVE;
+    double v[PER];
+    long id[PER];
+#pragma unroll
+    for (int u = 0; u < PER; u++) {
+        const int at = lane + WAVE * u;
+        const bool in = at < W * W && ci[at] != BEAM_NONE;
+        v[u] = in ? cv[at] : -INFINITY;
+        id[u] = in ? (long)(at / W) * vocab + ci[at] : 0x7FFFFFFFFFFFFFFFL;
+    }
+    for (int k = 0; k < W; k++) {
+        double bv = -INFINITY;
+        long bi = 0x7FFFFFFFFFFFFFFFL;
+#pragma unroll
+        for (int u = 0; u < PER; u++)
+            if (v[u] > bv || (v[u] == bv && id[u] < bi)) { bv = v[u]; bi = id[u]; }
+#pragma unroll
+        for (int s = 32; s >= 1; s >>= 1) {
+            const double ov = __shfl_xor(bv, s);
+            const long oi = __shfl_xor(bi, s);
+            if (ov > bv || (ov == bv && oi < bi)) { bv = ov; bi = oi; }
+        }
+#pragma unroll
+        for (int u = 0; u < PER; u++)
+            if (id[u] == bi) { v[u] = -INFINITY; id[u] = 0x7FFFFFFFFFFFFFFFL; }
+        if (lane == 0) {
+            // the inputs of the group have all been read: outputs may lie where they did
+            const int par = (int)(bi / vocab), tok = (int)(bi % vocab);
+            score_out[g * W + k] = (float)bv;
+            token_out[g * W + k] = tok;
+            parent_out[g * W + k] = par;
+            done_out[g * W + k] = sdone[par] != 0 || tok == end0 || tok == end1;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// reordering
+// ---------------------------------------------------------------------------
+// dst row w of every group = src row parent[w], over `slabs` states of
+// n_group * W rows, each row `runs` stretches of `run_bytes` used bytes.  A
+// thread owns one unit of T at the same place of all W rows: it reads every
+// row it needs before it writes any, so dst may be src, and rows that stay
+// where they are are then not touched.  Bound by the memory's rate.
+template <typename T, int WT>
+__global__ __launch_bounds__(NTH) void k_beam_reorder(uint8_t *dst, const uint8_t *src, const int *__restrict__ parent,
+                                                     int W, unsigned units, unsigned runs, size_t slab_stride,
+                                                     size_t seq_stride, size_t run_stride) {
+    const int g = blockIdx.y;
+    const unsigned u = blockIdx.x * NTH + threadIdx.x, run = u / units;
+    if (run >= runs) return;
+    const size_t at = (size_t)blockIdx.z * slab_stride + (size_t)g * W * seq_stride + (size_t)run * run_stride +
+                      (size_t)(u - run * units) * sizeof(T);
+    const bool same = dst == src;
+    T v[WT];
+    int p[WT];
+#pragma unroll
+    for (int w = 0; w < WT; w++) {
+        p[w] = w < W ? parent[g * W + w] : -1;
+        if (p[w] >= W || (same && p[w] == w)) p[w] = -1;
+        if (p[w] >= 0) v[w] = *(const T *)(src + at + (size_t)p[w] * seq_stride);
+    }
+#pragma unroll
+    for (int w = 0; w < WT; w++)
+        if (p[w] >= 0) *(T *)(dst + at + (size_t)w * seq_stride) = v[w];
+}
+
+// ---------------------------------------------------------------------------
+// launchers
+// ---------------------------------------------------------------------------
+extern "C" size_t qm_beam_select_work(int vocab, int n_group, int width) {
+    if (vocab < 1 || n_group < 1 || width < 1 || width > BEAM_MAX) return 0;
+    const size_t lists = (size_t)n_group * width * beam_pieces(vocab);
+    return lists * (sizeof(beam_sum) + (size_t)width * sizeof(beam_cand));
+}
+
+extern "C" int qm_beam_select(const float *logits, size_t ld, int vocab, int n_group, int width, const float *score,
+                              const int *done, int end0, int end1, float *score_out, int *done_out, int *token_out,
+                              int *parent_out, void *work, size_t work_bytes) {
+    if (n_group < 0 || width < 1 || width > BEAM_MAX || vocab < width || ld < (size_t)vocab) return QH_EINVAL;
+    if (end0 >= vocab || end1 >= vocab || (done && end0 < 0)) return QH_EINVAL;
+    if (n_group == 0) return QH_OK;
+    if (!logits || !score || !score_out || !done_out || !token_out || !parent_out || !work || ((uintptr_t)work & 7)) return QH_EINVAL;
+    const size_t pieces = beam_pieces(vocab);
+    if (pieces > QM_BEAM_MAX_PIECES || (long)n_group * width > 65535) return QH_ETOOBIG;
+    if (work_bytes < qm_beam_select_work(vocab, n_group, width)) return QH_ETOOBIG;
+    if (!stream()) return QH_ESTATE;
+    const int rows = n_group * width;
+    beam_sum *sums = (beam_sum *)work;
+    beam_cand *lists = (beam_cand *)(sums + (size_t)rows * pieces);
+    const dim3 grid((unsigned)((pieces + NTH / WAVE - 1) / (NTH / WAVE)), rows);
+    if (aligned16(logits) && ld % 4 == 0)
+        hipLaunchKernelGGL(k_beam_pieces<true>, grid, dim3(NTH), 0, stream(), logits, ld, vocab, rows, width, (int)pieces,
+                           score, done, sums, lists);
+    else
+        hipLaunchKernelGGL(k_beam_pieces<false>, grid, dim3(NTH), 0, stream(), logits, ld, vocab, rows, width, (int)pieces,
+                           score, done, sums, lists);
+    if (hipGetLastError() != hipSuccess) return QH_ELAUNCH;
+    hipLaunchKernelGGL(k_beam_pick, dim3(n_group), dim3(WAVE * width), 0, stream(), vocab, width, (int)pieces, score, done,
+                       end0, end1, sums, lists, score_out, done_out, token_out, parent_out);
+    return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
+}
+
+extern "C" int qm_beam_reorder(void *dst, const void *src, const int *parent, int n_group, int width, int slabs,
+                               size_t slab_stride, size_t seq_stride, int runs, size_t run_stride, size_t run_bytes) {
+    if (n_group < 0 || width < 1 || width > BEAM_MAX || slabs < 0 || runs < 0) return QH_EINVAL;
+    if (n_group == 0 || slabs == 0 || runs == 0 || run_bytes == 0) return QH_OK;
+    if (!dst || !src || !parent) return QH_EINVAL;
+    if (run_bytes % 4 || (runs > 1 && run_stride % 4) || seq_stride % 4 || (slabs > 1 && slab_stride % 4) ||
+        (((uintptr_t)dst | (uintptr_t)src) & 3))
+        return QH_EINVAL;
+    // rows, and the states, must not reach into one another
+    if (n_group > 65535 || slabs > 65535 || runs > 1 << 24 || run_bytes > (size_t)1 << 40 || seq_stride > (size_t)1 << 44 ||
+        slab_stride > (size_t)1 << 46 || run_stride > (size_t)1 << 40)
+        return QH_ETOOBIG;
+    const size_t row = (size_t)(runs - 1) * run_stride + run_bytes;
+    const size_t slab = ((size_t)n_group * width - 1) * seq_stride + row;
+    if ((runs > 1 && run_stride < run_bytes) || seq_stride < row || (slabs > 1 && slab_stride < slab)) return QH_EINVAL;
+    const size_t all = (size_t)(slabs - 1) * (slabs > 1 ? slab_stride : 0) + slab;
+    const uintptr_t d = (uintptr_t)dst, s = (uintptr_t)src;
+    if (d != s && d < s + all && s < d + all) return QH_EINVAL;
+    if (width == 1 && d == s) return QH_OK;
+    const bool wide = !((run_bytes | seq_stride | (runs > 1 ? run_stride : 0) | (slabs > 1 ? slab_stride : 0) | d | s) & 15);
+    const size_t units = run_bytes / (wide ? 16 : 4);
+    if (units * runs >= (size_t)1 << 31) return QH_ETOOBIG;
+    if (!stream()) return QH_ESTATE;
+    const dim3 grid((unsigned)((units * runs + NTH - 1) / NTH), n_group, slabs);
+#define REORDER(T, WT)                                                                                               \
+    hipLaunchKernelGGL((k_beam_reorder<T, WT>), grid, dim3(NTH), 0, stream(), (uint8_t *)dst, (const uint8_t *)src,  \
+                       parent, width, (unsigned)units, (unsigned)runs, slab_stride, seq_stride, run_stride)
+#define REORDER_W(T)                          \
+    do {                                      \
+        if (width <= 4) REORDER(T, 4);        \
+        else if (width <= 8) REORDER(T, 8);   \
+        else REORDER(T, 16);                  \
+    } while (0)
+    if (wide) REORDER_W(u32x4);
+    else REORDER_W(uint32_t);
+#undef REORDER_W
+#undef REORDER
+    return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
+}

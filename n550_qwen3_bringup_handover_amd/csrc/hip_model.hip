@@ -1,6 +1,7 @@
 // CDNA4 (gfx950) kernels of the device-resident Qwen3-0.6B forward besides
 // the projection GEMMs: row-wise residual + RMSNorm (with the embedding
-// gather folded in) and the fused attention step.  The arithmetic follows the
+// gather folded in) and the fused attention step; the 8-bit KV cache and beam
+// search are in kv8_kernels.h and beam_kernels.h, compiled into this unit.  The arithmetic follows the
 // reference's scalar ops (fpga_bringup/src/src/ops_scalar.c) and forward
 // (fpga_bringup/src/src/qwen3.c:276-576); sums are reduced in parallel, so
 // results agree to rounding, not bit for bit.
@@ -847,6 +848,10 @@ __global__ void k_zero_i32(int *p, int n) {
 // launchers
 // ---------------------------------------------------------------------------
 static inline hipStream_t stream() { return (hipStream_t)qh_stream(); }
+
+// the operators of a serving program: their kernels and launchers
+#include "kv8_kernels.h"
+#include "beam_kernels.h"
 
 template <bool BF>
 static int rows_norm(float *x, const float *r, const uint16_t *emb, const int *tok, int emb_rows, const uint16_t *nw,

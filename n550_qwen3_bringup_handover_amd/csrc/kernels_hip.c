@@ -7,7 +7,9 @@
  */
 #define _POSIX_C_SOURCE 199309L   /* clock_gettime */
 #include "qwen3_hip.h"
+#include "qwen3_hip_serve.h"
 #include "hip_shim.h"
+#include "model_shim.h"
 
 #include <stdint.h>
 #include <stdio.h>
@@ -613,6 +615,60 @@ int qwen3_hip_copy_dev(void *dst, const void *src, size_t bytes) {
 int qwen3_hip_read_dev(const void *src, size_t bytes) {
     READY_OR_RETURN();
     return note(qh_read(src, bytes));
+}
+
+/* ---- serving operators (qwen3_hip_serve.h) ------------------------------------------ */
+static qm_kv8_t kv8_of(const qwen3_hip_kv8 *c) {
+    const qm_kv8_t t = {c->format, c->kv_heads, c->head_dim, c->block, c->n_page, c->n_seq, c->max_blocks,
+                        c->k, c->v, c->k_scale, c->v_scale, c->k_tail, c->v_tail, c->table};
+    return t;
+}
+
+size_t qwen3_hip_kv8_bytes(const qwen3_hip_kv8 *c) {
+    if (!c) return 0;
+    const qm_kv8_t t = kv8_of(c);
+    return qm_kv8_bytes(&t);
+}
+
+int qwen3_hip_kv8_append_dev(const qwen3_hip_kv8 *c, const void *k, const void *v, size_t ldk, size_t ldv, int bf16,
+                             const int *row, const int *pos, int n, int rows, int max_rows) {
+    if (!c) return note(QWEN3_HIP_EINVAL);
+    READY_OR_RETURN();
+    const qm_kv8_t t = kv8_of(c);
+    return note(qm_kv8_append(&t, k, v, ldk, ldv, bf16, row, pos, n, rows, max_rows));
+}
+
+size_t qwen3_hip_kv8_attention_work(const qwen3_hip_kv8 *c, int q_heads, int n, int max_rows, int max_ctx) {
+    if (!c) return 0;
+    const qm_kv8_t t = kv8_of(c);
+    return qm_kv8_attention_work(&t, q_heads, n, max_rows, max_ctx);
+}
+
+int qwen3_hip_kv8_attention_dev(const qwen3_hip_kv8 *c, void *out, const void *q, size_t ldo, size_t ldq, int bf16,
+                                int q_heads, const int *row, const int *pos, int n, int rows, int max_rows, int max_ctx,
+                                float scale, void *work, size_t work_bytes) {
+    if (!c) return note(QWEN3_HIP_EINVAL);
+    READY_OR_RETURN();
+    const qm_kv8_t t = kv8_of(c);
+    return note(qm_kv8_attention(&t, out, q, ldo, ldq, bf16, q_heads, row, pos, n, rows, max_rows, max_ctx, scale, work,
+                                 work_bytes));
+}
+
+size_t qwen3_hip_beam_select_work(int vocab, int n_group, int width) { return qm_beam_select_work(vocab, n_group, width); }
+
+int qwen3_hip_beam_select_dev(const float *logits, size_t ld, int vocab, int n_group, int width, const float *score,
+                              const int *done, int end0, int end1, float *score_out, int *done_out, int *token_out,
+                              int *parent_out, void *work, size_t work_bytes) {
+    READY_OR_RETURN();
+    return note(qm_beam_select(logits, ld, vocab, n_group, width, score, done, end0, end1, score_out, done_out, token_out,
+                               parent_out, work, work_bytes));
+}
+
+int qwen3_hip_beam_reorder_dev(void *dst, const void *src, const int *parent, int n_group, int width, int slabs,
+                               size_t slab_stride, size_t seq_stride, int runs, size_t run_stride, size_t run_bytes) {
+    READY_OR_RETURN();
+    return note(qm_beam_reorder(dst, src, parent, n_group, width, slabs, slab_stride, seq_stride, runs, run_stride,
+                                run_bytes));
 }
 
 int qwen3_hip_capture_begin(void) { READY_OR_RETURN(); return note(qh_capture_begin()); }

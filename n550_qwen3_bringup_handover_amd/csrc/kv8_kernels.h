@@ -1,0 +1,836 @@
+// The 8-bit KV cache: storing rows into it and attention over it.  Compiled
+// into hip_model.hip.
+//
+// One layer's cache (qm_kv8_t): pages of B = 16, 32 or 64 tokens.  A finished
+// block lies in a page as one byte per value with one fp32 scale per kv head
+// for K and one for V; the unfinished block of a sequence lies in its tail as
+// bf16.  A block is quantised once, when its last row arrives, from the same
+// bf16 values whatever calls brought them, and never changes again, so beams
+// can share pages.
+//   x = bf16(row)           RNE; NaN -> 0, magnitudes saturate at the largest bf16
+//   a = max |x| over B x D, s = a / qmax (0 where a < 2^-100)
+//   code = rne(x / s)       e4m3 (qmax 448) or int8 (qmax 127); division and
+//                           scale rounded to fp32
+// K rows lie [slot][dim], V columns [dim][slot]: both products of attention
+// then read 8 or 16 contiguous bytes per lane in the order their MFMA wants.
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+#define KV8_TINY 0x1p-100f
+#define KV8_BF16_MAX 3.38953139e38f       // 0x7F7F as bf16
+
+template <int FMT>
+struct kv8_qmax { static constexpr float v = FMT == QM_KV8_E4M3 ? 448.0f : 127.0f; };
+
+// what a call says about entry e: its rows in the call's buffers and the
+// position of the first; false (the entry is left out) where these do not fit
+struct kv8_entry { int r0, cnt, pos; };
+__device__ __forceinline__ bool kv8_get(kv8_entry &t, const qm_kv8_t &c, const int *row, const int *pos, int e,
+                                        int rows, int max_rows) {
+    t.r0 = row ? row[e] : e;
+    const int r1 = row ? row[e + 1] : e + 1;
+    t.pos = pos[e];
+    if (t.r0 < 0 || r1 <= t.r0 || r1 > rows || r1 - t.r0 > max_rows) return false;
+    t.cnt = r1 - t.r0;
+    return t.pos >= 0 && t.pos <= c.max_blocks * c.block - t.cnt;
+}
+
+// ---------------------------------------------------------------------------
+// store
+// ---------------------------------------------------------------------------
+// a row's value as the cache holds it: bf16, finite
+__device__ __forceinline__ __bf16 kv8_held(float x) {
+    x = x == x ? x : 0.0f;
+    return (__bf16)fminf(fmaxf(x, -KV8_BF16_MAX), KV8_BF16_MAX);
+}
+
+template <int FMT>
+__device__ __forceinline__ uint32_t kv8_codes4(float a, float b, float c, float d, float s) {
+    if (s == 0.0f) return 0;
+    a /= s; b /= s; c /= s; d /= s;
+    if constexpr (FMT == QM_KV8_E4M3) {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+    } else {
+        auto i = [](float x) { return (uint32_t)(int)fminf(fmaxf(rintf(x), -127.0f), 127.0f) & 0xFFu; };
+        return i(a) | i(b) << 8 | i(c) << 16 | i(d) << 24;
+    }
+}
+
+// Block (h, e, z): kv head h of entry e, the z-th block its rows touch.  A
+// block that the rows finish is gathered in LDS as bf16 (rows that earlier
+// calls brought from the tail), its largest magnitudes found, its codes
+// written 16 bytes a thread.  The rows behind the last finished block go to
+// the tail, by z = 0 alone and after it has read the tail: two blocks of one
+// launch must not meet there.
+// Bound by its launch and two dependent reads for a decode step's rows.
+template <int FMT, int D, int B, bool BF>
+__global__ __launch_bounds__(NTH) void k_kv8_append(qm_kv8_t c, const void *__restrict__ kn, const void *__restrict__ vn,
+                                                   size_t ldk, size_t ldv, const int *__restrict__ row,
+                                                   const int *__restrict__ pos, int rows, int max_rows) {
+    const int h = blockIdx.x, e = blockIdx.y, z = blockIdx.z, tid = threadIdx.x;
+    kv8_entry t;
+    if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
+    const int end = t.pos + t.cnt, b0 = t.pos / B, bl = end / B, b = b0 + z;
+    if (b >= bl && z > 0) return;
+    auto k_at = [&](int p, int d) {
+        const size_t i = (size_t)(t.r0 + p - t.pos) * ldk + h * D + d;
+        return BF ? (float)((const __bf16 *)kn)[i] : ((const float *)kn)[i];
+    };
+    auto v_at = [&](int p, int d) {
+        const size_t i = (size_t)(t.r0 + p - t.pos) * ldv + h * D + d;
+        return BF ? (float)((const __bf16 *)vn)[i] : ((const float *)vn)[i];
+    };
+    __bf16 *kt = (__bf16 *)c.k_tail + ((size_t)e * c.heads + h) * (B * D);
+    __bf16 *vt = (__bf16 *)c.v_tail + ((size_t)e * c.heads + h) * (B * D);
+
+    if (b < bl) {
+        __shared__ __align__(16) __bf16 sk[B * D], sv[B * D];
+        __shared__ float red[2][NTH / WAVE];
+        float ak = 0.0f, av = 0.0f;
+        for (int i = tid; i < B * D; i += NTH) {
+            const int r = i / D, d = i % D, p = b * B + r;
+            const __bf16 x = p < t.pos ? kt[i] : kv8_held(k_at(p, d));
+            const __bf16 y = p < t.pos ? vt[d * B + r] : kv8_held(v_at(p, d));
+            sk[i] = x;
+            sv[i] = y;
+            ak = fmaxf(ak, fabsf((float)x));
+            av = fmaxf(av, fabsf((float)y));
+        }
+        ak = wave_max(ak);
+        av = wave_max(av);
+        if ((tid & 63) == 0) { red[0][tid >> 6] = ak; red[1][tid >> 6] = av; }
+        __syncthreads();
+        ak = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+        av = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+        const float ks = ak < KV8_TINY ? 0.0f : ak / kv8_qmax<FMT>::v;
+        const float vs = av < KV8_TINY ? 0.0f : av / kv8_qmax<FMT>::v;
+        const int page = c.table[(size_t)e * c.max_blocks + b];
+        if (page >= 0 && page < c.n_page) {               // the same for the whole block
+            const size_t at = (size_t)page * c.heads + h;
+            uint4 *ko = (uint4 *)(c.k + at * (B * D)), *vo = (uint4 *)(c.v + at * (B * D));
+            for (int u = tid; u < B * D / 16; u += NTH) {
+                const __bf16 *s = sk + 16 * u;
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    w[j] = kv8_codes4<FMT>((float)s[4 * j], (float)s[4 * j + 1], (float)s[4 * j + 2],
+                                           (float)s[4 * j + 3], ks);
+                ko[u] = make_uint4(w[0], w[1], w[2], w[3]);
+                const int d = u / (B / 16), r = u % (B / 16) * 16;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    w[j] = kv8_codes4<FMT>((float)sv[(r + 4 * j) * D + d], (float)sv[(r + 4 * j + 1) * D + d],
+                                           (float)sv[(r + 4 * j + 2) * D + d], (float)sv[(r + 4 * j + 3) * D + d], vs);
+                vo[u] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            if (tid == 0) {
+                c.k_scale[at] = ks;
+                c.v_scale[at] = vs;
+            }
+        }
+    }
+    if (z > 0) return;
+    const int from = max(t.pos, bl * B);
+    for (int i = tid; i < (end - from) * D; i += NTH) {
+        const int p = from + i / D, d = i % D;
+        kt[(p - bl * B) * D + d] = kv8_held(k_at(p, d));
+        vt[d * B + (p - bl * B)] = kv8_held(v_at(p, d));
+    }
+}
+
+// ---------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------
+// Both kernels work on S^T = K Q^T and O^T += V^T P^T with 16x16x32 bf16
+// MFMAs, the columns being query rows (row r, query head g of the kv head:
+// column r G + g), 64 keys a step.  8-bit codes are exact in bf16, so the
+// scales stay outside: K's multiplies the scores, V's the weights.
+// fp32 rows keep fp32 accuracy: q and the weights go through the matrix cores
+// as three bf16 pieces each (8 bits apiece: x - x1 - x2 - x3 < 2^-24 x).  bf16
+// rows are one piece; their weights are two where the bytes bound the kernel
+// and one in a prompt, whose results are rounded to bf16 anyway (the weights'
+// roundings, each its own, then add as much as that one does).
+//   S^T tile t, row m <-> key 16 (m / 4) + 4 t + m % 4 of the step, so that
+//   lane (c, h) = (lane % 16, lane / 16) ends up with keys 16 h + 4 t + i of
+//   column c: four tiles are 16 consecutive keys, which lie in one page (one
+//   scale) and, in V's columns, in 16 consecutive bytes.  The weights of
+//   tiles 2 s and 2 s + 1 are then, as they lie, the B operand of the MFMA
+//   over keys 16 h + 8 s .. + 7, and 8 bytes of V's column its A operand.
+template <int FMT>
+__device__ __forceinline__ bf16x8 kv8_bf16(uint32_t a, uint32_t b) {      // eight codes
+    union { bf16x2 p[4]; bf16x8 v; } r;
+    if constexpr (FMT == QM_KV8_E4M3) {
+        r.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
+        r.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
+        r.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
+        r.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            r.v[i] = (__bf16)(float)(int8_t)(a >> (8 * i));
+            r.v[4 + i] = (__bf16)(float)(int8_t)(b >> (8 * i));
+        }
+    }
+    return r.v;
+}
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// x as NP bf16 pieces
+template <int NP>
+__device__ __forceinline__ void kv8_pieces(f32x8 x, bf16x8 (&p)[NP]) {
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+        p[i] = __builtin_convertvector(x, bf16x8);
+        if (i + 1 < NP) x -= __builtin_convertvector(p[i], f32x8);
+    }
+}
+
+__device__ __forceinline__ f32x4 kv8_mma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// eight values of a query row
+template <bool BF, int NP>
+__device__ __forceinline__ void kv8_load_q(const void *q, size_t i, bool in, bf16x8 (&p)[NP]) {
+    if constexpr (BF) {
+        static_assert(NP == 1, "bf16 rows are one piece");
+        p[0] = in ? *(const bf16x8 *)((const __bf16 *)q + i) : bf16x8{};
+    } else {
+        f32x8 x = {};
+        if (in) {
+            const f32x4 a = *(const f32x4 *)((const float *)q + i), b = *(const f32x4 *)((const float *)q + i + 4);
+            x = f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        }
+        kv8_pieces<NP>(x, p);
+    }
+}
+
+// max and sum over the four lanes that share a column
+__device__ __forceinline__ float col_max(float v) {
+    f32x2 p = swap16(v);
+    v = fmaxf(p.x, p.y);
+    p = swap32(v);
+    return fmaxf(p.x, p.y);
+}
+__device__ __forceinline__ float col_sum(float v) {
+    f32x2 p = swap16(v);
+    v = p.x + p.y;
+    p = swap32(v);
+    return p.x + p.y;
+}
+
+// 1 / sum of weights; a row of which nothing was left (pages that are none) is 0
+__device__ __forceinline__ float kv8_inverse(float den) { return den == 0.0f ? 0.0f : 1.0f / den; }
+
+// the running softmax of one column tile: scores s (in units of log2 after the
+// factor f, masked entries -inf) become weights; returns what the sums so far
+// are to be multiplied by
+__device__ __forceinline__ float kv8_softmax(f32x4 (&s)[4], float &m, float &l) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; t++) mx = fmaxf(mx, fmaxf(fmaxf(s[t].x, s[t].y), fmaxf(s[t].z, s[t].w)));
+    const float nm = fmaxf(m, col_max(mx));
+    const float ref = nm == -INFINITY ? 0.0f : nm;       // nothing seen yet: every weight is 0
+    const float r = __builtin_amdgcn_exp2f(m - ref);
+    m = nm;
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref);
+            sum += s[t][i];
+        }
+    l = l * r + sum;
+    return r;
+}
+
+// ---- few columns: keys split over waves and blocks --------------------------
+// Block (split, head + heads * column tile, entry): four waves take the steps
+// of 64 keys in turn, wave w of split y steps 4 y + w, + 4 nsplit, ...; each
+// operand goes from memory straight into its MFMA's registers (K of the next
+// step is in flight during this step's V product).  The tail is one more step.
+// The waves' sums meet in LDS; with several splits each block leaves a partial
+// {m, l, -, -, o[D]} per column for k_kv8_merge.
+#define KV8_NW 4
+#define KV8_COLS 16
+template <int FMT, int D, bool BF>
+__global__ __launch_bounds__(WAVE *KV8_NW, 2) void k_kv8_few(qm_kv8_t c, void *__restrict__ out,
+                                                             const void *__restrict__ q, size_t ldo, size_t ldq,
+                                                             const int *__restrict__ row, const int *__restrict__ pos,
+                                                             int rows, int max_rows, int G, float f,
+                                                             float *__restrict__ part) {
+    constexpr int NP = BF ? 1 : 3, NW = BF ? 2 : 3;        // pieces of q, and of a weight
+    constexpr int KS = D / 32, DT = D / 16, LD = D + 4;
+    const int e = blockIdx.z, head = blockIdx.y % c.heads, ct = blockIdx.y / c.heads;
+    kv8_entry t;
+    if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
+    const int col0 = ct * KV8_COLS, ncol = t.cnt * G;
+    if (col0 >= ncol) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int cl = lane & 15, h = lane >> 4;
+    const int B = c.block, lb = __builtin_ctz(B);
+    const int full = (t.pos + t.cnt) >> lb << lb;                          // keys in finished blocks
+    const int kend = t.pos + min(t.cnt - 1, (col0 + KV8_COLS - 1) / G) + 1;   // keys the block's last column sees
+    const int ns = (min(full, kend) + 63) >> 6, stride = KV8_NW * gridDim.x;
+
+    const int col = col0 + cl;
+    const bool in = col < ncol;
+    const int qr = in ? col / G : 0, qg = in ? col % G : 0;
+    const int last = in ? t.pos + qr : -1;                                 // the column's last key
+    bf16x8 qf[KS][NP];
+#pragma unroll
+    for (int j = 0; j < KS; j++)
+        kv8_load_q<BF, NP>(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + (D / 4) * h + 8 * j, in, qf[j]);
+
+    const int *table = c.table + (size_t)e * c.max_blocks;
+    // page of the 16 keys at `key`, -1 where there is none
+    auto page_of = [&](int key) {
+        int p = -1;
+        if (key < full) p = table[key >> lb];
+        return (unsigned)p < (unsigned)c.n_page ? p : -1;
+    };
+    const int gk = (lane >> 2) & 3;                                        // the group its K row lies in
+    uint4 kk[4][D / 64], vv[DT];
+    auto load_k = [&](int s, int p) {
+        const int key = 64 * s + 16 * gk;
+        const uint8_t *b = c.k + (((size_t)p * c.heads + head) * B + ((key & (B - 1)) + (lane & 3))) * D + (D / 4) * h;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int u = 0; u < D / 64; u++)
+                kk[i][u] = p >= 0 ? *(const uint4 *)(b + (size_t)4 * i * D + 16 * u) : uint4{};
+    };
+    auto load_v = [&](int s, int p) {
+        const int key = 64 * s + 16 * h;
+        const uint8_t *b = c.v + (((size_t)p * c.heads + head) * D + cl) * B + (key & (B - 1));
+#pragma unroll
+        for (int i = 0; i < DT; i++) vv[i] = p >= 0 ? *(const uint4 *)(b + (size_t)16 * i * B) : uint4{};
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o[DT], s4[4];
+#pragma unroll
+    for (int i = 0; i < DT; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // weights p (times the page's V scale) as B operands of key half s2
+    auto weights = [&](int s2, float vs, bf16x8 (&pf)[NW]) {
+        const f32x4 a = s4[2 * s2] * vs, b = s4[2 * s2 + 1] * vs;
+        kv8_pieces<NW>(f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, pf);
+    };
+
+    int s = KV8_NW * blockIdx.x + wave;
+    int pk = -1, pv = -1;
+    if (s < ns) {
+        pk = page_of(64 * s + 16 * gk);
+        pv = page_of(64 * s + 16 * h);
+        load_k(s, pk);
+    }
+    for (; s < ns; s += stride) {
+        load_v(s, pv);
+        const float ks = pv >= 0 ? c.k_scale[(size_t)pv * c.heads + head] * f : 0.0f;
+        const float vs = pv >= 0 ? c.v_scale[(size_t)pv * c.heads + head] : 0.0f;
+        const int lim = pv >= 0 ? last - (64 * s + 16 * h) : -1;           // the group's last key that is seen
+        const int nx = s + stride;
+        int pkn = -1, pvn = -1;
+        if (nx < ns) {
+            pkn = page_of(64 * nx + 16 * gk);
+            pvn = page_of(64 * nx + 16 * h);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < KS; j++) {
+                const uint4 w = kk[i][j >> 1];
+                const bf16x8 kf = (j & 1) ? kv8_bf16<FMT>(w.z, w.w) : kv8_bf16<FMT>(w.x, w.y);
+#pragma unroll
+                for (int n = 0; n < NP; n++) a = kv8_mma(kf, qf[j][n], a);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) s4[i][r] = 4 * i + r <= lim ? a[r] * ks : -INFINITY;
+        }
+        if (nx < ns) load_k(nx, pkn);
+        const float rs = kv8_softmax(s4, m, l);
+#pragma unroll
+        for (int i = 0; i < DT; i++) o[i] *= rs;
+#pragma unroll
+        for (int s2 = 0; s2 < 2; s2++) {
+            bf16x8 pf[NW];
+            weights(s2, vs, pf);
+#pragma unroll
+            for (int i = 0; i < DT; i++) {
+                const bf16x8 vf = s2 ? kv8_bf16<FMT>(vv[i].z, vv[i].w) : kv8_bf16<FMT>(vv[i].x, vv[i].y);
+#pragma unroll
+                for (int n = 0; n < NW; n++) o[i] = kv8_mma(vf, pf[n], o[i]);
+            }
+        }
+        pv = pvn;
+    }
+
+    // the unfinished block, as step ns of the turn
+    if (kend > full && ns % stride == KV8_NW * (int)blockIdx.x + wave) {
+        const int nt = t.pos + t.cnt - full;                               // rows it holds, < B <= 64
+        const __bf16 *kt = (const __bf16 *)c.k_tail + ((size_t)e * c.heads + head) * ((size_t)B * D);
+        const __bf16 *vt = (const __bf16 *)c.v_tail + ((size_t)e * c.heads + head) * ((size_t)B * D);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int key = 16 * gk + 4 * i + (lane & 3);
+            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < KS; j++) {
+                const bf16x8 kf = key < nt ? *(const bf16x8 *)(kt + (size_t)key * D + (D / 4) * h + 8 * j) : bf16x8{};
+#pragma unroll
+                for (int n = 0; n < NP; n++) a = kv8_mma(kf, qf[j][n], a);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int k = 16 * h + 4 * i + r;
+                s4[i][r] = k < nt && full + k <= last ? a[r] * f : -INFINITY;
+            }
+        }
+        const float rs = kv8_softmax(s4, m, l);
+#pragma unroll
+        for (int i = 0; i < DT; i++) o[i] *= rs;
+#pragma unroll
+        for (int s2 = 0; s2 < 2; s2++) {
+            bf16x8 pf[NW];
+            weights(s2, 1.0f, pf);
+            const int k0 = 16 * h + 8 * s2;
+#pragma unroll
+            for (int i = 0; i < DT; i++) {
+                bf16x8 vf = {};
+                if (k0 < nt) vf = *(const bf16x8 *)(vt + (size_t)(16 * i + cl) * B + k0);
+#pragma unroll
+                for (int n = 0; n < 8; n++) vf[n] = k0 + n < nt ? vf[n] : (__bf16)0.0f;   // behind the last row: anything
+#pragma unroll
+                for (int n = 0; n < NW; n++) o[i] = kv8_mma(vf, pf[n], o[i]);
+            }
+        }
+    }
+
+    // merge the waves
+    __shared__ __align__(16) float so[KV8_NW][KV8_COLS][LD];
+    __shared__ float sm[KV8_NW][KV8_COLS], sl[KV8_NW][KV8_COLS];
+    l = col_sum(l);
+#pragma unroll
+    for (int i = 0; i < DT; i++) *(f32x4 *)&so[wave][cl][16 * i + 4 * h] = o[i];
+    if (h == 0) { sm[wave][cl] = m; sl[wave][cl] = l; }
+    __syncthreads();
+    constexpr int TPC = D / 4;                            // threads of a column
+    for (int i = tid; i < KV8_COLS * TPC; i += WAVE * KV8_NW) {
+        const int cc = i / TPC, d = i % TPC * 4, cg = col0 + cc;
+        if (cg >= ncol) continue;
+        float mx = sm[0][cc];
+#pragma unroll
+        for (int w = 1; w < KV8_NW; w++) mx = fmaxf(mx, sm[w][cc]);
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        float den = 0.0f;
+        f32x4 num = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < KV8_NW; w++) {
+            // a wave without keys weighs 0 (its sums are 0); one whose scores were all NaN keeps its NaN
+            const float g = __builtin_amdgcn_exp2f(sm[w][cc] - ref);
+            den += g * sl[w][cc];
+            num += *(const f32x4 *)&so[w][cc][d] * g;
+        }
+        if (gridDim.x == 1) {
+            num *= kv8_inverse(den);
+            const size_t at = (size_t)(t.r0 + cg / G) * ldo + (size_t)(head * G + cg % G) * D + d;
+            if constexpr (BF) *(uint2 *)((uint16_t *)out + at) = pack4(num);
+            else *(f32x4 *)((float *)out + at) = num;
+        } else {
+            float *p = part + ((((size_t)e * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * KV8_COLS + cc) * LD;
+            *(f32x4 *)(p + 4 + d) = num;
+            if (d == 0) { p[0] = mx; p[1] = den; }
+        }
+    }
+}
+
+// the splits' partials of k_kv8_few merged: D / 4 threads a column
+template <int D, bool BF>
+__global__ __launch_bounds__(NTH) void k_kv8_merge(qm_kv8_t c, void *__restrict__ out, size_t ldo,
+                                                   const int *__restrict__ row, const int *__restrict__ pos, int rows,
+                                                   int max_rows, int G, const float *__restrict__ part, int nsplit,
+                                                   int tiles) {
+    constexpr int TPC = D / 4, LD = D + 4;
+    const int e = blockIdx.z, head = blockIdx.y;
+    kv8_entry t;
+    if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
+    const int col = blockIdx.x * (NTH / TPC) + threadIdx.x / TPC, d = threadIdx.x % TPC * 4;
+    if (col >= t.cnt * G) return;
+    const int y = col / KV8_COLS * c.heads + head;
+    const float *p = part + (((size_t)e * (tiles * c.heads) + y) * nsplit * KV8_COLS + col % KV8_COLS) * LD;
+    float mx = -INFINITY;
+    for (int s = 0; s < nsplit; s++) mx = fmaxf(mx, p[(size_t)s * KV8_COLS * LD]);
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    float den = 0.0f;
+    f32x4 num = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < nsplit; s++) {
+        const float *ps = p + (size_t)s * KV8_COLS * LD;
+        const float g = __builtin_amdgcn_exp2f(ps[0] - ref);
+        den += g * ps[1];
+        num += *(const f32x4 *)(ps + 4 + d) * g;
+    }
+    num *= kv8_inverse(den);
+    const size_t at = (size_t)(t.r0 + col / G) * ldo + (size_t)(head * G + col % G) * D + d;
+    if constexpr (BF) *(uint2 *)((uint16_t *)out + at) = pack4(num);
+    else *(f32x4 *)((float *)out + at) = num;
+}
+
+// ---- many columns: a prompt's rows ------------------------------------------
+// Block b: kv head b % heads (each XCD serves a head's pages from its own L2
+// where there are eight), the column tiles with the longest contexts first.
+// Four waves of 32 columns share each step's 64 keys in LDS, converted to bf16
+// once and laid out as the MFMAs' operands (16 bytes a lane, conflict-free);
+// the next step's codes are in flight while this one is computed.
+#define KV8_MANY 128                   // columns of a block
+template <int FMT, int D, bool BF>
+__global__ __launch_bounds__(NTH, 2) void k_kv8_many(qm_kv8_t c, void *__restrict__ out, const void *__restrict__ q,
+                                                    size_t ldo, size_t ldq, const int *__restrict__ row,
+                                                    const int *__restrict__ pos, int rows, int max_rows, int G, float f) {
+    constexpr int NP = BF ? 1 : 3, KS = D / 32, DT = D / 16, CT = 2;
+    constexpr int UN = 64 * D / 16 / NTH;                 // 16-code units of K, and of V, a thread stages
+    const int e = blockIdx.y, head = blockIdx.x % c.heads;
+    kv8_entry t;
+    if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
+    const int ncol = t.cnt * G, tiles = (ncol + KV8_MANY - 1) / KV8_MANY;
+    const int tile = tiles - 1 - (int)(blockIdx.x / c.heads);
+    if (tile < 0) return;
+    const int col0 = tile * KV8_MANY;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int cl = lane & 15, h = lane >> 4;
+    const int B = c.block, lb = __builtin_ctz(B);
+    const int end = t.pos + t.cnt, full = end >> lb << lb;
+    const int kend = t.pos + min(t.cnt - 1, (col0 + KV8_MANY - 1) / G) + 1;
+    const int ns = (kend + 63) >> 6;
+
+    __shared__ __align__(16) bf16x8 lk[2][4 * KS * 64], lv[2][2 * DT * 64];
+
+    // the wave's columns
+    const int w0 = col0 + wave * 16 * CT;
+    int last[CT];
+    bf16x8 qf[CT][KS][NP];
+#pragma unroll
+    for (int n = 0; n < CT; n++) {
+        const int col = w0 + 16 * n + cl;
+        const bool in = col < ncol;
+        const int qr = in ? col / G : 0, qg = in ? col % G : 0;
+        last[n] = in ? t.pos + qr : -1;
+#pragma unroll
+        for (int j = 0; j < KS; j++)
+            kv8_load_q<BF, NP>(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + 32 * j + 8 * h, in, qf[n][j]);
+    }
+    const int wfirst = w0 < ncol ? t.pos + w0 / G : -1;                    // keys all the wave's columns see, and any
+    const int wlast = w0 < ncol ? t.pos + min(t.cnt - 1, (w0 + 16 * CT - 1) / G) : -1;
+    const bool whole = w0 + 16 * CT <= ncol;
+
+    const int *table = c.table + (size_t)e * c.max_blocks;
+    auto page_of = [&](int key) {
+        int p = -1;
+        if (key < full) p = table[key >> lb];
+        return (unsigned)p < (unsigned)c.n_page ? p : -1;
+    };
+    // unit u of a step: K 16 dims of key u / (D / 16); V 16 keys of a dim, in
+    // the order they lie in their pages
+    const int sub = B / 16, lsub = lb - 4;
+    auto v_group = [&](int u) { return (u >> lsub) / D * sub + (u & (sub - 1)); };
+    auto v_dim = [&](int u) { return (u >> lsub) & (D - 1); };
+    uint4 ku[UN], vu[UN];
+    auto load = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < UN; i++) {
+            const int u = tid + NTH * i, key = 64 * s + u / (D / 16);
+            const int p = page_of(key);
+            ku[i] = p >= 0 ? *(const uint4 *)(c.k + (((size_t)p * c.heads + head) * B + (key & (B - 1))) * D + u % (D / 16) * 16)
+                           : uint4{};
+            const int kv = 64 * s + 16 * v_group(u), pv = page_of(kv);
+            vu[i] = pv >= 0 ? *(const uint4 *)(c.v + (((size_t)pv * c.heads + head) * D + v_dim(u)) * B + (kv & (B - 1)))
+                            : uint4{};
+        }
+    };
+    auto put_k = [&](int b, int u, bf16x8 x, bf16x8 y) {
+        const int key = u / (D / 16), ds = u % (D / 16);
+        const int at = ((((key >> 2) & 3) * KS + (ds >> 1)) * 64) + (ds & 1) * 32 + ((key >> 4) << 2 | (key & 3));
+        lk[b][at] = x;
+        lk[b][at + 16] = y;
+    };
+    auto put_v = [&](int b, int u, bf16x8 x, bf16x8 y) {
+        const int d = v_dim(u), at = (d >> 4) * 64 + v_group(u) * 16 + (d & 15);
+        lv[b][at] = x;
+        lv[b][DT * 64 + at] = y;
+    };
+    auto put = [&](int b, int s) {
+#pragma unroll
+        for (int i = 0; i < UN; i++) {
+            const int u = tid + NTH * i;
+            put_k(b, u, kv8_bf16<FMT>(ku[i].x, ku[i].y), kv8_bf16<FMT>(ku[i].z, ku[i].w));
+            put_v(b, u, kv8_bf16<FMT>(vu[i].x, vu[i].y), kv8_bf16<FMT>(vu[i].z, vu[i].w));
+        }
+        if (64 * s + 64 <= full) return;
+        // the step reaches into the unfinished block: its groups come from the tail
+        const __bf16 *kt = (const __bf16 *)c.k_tail + ((size_t)e * c.heads + head) * ((size_t)B * D);
+        const __bf16 *vt = (const __bf16 *)c.v_tail + ((size_t)e * c.heads + head) * ((size_t)B * D);
+        for (int i = 0; i < UN; i++) {
+            const int u = tid + NTH * i, key = 64 * s + u / (D / 16), ds = u % (D / 16);
+            if (key >= full && key < end) {
+                const bf16x8 *p = (const bf16x8 *)(kt + (size_t)(key - full) * D + ds * 16);
+                put_k(b, u, p[0], p[1]);
+            }
+            const int kv = 64 * s + 16 * v_group(u);
+            if (kv >= full && kv < end) {
+                const bf16x8 *p = (const bf16x8 *)(vt + (size_t)v_dim(u) * B + (kv - full));
+                bf16x8 x = p[0], y = p[1];
+#pragma unroll
+                for (int n = 0; n < 8; n++) {             // behind the last row: anything
+                    x[n] = kv + n < end ? x[n] : (__bf16)0.0f;
+                    y[n] = kv + 8 + n < end ? y[n] : (__bf16)0.0f;
+                }
+                put_v(b, u, x, y);
+            }
+        }
+    };
+    float ksn = 0.0f, vsn = 0.0f;                          // the next step's scales of this lane's 16 keys
+    int okn = 0;
+    auto scales = [&](int s) {
+        const int key = 64 * s + 16 * h, p = page_of(key);
+        okn = p >= 0 || (key >= full && key < end);
+        ksn = p >= 0 ? c.k_scale[(size_t)p * c.heads + head] * f : f;
+        vsn = p >= 0 ? c.v_scale[(size_t)p * c.heads + head] : 1.0f;
+    };
+
+    float m[CT], l[CT];
+    f32x4 o[DT][CT];
+#pragma unroll
+    for (int n = 0; n < CT; n++) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DT; i++) o[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    load(0);
+    scales(0);
+    for (int s = 0; s < ns; s++) {
+        const int b = s & 1;
+        put(b, s);
+        const float ks = ksn, vs = vsn;
+        const int ok = okn;
+        __syncthreads();                                  // this buffer is full; the other one's readers are done
+        if (s + 1 < ns) {
+            load(s + 1);
+            scales(s + 1);
+        }
+        if (64 * s > wlast) continue;                     // uniform per wave: nothing of it is seen
+        f32x4 s4[CT][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            f32x4 a[CT];
+#pragma unroll
+            for (int n = 0; n < CT; n++) a[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < KS; j++) {
+                const bf16x8 kf = lk[b][(i * KS + j) * 64 + lane];
+#pragma unroll
+                for (int n = 0; n < CT; n++)
+#pragma unroll
+                    for (int x = 0; x < NP; x++) a[n] = kv8_mma(kf, qf[n][j][x], a[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < CT; n++) s4[n][i] = a[n] * ks;
+        }
+        const bool clear = whole && 64 * s + 63 <= wfirst && __all(ok);
+        if (!clear) {
+#pragma unroll
+            for (int n = 0; n < CT; n++) {
+                const int lim = ok ? last[n] - (64 * s + 16 * h) : -1;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s4[n][i][r] = 4 * i + r <= lim ? s4[n][i][r] : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < CT; n++) {
+            const float rs = kv8_softmax(s4[n], m[n], l[n]);
+#pragma unroll
+            for (int i = 0; i < DT; i++) o[i][n] *= rs;
+        }
+#pragma unroll
+        for (int s2 = 0; s2 < 2; s2++) {
+            bf16x8 pf[CT][NP];
+#pragma unroll
+            for (int n = 0; n < CT; n++) {
+                const f32x4 x = s4[n][2 * s2] * vs, y = s4[n][2 * s2 + 1] * vs;
+                kv8_pieces<NP>(f32x8{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w}, pf[n]);
+            }
+#pragma unroll
+            for (int i = 0; i < DT; i++) {
+                const bf16x8 vf = lv[b][(s2 * DT + i) * 64 + lane];
+#pragma unroll
+                for (int n = 0; n < CT; n++)
+#pragma unroll
+                    for (int x = 0; x < NP; x++) o[i][n] = kv8_mma(vf, pf[n][x], o[i][n]);
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < CT; n++) {
+        const int col = w0 + 16 * n + cl;
+        const float inv = kv8_inverse(col_sum(l[n]));
+        if (col >= ncol) continue;
+        const size_t at = (size_t)(t.r0 + col / G) * ldo + (size_t)(head * G + col % G) * D + 4 * h;
+#pragma unroll
+        for (int i = 0; i < DT; i++) {
+            const f32x4 x = o[i][n] * inv;
+            if constexpr (BF) *(uint2 *)((uint16_t *)out + at + 16 * i) = pack4(x);
+            else *(f32x4 *)((float *)out + at + 16 * i) = x;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// launchers
+// ---------------------------------------------------------------------------
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+static int kv8_sizes(const qm_kv8_t *c) {
+    if (c->format != QM_KV8_E4M3 && c->format != QM_KV8_INT8) return QH_EINVAL;
+    if (c->head_dim != 64 && c->head_dim != 128) return QH_EINVAL;
+    if (c->block != 16 && c->block != 32 && c->block != 64) return QH_EINVAL;
+    if (c->heads < 1 || c->heads > QM_KV8_MAX_HEADS || c->n_page < 1 || c->n_seq < 1 || c->max_blocks < 1) return QH_EINVAL;
+    return (long)c->max_blocks * c->block > QM_KV8_MAX_CTX ? QH_ETOOBIG : QH_OK;
+}
+static int kv8_check(const qm_kv8_t *c) {
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || !c->k_tail || !c->v_tail || !c->table) return QH_EINVAL;
+    const int rc = kv8_sizes(c);
+    if (rc) return rc;
+    if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->k_tail) || !aligned16(c->v_tail)) return QH_EINVAL;
+    return QH_OK;
+}
+// rows of `cols` values at stride ld, loaded 16 bytes at a time
+static bool kv8_rows_ok(const void *p, size_t ld, int cols, int bf16) {
+    return p && aligned16(p) && ld >= (size_t)cols && ld % (bf16 ? 8 : 4) == 0;
+}
+static int kv8_call_check(const qm_kv8_t *c, const int *row, const int *pos, int n, int rows, int max_rows) {
+    if (n < 0 || n > c->n_seq || n > QM_KV8_MAX_SEQS || !pos || rows < 0 || max_rows < 1) return QH_EINVAL;
+    if (!row && (rows != n || max_rows != 1)) return QH_EINVAL;
+    if ((long)max_rows > (long)c->max_blocks * c->block) return QH_EINVAL;
+    return QH_OK;
+}
+
+#define KV8_SWITCH(CALL)                                                        \
+    do {                                                                        \
+        if (c->format == QM_KV8_E4M3) {                                         \
+            if (c->head_dim == 128) { if (bf16) CALL(QM_KV8_E4M3, 128, true); else CALL(QM_KV8_E4M3, 128, false); } \
+            else { if (bf16) CALL(QM_KV8_E4M3, 64, true); else CALL(QM_KV8_E4M3, 64, false); }                      \
+        } else {                                                                \
+            if (c->head_dim == 128) { if (bf16) CALL(QM_KV8_INT8, 128, true); else CALL(QM_KV8_INT8, 128, false); } \
+            else { if (bf16) CALL(QM_KV8_INT8, 64, true); else CALL(QM_KV8_INT8, 64, false); }                      \
+        }                                                                       \
+    } while (0)
+
+extern "C" size_t qm_kv8_bytes(const qm_kv8_t *c) {
+    if (!c || kv8_sizes(c)) return 0;
+    const size_t values = 2 * (size_t)c->heads * c->block * c->head_dim;       // K and V of a block
+    return c->n_page * (values + 2 * (size_t)c->heads * sizeof(float)) +
+           c->n_seq * (2 * values + (size_t)c->max_blocks * sizeof(int));
+}
+
+extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, size_t ldk, size_t ldv, int bf16,
+                             const int *row, const int *pos, int n, int rows, int max_rows) {
+    int rc = kv8_check(c);
+    if (!rc) rc = kv8_call_check(c, row, pos, n, rows, max_rows);
+    if (rc) return rc;
+    if (n == 0 || rows == 0) return QH_OK;
+    if (!kv8_rows_ok(k, ldk, c->heads * c->head_dim, bf16) || !kv8_rows_ok(v, ldv, c->heads * c->head_dim, bf16))
+        return QH_EINVAL;
+    // blocks that max_rows rows touch at most, wherever they start
+    const dim3 grid(c->heads, n, (max_rows + c->block - 2) / c->block + 1);
+    if (grid.z > 65535) return QH_ETOOBIG;
+    if (!stream()) return QH_ESTATE;
+#define APPEND_B(F, D_, B_, BF_) \
+    hipLaunchKernelGGL((k_kv8_append<F, D_, B_, BF_>), grid, dim3(NTH), 0, stream(), *c, k, v, ldk, ldv, row, pos, rows, max_rows)
+#define APPEND(F, D_, BF_)                                  \
+    do {                                                    \
+        if (c->block == 16) APPEND_B(F, D_, 16, BF_);       \
+        else if (c->block == 32) APPEND_B(F, D_, 32, BF_);  \
+        else APPEND_B(F, D_, 64, BF_);                      \
+    } while (0)
+    KV8_SWITCH(APPEND);
+#undef APPEND
+#undef APPEND_B
+    return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
+}
+
+// Key splits of k_kv8_few: enough blocks for the CUs, at least a step for each
+// wave of a split.
+#define KV8_MAX_SPLITS 32
+#define KV8_FEW_COLS 64                // columns up to which the keys are split instead
+static int kv8_splits(const qm_kv8_t *c, int n, int tiles, int max_ctx) {
+    const long blocks = (long)n * c->heads * tiles;
+    const int steps = (max_ctx + 63) / 64 + 1;
+    int s = 1;
+    while (2 * s <= KV8_MAX_SPLITS && blocks * s < 512 && 2 * s * KV8_NW <= steps) s *= 2;
+    return s;
+}
+
+extern "C" size_t qm_kv8_attention_work(const qm_kv8_t *c, int q_heads, int n, int max_rows, int max_ctx) {
+    if (!c || c->heads < 1 || q_heads < c->heads || n < 1 || max_rows < 1) return 0;
+    const long cols = (long)max_rows * (q_heads / c->heads);
+    if (cols > KV8_FEW_COLS) return 0;
+    const int tiles = (int)((cols + KV8_COLS - 1) / KV8_COLS), s = kv8_splits(c, n, tiles, max_ctx);
+    return s == 1 ? 0 : (size_t)n * c->heads * tiles * s * KV8_COLS * (c->head_dim + 4) * sizeof(float);
+}
+
+extern "C" int qm_kv8_attention(const qm_kv8_t *c, void *out, const void *q, size_t ldo, size_t ldq, int bf16, int q_heads,
+                                const int *row, const int *pos, int n, int rows, int max_rows, int max_ctx, float scale,
+                                void *work, size_t work_bytes) {
+    int rc = kv8_check(c);
+    if (!rc) rc = kv8_call_check(c, row, pos, n, rows, max_rows);
+    if (rc) return rc;
+    if (q_heads < 1 || q_heads % c->heads || q_heads / c->heads > QM_KV8_MAX_GROUP) return QH_EINVAL;
+    if (max_ctx < 1 || max_ctx > c->max_blocks * c->block || !(fabsf(scale) < INFINITY)) return QH_EINVAL;
+    if (n == 0 || rows == 0) return QH_OK;
+    if (!kv8_rows_ok(q, ldq, q_heads * c->head_dim, bf16) || !kv8_rows_ok(out, ldo, q_heads * c->head_dim, bf16))
+        return QH_EINVAL;
+    const int G = q_heads / c->heads;
+    const long cols = (long)max_rows * G;
+    const float f = scale * 1.44269504088896340736f;     // the softmax runs on powers of two
+    if (cols > KV8_FEW_COLS) {
+        const long tiles = (cols + KV8_MANY - 1) / KV8_MANY;
+        if (tiles * c->heads * NTH >= 1L << 32) return QH_ETOOBIG;
+        if (!stream()) return QH_ESTATE;
+        const dim3 grid((unsigned)(tiles * c->heads), n);
+#define MANY(F, D_, BF_)                                                                                             \
+    hipLaunchKernelGGL((k_kv8_many<F, D_, BF_>), grid, dim3(NTH), 0, stream(), *c, out, q, ldo, ldq, row, pos, rows, \
+                       max_rows, G, f)
+        KV8_SWITCH(MANY);
+#undef MANY
+        return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
+    }
+    const int tiles = (int)((cols + KV8_COLS - 1) / KV8_COLS), ns = kv8_splits(c, n, tiles, max_ctx);
+    if (ns > 1 && (!work || !aligned16(work))) return QH_EINVAL;
+    if (work_bytes < qm_kv8_attention_work(c, q_heads, n, max_rows, max_ctx)) return QH_ETOOBIG;
+    if (!stream()) return QH_ESTATE;
+    const dim3 grid(ns, c->heads * tiles, n);
+#define FEW(F, D_, BF_)                                                                                             \
+    hipLaunchKernelGGL((k_kv8_few<F, D_, BF_>), grid, dim3(WAVE *KV8_NW), 0, stream(), *c, out, q, ldo, ldq, row, pos, \
+                       rows, max_rows, G, f, (float *)work)
+    KV8_SWITCH(FEW);
+#undef FEW
+    if (hipGetLastError() != hipSuccess) return QH_ELAUNCH;
+    if (ns > 1) {
+        const int per = NTH / (c->head_dim / 4);
+        const dim3 mg((unsigned)((cols + per - 1) / per), c->heads, n);
+#define MERGE(D_, BF_)                                                                                               \
+    hipLaunchKernelGGL((k_kv8_merge<D_, BF_>), mg, dim3(NTH), 0, stream(), *c, out, ldo, row, pos, rows, max_rows, G, \
+                       (const float *)work, ns, tiles)
+        if (c->head_dim == 128) { if (bf16) MERGE(128, true); else MERGE(128, false); }
+        else { if (bf16) MERGE(64, true); else MERGE(64, false); }
+#undef MERGE
+    }
+    return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
+}

@@ -108,6 +108,39 @@ int qm_decode_layers_persist(const uint16_t *const *w, int layers, const uint16_
                              const float *rsin, int max_seq, float eps, float *x_out, float *dn_out);
 int qm_persist_errors(unsigned *flags);
 
+/* ---- 8-bit KV cache (kv8_kernels.h) and beam search (beam_kernels.h) -------
+ * One layer's cache; device pointers.  What the fields hold, and what the
+ * calls do: include/qwen3_hip_serve.h */
+#define QM_KV8_E4M3 0
+#define QM_KV8_INT8 1
+#define QM_KV8_MAX_HEADS 256
+#define QM_KV8_MAX_GROUP 64          /* query heads of a kv head */
+#define QM_KV8_MAX_CTX (1 << 20)     /* positions of a sequence */
+#define QM_KV8_MAX_SEQS 65535
+typedef struct {
+    int format, heads, head_dim, block, n_page, n_seq, max_blocks;
+    uint8_t *k, *v;
+    float *k_scale, *v_scale;
+    uint16_t *k_tail, *v_tail;
+    const int *table;
+} qm_kv8_t;
+size_t qm_kv8_bytes(const qm_kv8_t *c);
+int qm_kv8_append(const qm_kv8_t *c, const void *k_d, const void *v_d, size_t ldk, size_t ldv, int bf16,
+                  const int *row_d, const int *pos_d, int n, int rows, int max_rows);
+size_t qm_kv8_attention_work(const qm_kv8_t *c, int q_heads, int n, int max_rows, int max_ctx);
+int qm_kv8_attention(const qm_kv8_t *c, void *out_d, const void *q_d, size_t ldo, size_t ldq, int bf16, int q_heads,
+                     const int *row_d, const int *pos_d, int n, int rows, int max_rows, int max_ctx, float scale,
+                     void *work_d, size_t work_bytes);
+
+#define QM_BEAM_MAX_WIDTH 16
+#define QM_BEAM_MAX_PIECES 1024      /* of 2,048 logits each */
+size_t qm_beam_select_work(int vocab, int n_group, int width);
+int qm_beam_select(const float *logits_d, size_t ld, int vocab, int n_group, int width, const float *score_d,
+                   const int *done_d, int end0, int end1, float *score_out_d, int *done_out_d, int *token_out_d,
+                   int *parent_out_d, void *work_d, size_t work_bytes);
+int qm_beam_reorder(void *dst_d, const void *src_d, const int *parent_d, int n_group, int width, int slabs,
+                    size_t slab_stride, size_t seq_stride, int runs, size_t run_stride, size_t run_bytes);
+
 /* tok[0 .. n) = the host's tokens (n <= QM_MAX_CHUNK) and *pos = pos0, both
  * passed as kernel arguments: the caller's buffer is read before the return */
 int qm_set_tokens(int *tok_d, const int *tokens, int n, int *pos_d, int pos0);

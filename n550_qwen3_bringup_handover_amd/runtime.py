@@ -1,5 +1,6 @@
-"""Loader for libqwen3_hip.so — the MI355X GEMM plug-in and device-resident
-forward (C ABI in include/qwen3_hip.h and include/qwen3_hip_model.h).
+"""Loader for libqwen3_hip.so — the MI355X GEMM plug-in, device-resident
+forward and serving operators (C ABI in include/qwen3_hip.h,
+include/qwen3_hip_model.h and include/qwen3_hip_serve.h).
 
 The library is built in-tree (`build()`, or `make -C <pkg>/csrc`) and loaded
 from this directory only.  There is no CPU fallback: if the library is
@@ -14,7 +15,8 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libqwen3_hip.so")
 HEADER = os.path.join(os.path.dirname(PKG_DIR), "include", "qwen3_hip.h")
 MODEL_HEADER = os.path.join(os.path.dirname(PKG_DIR), "include", "qwen3_hip_model.h")
-HEADERS = (HEADER, MODEL_HEADER)
+SERVE_HEADER = os.path.join(os.path.dirname(PKG_DIR), "include", "qwen3_hip_serve.h")
+HEADERS = (HEADER, MODEL_HEADER, SERVE_HEADER)
 
 F32P = ctypes.POINTER(ctypes.c_float)
 U16P = ctypes.POINTER(ctypes.c_uint16)
@@ -22,6 +24,15 @@ I32P = ctypes.POINTER(ctypes.c_int)
 VP = ctypes.c_void_p
 
 _lib = None
+
+
+class Kv8(ctypes.Structure):
+    """qwen3_hip_kv8 (include/qwen3_hip_serve.h): one layer's 8-bit KV cache"""
+    _fields_ = ([(n, ctypes.c_int) for n in ("format", "kv_heads", "head_dim", "block", "n_page", "n_seq", "max_blocks")]
+                + [(n, VP) for n in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail", "table")])
+
+
+KV8P = ctypes.POINTER(Kv8)
 
 
 class Qwen3HipError(RuntimeError):
@@ -108,6 +119,19 @@ _PROTOS = {
     "qwen3_hip_batch_logits": (ctypes.c_int, [VP, F32P]),
     "qwen3_hip_batch_set_graph": (ctypes.c_int, [VP, ctypes.c_int]),
     "qwen3_hip_batch_timing": (ctypes.c_int, [VP, ctypes.POINTER(ctypes.c_double)]),
+    # include/qwen3_hip_serve.h
+    "qwen3_hip_kv8_bytes": (ctypes.c_size_t, [KV8P]),
+    "qwen3_hip_kv8_append_dev": (ctypes.c_int, [KV8P, VP, VP, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_int, VP, VP,
+                                                ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "qwen3_hip_kv8_attention_work": (ctypes.c_size_t, [KV8P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "qwen3_hip_kv8_attention_dev": (ctypes.c_int, [KV8P, VP, VP, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_int,
+                                                   ctypes.c_int, VP, VP, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                   ctypes.c_int, ctypes.c_float, VP, ctypes.c_size_t]),
+    "qwen3_hip_beam_select_work": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "qwen3_hip_beam_select_dev": (ctypes.c_int, [VP, ctypes.c_size_t, ctypes.c_int, ctypes.c_int, ctypes.c_int, VP, VP,
+                                                 ctypes.c_int, ctypes.c_int, VP, VP, VP, VP, VP, ctypes.c_size_t]),
+    "qwen3_hip_beam_reorder_dev": (ctypes.c_int, [VP, VP, VP, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_size_t,
+                                                  ctypes.c_size_t, ctypes.c_int, ctypes.c_size_t, ctypes.c_size_t]),
 }
 
 # qwen3_hip_dump_fn
@@ -115,7 +139,7 @@ DUMP_FN = ctypes.CFUNCTYPE(None, VP, ctypes.c_int, ctypes.c_char_p, F32P, ctypes
 
 
 def header_symbols():
-    """Function names declared in include/qwen3_hip.h and qwen3_hip_model.h."""
+    """Function names declared in the public headers."""
     import re
     names = set()
     for h in HEADERS:

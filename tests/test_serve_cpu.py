@@ -1,0 +1,138 @@
+"""The serving operators' argument checks, on a machine without a GPU: every refusal is made before anything is
+launched, so the addresses below are never used.  Accepted calls end at the missing stream."""
+import ctypes
+
+import pytest
+
+from n550_qwen3_bringup_handover_amd import abi, runtime
+
+VP, SZ = ctypes.c_void_p, ctypes.c_size_t
+EINVAL, ESTATE, ETOOBIG = 1, 7, 8
+A = 1 << 20                       # a 16-byte aligned address
+
+pytestmark = pytest.mark.skipif(runtime.gpu_visible(), reason="accepted calls would launch")
+
+
+class Shim(ctypes.Structure):     # qm_kv8_t has qwen3_hip_kv8's fields in its order
+    _fields_ = runtime.Kv8._fields_
+
+
+def cache(**kw):
+    d = dict(format=0, kv_heads=8, head_dim=128, block=32, n_page=64, n_seq=4, max_blocks=16, k=A, v=A, k_scale=A, v_scale=A,
+             k_tail=A, v_tail=A, table=A)
+    d.update(kw)
+    return Shim(*[d[n] for n, _ in Shim._fields_])
+
+
+def append(c=None, k=A, v=A, ldk=1024, ldv=1024, bf16=0, row=A, pos=A, n=4, rows=9, most=3):
+    f = runtime.lib().qm_kv8_append
+    return f(ctypes.byref(c or cache()), VP(k), VP(v), SZ(ldk), SZ(ldv), bf16, VP(row), VP(pos), n, rows, most)
+
+
+def attend(c=None, out=A, q=A, ldo=2048, ldq=2048, bf16=0, heads=16, row=A, pos=A, n=4, rows=9, most=3, ctx=512, scale=0.1,
+           work=A, bytes=1 << 30):
+    f = runtime.lib().qm_kv8_attention
+    return f(ctypes.byref(c or cache()), VP(out), VP(q), SZ(ldo), SZ(ldq), bf16, heads, VP(row), VP(pos), n, rows, most, ctx,
+             ctypes.c_float(scale), VP(work), SZ(bytes))
+
+
+BAD_CACHES = [dict(format=2), dict(format=-1), dict(kv_heads=0), dict(kv_heads=257), dict(head_dim=96), dict(block=8),
+              dict(block=128), dict(n_page=0), dict(n_seq=0), dict(max_blocks=0), dict(k=None), dict(v=A + 8),
+              dict(k_scale=None), dict(v_tail=A + 2), dict(k_tail=None), dict(table=None)]
+
+
+@pytest.mark.parametrize("bad", BAD_CACHES)
+def test_caches_that_are_refused(bad):
+    assert append(cache(**bad)) == EINVAL
+    assert attend(cache(**bad)) == EINVAL
+
+
+def test_caches_at_their_limits():
+    assert append(cache(max_blocks=(1 << 20) // 32)) == ESTATE
+    assert append(cache(max_blocks=(1 << 20) // 32 + 1)) == ETOOBIG
+    assert append(cache(max_blocks=1 << 30)) == ETOOBIG
+    assert append(cache(kv_heads=256), ldk=256 * 128, ldv=256 * 128) == ESTATE
+
+
+@pytest.mark.parametrize("bad", [dict(k=None), dict(v=A + 4), dict(ldk=1023), dict(ldv=1026), dict(pos=None), dict(n=5),
+                                 dict(n=-1), dict(rows=-1), dict(most=0), dict(most=513), dict(row=None),
+                                 dict(ldk=1028, bf16=1)])
+def test_appends_that_are_refused(bad):
+    assert append() == ESTATE
+    assert append(**bad) == EINVAL
+
+
+def test_nothing_to_do():
+    assert append(n=0) == 0 and append(rows=0, k=None, v=None) == 0
+    assert attend(n=0) == 0 and attend(rows=0, q=None, out=None) == 0
+
+
+@pytest.mark.parametrize("bad", [dict(out=None), dict(q=A + 4), dict(ldo=2047), dict(ldq=2044 + 2), dict(heads=12), dict(heads=0),
+                                 dict(heads=8 * 65, ldo=1 << 17, ldq=1 << 17), dict(n=5), dict(row=None), dict(ctx=0),
+                                 dict(ctx=513), dict(scale=float("nan")), dict(scale=float("inf")), dict(work=None),
+                                 dict(work=A + 4), dict(most=513), dict(pos=None)])
+def test_attentions_that_are_refused(bad):
+    assert attend() == ESTATE
+    assert attend(**bad) == EINVAL
+
+
+def test_attention_needs_its_workspace():
+    c = cache()
+    need = runtime.lib().qwen3_hip_kv8_attention_work(ctypes.cast(ctypes.byref(c), runtime.KV8P), 16, 4, 3, 512)
+    assert need > 0
+    assert attend(c, bytes=need) == ESTATE
+    assert attend(c, bytes=need - 1) == ETOOBIG
+    # a prompt's launch needs none
+    assert runtime.lib().qwen3_hip_kv8_attention_work(ctypes.cast(ctypes.byref(c), runtime.KV8P), 16, 4, 200, 512) == 0
+    assert attend(c, rows=800, most=200, work=None, bytes=0) == ESTATE
+
+
+def test_bytes_of_a_cache():
+    c = abi.kv8_cache("e4m3", 8, 128, 32, 64, 4, 16, *[None] * 7)
+    assert abi.kv8_bytes(c) == 64 * 8 * (2 * 32 * 128 + 8) + 4 * (8 * 2 * 2 * 32 * 128 + 16 * 4)
+    c.block = 48
+    assert abi.kv8_bytes(c) == 0
+
+
+def select(x=A, ld=1000, vocab=1000, groups=2, width=4, score=A, done=A, e0=1, e1=-1, so=A, do=A, tok=A, par=A, work=A,
+           bytes=1 << 30):
+    f = runtime.lib().qm_beam_select
+    return f(VP(x), SZ(ld), vocab, groups, width, VP(score), VP(done), e0, e1, VP(so), VP(do), VP(tok), VP(par), VP(work), SZ(bytes))
+
+
+@pytest.mark.parametrize("bad", [dict(x=None), dict(ld=999), dict(vocab=3), dict(groups=-1), dict(width=0), dict(width=17),
+                                 dict(score=None), dict(e0=1000), dict(e1=1000), dict(e0=-1), dict(so=None), dict(do=None),
+                                 dict(tok=None), dict(par=None), dict(work=None), dict(work=A + 4)])
+def test_choices_that_are_refused(bad):
+    assert select() == ESTATE
+    assert select(**bad) == EINVAL
+
+
+def test_choices_at_their_limits():
+    assert select(groups=0, x=None) == 0
+    assert select(done=None, e0=-1) == ESTATE
+    assert select(vocab=1 << 21, ld=1 << 21) == ESTATE
+    assert select(vocab=(1 << 21) + 1, ld=1 << 22) == ETOOBIG
+    need = runtime.lib().qwen3_hip_beam_select_work(1000, 2, 4)
+    assert select(bytes=need) == ESTATE and select(bytes=need - 1) == ETOOBIG
+    assert runtime.lib().qwen3_hip_beam_select_work(1000, 2, 17) == 0
+
+
+def reorder(dst=A, src=A, parent=A, groups=2, width=4, slabs=3, slab=1 << 16, seq=4096, runs=2, run=1024, used=512):
+    f = runtime.lib().qm_beam_reorder
+    return f(VP(dst), VP(src), VP(parent), groups, width, slabs, SZ(slab), SZ(seq), runs, SZ(run), SZ(used))
+
+
+@pytest.mark.parametrize("bad", [dict(dst=None), dict(src=None), dict(parent=None), dict(groups=-1), dict(width=0), dict(width=17),
+                                 dict(slabs=-1), dict(runs=-1), dict(used=510), dict(seq=4098), dict(run=500), dict(seq=1020),
+                                 dict(slab=16384), dict(src=A + 16), dict(src=A + 2), dict(src=A + (2 << 16))])
+def test_reorders_that_are_refused(bad):
+    assert reorder() == ESTATE and reorder(src=A + (3 << 16)) == ESTATE
+    assert reorder(**bad) == EINVAL
+
+
+def test_reorders_at_their_limits():
+    assert reorder(groups=0, src=None) == 0 and reorder(slabs=0) == 0 and reorder(runs=0) == 0 and reorder(used=0) == 0
+    assert reorder(width=1) == 0                      # in place, one beam: nothing moves
+    assert reorder(groups=65536, slab=1 << 40) == ETOOBIG
+    assert reorder(runs=1, used=1 << 36, seq=1 << 36, slab=1 << 40) == ETOOBIG

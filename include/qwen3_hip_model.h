@@ -175,6 +175,15 @@ typedef struct qwen3_hip_batch qwen3_hip_batch;
  * qwen3_hip_model_max_seq(model). */
 int qwen3_hip_batch_open(qwen3_hip_batch **batch, qwen3_hip_model *model, int n_seq, int max_ctx);
 
+/* The same with the KV caches in 8 bits (format: QWEN3_HIP_KV8_E4M3 or _INT8
+ * of qwen3_hip_serve.h, which says what a cache of blocks of 32 tokens holds):
+ * 57,568 bytes per position, rounded up to blocks, and 3.7 MB per sequence for
+ * the unfinished blocks, instead of 229,376 per position.  Every call below
+ * takes either kind.  Attention, a prompt's included, reads K and V as the
+ * cache holds them, so logits differ from an fp32 batch's by the codes'
+ * roundings. */
+int qwen3_hip_batch_open_kv8(qwen3_hip_batch **batch, qwen3_hip_model *model, int n_seq, int max_ctx, int format);
+
 void qwen3_hip_batch_close(qwen3_hip_batch *batch);
 
 /* Prefill sequence seq (0 .. n_seq-1) with n_prompt tokens (1 .. max_ctx-1)
@@ -192,6 +201,20 @@ int qwen3_hip_batch_prefill(qwen3_hip_batch *batch, int seq, const int *prompt, 
  * does not stop a sequence (callers cut at it). */
 int qwen3_hip_batch_decode(qwen3_hip_batch *batch, int n_decode, int *out);
 
+/* Beam search of n_seq / width groups at once (width 1 .. 16, a divisor of
+ * n_seq): group g searches behind its own prompt, n_prompt[g] tokens, the
+ * prompts one after another in `prompts`.  n_tokens steps choose, from the
+ * logits of the prompt and then of each step, the `width` continuations with
+ * the largest sums of log-probabilities (qwen3_hip_beam_select_dev); the
+ * beams' caches follow their parents, 8-bit ones by sharing finished blocks.
+ * With stop_at_eos a beam that has produced an EOS is finished: it keeps its
+ * score and is padded with EOS (151645).  out[(g * width + k) * n_tokens + i]:
+ * token i of group g's k-th best beam; scores[g * width + k] its sum.
+ * n_prompt[g] + n_tokens - 1 <= max_ctx.  The sequences are empty afterwards:
+ * prefill them before a decode. */
+int qwen3_hip_batch_beam(qwen3_hip_batch *batch, int width, const int *prompts, const int *n_prompt, int n_tokens,
+                         int stop_at_eos, int *out, float *scores);
+
 /* Logits of the last decode step, n_seq x vocab floats (synchronous copy). */
 int qwen3_hip_batch_logits(qwen3_hip_batch *batch, float *out);
 
@@ -200,7 +223,8 @@ int qwen3_hip_batch_logits(qwen3_hip_batch *batch, float *out);
  * launches (0); both compute the same thing. */
 int qwen3_hip_batch_set_graph(qwen3_hip_batch *batch, int on);
 
-/* Wall-clock ms of the last qwen3_hip_batch_decode call. */
+/* Wall-clock ms of the last qwen3_hip_batch_decode call, or of the steps of the
+ * last qwen3_hip_batch_beam call. */
 int qwen3_hip_batch_timing(const qwen3_hip_batch *batch, double *decode_ms);
 
 #ifdef __cplusplus

@@ -274,8 +274,44 @@ __global__ __launch_bounds__(NTH) void k_beam_reorder(uint8_t *dst, const uint8_
 }
 
 // ---------------------------------------------------------------------------
+// A search's bookkeeping.  Start: the first beam of each group alone is in use.
+// Step: the choice goes to row `step` of the history {token, parent}[n], and
+// positions advance by adv.
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(NTH) void k_beam_start(float *score, int *done, int n, int W) {
+    const int i = blockIdx.x * NTH + threadIdx.x;
+    if (i < n) {
+        score[i] = i % W ? -INFINITY : 0.0f;
+        done[i] = 0;
+    }
+}
+__global__ __launch_bounds__(NTH) void k_beam_record(int *hist, const int *token, const int *parent, int *pos, int n, int step,
+                                                    int adv) {
+    const int i = blockIdx.x * NTH + threadIdx.x;
+    if (i < n) {
+        hist[((size_t)step * n + i) * 2] = token[i];
+        hist[((size_t)step * n + i) * 2 + 1] = parent[i];
+        pos[i] += adv;
+    }
+}
+
+// ---------------------------------------------------------------------------
 // launchers
 // ---------------------------------------------------------------------------
+extern "C" int qm_beam_start(float *score, int *done, int n, int width) {
+    if (!score || !done || n <= 0 || width <= 0) return QH_EINVAL;
+    if (!stream()) return QH_ESTATE;
+    hipLaunchKernelGGL(k_beam_start, dim3((n + NTH - 1) / NTH), dim3(NTH), 0, stream(), score, done, n, width);
+    return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
+}
+extern "C" int qm_beam_record(int *hist, const int *token, const int *parent, int *pos, int n, int step, int adv) {
+    if (!hist || !token || !parent || !pos || n <= 0 || step < 0) return QH_EINVAL;
+    if (!stream()) return QH_ESTATE;
+    hipLaunchKernelGGL(k_beam_record, dim3((n + NTH - 1) / NTH), dim3(NTH), 0, stream(), hist, token, parent, pos, n, step,
+                       adv);
+    return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
+}
+
 extern "C" size_t qm_beam_select_work(int vocab, int n_group, int width) {
     if (vocab < 1 || n_group < 1 || width < 1 || width > BEAM_MAX) return 0;
     const size_t lists = (size_t)n_group * width * beam_pieces(vocab);

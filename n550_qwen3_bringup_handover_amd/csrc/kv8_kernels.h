@@ -38,6 +38,45 @@ __device__ __forceinline__ bool kv8_get(kv8_entry &t, const qm_kv8_t &c, const i
 }
 
 // ---------------------------------------------------------------------------
+// The model's q and k rows before they meet the cache: QK-norm and RoPE
+// (qwen3.c:298-305, ops_scalar.c:21-35) of row i at position pos[i] (each) or
+// *pos + i.  k in place; q in place or, where qb is set, as bf16 [nt][2048].
+// grid = (nt, 6): wave w of block (i, b) takes head 4 b + w of q's 16 and k's 8.
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(NTH) void k_qk_rope(float *__restrict__ qkv, uint16_t *__restrict__ qb,
+                                                const uint16_t *__restrict__ qn, const uint16_t *__restrict__ kn,
+                                                const float *__restrict__ rcos, const float *__restrict__ rsin,
+                                                const int *__restrict__ pos_d, int each, int max_seq, float eps) {
+    constexpr int QH = NKV * GRP;
+    const int i = blockIdx.x, lane = threadIdx.x & 63, hd = blockIdx.y * 4 + (threadIdx.x >> 6);
+    const int pos = each ? pos_d[i] : *pos_d + i;
+    if (pos < 0 || pos >= max_seq) return;
+    float *x = qkv + (size_t)i * QKV_LD + hd * HD;           // k's heads lie behind q's
+    const uint16_t *w = hd < QH ? qn : kn;
+    const float x0 = x[lane], x1 = x[lane + 64];
+    const float c = rcos[(size_t)pos * (HD / 2) + lane], sn = rsin[(size_t)pos * (HD / 2) + lane];
+    const float sc = 1.0f / sqrtf(wave_sum(sumsq2(x0, x1)) / (float)HD + eps);
+    float o0, o1;
+    rope_pair((x0 * sc) * bf16f(w[lane]), (x1 * sc) * bf16f(w[lane + 64]), c, sn, o0, o1);
+    if (qb && hd < QH) {
+        __bf16 *o = (__bf16 *)qb + (size_t)i * (QH * HD) + hd * HD;
+        o[lane] = (__bf16)o0;
+        o[lane + 64] = (__bf16)o1;
+    } else {
+        x[lane] = o0;
+        x[lane + 64] = o1;
+    }
+}
+
+// blocks of sequence s that are not finished (from pos[s] / block on; all where
+// pos is NULL) get its own pages, s * max_blocks + block index
+__global__ __launch_bounds__(NTH) void k_kv8_own(int *__restrict__ table, const int *__restrict__ pos, int block,
+                                                int max_blocks) {
+    const int s = blockIdx.y, b = blockIdx.x * NTH + threadIdx.x;
+    if (b < max_blocks && (!pos || b >= pos[s] / block)) table[(size_t)s * max_blocks + b] = s * max_blocks + b;
+}
+
+// ---------------------------------------------------------------------------
 // store
 // ---------------------------------------------------------------------------
 // a row's value as the cache holds it: bf16, finite
@@ -737,6 +776,23 @@ extern "C" size_t qm_kv8_bytes(const qm_kv8_t *c) {
     const size_t values = 2 * (size_t)c->heads * c->block * c->head_dim;       // K and V of a block
     return c->n_page * (values + 2 * (size_t)c->heads * sizeof(float)) +
            c->n_seq * (2 * values + (size_t)c->max_blocks * sizeof(int));
+}
+
+extern "C" int qm_qk_rope(float *qkv, uint16_t *qb, const uint16_t *qn, const uint16_t *kn, const float *rcos,
+                          const float *rsin, const int *pos, int each, int nt, int max_seq, float eps) {
+    if (!qkv || !qn || !kn || !rcos || !rsin || !pos || nt <= 0 || max_seq <= 0) return QH_EINVAL;
+    if (!stream()) return QH_ESTATE;
+    hipLaunchKernelGGL(k_qk_rope, dim3(nt, (NKV * GRP + NKV) / 4), dim3(NTH), 0, stream(), qkv, qb, qn, kn, rcos, rsin, pos,
+                       each, max_seq, eps);
+    return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
+}
+
+extern "C" int qm_kv8_own(int *table, const int *pos, int n_seq, int block, int max_blocks) {
+    if (!table || n_seq <= 0 || n_seq > 65535 || block <= 0 || max_blocks <= 0) return QH_EINVAL;
+    if (!stream()) return QH_ESTATE;
+    hipLaunchKernelGGL(k_kv8_own, dim3((max_blocks + NTH - 1) / NTH, n_seq), dim3(NTH), 0, stream(), table, pos, block,
+                       max_blocks);
+    return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
 }
 
 extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, size_t ldk, size_t ldv, int bf16,

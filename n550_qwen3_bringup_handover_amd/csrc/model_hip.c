@@ -336,17 +336,81 @@ static size_t kv_layer_floats(const qwen3_hip_model *m) {
     return (size_t)QW3M_N_KV_HEADS * m->max_seq * QW3M_HEAD_DIM;
 }
 
+/* a batch's 8-bit caches: layer 0's, and what to add for the next layer's */
+#define KV8_BLOCK 32
+typedef struct {
+    qm_kv8_t c;
+    size_t codes, scales, tails;       /* per layer: bytes of K, floats, bf16 values */
+    int *row;                          /* [2]: a prompt pass's row offsets 0, nt */
+    void *work;
+    size_t work_bytes;
+} kv8_t;
+
+static qm_kv8_t kv8_layer(const kv8_t *k, int l) {
+    qm_kv8_t c = k->c;
+    c.k += l * k->codes;
+    c.v += l * k->codes;
+    c.k_scale += l * k->scales;
+    c.v_scale += l * k->scales;
+    c.k_tail += l * k->tails;
+    c.v_tail += l * k->tails;
+    return c;
+}
+/* the cache of sequence seq alone */
+static kv8_t kv8_seq(const kv8_t *k, int seq) {
+    kv8_t s = *k;
+    const size_t tail = (size_t)k->c.heads * k->c.block * k->c.head_dim;
+    s.c.table += (size_t)seq * k->c.max_blocks;
+    s.c.k_tail += seq * tail;
+    s.c.v_tail += seq * tail;
+    s.c.n_seq = 1;
+    return s;
+}
+
 /* where a chunk's K/V go: layer l's cache of one sequence starts at
- * kc + l * layer_stride (layout in hip_model.hip, max_seq positions) */
+ * kc + l * layer_stride (layout in hip_model.hip, max_seq positions), or the
+ * 8-bit cache kv8 of that sequence */
 typedef struct {
     float *kc, *vc;
     size_t layer_stride;
     int max_seq;
+    const kv8_t *kv8;
 } kv_t;
 
 static kv_t model_kv(qwen3_hip_model *m) {
-    const kv_t kv = {m->kc, m->vc, kv_layer_floats(m), m->max_seq};
+    const kv_t kv = {m->kc, m->vc, kv_layer_floats(m), m->max_seq, NULL};
     return kv;
+}
+
+/* 1 / sqrt(head_dim), the constant of qwen3.c:311 */
+#define ATT_SCALE 0.08838834764831845f
+
+/* attention of nt rows of m->qkv over an 8-bit cache: q and k are normalised
+ * and rotated, k and v stored, then read back through the cache.  n sequences
+ * of one row (pos[i]), or one sequence's nt rows at *pos ... */
+static int attend_kv8(qwen3_hip_model *m, const kv8_t *k, int l, const layer_t *L, int n, int nt, const int *pos,
+                      int ctx, int bf16) {
+    const qm_kv8_t c = kv8_layer(k, l);
+    const int each = n == nt;          /* a row of each sequence */
+    /* bf16 rows: the output takes the first half of the buffer, q the second */
+    uint16_t *qb = bf16 ? (uint16_t *)m->att + (size_t)nt * QW3M_Q_DIM : NULL;
+    int rc = qm_qk_rope(m->qkv, qb, L->qn, L->kn, m->rcos, m->rsin, pos, each, nt, m->max_seq, QW3M_RMS_EPS);
+    if (!rc) rc = qm_kv8_append(&c, m->qkv + QW3M_Q_DIM, m->qkv + QW3M_Q_DIM + QW3M_KV_DIM, QKV_N, QKV_N, 0,
+                                each ? NULL : k->row, pos, n, nt, each ? 1 : nt);
+    if (!rc) rc = qm_kv8_attention(&c, m->att, bf16 ? (const void *)qb : m->qkv, QW3M_Q_DIM, bf16 ? QW3M_Q_DIM : QKV_N,
+                                   bf16, QW3M_N_HEADS, each ? NULL : k->row, pos, n, nt, each ? 1 : nt, ctx,
+                                   ATT_SCALE, k->work, k->work_bytes);
+    return rc;
+}
+
+/* attention of a chunk of nt tokens at pos0, the cache's entries written */
+static int attend_chunk(qwen3_hip_model *m, const kv_t *kv, int l, const layer_t *L, int nt, int pos0, int bf16) {
+    if (kv->kv8) return attend_kv8(m, kv->kv8, l, L, 1, nt, m->state + 1, pos0 + nt, bf16);
+    float *kc = kv->kc + l * kv->layer_stride, *vc = kv->vc + l * kv->layer_stride;
+    return bf16 ? qm_attention_bf16(m->qkv, (uint16_t *)m->att, m->cpart, kc, vc, L->qn, L->kn, m->rcos, m->rsin,
+                                    m->state + 1, nt, kv->max_seq, pos0 + nt, QW3M_RMS_EPS)
+                : qm_attention(m->qkv, m->att, m->cpart, kc, vc, L->qn, L->kn, m->rcos, m->rsin, m->state + 1, nt,
+                               kv->max_seq, pos0 + nt, QW3M_RMS_EPS);
 }
 
 /* the layers of a chunk of more than BF16_ROWS tokens with the inputs of all
@@ -367,9 +431,7 @@ static int run_layers_bf16(qwen3_hip_model *m, const kv_t *kv, int nt, int pos0)
         rc = qm_rows_norm_bf16(m->x, l == 0 || dks ? NULL : m->dn, l == 0 ? m->embed : NULL, m->tok_in, V, L->in_norm,
                                xb, nt, H, eps, dpart, dks);
         if (!rc) rc = qh_gemm_bf16a(m->qkv, xb, L->wqkv, nt, H, QKV_N);
-        if (!rc) rc = qm_attention_bf16(m->qkv, att, m->cpart, kv->kc + l * kv->layer_stride,
-                                        kv->vc + l * kv->layer_stride, L->qn, L->kn, m->rcos, m->rsin, m->state + 1,
-                                        nt, kv->max_seq, pos0 + nt, eps);
+        if (!rc) rc = attend_chunk(m, kv, l, L, nt, pos0, 1);
         if (!rc) rc = qh_gemm_split_bf16a(m->ob, att, L->wo, nt, QW3M_Q_DIM, H, &opart, &oks);
         if (!rc) rc = qm_rows_norm_bf16(m->x, oks ? NULL : m->ob, NULL, NULL, 0, L->post_norm, xb, nt, H, eps, opart,
                                         oks);
@@ -413,9 +475,7 @@ static int run_chunk(qwen3_hip_model *m, const kv_t *kv, int nt, int pos0, int w
         DUMP(l, "q_proj_out", m->qkv, QKV_N, 0, QW3M_Q_DIM);
         DUMP(l, "k_proj_out", m->qkv, QKV_N, QW3M_Q_DIM, QW3M_KV_DIM);
         DUMP(l, "v_proj_out", m->qkv, QKV_N, QW3M_Q_DIM + QW3M_KV_DIM, QW3M_KV_DIM);
-        if (!rc) rc = qm_attention(m->qkv, m->att, m->cpart, kv->kc + l * kv->layer_stride,
-                                   kv->vc + l * kv->layer_stride, L->qn, L->kn, m->rcos, m->rsin,
-                                   m->state + 1, nt, kv->max_seq, pos0 + nt, eps);
+        if (!rc) rc = attend_chunk(m, kv, l, L, nt, pos0, 0);
         DUMP(l, "attn_out", m->att, QW3M_Q_DIM, 0, QW3M_Q_DIM);
         if (!rc) rc = dumping ? qh_gemm(m->ob, m->att, L->wo, nt, QW3M_Q_DIM, H)
                               : qh_gemm_split(m->ob, m->att, L->wo, nt, QW3M_Q_DIM, H, &opart, &oks);
@@ -533,6 +593,7 @@ static int prefill(qwen3_hip_model *m, const kv_t *kv, const int *prompt, int n,
     for (int p0 = 0; p0 < n && !rc; p0 += each) {
         *last = n - p0 < each ? n - p0 : each;
         rc = load_chunk(m, prompt + p0, *last, p0);
+        if (!rc && kv->kv8) rc = qm_set_i32(kv->kv8->row + 1, *last);
         if (!rc) rc = run_chunk(m, kv, *last, p0, p0 + *last == n);
     }
     return rc;
@@ -646,7 +707,9 @@ struct qwen3_hip_batch {
     qwen3_hip_model *m;
     int n_seq, max_ctx, out_ld;
     size_t kv_seq;                     /* floats of one sequence's cache in one layer */
-    float *kc, *vc;                    /* [NL][n_seq][kv_seq] */
+    float *kc, *vc;                    /* [NL][n_seq][kv_seq]; NULL with 8-bit caches */
+    kv8_t kv8;                         /* c.k NULL with fp32 caches */
+    int *table;                        /* kv8.c.table */
     float *logits;                     /* [n_seq][V] of the last decode step */
     float *part;                       /* [n_seq][QM_BATCH_PART_FLOATS] */
     int *tok, *pos, *plen;             /* [n_seq]: next token fed, its position, prompt length */
@@ -655,19 +718,31 @@ struct qwen3_hip_batch {
     int *h_plen;                       /* host: prompt length of each sequence */
     int *h_out;                        /* host staging of out */
     int use_graph;
-    int graph_id;
+    int graph_id[2];                   /* the greedy step and the beams' forward, -1 until captured */
     int have_logits;
     double t_decode_ms;
+    /* beam search, allocated by the first: per sequence score, finished, parent;
+     * {token, parent} of every step; the choice's workspace */
+    float *score;
+    int *done, *parent, *hist;
+    void *swork;
+    size_t swork_bytes;
     qwen3_hip_batch *next;             /* the model's list of open batches */
 };
 
-/* A batch's graph holds the model's device addresses: when the model closes
- * first, its batches lose the graph and the model, and later calls on them
+/* A batch's graphs hold the model's device addresses: when the model closes
+ * first, its batches lose the graphs and the model, and later calls on them
  * return QWEN3_HIP_ESTATE instead of touching freed memory. */
+static void drop_graphs(qwen3_hip_batch *b) {
+    for (int g = 0; g < 2; g++) {
+        if (b->graph_id[g] >= 0) (void)qh_graph_destroy(b->graph_id[g]);
+        b->graph_id[g] = -1;
+    }
+}
+
 static void detach_batches(qwen3_hip_model *m) {
     for (qwen3_hip_batch *b = m->batches; b; b = b->next) {
-        if (b->graph_id >= 0) (void)qh_graph_destroy(b->graph_id);
-        b->graph_id = -1;
+        drop_graphs(b);
         b->m = NULL;
     }
     m->batches = NULL;
@@ -681,8 +756,9 @@ void qwen3_hip_batch_close(qwen3_hip_batch *b) {
         while (*pp && *pp != b) pp = &(*pp)->next;
         if (*pp) *pp = b->next;
     }
-    if (b->graph_id >= 0) (void)qh_graph_destroy(b->graph_id);
-    void *bufs[] = {b->kc, b->vc, b->logits, b->part, b->tok, b->pos, b->plen, b->out};
+    drop_graphs(b);
+    void *bufs[] = {b->kc, b->vc, b->logits, b->part, b->tok, b->pos, b->plen, b->out, b->kv8.c.k, b->kv8.c.k_scale,
+                    b->kv8.c.k_tail, b->table, b->kv8.row, b->kv8.work, b->score, b->done, b->parent, b->hist, b->swork};
     for (size_t i = 0; i < sizeof bufs / sizeof bufs[0]; i++) (void)qh_free(bufs[i]);
     free(b->h_next);
     free(b->h_plen);
@@ -690,7 +766,49 @@ void qwen3_hip_batch_close(qwen3_hip_batch *b) {
     free(b);
 }
 
-int qwen3_hip_batch_open(qwen3_hip_batch **out, qwen3_hip_model *m, int n_seq, int max_ctx) {
+/* the 8-bit caches of a batch: pages s * max_blocks .. of sequence s, its
+ * tails one allocation [K, V][layer][sequence] so that beams reorder them in
+ * one call.  Blocks of 32 tokens: 131 KB of tail per sequence and layer and a
+ * scale for 4,096 values; 16 halves the one and doubles the scales, 64 the
+ * other way, with no other cost in the kernels. */
+static int open_kv8(qwen3_hip_batch *b, int format) {
+    qm_kv8_t *c = &b->kv8.c;
+    c->format = format;
+    c->heads = QW3M_N_KV_HEADS;
+    c->head_dim = QW3M_HEAD_DIM;
+    c->block = KV8_BLOCK;
+    c->n_seq = b->n_seq;
+    c->max_blocks = (b->max_ctx + KV8_BLOCK - 1) / KV8_BLOCK;
+    c->n_page = b->n_seq * c->max_blocks;
+    const size_t unit = (size_t)c->heads * c->block * c->head_dim;      /* values of a block */
+    b->kv8.codes = c->n_page * unit;
+    b->kv8.scales = (size_t)c->n_page * c->heads;
+    b->kv8.tails = b->n_seq * unit;
+    int rc = qh_malloc((void **)&c->k, 2 * NL * b->kv8.codes);
+    if (!rc) rc = qh_malloc((void **)&c->k_scale, 2 * NL * b->kv8.scales * sizeof(float));
+    if (!rc) rc = qh_malloc((void **)&c->k_tail, 2 * NL * b->kv8.tails * sizeof(uint16_t));
+    if (!rc) rc = qh_malloc((void **)&b->table, (size_t)c->n_page * sizeof(int));
+    if (!rc) rc = qh_malloc((void **)&b->kv8.row, 2 * sizeof(int));
+    if (rc) return rc;
+    c->v = c->k + NL * b->kv8.codes;
+    c->v_scale = c->k_scale + NL * b->kv8.scales;
+    c->v_tail = c->k_tail + NL * b->kv8.tails;
+    c->table = b->table;
+    /* of a step of every sequence, and of the short passes of a prompt that
+     * split the keys */
+    b->kv8.work_bytes = qm_kv8_attention_work(c, QW3M_N_HEADS, b->n_seq, 1, b->max_ctx);
+    for (int rows = 1; rows <= QM_MAX_CHUNK; rows++) {
+        const size_t w = qm_kv8_attention_work(c, QW3M_N_HEADS, 1, rows, b->max_ctx);
+        if (w > b->kv8.work_bytes) b->kv8.work_bytes = w;
+    }
+    rc = qh_malloc(&b->kv8.work, b->kv8.work_bytes);
+    if (!rc) rc = qm_zero_i32(b->kv8.row, 2);
+    if (!rc) rc = qm_kv8_own(b->table, NULL, b->n_seq, c->block, c->max_blocks);
+    return rc;
+}
+
+/* format: QM_KV8_*, or -1 for fp32 caches */
+static int batch_open(qwen3_hip_batch **out, qwen3_hip_model *m, int n_seq, int max_ctx, int format) {
     if (!out) return QWEN3_HIP_EINVAL;
     *out = NULL;
     if (!m || n_seq < 1 || n_seq > QM_MAX_CHUNK || max_ctx < 2 || max_ctx > m->max_seq) return QWEN3_HIP_EINVAL;
@@ -702,7 +820,7 @@ int qwen3_hip_batch_open(qwen3_hip_batch **out, qwen3_hip_model *m, int n_seq, i
     b->out_ld = max_ctx + 1;
     b->kv_seq = (size_t)QW3M_N_KV_HEADS * max_ctx * QW3M_HEAD_DIM;
     b->use_graph = 1;
-    b->graph_id = -1;
+    b->graph_id[0] = b->graph_id[1] = -1;
     int rc = QWEN3_HIP_ENOMEM;
     b->h_next = (int *)malloc((size_t)n_seq * sizeof(int));
     b->h_plen = (int *)calloc((size_t)n_seq, sizeof(int));
@@ -713,11 +831,15 @@ int qwen3_hip_batch_open(qwen3_hip_batch **out, qwen3_hip_model *m, int n_seq, i
     do {                                                                  \
         if ((rc = qh_malloc((void **)&(ptr), (bytes))) != 0) goto fail;   \
     } while (0)
-    const size_t kv_bytes = (size_t)NL * n_seq * b->kv_seq * sizeof(float);
-    DEV(b->kc, kv_bytes);
-    DEV(b->vc, kv_bytes);
+    if (format >= 0) {
+        if ((rc = open_kv8(b, format)) != 0) goto fail;
+    } else {
+        const size_t kv_bytes = (size_t)NL * n_seq * b->kv_seq * sizeof(float);
+        DEV(b->kc, kv_bytes);
+        DEV(b->vc, kv_bytes);
+        DEV(b->part, (size_t)n_seq * QM_BATCH_PART_FLOATS * sizeof(float));
+    }
     DEV(b->logits, (size_t)n_seq * V * sizeof(float));
-    DEV(b->part, (size_t)n_seq * QM_BATCH_PART_FLOATS * sizeof(float));
     DEV(b->tok, (size_t)n_seq * sizeof(int));
     DEV(b->pos, (size_t)n_seq * sizeof(int));
     DEV(b->plen, (size_t)n_seq * sizeof(int));
@@ -737,11 +859,34 @@ fail:
     return rc;
 }
 
+int qwen3_hip_batch_open(qwen3_hip_batch **out, qwen3_hip_model *m, int n_seq, int max_ctx) {
+    return batch_open(out, m, n_seq, max_ctx, -1);
+}
+
+int qwen3_hip_batch_open_kv8(qwen3_hip_batch **out, qwen3_hip_model *m, int n_seq, int max_ctx, int format) {
+    if (out) *out = NULL;
+    if (format != QM_KV8_E4M3 && format != QM_KV8_INT8) return QWEN3_HIP_EINVAL;
+    return batch_open(out, m, n_seq, max_ctx, format);
+}
+
 int qwen3_hip_batch_set_graph(qwen3_hip_batch *b, int on) {
     if (!b) return QWEN3_HIP_EINVAL;
     if (!b->m) return QWEN3_HIP_ESTATE;
     b->use_graph = on ? 1 : 0;
     return QWEN3_HIP_OK;
+}
+
+/* a prompt into sequence seq's cache; its last row's logits in the model's
+ * buffer */
+static int batch_prompt(qwen3_hip_batch *b, int seq, const int *prompt, int n_prompt) {
+    const int has8 = b->kv8.c.k != NULL;
+    kv8_t k8 = b->kv8;
+    if (has8) k8 = kv8_seq(&b->kv8, seq);
+    const kv_t kv = {has8 ? NULL : b->kc + (size_t)seq * b->kv_seq, has8 ? NULL : b->vc + (size_t)seq * b->kv_seq,
+                     (size_t)b->n_seq * b->kv_seq, b->max_ctx, has8 ? &k8 : NULL};
+    b->m->have_logits = 0;             /* the model's logits buffer is reused */
+    int nt = 0;
+    return prefill(b->m, &kv, prompt, n_prompt, &nt);
 }
 
 int qwen3_hip_batch_prefill(qwen3_hip_batch *b, int seq, const int *prompt, int n_prompt) {
@@ -751,12 +896,8 @@ int qwen3_hip_batch_prefill(qwen3_hip_batch *b, int seq, const int *prompt, int 
     int rc = check_tokens(prompt, n_prompt);
     if (rc) return rc;
     qwen3_hip_model *m = b->m;
-    const kv_t kv = {b->kc + (size_t)seq * b->kv_seq, b->vc + (size_t)seq * b->kv_seq,
-                     (size_t)b->n_seq * b->kv_seq, b->max_ctx};
     b->h_next[seq] = -1;
-    m->have_logits = 0;             /* the model's logits buffer is reused below */
-    int nt = 0;
-    rc = prefill(m, &kv, prompt, n_prompt, &nt);
+    rc = batch_prompt(b, seq, prompt, n_prompt);
     /* first token: out[seq][0] at pos - plen + 1 = 0, then pos = n_prompt */
     if (!rc) rc = qm_set_i32(b->pos + seq, n_prompt - 1);
     if (!rc) rc = qm_set_i32(b->plen + seq, n_prompt);
@@ -770,12 +911,13 @@ int qwen3_hip_batch_prefill(qwen3_hip_batch *b, int seq, const int *prompt, int 
     return rc;
 }
 
-/* one decode step of every sequence: token tok[s] at position pos[s].  When
+/* the logits of one decode step of every sequence: token tok[s] at position
+ * pos[s], K and V appended.  When
  * the o and down projections split K (the skinny kernel up to 16 sequences,
  * the ring tiles above 64 and, for down, from 17), their
  * slice sums are added by the residual + RMSNorm kernel that consumes them
  * (the sums a reduction launch would form), one launch fewer each. */
-static int batch_step(qwen3_hip_batch *b) {
+static int batch_forward(qwen3_hip_batch *b) {
     qwen3_hip_model *m = b->m;
     const int n = b->n_seq;
     const float eps = QW3M_RMS_EPS;
@@ -788,9 +930,10 @@ static int batch_step(qwen3_hip_batch *b) {
         if (l == 0) rc = qm_rows_norm(m->x, NULL, m->embed, b->tok, V, L->in_norm, m->xb, n, H, eps);
         else rc = qm_rows_norm_split(m->x, dks ? NULL : m->dn, NULL, NULL, 0, L->in_norm, m->xb, n, H, eps, dpart, dks);
         if (!rc) rc = qh_gemm(m->qkv, m->xb, L->wqkv, n, H, QKV_N);
-        if (!rc) rc = qm_attention_decode_batch(m->qkv, m->att, b->part, b->kc + l * lstride, b->vc + l * lstride,
-                                                b->kv_seq, L->qn, L->kn, m->rcos, m->rsin, b->pos, n,
-                                                b->max_ctx, eps);
+        if (!rc && b->kv8.c.k) rc = attend_kv8(m, &b->kv8, l, L, n, n, b->pos, b->max_ctx, 0);
+        else if (!rc) rc = qm_attention_decode_batch(m->qkv, m->att, b->part, b->kc + l * lstride, b->vc + l * lstride,
+                                                     b->kv_seq, L->qn, L->kn, m->rcos, m->rsin, b->pos, n,
+                                                     b->max_ctx, eps);
         if (!rc) rc = qh_gemm_split(m->ob, m->att, L->wo, n, QW3M_Q_DIM, H, &opart, &oks);
         if (!rc) rc = qm_rows_norm_split(m->x, oks ? NULL : m->ob, NULL, NULL, 0, L->post_norm, m->xb, n, H, eps,
                                          opart, oks);
@@ -800,8 +943,37 @@ static int batch_step(qwen3_hip_batch *b) {
     if (!rc) rc = qm_rows_norm_split(m->x, dks ? NULL : m->dn, NULL, NULL, 0, m->final_norm, m->xb, n, H, eps,
                                      dpart, dks);
     if (!rc) rc = qh_gemm(b->logits, m->xb, m->embed, n, H, V);
-    if (!rc) rc = qm_argmax_rows(b->logits, V, n, b->tok, b->pos, b->plen, b->out, b->out_ld);
     return rc;
+}
+
+/* the forward and the greedy choice of every sequence's next token (0), or the
+ * forward alone (1) */
+static int batch_step(qwen3_hip_batch *b, int which) {
+    int rc = batch_forward(b);
+    if (!rc && which == 0) rc = qm_argmax_rows(b->logits, V, b->n_seq, b->tok, b->pos, b->plen, b->out, b->out_ld);
+    return rc;
+}
+
+/* step i of a call: with graphs on, a first step runs eagerly (any workspace
+ * its GEMM plans need is allocated then, outside capture); later steps replay
+ * the one captured step */
+static int batch_run(qwen3_hip_batch *b, int i, int which) {
+    int *id = &b->graph_id[which];
+    if (!b->use_graph || (*id < 0 && i == 0)) return batch_step(b, which);
+    if (*id < 0) {
+        int rc = qh_capture_begin();
+        if (rc) return rc;
+        const int rc2 = batch_step(b, which);
+        int gid = -1;
+        rc = qh_capture_end(&gid);
+        if (!rc) rc = rc2;
+        if (rc) {
+            if (gid >= 0) (void)qh_graph_destroy(gid);
+            return rc;
+        }
+        *id = gid;
+    }
+    return qh_graph_launch(*id);
 }
 
 int qwen3_hip_batch_decode(qwen3_hip_batch *b, int n_decode, int *out) {
@@ -811,29 +983,7 @@ int qwen3_hip_batch_decode(qwen3_hip_batch *b, int n_decode, int *out) {
         if (b->h_next[s] < 0 || (long)b->h_next[s] + n_decode > b->max_ctx) return QWEN3_HIP_EINVAL;
     int rc = QWEN3_HIP_OK;
     const double t0 = now_ms();
-    for (int i = 0; i < n_decode && !rc; i++) {
-        /* with graphs on, a first step runs eagerly (any workspace its GEMM
-           plans need is allocated then, outside capture); later steps replay
-           the one captured step */
-        if (!b->use_graph || (b->graph_id < 0 && i == 0)) {
-            rc = batch_step(b);
-            continue;
-        }
-        if (b->graph_id < 0) {
-            rc = qh_capture_begin();
-            if (rc) break;
-            const int rc2 = batch_step(b);
-            int gid = -1;
-            rc = qh_capture_end(&gid);
-            if (!rc) rc = rc2;
-            if (rc) {
-                if (gid >= 0) (void)qh_graph_destroy(gid);
-                break;
-            }
-            b->graph_id = gid;
-        }
-        rc = qh_graph_launch(b->graph_id);
-    }
+    for (int i = 0; i < n_decode && !rc; i++) rc = batch_run(b, i, 0);
     if (!rc) rc = qh_sync();
     b->t_decode_ms = now_ms() - t0;
     if (rc) return rc;
@@ -848,6 +998,111 @@ int qwen3_hip_batch_decode(qwen3_hip_batch *b, int n_decode, int *out) {
         b->h_next[s] += n_decode;
     }
     return QWEN3_HIP_OK;
+}
+
+/* ---- beam search ------------------------------------------------------------ */
+
+static int beam_buffers(qwen3_hip_batch *b, int width) {
+    const size_t n = (size_t)b->n_seq;
+    const size_t need = qm_beam_select_work(V, b->n_seq / width, width);
+    int rc = QWEN3_HIP_OK;
+    if (!b->score) rc = qh_malloc((void **)&b->score, n * sizeof(float));
+    if (!rc && !b->done) rc = qh_malloc((void **)&b->done, n * sizeof(int));
+    if (!rc && !b->parent) rc = qh_malloc((void **)&b->parent, n * sizeof(int));
+    if (!rc && !b->hist) rc = qh_malloc((void **)&b->hist, 2 * n * b->max_ctx * sizeof(int));
+    if (!rc && need > b->swork_bytes) {
+        rc = qh_sync();
+        if (!rc) rc = qh_free(b->swork);
+        b->swork = NULL;
+        b->swork_bytes = 0;
+        if (!rc) rc = qh_malloc(&b->swork, need);
+        if (!rc) b->swork_bytes = need;
+    }
+    return rc;
+}
+
+/* every sequence's state after its parent's, `rows` positions of the longest:
+ * fp32 caches move; of 8-bit ones the tables and the unfinished blocks do,
+ * finished blocks are shared, and a sequence's next ones are its own again */
+static int beam_states(qwen3_hip_batch *b, int width, int rows) {
+    const int n = b->n_seq, g = n / width;
+    if (b->kv8.c.k) {
+        const qm_kv8_t *c = &b->kv8.c;
+        const size_t tail = (size_t)c->heads * c->block * c->head_dim * sizeof(uint16_t);
+        const size_t line = (size_t)c->max_blocks * sizeof(int);
+        int rc = qm_beam_reorder(c->k_tail, c->k_tail, b->parent, g, width, 2 * NL, n * tail, tail, 1, tail, tail);
+        if (!rc) rc = qm_beam_reorder(b->table, b->table, b->parent, g, width, 1, n * line, line, 1, line, line);
+        if (!rc) rc = qm_kv8_own(b->table, b->pos, n, c->block, c->max_blocks);
+        return rc;
+    }
+    const size_t seq = b->kv_seq * sizeof(float), ctx = (size_t)b->max_ctx;
+    int rc = qm_beam_reorder(b->kc, b->kc, b->parent, g, width, NL, n * seq, seq, QW3M_KV_DIM / 4, ctx * 16,
+                             (size_t)rows * 16);
+    if (!rc) rc = qm_beam_reorder(b->vc, b->vc, b->parent, g, width, NL, n * seq, seq, QW3M_N_KV_HEADS,
+                                  ctx * QW3M_HEAD_DIM * 4, (size_t)rows * QW3M_HEAD_DIM * 4);
+    return rc;
+}
+
+int qwen3_hip_batch_beam(qwen3_hip_batch *b, int width, const int *prompts, const int *n_prompt, int n_tokens,
+                         int stop_at_eos, int *out, float *scores) {
+    if (!b || !prompts || !n_prompt || !out || !scores || n_tokens < 1) return QWEN3_HIP_EINVAL;
+    if (!b->m) return QWEN3_HIP_ESTATE;
+    if (width < 1 || width > QM_BEAM_MAX_WIDTH || b->n_seq % width) return QWEN3_HIP_EINVAL;
+    const int n = b->n_seq, groups = n / width;
+    int longest = 0, rc = QWEN3_HIP_OK;
+    size_t total = 0;
+    for (int g = 0; g < groups; g++) {
+        if (n_prompt[g] < 1 || n_prompt[g] >= b->max_ctx || (long)n_prompt[g] + n_tokens - 1 > b->max_ctx)
+            return QWEN3_HIP_EINVAL;
+        if (n_prompt[g] > longest) longest = n_prompt[g];
+        if ((rc = check_tokens(prompts + total, n_prompt[g])) != 0) return rc;
+        total += (size_t)n_prompt[g];
+    }
+    if (qh_capturing()) return QWEN3_HIP_ERUNTIME;   /* prompts come from the host */
+    if ((rc = beam_buffers(b, width)) != 0) return rc;
+    int *hist = (int *)malloc((size_t)n_tokens * n * 2 * sizeof(int));
+    if (!hist) return QWEN3_HIP_ENOMEM;
+
+    const double t0 = now_ms();
+    double t1 = t0;
+    for (int s = 0; s < n; s++) b->h_next[s] = -1;   /* whatever happens, the sequences are the search's now */
+    b->have_logits = 0;
+    const int *p = prompts;
+    for (int g = 0; g < groups && !rc; p += n_prompt[g++]) {
+        rc = batch_prompt(b, g * width, p, n_prompt[g]);
+        if (!rc) rc = qh_d2d(b->logits + (size_t)g * width * V, b->m->logits, (size_t)V * sizeof(float));
+        for (int w = 0; w < width && !rc; w++) rc = qm_set_i32(b->pos + g * width + w, n_prompt[g]);
+    }
+    if (!rc) rc = qm_beam_start(b->score, b->done, n, width);
+    if (!rc) rc = qh_sync();
+    t1 = now_ms();
+    for (int t = 0; t < n_tokens && !rc; t++) {
+        rc = qm_beam_select(b->logits, V, V, groups, width, b->score, stop_at_eos ? b->done : NULL,
+                            stop_at_eos ? QW3M_EOS0 : -1, stop_at_eos ? QW3M_EOS1 : -1, b->score, b->done, b->tok, b->parent,
+                            b->swork, b->swork_bytes);
+        if (!rc) rc = qm_beam_record(b->hist, b->tok, b->parent, b->pos, n, t, t > 0);
+        if (rc || t + 1 == n_tokens) break;
+        rc = beam_states(b, width, longest + t);
+        if (!rc) rc = batch_run(b, t, 1);
+    }
+    if (!rc) rc = qh_sync();
+    else (void)qh_sync();              /* steps already launched */
+    b->t_decode_ms = now_ms() - t1;
+    if (b->kv8.c.k) {                  /* every sequence has its own pages again */
+        const int rc2 = qm_kv8_own(b->table, NULL, n, b->kv8.c.block, b->kv8.c.max_blocks);
+        if (!rc) rc = rc2;
+    }
+    if (!rc) rc = qh_d2h(hist, b->hist, (size_t)n_tokens * n * 2 * sizeof(int));
+    if (!rc) rc = qh_d2h(scores, b->score, (size_t)n * sizeof(float));
+    if (!rc) rc = qh_sync();
+    for (int s = 0; s < n && !rc; s++)
+        for (int t = n_tokens - 1, at = s; t >= 0; t--) {
+            const int *h = hist + ((size_t)t * n + at) * 2;
+            out[(size_t)s * n_tokens + t] = h[0];
+            at = s / width * width + h[1];
+        }
+    free(hist);
+    return rc;
 }
 
 int qwen3_hip_batch_logits(qwen3_hip_batch *b, float *out) {

@@ -132,12 +132,24 @@ int qm_kv8_attention(const qm_kv8_t *c, void *out_d, const void *q_d, size_t ldo
                      const int *row_d, const int *pos_d, int n, int rows, int max_rows, int max_ctx, float scale,
                      void *work_d, size_t work_bytes);
 
+/* QK-norm + RoPE of qkv rows ([nt][4096]) at positions pos_d[i] (each) or
+ * *pos_d + i: k in place, q in place or as bf16 [nt][2048] into qb_d */
+int qm_qk_rope(float *qkv_d, uint16_t *qb_d, const uint16_t *qn_d, const uint16_t *kn_d, const float *rcos_d,
+               const float *rsin_d, const int *pos_d, int each, int nt, int max_seq, float eps);
+/* table entries of unfinished blocks (all where pos_d is NULL) = the
+ * sequence's own pages, s * max_blocks + block index */
+int qm_kv8_own(int *table_d, const int *pos_d, int n_seq, int block, int max_blocks);
+
 #define QM_BEAM_MAX_WIDTH 16
 #define QM_BEAM_MAX_PIECES 1024      /* of 2,048 logits each */
 size_t qm_beam_select_work(int vocab, int n_group, int width);
 int qm_beam_select(const float *logits_d, size_t ld, int vocab, int n_group, int width, const float *score_d,
                    const int *done_d, int end0, int end1, float *score_out_d, int *done_out_d, int *token_out_d,
                    int *parent_out_d, void *work_d, size_t work_bytes);
+/* score = 0 for the first beam of a group, -inf for the others; done = 0 */
+int qm_beam_start(float *score_d, int *done_d, int n, int width);
+/* hist_d[step][i] = {token_d[i], parent_d[i]}; pos_d[i] += adv */
+int qm_beam_record(int *hist_d, const int *token_d, const int *parent_d, int *pos_d, int n, int step, int adv);
 int qm_beam_reorder(void *dst_d, const void *src_d, const int *parent_d, int n_group, int width, int slabs,
                     size_t slab_stride, size_t seq_stride, int runs, size_t run_stride, size_t run_bytes);
 

@@ -12,6 +12,7 @@ import ctypes
 import numpy as np
 
 from . import runtime
+from .abi import KV8_FORMATS
 from .runtime import F32P, I32P, VP
 
 LAYOUT_ROW = 0
@@ -170,12 +171,19 @@ class Model:
 class Batch:
     """n_seq sequences decoded together on one Model (qwen3_hip_batch_*):
     prefill each sequence, then decode steps feed one token of every
-    sequence at once (M = n_seq projections)."""
+    sequence at once (M = n_seq projections).  kv: how the caches are held,
+    "fp32", or in 8 bits as "e4m3" or "int8"."""
 
-    def __init__(self, model, n_seq, max_ctx):
+    def __init__(self, model, n_seq, max_ctx, kv="fp32"):
         L = runtime.lib()
         h = VP()
-        _rc(L.qwen3_hip_batch_open(ctypes.byref(h), model._h, n_seq, max_ctx), "qwen3_hip_batch_open")
+        if kv == "fp32":
+            _rc(L.qwen3_hip_batch_open(ctypes.byref(h), model._h, n_seq, max_ctx), "qwen3_hip_batch_open")
+        elif kv in KV8_FORMATS:
+            _rc(L.qwen3_hip_batch_open_kv8(ctypes.byref(h), model._h, n_seq, max_ctx, KV8_FORMATS[kv]),
+                "qwen3_hip_batch_open_kv8")
+        else:
+            raise ValueError(f"unknown cache kind {kv!r}")
         self._h = h
         self.n_seq = n_seq
         self.max_ctx = max_ctx
@@ -204,6 +212,20 @@ class Batch:
             "qwen3_hip_batch_decode")
         return out
 
+    def beam(self, prompts, width, n_tokens, stop_at_eos=False):
+        """Beam search behind each of n_seq / width prompts: tokens
+        [groups, width, n_tokens] and scores [groups, width], best first."""
+        ps = [_i32(p) for p in prompts]
+        if len(ps) * width != self.n_seq:
+            raise ValueError(f"{len(ps)} prompts of {width} beams on {self.n_seq} sequences")
+        flat, lens = np.concatenate(ps), _i32([p.size for p in ps])
+        out = np.zeros((len(ps), width, n_tokens), dtype=np.int32)
+        scores = np.zeros((len(ps), width), dtype=np.float32)
+        _rc(runtime.lib().qwen3_hip_batch_beam(self._h, width, flat.ctypes.data_as(I32P), lens.ctypes.data_as(I32P), n_tokens,
+                                               1 if stop_at_eos else 0, out.ctypes.data_as(I32P),
+                                               scores.ctypes.data_as(F32P)), "qwen3_hip_batch_beam")
+        return out, scores
+
     def logits(self):
         out = np.empty((self.n_seq, VOCAB), dtype=np.float32)
         _rc(runtime.lib().qwen3_hip_batch_logits(self._h, out.ctypes.data_as(F32P)), "qwen3_hip_batch_logits")
@@ -221,9 +243,11 @@ class Batch:
 def main(argv=None):
     """Greedy generation on a seeded random-init blob:
     python -m n550_qwen3_bringup_handover_amd.model [--seed S] [--prompt N] [--decode N]
-                                                     [--repeat R] [--eager] [--tile] [--batch B]
+                                                     [--repeat R] [--eager] [--tile]
+                                                     [--batch B [--kv fp32|e4m3|int8] [--beams W]]
     With --batch B, B sequences with their own random prompts of --prompt
-    tokens are decoded together (--repeat calls of --decode steps each)."""
+    tokens are decoded together (--repeat calls of --decode steps each), their
+    caches held as --kv says; with --beams W they are B / W beam searches."""
     import argparse
     ap = argparse.ArgumentParser(description=main.__doc__)
     ap.add_argument("--seed", type=lambda v: int(v, 0), default=0x03550040)
@@ -236,6 +260,8 @@ def main(argv=None):
     ap.add_argument("--tile", action="store_true", help="tile-major blob")
     ap.add_argument("--batch", type=int, default=0,
                     help="decode this many sequences together (each with its own random prompt)")
+    ap.add_argument("--kv", choices=("fp32", *KV8_FORMATS), default="fp32", help="how a batch's caches are held")
+    ap.add_argument("--beams", type=int, default=0, help="beams of each search of a batch")
     args = ap.parse_args(argv)
     blob = qw3m_random(args.seed, LAYOUT_TILE if args.tile else LAYOUT_ROW, threads=16)
     if args.batch:
@@ -260,9 +286,17 @@ def _main_batch(args, blob):
     import time
     rng = np.random.default_rng(args.seed)
     ctx = args.prompt + args.decode * args.repeat
-    with Model(blob, max_seq=ctx) as m, Batch(m, args.batch, ctx) as b:
+    with Model(blob, max_seq=ctx) as m, Batch(m, args.batch, ctx, args.kv) as b:
         del blob
         b.set_graph(not args.eager)
+        if args.beams:
+            prompts = [rng.integers(0, VOCAB, args.prompt).astype(np.int32) for _ in range(args.batch // args.beams)]
+            for r in range(args.repeat):
+                out, scores = b.beam(prompts, args.beams, args.decode)
+                dec = b.timing()
+                print(f"run {r}: {args.decode} steps of {len(prompts)} x {args.beams} beams {dec:.3f} ms; best of search 0 "
+                      f"{scores[0, 0]:.3f} {out[0, 0, :8].tolist()}", flush=True)
+            return 0
         t0 = time.time()
         for s in range(args.batch):
             b.prefill(s, rng.integers(0, VOCAB, args.prompt).astype(np.int32))

@@ -113,9 +113,11 @@ _PROTOS = {
     "qwen3_hip_model_persist_errors": (ctypes.c_int, [VP, ctypes.POINTER(ctypes.c_uint)]),
     "qwen3_hip_model_set_dump": (ctypes.c_int, [VP, VP, VP]),
     "qwen3_hip_batch_open": (ctypes.c_int, [ctypes.POINTER(VP), VP, ctypes.c_int, ctypes.c_int]),
+    "qwen3_hip_batch_open_kv8": (ctypes.c_int, [ctypes.POINTER(VP), VP, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "qwen3_hip_batch_close": (None, [VP]),
     "qwen3_hip_batch_prefill": (ctypes.c_int, [VP, ctypes.c_int, I32P, ctypes.c_int]),
     "qwen3_hip_batch_decode": (ctypes.c_int, [VP, ctypes.c_int, I32P]),
+    "qwen3_hip_batch_beam": (ctypes.c_int, [VP, ctypes.c_int, I32P, I32P, ctypes.c_int, ctypes.c_int, I32P, F32P]),
     "qwen3_hip_batch_logits": (ctypes.c_int, [VP, F32P]),
     "qwen3_hip_batch_set_graph": (ctypes.c_int, [VP, ctypes.c_int]),
     "qwen3_hip_batch_timing": (ctypes.c_int, [VP, ctypes.POINTER(ctypes.c_double)]),

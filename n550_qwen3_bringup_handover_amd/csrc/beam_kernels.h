@@ -18,11 +18,13 @@
 #define BEAM_PIECE 2048                // logits of a wave: 32 a lane
 #define BEAM_V (BEAM_PIECE / WAVE)
 #define BEAM_NONE 0x7FFFFFFF           // the index of no candidate
+#define BEAM_E 32                      // list entries a lane of the second launch holds: vocab x W up to 4 M
 
 struct beam_cand { float v; int i; };
 struct beam_sum { float m, s; };
 
-// workspace: sums [row][piece], lists [row][piece][W]
+// workspace: sums [row][piece], lists [row][W][piece] (by rank: the lanes of the
+// second launch then hold entries of like ranks)
 static size_t beam_pieces(int vocab) { return ((size_t)vocab + BEAM_PIECE - 1) / BEAM_PIECE; }
 
 template <int CTRL>
@@ -43,36 +45,64 @@ __device__ __forceinline__ bool beam_before(float av, int ai, float bv, int bi) 
     return av > bv || (av == bv && ai < bi);
 }
 
-// Wave: one piece of one row.  Each lane keeps its best and second best;
-// W times the wave's best is taken and its lane moves up, scanning its values
-// again only after its second was used.
+// A wave's choice of W among what its lanes hold: W times the largest of the
+// lanes' maxima is dropped; what reaches the last of them, T, are at least W
+// values and hardly more, which go to LDS, where each finds its rank by
+// counting who comes before it.  Where more than a lane each reach T (equal
+// values), or fewer than W are finite, the callers choose one at a time.
+#define BEAM_CAP WAVE
+__device__ __forceinline__ float beam_threshold(float lane_max, int W) {
+    float t = -INFINITY;
+    for (int w = 0; w < W; w++) {
+        t = wave_max(lane_max);
+        lane_max = lane_max == t ? -INFINITY : lane_max;
+    }
+    return t;
+}
+__device__ __forceinline__ void beam_collect(beam_cand *cand, int &n, bool in, float v, int i) {
+    const unsigned long long mask = __ballot(in);
+    if (mask) {
+        const int at = n + __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
+        if (in && at < BEAM_CAP) cand[at] = beam_cand{v, i};
+        n += __popcll(mask);
+    }
+}
+__device__ __forceinline__ int beam_rank(const beam_cand *cand, int n, beam_cand t) {
+    int rank = 0;
+#pragma unroll 4
+    for (int u = 0; u < n; u++) rank += beam_before(cand[u].v, cand[u].i, t.v, t.i);
+    return rank;
+}
+
+// Wave: one piece of one row, 32 logits a lane in registers.
 template <bool VEC>
 __global__ __launch_bounds__(NTH) void k_beam_pieces(const float *__restrict__ logits, size_t ld, int vocab, int rows,
                                                     int W, int pieces, const float *__restrict__ score,
                                                     const int *__restrict__ done, beam_sum *__restrict__ sums,
                                                     beam_cand *__restrict__ lists) {
+    __shared__ beam_cand cands[NTH / WAVE][BEAM_CAP];
     const int lane = threadIdx.x & 63;
     const int piece = blockIdx.x * (NTH / WAVE) + (threadIdx.x >> 6), r = blockIdx.y;
     if (piece >= pieces) return;
-    beam_cand *out = lists + ((size_t)r * pieces + piece) * W;
-    // a finished beam's row is not read; a beam that cannot be chosen for its
-    // score offers its first tokens, in case nothing else is left
-    const bool over = done && done[r] != 0;
-    if (over || score[r] == -INFINITY) {
-        if (lane < W) out[lane] = beam_cand{-INFINITY, !over && piece == 0 && lane < vocab ? lane : BEAM_NONE};
-        if (lane == 0) sums[(size_t)r * pieces + piece] = beam_sum{-INFINITY, 0.0f};
-        return;
-    }
+    beam_cand *out = lists + (size_t)r * pieces * W + piece;             // entry w at w * pieces
     const float *x = logits + (size_t)r * ld;
     const int base = piece * BEAM_PIECE;
     float v[BEAM_V];
     auto at = [&](int k) { return VEC ? base + (k >> 2) * (4 * WAVE) + 4 * lane + (k & 3) : base + k * WAVE + lane; };
+    // a finished beam's row is not read; a beam that cannot be chosen for its
+    // score offers its first tokens, in case nothing else is left
+    const bool over = done && done[r] != 0;
+    if (over || score[r] == -INFINITY) {
+        if (lane < W) out[(size_t)lane * pieces] = beam_cand{-INFINITY, !over && piece == 0 && lane < vocab ? lane : BEAM_NONE};
+        if (lane == 0) sums[(size_t)r * pieces + piece] = beam_sum{-INFINITY, 0.0f};
+        return;
+    }
     if constexpr (VEC) {
 #pragma unroll
         for (int k = 0; k < BEAM_V; k += 4) {
             const int i = at(k);
             f32x4 t = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (i + 3 < vocab) t = __builtin_nontemporal_load((const f32x4 *)(x + i));
+            if (i + 3 < vocab) t = *(const f32x4 *)(x + i);
             else {
 #pragma unroll
                 for (int u = 0; u < 4; u++)
@@ -85,70 +115,56 @@ __global__ __launch_bounds__(NTH) void k_beam_pieces(const float *__restrict__ l
 #pragma unroll
         for (int k = 0; k < BEAM_V; k++) v[k] = at(k) < vocab ? x[at(k)] : -INFINITY;
     }
-    float mx = -INFINITY;
+    float lm = -INFINITY;
 #pragma unroll
     for (int k = 0; k < BEAM_V; k++) {
-        v[k] = v[k] == v[k] ? v[k] : -INFINITY;           // a NaN is never chosen
-        mx = fmaxf(mx, v[k]);
+        v[k] = fmaxf(v[k], -INFINITY);                    // a NaN is never chosen
+        lm = fmaxf(lm, v[k]);
     }
-    mx = wave_max(mx);
+    const float mx = wave_max(lm);
     float sum = 0.0f;
     if (mx > -INFINITY) {
+        // +inf gives NaN: a row without probabilities
 #pragma unroll
-        for (int k = 0; k < BEAM_V; k++) sum += expf(v[k] - mx);
+        for (int k = 0; k < BEAM_V; k++) sum += __builtin_amdgcn_exp2f((v[k] - mx) * 1.44269504088896340736f);
     }
     sum = wave_sum(sum);
     if (lane == 0) sums[(size_t)r * pieces + piece] = beam_sum{mx, sum};
 
-    float v1 = -INFINITY, v2 = -INFINITY;
-    int i1 = BEAM_NONE, i2 = BEAM_NONE;
-    // the best two that come behind (pv, pi)
-    auto scan = [&](float pv, int pi) {
-        v1 = v2 = -INFINITY;
-        i1 = i2 = BEAM_NONE;
+    const float thr = beam_threshold(lm, W);
+    beam_cand *cand = cands[threadIdx.x >> 6];
+    int n = 0;
+    if (thr > -INFINITY) {
+#pragma unroll
+        for (int k = 0; k < BEAM_V; k++) beam_collect(cand, n, v[k] >= thr, v[k], at(k));
+        if (n <= BEAM_CAP) {
+            if (lane < n) {
+                const beam_cand t = cand[lane];
+                const int rank = beam_rank(cand, n, t);
+                if (rank < W) out[(size_t)rank * pieces] = t;
+            }
+            return;
+        }
+    }
+    // one at a time: the first that comes behind the last one taken
+    float pv = INFINITY;
+    int pi = -1;
+    for (int w = 0; w < W; w++) {
+        float bv = -INFINITY;
+        int bi = BEAM_NONE;
 #pragma unroll
         for (int k = 0; k < BEAM_V; k++) {
             const int i = at(k);
-            if (i < vocab && beam_before(pv, pi, v[k], i)) {
-                if (beam_before(v[k], i, v1, i1)) {
-                    v2 = v1; i2 = i1;
-                    v1 = v[k]; i1 = i;
-                } else if (beam_before(v[k], i, v2, i2)) {
-                    v2 = v[k]; i2 = i;
-                }
-            }
+            if (i < vocab && beam_before(pv, pi, v[k], i) && beam_before(v[k], i, bv, bi)) { bv = v[k]; bi = i; }
         }
-    };
-    scan(INFINITY, -1);
-    for (int w = 0; w < W; w++) {
-        const float bv = wave_max(v1);
-        const int bi = wave_min_int(v1 == bv ? i1 : BEAM_NONE);
-        if (lane == 0) out[w] = beam_cand{bv, bi};
-        const bool mine = i1 == bi && bi != BEAM_NONE;
-        if (mine) { v1 = v2; i1 = i2; v2 = -INFINITY; i2 = BEAM_NONE; }
-        // i2 used up and i1 as well: look again behind what was taken
-        if (__any(mine && i1 == BEAM_NONE)) {
-            if (mine && i1 == BEAM_NONE) scan(bv, bi);
-        }
+        pv = wave_max(bv);
+        pi = wave_min_int(bv == pv ? bi : BEAM_NONE);
+        if (lane == 0) out[(size_t)w * pieces] = beam_cand{pv, pi};
     }
 }
 
-__device__ __forceinline__ bool beam_before(double av, int ai, double bv, int bi) {
-    return av > bv || (av == bv && ai < bi);
-}
-// the wave's best (score, index), in every lane
-__device__ __forceinline__ void beam_wave_best(double &v, int &i) {
-#pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) {
-        const double ov = __shfl_xor(v, s);
-        const int oi = __shfl_xor(i, s);
-        if (beam_before(ov, oi, v, i)) { v = ov; i = oi; }
-    }
-}
-
-// Block: one group.  Wave w joins row w's sums and merges its pieces' lists
-// (each lane walks its own lists' heads); then wave 0 picks W of the W x W
-// rows' best.
+// Block: one group.  Wave w joins row w's sums and finds the row's best W in
+// its pieces' lists; then one thread for each of the W x W counts its rank.
 __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, int pieces, const float *score,
                                                              const int *done, int end0, int end1,
                                                              const beam_sum *__restrict__ sums,
@@ -157,88 +173,93 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
                                                              int *__restrict__ parent_out) {
     const int g = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     __shared__ double cv[BEAM_MAX * BEAM_MAX];
-    __shared__ int ci[BEAM_MAX * BEAM_MAX];              // token
-    __shared__ unsigned char head[BEAM_MAX][QM_BEAM_MAX_PIECES];
+    __shared__ long cid[BEAM_MAX * BEAM_MAX];             // w V + token, BEAM_NOWHERE for no candidate
+    __shared__ beam_cand cands[BEAM_MAX][BEAM_CAP];
     __shared__ int sdone[BEAM_MAX];
-    const int r = g * W + w;                              // grid: W waves a block
+    constexpr long BEAM_NOWHERE = 0x7FFFFFFFFFFFFFFFL;
+    const int r = g * W + w;                              // launched with W waves
     const bool over = done && done[r] != 0;
     const double base = score[r];
     if (lane == 0) sdone[w] = over;
     if (over) {
         if (lane < W) {
             cv[w * W + lane] = lane == 0 ? base : -INFINITY;
-            ci[w * W + lane] = lane == 0 ? end0 : BEAM_NONE;
+            cid[w * W + lane] = lane == 0 ? (long)w * vocab + end0 : BEAM_NOWHERE;
         }
     } else {
-        // log of the sum of e^x over the row
         const beam_sum *ps = sums + (size_t)r * pieces;
+        const beam_cand *pl = lists + (size_t)r * pieces * W;
+        const int entries = pieces * W;
+        // the first BEAM_E x 64 entries of the lists in registers, all loads in flight
+        beam_cand t[BEAM_E];
+#pragma unroll
+        for (int k = 0; k < BEAM_E; k++) {
+            t[k] = beam_cand{-INFINITY, BEAM_NONE};
+            if (WAVE * (k / 8 * 8) < entries && WAVE * k + lane < entries) t[k] = pl[WAVE * k + lane];
+        }
         float mx = -INFINITY;
+#pragma unroll 2
         for (int p = lane; p < pieces; p += WAVE) mx = fmaxf(mx, ps[p].m);
         mx = wave_max(mx);
+        // log of the sum of e^x over the row
         double sum = 0.0;
         for (int p = lane; p < pieces; p += WAVE)
             if (ps[p].m > -INFINITY) sum += (double)ps[p].s * exp((double)ps[p].m - (double)mx);
 #pragma unroll
         for (int s = 32; s >= 1; s >>= 1) sum += __shfl_xor(sum, s);
         const double lse = (double)mx + log(sum);
-        const beam_cand *pl = lists + (size_t)r * pieces * W;
-        for (int p = lane; p < pieces; p += WAVE) head[w][p] = 0;
-        for (int k = 0; k < W; k++) {
-            float bv = -INFINITY;
-            int bi = BEAM_NONE, bp = -1;
-            for (int p = lane; p < pieces; p += WAVE) {
-                const int hd = head[w][p];
-                if (hd >= W) continue;
-                const beam_cand t = pl[(size_t)p * W + hd];
-                if (beam_before(t.v, t.i, bv, bi)) { bv = t.v; bi = t.i; bp = p; }
+        auto put = [&](int k, float v, int i) {
+            const double t = base + ((double)v - lse);
+            cv[w * W + k] = t == t ? t : -INFINITY;       // no probabilities, no score
+            cid[w * W + k] = i == BEAM_NONE ? BEAM_NOWHERE : (long)w * vocab + i;
+        };
+        float lm = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < BEAM_E; k++) lm = fmaxf(lm, t[k].v);
+        const float thr = entries <= WAVE * BEAM_E ? beam_threshold(lm, W) : -INFINITY;
+        beam_cand *cand = cands[w];
+        int n = 0;
+        if (thr > -INFINITY) {
+#pragma unroll
+            for (int k = 0; k < BEAM_E; k++)
+                if (WAVE * (k / 8 * 8) < entries) beam_collect(cand, n, t[k].v >= thr, t[k].v, t[k].i);
+        }
+        if (n > 0 && n <= BEAM_CAP) {
+            if (lane < n) {
+                const beam_cand t = cand[lane];
+                const int rank = beam_rank(cand, n, t);
+                if (rank < W) put(rank, t.v, t.i);
             }
-            const float wv = wave_max(bv);
-            const int wi = wave_min_int(bv == wv ? bi : BEAM_NONE);
-            if (bp >= 0 && bi == wi) head[w][bp]++;
-            if (lane == 0) {
-                const double t = base + ((double)wv - lse);
-                cv[w * W + k] = t == t ? t : -INFINITY;   // no probabilities, no score
-                ci[w * W + k] = wi;
+        } else {
+            float pv = INFINITY;
+            int pi = -1;
+            for (int k = 0; k < W; k++) {
+                float bv = -INFINITY;
+                int bi = BEAM_NONE;
+                for (int i = lane; i < entries; i += WAVE) {
+                    const beam_cand t = pl[i];
+                    if (beam_before(pv, pi, t.v, t.i) && beam_before(t.v, t.i, bv, bi)) { bv = t.v; bi = t.i; }
+                }
+                pv = wave_max(bv);
+                pi = wave_min_int(bv == pv ? bi : BEAM_NONE);
+                if (lane == 0) put(k, pv, pi);
             }
         }
     }
-    __syncthreads();
-    if (w > 0) return;
-    // BEAM_MAX^2 / 64 candidates a lane, by place w' W + k; a tie goes to the
-    // lowest w' V + token
-    constexpr int PER = BEAM_MAX * BEAM_MAX / WAVE;
-    double v[PER];
-    long id[PER];
-#pragma unroll
-    for (int u = 0; u < PER; u++) {
-        const int at = lane + WAVE * u;
-        const bool in = at < W * W && ci[at] != BEAM_NONE;
-        v[u] = in ? cv[at] : -INFINITY;
-        id[u] = in ? (long)(at / W) * vocab + ci[at] : 0x7FFFFFFFFFFFFFFFL;
-    }
-    for (int k = 0; k < W; k++) {
-        double bv = -INFINITY;
-        long bi = 0x7FFFFFFFFFFFFFFFL;
-#pragma unroll
-        for (int u = 0; u < PER; u++)
-            if (v[u] > bv || (v[u] == bv && id[u] < bi)) { bv = v[u]; bi = id[u]; }
-#pragma unroll
-        for (int s = 32; s >= 1; s >>= 1) {
-            const double ov = __shfl_xor(bv, s);
-            const long oi = __shfl_xor(bi, s);
-            if (ov > bv || (ov == bv && oi < bi)) { bv = ov; bi = oi; }
-        }
-#pragma unroll
-        for (int u = 0; u < PER; u++)
-            if (id[u] == bi) { v[u] = -INFINITY; id[u] = 0x7FFFFFFFFFFFFFFFL; }
-        if (lane == 0) {
-            // the inputs of the group have all been read: outputs may lie where they did
-            const int par = (int)(bi / vocab), tok = (int)(bi % vocab);
-            score_out[g * W + k] = (float)bv;
-            token_out[g * W + k] = tok;
-            parent_out[g * W + k] = par;
-            done_out[g * W + k] = sdone[par] != 0 || tok == end0 || tok == end1;
-        }
+    __syncthreads();                                      // the group's inputs have been read: outputs may lie there
+    const int i = threadIdx.x;
+    if (i >= W * W) return;
+    const double v = cv[i];
+    const long id = cid[i];
+    int rank = 0;
+#pragma unroll 8
+    for (int u = 0; u < W * W; u++) rank += cv[u] > v || (cv[u] == v && cid[u] < id);
+    if (rank < W && id != BEAM_NOWHERE) {
+        const int par = i / W, tok = (int)(id - (long)par * vocab);
+        score_out[g * W + rank] = (float)v;
+        token_out[g * W + rank] = tok;
+        parent_out[g * W + rank] = par;
+        done_out[g * W + rank] = sdone[par] != 0 || tok == end0 || tok == end1;
     }
 }
 

@@ -98,73 +98,97 @@ __device__ __forceinline__ uint32_t kv8_codes4(float a, float b, float c, float 
     }
 }
 
-// Block (h, e, z): kv head h of entry e, the z-th block its rows touch.  A
-// block that the rows finish is gathered in LDS as bf16 (rows that earlier
-// calls brought from the tail), its largest magnitudes found, its codes
-// written 16 bytes a thread.  The rows behind the last finished block go to
-// the tail, by z = 0 alone and after it has read the tail: two blocks of one
-// launch must not meet there.
-// Bound by its launch and two dependent reads for a decode step's rows.
+// sixteen consecutive values, 16-byte aligned (BF) or 16-byte aligned fp32
+template <bool BF>
+__device__ __forceinline__ void kv8_load16(const void *p, size_t i, __bf16 (&x)[16]) {
+    if constexpr (BF) {
+        const bf16x8 a = *(const bf16x8 *)((const __bf16 *)p + i), b = *(const bf16x8 *)((const __bf16 *)p + i + 8);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] = kv8_held((float)a[j]);
+            x[8 + j] = kv8_held((float)b[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const f32x4 a = *(const f32x4 *)((const float *)p + i + j);
+#pragma unroll
+            for (int u = 0; u < 4; u++) x[j + u] = kv8_held(a[u]);
+        }
+    }
+}
+
+// Block (h, e, z): kv head h of entry e, the z-th block its rows touch; B D / 16
+// threads, so that a finished block is one unit of 16 values of K (of a row)
+// and one of V (of a column: 16 rows of one dim) a thread, in registers from
+// the load to the codes: all loads of a block in flight at once, its largest
+// magnitudes the only exchange.  Rows that earlier calls brought come from the
+// tail.  The rows behind the last finished block go to the tail, by z = 0
+// alone and after it has read the tail: two blocks of one launch must not meet
+// there.
 template <int FMT, int D, int B, bool BF>
-__global__ __launch_bounds__(NTH) void k_kv8_append(qm_kv8_t c, const void *__restrict__ kn, const void *__restrict__ vn,
-                                                   size_t ldk, size_t ldv, const int *__restrict__ row,
-                                                   const int *__restrict__ pos, int rows, int max_rows) {
+__global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void *__restrict__ kn,
+                                                         const void *__restrict__ vn, size_t ldk, size_t ldv,
+                                                         const int *__restrict__ row, const int *__restrict__ pos, int rows,
+                                                         int max_rows) {
+    constexpr int NT = B * D / 16, NWV = NT / WAVE;
     const int h = blockIdx.x, e = blockIdx.y, z = blockIdx.z, tid = threadIdx.x;
     kv8_entry t;
     if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
     const int end = t.pos + t.cnt, b0 = t.pos / B, bl = end / B, b = b0 + z;
     if (b >= bl && z > 0) return;
-    auto k_at = [&](int p, int d) {
-        const size_t i = (size_t)(t.r0 + p - t.pos) * ldk + h * D + d;
-        return BF ? (float)((const __bf16 *)kn)[i] : ((const float *)kn)[i];
-    };
-    auto v_at = [&](int p, int d) {
-        const size_t i = (size_t)(t.r0 + p - t.pos) * ldv + h * D + d;
-        return BF ? (float)((const __bf16 *)vn)[i] : ((const float *)vn)[i];
-    };
     __bf16 *kt = (__bf16 *)c.k_tail + ((size_t)e * c.heads + h) * (B * D);
     __bf16 *vt = (__bf16 *)c.v_tail + ((size_t)e * c.heads + h) * (B * D);
 
     if (b < bl) {
-        __shared__ __align__(16) __bf16 sk[B * D], sv[B * D];
-        __shared__ float red[2][NTH / WAVE];
-        float ak = 0.0f, av = 0.0f;
-        for (int i = tid; i < B * D; i += NTH) {
-            const int r = i / D, d = i % D, p = b * B + r;
-            const __bf16 x = p < t.pos ? kt[i] : kv8_held(k_at(p, d));
-            const __bf16 y = p < t.pos ? vt[d * B + r] : kv8_held(v_at(p, d));
-            sk[i] = x;
-            sv[i] = y;
-            ak = fmaxf(ak, fabsf((float)x));
-            av = fmaxf(av, fabsf((float)y));
+        const int page = c.table[(size_t)e * c.max_blocks + b];
+        const int have = max(t.pos - b * B, 0);           // rows in the tail, < B
+        const int p0 = t.r0 + b * B - t.pos;              // row of the block's slot 0 (before r0 where some are in the tail)
+        const int kr = tid / (D / 16), kd = tid % (D / 16) * 16;       // K: slot and dims
+        const int vd = tid % D, vr = tid / D * 16;                     // V: dim and slots
+        __bf16 x[16], y[16];
+        kv8_load16<BF>(kn, (size_t)(p0 + max(kr, have)) * ldk + h * D + kd, x);
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const size_t i = (size_t)(p0 + max(vr + j, have)) * ldv + h * D + vd;
+            y[j] = kv8_held(BF ? (float)((const __bf16 *)vn)[i] : ((const float *)vn)[i]);
         }
+        if (have > 0) {
+            if (kr < have) kv8_load16<true>(kt, kr * D + kd, x);
+            __bf16 o[16];
+            kv8_load16<true>(vt, vd * B + vr, o);
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (vr + j < have) y[j] = o[j];
+        }
+        float ak = 0.0f, av = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            ak = fmaxf(ak, fabsf((float)x[j]));
+            av = fmaxf(av, fabsf((float)y[j]));
+        }
+        __shared__ float red[2][NWV];
         ak = wave_max(ak);
         av = wave_max(av);
         if ((tid & 63) == 0) { red[0][tid >> 6] = ak; red[1][tid >> 6] = av; }
-        __syncthreads();
-        ak = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-        av = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+        __syncthreads();                                  // the tail has been read, too
+#pragma unroll
+        for (int w = 0; w < NWV; w++) {
+            ak = fmaxf(ak, red[0][w]);
+            av = fmaxf(av, red[1][w]);
+        }
         const float ks = ak < KV8_TINY ? 0.0f : ak / kv8_qmax<FMT>::v;
         const float vs = av < KV8_TINY ? 0.0f : av / kv8_qmax<FMT>::v;
-        const int page = c.table[(size_t)e * c.max_blocks + b];
         if (page >= 0 && page < c.n_page) {               // the same for the whole block
             const size_t at = (size_t)page * c.heads + h;
-            uint4 *ko = (uint4 *)(c.k + at * (B * D)), *vo = (uint4 *)(c.v + at * (B * D));
-            for (int u = tid; u < B * D / 16; u += NTH) {
-                const __bf16 *s = sk + 16 * u;
-                uint32_t w[4];
+            uint32_t u[4], w[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    w[j] = kv8_codes4<FMT>((float)s[4 * j], (float)s[4 * j + 1], (float)s[4 * j + 2],
-                                           (float)s[4 * j + 3], ks);
-                ko[u] = make_uint4(w[0], w[1], w[2], w[3]);
-                const int d = u / (B / 16), r = u % (B / 16) * 16;
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    w[j] = kv8_codes4<FMT>((float)sv[(r + 4 * j) * D + d], (float)sv[(r + 4 * j + 1) * D + d],
-                                           (float)sv[(r + 4 * j + 2) * D + d], (float)sv[(r + 4 * j + 3) * D + d], vs);
-                vo[u] = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int j = 0; j < 4; j++) {
+                u[j] = kv8_codes4<FMT>((float)x[4 * j], (float)x[4 * j + 1], (float)x[4 * j + 2], (float)x[4 * j + 3], ks);
+                w[j] = kv8_codes4<FMT>((float)y[4 * j], (float)y[4 * j + 1], (float)y[4 * j + 2], (float)y[4 * j + 3], vs);
             }
+            *(uint4 *)(c.k + at * (B * D) + kr * D + kd) = make_uint4(u[0], u[1], u[2], u[3]);
+            *(uint4 *)(c.v + at * (B * D) + vd * B + vr) = make_uint4(w[0], w[1], w[2], w[3]);
             if (tid == 0) {
                 c.k_scale[at] = ks;
                 c.v_scale[at] = vs;
@@ -173,10 +197,13 @@ __global__ __launch_bounds__(NTH) void k_kv8_append(qm_kv8_t c, const void *__re
     }
     if (z > 0) return;
     const int from = max(t.pos, bl * B);
-    for (int i = tid; i < (end - from) * D; i += NTH) {
+    for (int i = tid; i < (end - from) * D; i += NT) {
         const int p = from + i / D, d = i % D;
-        kt[(p - bl * B) * D + d] = kv8_held(k_at(p, d));
-        vt[d * B + (p - bl * B)] = kv8_held(v_at(p, d));
+        const size_t r = t.r0 + p - t.pos;
+        const float a = BF ? (float)((const __bf16 *)kn)[r * ldk + h * D + d] : ((const float *)kn)[r * ldk + h * D + d];
+        const float o = BF ? (float)((const __bf16 *)vn)[r * ldv + h * D + d] : ((const float *)vn)[r * ldv + h * D + d];
+        kt[(p - bl * B) * D + d] = kv8_held(a);
+        vt[d * B + (p - bl * B)] = kv8_held(o);
     }
 }
 
@@ -232,21 +259,29 @@ __device__ __forceinline__ f32x4 kv8_mma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// eight values of a query row
-template <bool BF, int NP>
-__device__ __forceinline__ void kv8_load_q(const void *q, size_t i, bool in, bf16x8 (&p)[NP]) {
-    if constexpr (BF) {
-        static_assert(NP == 1, "bf16 rows are one piece");
-        p[0] = in ? *(const bf16x8 *)((const __bf16 *)q + i) : bf16x8{};
-    } else {
-        f32x8 x = {};
-        if (in) {
-            const f32x4 a = *(const f32x4 *)((const float *)q + i), b = *(const f32x4 *)((const float *)q + i + 4);
-            x = f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+// eight values of a query row, and their pieces
+template <bool BF>
+struct kv8_row {
+    f32x4 a, b;
+    __device__ __forceinline__ void load(const void *q, size_t i, bool in) {
+        a = b = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (BF) {
+            if (in) a = *(const f32x4 *)((const __bf16 *)q + i);
+        } else if (in) {
+            a = *(const f32x4 *)((const float *)q + i);
+            b = *(const f32x4 *)((const float *)q + i + 4);
         }
-        kv8_pieces<NP>(x, p);
     }
-}
+    template <int NP>
+    __device__ __forceinline__ void pieces(bf16x8 (&p)[NP]) const {
+        if constexpr (BF) {
+            static_assert(NP == 1, "bf16 rows are one piece");
+            p[0] = __builtin_bit_cast(bf16x8, a);
+        } else {
+            kv8_pieces<NP>(f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, p);
+        }
+    }
+};
 
 // max and sum over the four lanes that share a column
 __device__ __forceinline__ float col_max(float v) {
@@ -289,16 +324,16 @@ __device__ __forceinline__ float kv8_softmax(f32x4 (&s)[4], float &m, float &l) 
 }
 
 // ---- few columns: keys split over waves and blocks --------------------------
-// Block (split, head + heads * column tile, entry): four waves take the steps
-// of 64 keys in turn, wave w of split y steps 4 y + w, + 4 nsplit, ...; each
+// Block (split, head + heads * column tile, entry): its NWV waves take the steps
+// of 64 keys in turn, wave w of split y steps NWV y + w, + NWV nsplit, ...; each
 // operand goes from memory straight into its MFMA's registers (K of the next
 // step is in flight during this step's V product).  The tail is one more step.
 // The waves' sums meet in LDS; with several splits each block leaves a partial
 // {m, l, -, -, o[D]} per column for k_kv8_merge.
-#define KV8_NW 4
 #define KV8_COLS 16
-template <int FMT, int D, bool BF>
-__global__ __launch_bounds__(WAVE *KV8_NW, 2) void k_kv8_few(qm_kv8_t c, void *__restrict__ out,
+#define KV8_MAX_SPLITS 32
+template <int FMT, int D, bool BF, int NWV>
+__global__ __launch_bounds__(WAVE *NWV, 2) void k_kv8_few(qm_kv8_t c, void *__restrict__ out,
                                                              const void *__restrict__ q, size_t ldo, size_t ldq,
                                                              const int *__restrict__ row, const int *__restrict__ pos,
                                                              int rows, int max_rows, int G, float f,
@@ -306,34 +341,29 @@ __global__ __launch_bounds__(WAVE *KV8_NW, 2) void k_kv8_few(qm_kv8_t c, void *_
     constexpr int NP = BF ? 1 : 3, NW = BF ? 2 : 3;        // pieces of q, and of a weight
     constexpr int KS = D / 32, DT = D / 16, LD = D + 4;
     const int e = blockIdx.z, head = blockIdx.y % c.heads, ct = blockIdx.y / c.heads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int cl = lane & 15, h = lane >> 4;
+    const int gk = (lane >> 2) & 3;                                        // the group of 16 keys its K row lies in
+    const int B = c.block, lb = __builtin_ctz(B);
+    const int *table = c.table + (size_t)e * c.max_blocks;
+    // table entry of a key, and the page it stands for, -1 where there is none.
+    // The first step's are read before anything says how long the sequence is
+    auto entry_of = [&](int key) { return (key >> lb) < c.max_blocks ? table[key >> lb] : -1; };
+    int s = NWV * blockIdx.x + wave;
+    int pk = entry_of(64 * s + 16 * gk), pv = entry_of(64 * s + 16 * h);
     kv8_entry t;
     if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
     const int col0 = ct * KV8_COLS, ncol = t.cnt * G;
     if (col0 >= ncol) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int cl = lane & 15, h = lane >> 4;
-    const int B = c.block, lb = __builtin_ctz(B);
     const int full = (t.pos + t.cnt) >> lb << lb;                          // keys in finished blocks
     const int kend = t.pos + min(t.cnt - 1, (col0 + KV8_COLS - 1) / G) + 1;   // keys the block's last column sees
-    const int ns = (min(full, kend) + 63) >> 6, stride = KV8_NW * gridDim.x;
+    const int ns = (min(full, kend) + 63) >> 6, stride = NWV * gridDim.x;
 
     const int col = col0 + cl;
     const bool in = col < ncol;
     const int qr = in ? col / G : 0, qg = in ? col % G : 0;
     const int last = in ? t.pos + qr : -1;                                 // the column's last key
-    bf16x8 qf[KS][NP];
-#pragma unroll
-    for (int j = 0; j < KS; j++)
-        kv8_load_q<BF, NP>(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + (D / 4) * h + 8 * j, in, qf[j]);
-
-    const int *table = c.table + (size_t)e * c.max_blocks;
-    // page of the 16 keys at `key`, -1 where there is none
-    auto page_of = [&](int key) {
-        int p = -1;
-        if (key < full) p = table[key >> lb];
-        return (unsigned)p < (unsigned)c.n_page ? p : -1;
-    };
-    const int gk = (lane >> 2) & 3;                                        // the group its K row lies in
+    auto page_of = [&](int key, int p) { return key < full && (unsigned)p < (unsigned)c.n_page ? p : -1; };
     uint4 kk[4][D / 64], vv[DT];
     auto load_k = [&](int s, int p) {
         const int key = 64 * s + 16 * gk;
@@ -361,13 +391,18 @@ __global__ __launch_bounds__(WAVE *KV8_NW, 2) void k_kv8_few(qm_kv8_t c, void *_
         kv8_pieces<NW>(f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, pf);
     };
 
-    int s = KV8_NW * blockIdx.x + wave;
-    int pk = -1, pv = -1;
+    kv8_row<BF> qr_[KS];
+#pragma unroll
+    for (int j = 0; j < KS; j++)
+        qr_[j].load(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + (D / 4) * h + 8 * j, in);
     if (s < ns) {
-        pk = page_of(64 * s + 16 * gk);
-        pv = page_of(64 * s + 16 * h);
+        pk = page_of(64 * s + 16 * gk, pk);
+        pv = page_of(64 * s + 16 * h, pv);
         load_k(s, pk);
     }
+    bf16x8 qf[KS][NP];
+#pragma unroll
+    for (int j = 0; j < KS; j++) qr_[j].pieces(qf[j]);
     for (; s < ns; s += stride) {
         load_v(s, pv);
         const float ks = pv >= 0 ? c.k_scale[(size_t)pv * c.heads + head] * f : 0.0f;
@@ -376,8 +411,9 @@ __global__ __launch_bounds__(WAVE *KV8_NW, 2) void k_kv8_few(qm_kv8_t c, void *_
         const int nx = s + stride;
         int pkn = -1, pvn = -1;
         if (nx < ns) {
-            pkn = page_of(64 * nx + 16 * gk);
-            pvn = page_of(64 * nx + 16 * h);
+            const int kk_ = 64 * nx + 16 * gk, kv_ = 64 * nx + 16 * h;
+            pkn = page_of(kk_, entry_of(kk_));
+            pvn = page_of(kv_, entry_of(kv_));
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -391,8 +427,10 @@ __global__ __launch_bounds__(WAVE *KV8_NW, 2) void k_kv8_few(qm_kv8_t c, void *_
             }
 #pragma unroll
             for (int r = 0; r < 4; r++) s4[i][r] = 4 * i + r <= lim ? a[r] * ks : -INFINITY;
+            if constexpr (FMT == QM_KV8_INT8) __builtin_amdgcn_sched_barrier(0);   // fp32 halfway: one tile's at a time
         }
         if (nx < ns) load_k(nx, pkn);
+        __builtin_amdgcn_sched_barrier(0);                // V's codes are not converted before they are needed
         const float rs = kv8_softmax(s4, m, l);
 #pragma unroll
         for (int i = 0; i < DT; i++) o[i] *= rs;
@@ -406,25 +444,36 @@ __global__ __launch_bounds__(WAVE *KV8_NW, 2) void k_kv8_few(qm_kv8_t c, void *_
 #pragma unroll
                 for (int n = 0; n < NW; n++) o[i] = kv8_mma(vf, pf[n], o[i]);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         pv = pvn;
     }
 
-    // the unfinished block, as step ns of the turn
-    if (kend > full && ns % stride == KV8_NW * (int)blockIdx.x + wave) {
+    // the unfinished block, as step ns of the turn.  Its rows are read whether
+    // they are there or not (within the tail): scores of keys that are not are
+    // masked, and V is cleared where they lie, as it may hold anything
+    if (kend > full && ns % stride == NWV * (int)blockIdx.x + wave) {
         const int nt = t.pos + t.cnt - full;                               // rows it holds, < B <= 64
         const __bf16 *kt = (const __bf16 *)c.k_tail + ((size_t)e * c.heads + head) * ((size_t)B * D);
         const __bf16 *vt = (const __bf16 *)c.v_tail + ((size_t)e * c.heads + head) * ((size_t)B * D);
+        bf16x8 tk[4][KS], tv[2][DT];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < KS; j++)
+                tk[i][j] = *(const bf16x8 *)(kt + (size_t)min(16 * gk + 4 * i + (lane & 3), B - 1) * D + (D / 4) * h + 8 * j);
+#pragma unroll
+        for (int s2 = 0; s2 < 2; s2++)
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+                tv[s2][i] = *(const bf16x8 *)(vt + (size_t)(16 * i + cl) * B + min(16 * h + 8 * s2, B - 8));
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int key = 16 * gk + 4 * i + (lane & 3);
             f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < KS; j++) {
-                const bf16x8 kf = key < nt ? *(const bf16x8 *)(kt + (size_t)key * D + (D / 4) * h + 8 * j) : bf16x8{};
+            for (int j = 0; j < KS; j++)
 #pragma unroll
-                for (int n = 0; n < NP; n++) a = kv8_mma(kf, qf[j][n], a);
-            }
+                for (int n = 0; n < NP; n++) a = kv8_mma(tk[i][j], qf[j][n], a);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int k = 16 * h + 4 * i + r;
@@ -438,13 +487,15 @@ __global__ __launch_bounds__(WAVE *KV8_NW, 2) void k_kv8_few(qm_kv8_t c, void *_
         for (int s2 = 0; s2 < 2; s2++) {
             bf16x8 pf[NW];
             weights(s2, 1.0f, pf);
-            const int k0 = 16 * h + 8 * s2;
+            const int there = nt - (16 * h + 8 * s2);
+            // 32 bits, two keys, at a time
+            typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+            u4 mask;
+#pragma unroll
+            for (int n = 0; n < 4; n++) mask[n] = there > 2 * n + 1 ? ~0u : there == 2 * n + 1 ? 0xFFFFu : 0u;
 #pragma unroll
             for (int i = 0; i < DT; i++) {
-                bf16x8 vf = {};
-                if (k0 < nt) vf = *(const bf16x8 *)(vt + (size_t)(16 * i + cl) * B + k0);
-#pragma unroll
-                for (int n = 0; n < 8; n++) vf[n] = k0 + n < nt ? vf[n] : (__bf16)0.0f;   // behind the last row: anything
+                const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u4, tv[s2][i]) & mask);
 #pragma unroll
                 for (int n = 0; n < NW; n++) o[i] = kv8_mma(vf, pf[n], o[i]);
             }
@@ -452,25 +503,25 @@ __global__ __launch_bounds__(WAVE *KV8_NW, 2) void k_kv8_few(qm_kv8_t c, void *_
     }
 
     // merge the waves
-    __shared__ __align__(16) float so[KV8_NW][KV8_COLS][LD];
-    __shared__ float sm[KV8_NW][KV8_COLS], sl[KV8_NW][KV8_COLS];
+    __shared__ __align__(16) float so[NWV][KV8_COLS][LD];
+    __shared__ float sm[NWV][KV8_COLS], sl[NWV][KV8_COLS];
     l = col_sum(l);
 #pragma unroll
     for (int i = 0; i < DT; i++) *(f32x4 *)&so[wave][cl][16 * i + 4 * h] = o[i];
     if (h == 0) { sm[wave][cl] = m; sl[wave][cl] = l; }
     __syncthreads();
     constexpr int TPC = D / 4;                            // threads of a column
-    for (int i = tid; i < KV8_COLS * TPC; i += WAVE * KV8_NW) {
+    for (int i = tid; i < KV8_COLS * TPC; i += WAVE * NWV) {
         const int cc = i / TPC, d = i % TPC * 4, cg = col0 + cc;
         if (cg >= ncol) continue;
         float mx = sm[0][cc];
 #pragma unroll
-        for (int w = 1; w < KV8_NW; w++) mx = fmaxf(mx, sm[w][cc]);
+        for (int w = 1; w < NWV; w++) mx = fmaxf(mx, sm[w][cc]);
         const float ref = mx == -INFINITY ? 0.0f : mx;
         float den = 0.0f;
         f32x4 num = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < KV8_NW; w++) {
+        for (int w = 0; w < NWV; w++) {
             // a wave without keys weighs 0 (its sums are 0); one whose scores were all NaN keeps its NaN
             const float g = __builtin_amdgcn_exp2f(sm[w][cc] - ref);
             den += g * sl[w][cc];
@@ -489,31 +540,60 @@ __global__ __launch_bounds__(WAVE *KV8_NW, 2) void k_kv8_few(qm_kv8_t c, void *_
     }
 }
 
-// the splits' partials of k_kv8_few merged: D / 4 threads a column
+// the splits' partials of k_kv8_few merged: a wave a column, its D / 4 lanes
+// twice (D = 128) or four times (64) over the splits, so that all are read at
+// once
 template <int D, bool BF>
 __global__ __launch_bounds__(NTH) void k_kv8_merge(qm_kv8_t c, void *__restrict__ out, size_t ldo,
                                                    const int *__restrict__ row, const int *__restrict__ pos, int rows,
                                                    int max_rows, int G, const float *__restrict__ part, int nsplit,
                                                    int tiles) {
-    constexpr int TPC = D / 4, LD = D + 4;
-    const int e = blockIdx.z, head = blockIdx.y;
+    constexpr int TPC = D / 4, LD = D + 4, GR = WAVE / TPC, PER = KV8_MAX_SPLITS / GR;
+    const int e = blockIdx.z, head = blockIdx.y, lane = threadIdx.x & 63;
     kv8_entry t;
     if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
-    const int col = blockIdx.x * (NTH / TPC) + threadIdx.x / TPC, d = threadIdx.x % TPC * 4;
+    const int col = blockIdx.x * (NTH / WAVE) + (threadIdx.x >> 6), d = lane % TPC * 4, gr = lane / TPC;
     if (col >= t.cnt * G) return;
     const int y = col / KV8_COLS * c.heads + head;
     const float *p = part + (((size_t)e * (tiles * c.heads) + y) * nsplit * KV8_COLS + col % KV8_COLS) * LD;
+    float ms[PER], ls[PER];
+    f32x4 o[PER];
+#pragma unroll
+    for (int u = 0; u < PER; u++) {
+        const int s = u * GR + gr;
+        ms[u] = -INFINITY;
+        ls[u] = 0.0f;
+        o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (u * GR < nsplit && s < nsplit) {
+            const float *ps = p + (size_t)s * KV8_COLS * LD;
+            ms[u] = ps[0];
+            ls[u] = ps[1];
+            o[u] = *(const f32x4 *)(ps + 4 + d);
+        }
+    }
     float mx = -INFINITY;
-    for (int s = 0; s < nsplit; s++) mx = fmaxf(mx, p[(size_t)s * KV8_COLS * LD]);
+#pragma unroll
+    for (int u = 0; u < PER; u++) mx = fmaxf(mx, ms[u]);
+    mx = wave_max(mx);
     const float ref = mx == -INFINITY ? 0.0f : mx;
     float den = 0.0f;
     f32x4 num = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < nsplit; s++) {
-        const float *ps = p + (size_t)s * KV8_COLS * LD;
-        const float g = __builtin_amdgcn_exp2f(ps[0] - ref);
-        den += g * ps[1];
-        num += *(const f32x4 *)(ps + 4 + d) * g;
+#pragma unroll
+    for (int u = 0; u < PER; u++) {
+        const float g = __builtin_amdgcn_exp2f(ms[u] - ref);
+        den += g * ls[u];
+        num += o[u] * g;
     }
+    auto join = [](float x) {                             // the groups of lanes
+        f32x2 q;
+        if constexpr (GR == 4) { q = swap16(x); x = q.x + q.y; }
+        q = swap32(x);
+        return q.x + q.y;
+    };
+    den = join(den);
+#pragma unroll
+    for (int i = 0; i < 4; i++) num[i] = join(num[i]);
+    if (gr > 0) return;
     num *= kv8_inverse(den);
     const size_t at = (size_t)(t.r0 + col / G) * ldo + (size_t)(head * G + col % G) * D + d;
     if constexpr (BF) *(uint2 *)((uint16_t *)out + at) = pack4(num);
@@ -560,8 +640,11 @@ __global__ __launch_bounds__(NTH, 2) void k_kv8_many(qm_kv8_t c, void *__restric
         const int qr = in ? col / G : 0, qg = in ? col % G : 0;
         last[n] = in ? t.pos + qr : -1;
 #pragma unroll
-        for (int j = 0; j < KS; j++)
-            kv8_load_q<BF, NP>(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + 32 * j + 8 * h, in, qf[n][j]);
+        for (int j = 0; j < KS; j++) {
+            kv8_row<BF> x;
+            x.load(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + 32 * j + 8 * h, in);
+            x.pieces(qf[n][j]);
+        }
     }
     const int wfirst = w0 < ncol ? t.pos + w0 / G : -1;                    // keys all the wave's columns see, and any
     const int wlast = w0 < ncol ? t.pos + min(t.cnt - 1, (w0 + 16 * CT - 1) / G) : -1;
@@ -808,7 +891,8 @@ extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, si
     if (grid.z > 65535) return QH_ETOOBIG;
     if (!stream()) return QH_ESTATE;
 #define APPEND_B(F, D_, B_, BF_) \
-    hipLaunchKernelGGL((k_kv8_append<F, D_, B_, BF_>), grid, dim3(NTH), 0, stream(), *c, k, v, ldk, ldv, row, pos, rows, max_rows)
+    hipLaunchKernelGGL((k_kv8_append<F, D_, B_, BF_>), grid, dim3(B_ *D_ / 16), 0, stream(), *c, k, v, ldk, ldv, row, pos, rows, \
+                       max_rows)
 #define APPEND(F, D_, BF_)                                  \
     do {                                                    \
         if (c->block == 16) APPEND_B(F, D_, 16, BF_);       \
@@ -821,23 +905,27 @@ extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, si
     return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
 }
 
-// Key splits of k_kv8_few: enough blocks for the CUs, at least a step for each
-// wave of a split.
-#define KV8_MAX_SPLITS 32
 #define KV8_FEW_COLS 64                // columns up to which the keys are split instead
-static int kv8_splits(const qm_kv8_t *c, int n, int tiles, int max_ctx) {
+// The launch of k_kv8_few: four waves a block where the blocks fill the CUs
+// twice, eight otherwise; the keys split over blocks where a wave would walk
+// more than three steps, as long as each still walks one and CUs are idle.
+struct kv8_plan { int waves, splits; };
+static kv8_plan kv8_few_plan(const qm_kv8_t *c, int n, int tiles, int max_ctx) {
     const long blocks = (long)n * c->heads * tiles;
     const int steps = (max_ctx + 63) / 64 + 1;
-    int s = 1;
-    while (2 * s <= KV8_MAX_SPLITS && blocks * s < 512 && 2 * s * KV8_NW <= steps) s *= 2;
-    return s;
+    if (blocks >= 512) return kv8_plan{4, 1};
+    if (steps <= 24) return kv8_plan{8, 1};
+    long s = (steps + 15) / 16, room = (320 + blocks - 1) / blocks;
+    if (s > room) s = room;
+    if (s > KV8_MAX_SPLITS) s = KV8_MAX_SPLITS;
+    return kv8_plan{8, (int)s};
 }
 
 extern "C" size_t qm_kv8_attention_work(const qm_kv8_t *c, int q_heads, int n, int max_rows, int max_ctx) {
     if (!c || c->heads < 1 || q_heads < c->heads || n < 1 || max_rows < 1) return 0;
     const long cols = (long)max_rows * (q_heads / c->heads);
     if (cols > KV8_FEW_COLS) return 0;
-    const int tiles = (int)((cols + KV8_COLS - 1) / KV8_COLS), s = kv8_splits(c, n, tiles, max_ctx);
+    const int tiles = (int)((cols + KV8_COLS - 1) / KV8_COLS), s = kv8_few_plan(c, n, tiles, max_ctx).splits;
     return s == 1 ? 0 : (size_t)n * c->heads * tiles * s * KV8_COLS * (c->head_dim + 4) * sizeof(float);
 }
 
@@ -867,19 +955,27 @@ extern "C" int qm_kv8_attention(const qm_kv8_t *c, void *out, const void *q, siz
 #undef MANY
         return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
     }
-    const int tiles = (int)((cols + KV8_COLS - 1) / KV8_COLS), ns = kv8_splits(c, n, tiles, max_ctx);
+    const int tiles = (int)((cols + KV8_COLS - 1) / KV8_COLS);
+    const kv8_plan plan = kv8_few_plan(c, n, tiles, max_ctx);
+    const int ns = plan.splits;
     if (ns > 1 && (!work || !aligned16(work))) return QH_EINVAL;
     if (work_bytes < qm_kv8_attention_work(c, q_heads, n, max_rows, max_ctx)) return QH_ETOOBIG;
     if (!stream()) return QH_ESTATE;
     const dim3 grid(ns, c->heads * tiles, n);
-#define FEW(F, D_, BF_)                                                                                             \
-    hipLaunchKernelGGL((k_kv8_few<F, D_, BF_>), grid, dim3(WAVE *KV8_NW), 0, stream(), *c, out, q, ldo, ldq, row, pos, \
+#define FEW_W(F, D_, BF_, W_)                                                                                          \
+    hipLaunchKernelGGL((k_kv8_few<F, D_, BF_, W_>), grid, dim3(WAVE *W_), 0, stream(), *c, out, q, ldo, ldq, row, pos, \
                        rows, max_rows, G, f, (float *)work)
+#define FEW(F, D_, BF_)                             \
+    do {                                            \
+        if (plan.waves == 4) FEW_W(F, D_, BF_, 4);  \
+        else FEW_W(F, D_, BF_, 8);                  \
+    } while (0)
     KV8_SWITCH(FEW);
 #undef FEW
+#undef FEW_W
     if (hipGetLastError() != hipSuccess) return QH_ELAUNCH;
     if (ns > 1) {
-        const int per = NTH / (c->head_dim / 4);
+        const int per = NTH / WAVE;
         const dim3 mg((unsigned)((cols + per - 1) / per), c->heads, n);
 #define MERGE(D_, BF_)                                                                                               \
     hipLaunchKernelGGL((k_kv8_merge<D_, BF_>), mg, dim3(NTH), 0, stream(), *c, out, ldo, row, pos, rows, max_rows, G, \

@@ -234,6 +234,23 @@ def test_attention_of_several_rows(fmt, dim, block, heads, group, bf16, counts, 
     c.check_attention(rng, pos, counts, group, bf16)
 
 
+@pytest.mark.parametrize("fmt,dim,block,heads,group,bf16,counts", [
+    ("e4m3", 128, 32, 1, 2, False, [1, 1, 1, 1]), ("int8", 128, 64, 1, 8, True, [1, 1, 1, 1]),
+    ("e4m3", 64, 16, 2, 1, True, [1, 1, 0, 1]), ("int8", 64, 32, 1, 3, False, [1, 1, 1, 1]),
+    ("e4m3", 128, 32, 1, 2, False, [17, 1, 30, 2]), ("int8", 128, 16, 1, 4, True, [3, 16, 1, 0])])
+def test_attention_split_over_blocks(fmt, dim, block, heads, group, bf16, counts):
+    """long and short contexts in one call, the keys of each split over blocks and merged"""
+    print(f"splits {fmt} dim {dim} block {block} group {group} bf16 {bf16} {counts}", flush=True)
+    rng = np.random.default_rng([dim, block, group])
+    before = [3000, 1535, 64, 2047]
+    c = Cache(rng, fmt, heads, dim, block, 4, 3072 // block)
+    c.append(rng, before, bf16)
+    pos = c.append(rng, counts, bf16)
+    for ctx in (3072, 1700):
+        assert abi.kv8_attention_work(c.c, heads * group, 4, max(counts), ctx) > 0
+        c.check_attention(rng, pos, counts, group, bf16, max_ctx=ctx)
+
+
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("counts", [[1, 1], [40, 70]])
 def test_a_row_that_is_not_finite_stays_alone(bf16, counts):
@@ -310,20 +327,20 @@ def test_steps_replayed_from_a_graph(lib):
     """append and attention of a decode step recorded once, replayed with eager calls of other sizes between: every
     replay gives the eager calls' bits"""
     rng = np.random.default_rng(11)
-    c = Cache(rng, "e4m3", 2, 128, 32, 3, 16)
-    c.append(rng, [200, 31, 400], False)
+    c = Cache(rng, "e4m3", 2, 128, 32, 3, 80)
+    c.append(rng, [2000, 31, 400], False)
     kv = rng.standard_normal((2, 3, 2, 128)).astype(np.float32)
     q = rng.standard_normal((3, 4, 128)).astype(np.float32)
     up = abi.DeviceBuffer.from_array
-    kd, vd, qd, pd = up(kv[0]), up(kv[1]), up(q), up(np.array([200, 31, 400], np.int32))
+    kd, vd, qd, pd = up(kv[0]), up(kv[1]), up(q), up(np.array([2000, 31, 400], np.int32))
     od = up(np.zeros(q.shape, np.float32))
-    work = abi.kv8_attention_work(c.c, 4, 3, 1, 512)
-    assert work > 0
+    work = abi.kv8_attention_work(c.c, 4, 3, 1, 2560)
+    assert work > 0                                    # its keys are split over blocks
     wd = abi.DeviceBuffer(work)
 
     def step():
         abi.kv8_append_dev(c.c, kd.ptr, vd.ptr, 256, 256, False, None, pd.ptr, 3, 3, 1)
-        abi.kv8_attention_dev(c.c, od.ptr, qd.ptr, 512, 512, False, 4, None, pd.ptr, 3, 3, 1, 512, 0.09, wd.ptr, work)
+        abi.kv8_attention_dev(c.c, od.ptr, qd.ptr, 512, 512, False, 4, None, pd.ptr, 3, 3, 1, 2560, 0.09, wd.ptr, work)
 
     step()
     abi.sync()

@@ -76,7 +76,7 @@ int qwen3_hip_kv8_append_dev(const qwen3_hip_kv8 *cache, const void *k_d, const 
  * pos_d[i] + r, over positions 0 .. pos_d[i] + r of the cache, to which the
  * entry's rows have been appended (qwen3_hip_kv8_append_dev with the same
  * row_d and pos_d):
- *   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j)
+ *   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j),  scale > 0
  * q_d and out_d: [q_heads][head_dim] per row, both fp32 or, where bf16 is set,
  * both bf16; query head h reads kv head h / (q_heads / kv_heads), at most 64
  * query heads a kv head.  fp32 rows are computed with fp32 accuracy

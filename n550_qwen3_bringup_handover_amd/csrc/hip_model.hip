@@ -16,6 +16,7 @@
 //   rope tables   [max_seq][64] cos and sin, built on the host with the
 //                 reference formula (ops_scalar.c:21-35)
 #include <hip/hip_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "hip_shim.h"

@@ -234,11 +234,22 @@ __device__ __forceinline__ bf16x8 kv8_bf16(uint32_t a, uint32_t b) {      // eig
         r.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
         r.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
     } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            r.v[i] = (__bf16)(float)(int8_t)(a >> (8 * i));
-            r.v[4 + i] = (__bf16)(float)(int8_t)(b >> (8 * i));
-        }
+        // three instructions for two codes, and two registers halfway: left to
+        // the scheduler the fp32 values of many codes are made first, and spill
+#define KV8_I8(R, X, B0, B1)                                                                                    \
+    do {                                                                                                        \
+        float t0, t1;                                                                                           \
+        asm("v_cvt_f32_i32_sdwa %1, sext(%3) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:" B0 "\n\t"           \
+            "v_cvt_f32_i32_sdwa %2, sext(%3) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:" B1 "\n\t"           \
+            "v_cvt_pk_bf16_f32 %0, %1, %2"                                                                      \
+            : "=v"(R), "=&v"(t0), "=&v"(t1)                                                                     \
+            : "v"(X));                                                                                          \
+    } while (0)
+        KV8_I8(r.p[0], a, "BYTE_0", "BYTE_1");
+        KV8_I8(r.p[1], a, "BYTE_2", "BYTE_3");
+        KV8_I8(r.p[2], b, "BYTE_0", "BYTE_1");
+        KV8_I8(r.p[3], b, "BYTE_2", "BYTE_3");
+#undef KV8_I8
     }
     return r.v;
 }
@@ -300,14 +311,14 @@ __device__ __forceinline__ float col_sum(float v) {
 // 1 / sum of weights; a row of which nothing was left (pages that are none) is 0
 __device__ __forceinline__ float kv8_inverse(float den) { return den == 0.0f ? 0.0f : 1.0f / den; }
 
-// the running softmax of one column tile: scores s (in units of log2 after the
-// factor f, masked entries -inf) become weights; returns what the sums so far
-// are to be multiplied by
-__device__ __forceinline__ float kv8_softmax(f32x4 (&s)[4], float &m, float &l) {
+// the running softmax of one column tile: raw products s (masked ones -inf), of
+// which k > 0 times each is the score in units of log2, become weights; returns
+// what the sums so far are to be multiplied by
+__device__ __forceinline__ float kv8_softmax(f32x4 (&s)[4], float k, float &m, float &l) {
     float mx = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 4; t++) mx = fmaxf(mx, fmaxf(fmaxf(s[t].x, s[t].y), fmaxf(s[t].z, s[t].w)));
-    const float nm = fmaxf(m, col_max(mx));
+    const float nm = fmaxf(m, col_max(mx * k));
     const float ref = nm == -INFINITY ? 0.0f : nm;       // nothing seen yet: every weight is 0
     const float r = __builtin_amdgcn_exp2f(m - ref);
     m = nm;
@@ -316,32 +327,42 @@ __device__ __forceinline__ float kv8_softmax(f32x4 (&s)[4], float &m, float &l) 
     for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref);
+            // the product rounded as the maximum's was: at 1e31 a fused one is off by 1e24
+            s[t][i] = __builtin_amdgcn_exp2f(mul_add(s[t][i], k, -ref));
             sum += s[t][i];
         }
     l = l * r + sum;
     return r;
 }
 
-// ---- few columns: keys split over waves and blocks --------------------------
-// Block (split, head + heads * column tile, entry): its NWV waves take the steps
-// of 64 keys in turn, wave w of split y steps NWV y + w, + NWV nsplit, ...; each
-// operand goes from memory straight into its MFMA's registers (K of the next
-// step is in flight during this step's V product).  The tail is one more step.
-// The waves' sums meet in LDS; with several splits each block leaves a partial
-// {m, l, -, -, o[D]} per column for k_kv8_merge.
+// A block has CG x KG waves on COLS = 16 CT CG columns of one kv head: wave
+// (cg, kg) takes 16 CT of the columns and, of the steps of 64 keys, in turn
+// with the other groups of keys and the other splits, its own; each operand
+// goes from memory straight into its MFMA's registers, converted on the way
+// (K of the next step is in flight during this step's V product), so that
+// waves never wait for one another until the groups' sums meet in LDS at the
+// end.  The unfinished block is one more step.  With several splits (blocks on
+// the same columns) each block leaves a partial {m, l, -, -, o[D]} per column
+// for k_kv8_merge.
+//   few columns (decode, a few rows): CT = CG = 1, the keys split over four or
+//   eight waves and over blocks
+//   many (a prompt): two groups of keys, two of columns; the column tiles with
+//   the longest contexts first, or, where all blocks fit the CUs at once, so
+//   that the two blocks of a CU are a long and a short one
 #define KV8_COLS 16
 #define KV8_MAX_SPLITS 32
-template <int FMT, int D, bool BF, int NWV>
-__global__ __launch_bounds__(WAVE *NWV, 2) void k_kv8_few(qm_kv8_t c, void *__restrict__ out,
-                                                             const void *__restrict__ q, size_t ldo, size_t ldq,
-                                                             const int *__restrict__ row, const int *__restrict__ pos,
-                                                             int rows, int max_rows, int G, float f,
-                                                             float *__restrict__ part) {
-    constexpr int NP = BF ? 1 : 3, NW = BF ? 2 : 3;        // pieces of q, and of a weight
-    constexpr int KS = D / 32, DT = D / 16, LD = D + 4;
-    const int e = blockIdx.z, head = blockIdx.y % c.heads, ct = blockIdx.y / c.heads;
+enum { KV8_AS_IS, KV8_LONG_FIRST, KV8_PAIRED };
+template <int FMT, int D, bool BF, int CT, int CG, int KG>
+__global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void *__restrict__ out,
+                                                               const void *__restrict__ q, size_t ldo, size_t ldq,
+                                                               const int *__restrict__ row, const int *__restrict__ pos,
+                                                               int rows, int max_rows, int G, float f, int nsplit,
+                                                               int order, float *__restrict__ part) {
+    constexpr int NP = BF ? 1 : 3, NW = !BF ? 3 : CT == 1 ? 2 : 1;         // pieces of q, and of a weight
+    constexpr int KS = D / 32, DT = D / 16, LD = D + 4, COLS = 16 * CT * CG, NT = WAVE * CG * KG;
+    const int e = blockIdx.y, split = blockIdx.x % nsplit, x = blockIdx.x / nsplit, head = x % c.heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int cg = wave % CG, kg = wave / CG;
     const int cl = lane & 15, h = lane >> 4;
     const int gk = (lane >> 2) & 3;                                        // the group of 16 keys its K row lies in
     const int B = c.block, lb = __builtin_ctz(B);
@@ -349,20 +370,32 @@ __global__ __launch_bounds__(WAVE *NWV, 2) void k_kv8_few(qm_kv8_t c, void *__re
     // table entry of a key, and the page it stands for, -1 where there is none.
     // The first step's are read before anything says how long the sequence is
     auto entry_of = [&](int key) { return (key >> lb) < c.max_blocks ? table[key >> lb] : -1; };
-    int s = NWV * blockIdx.x + wave;
+    int s = KG * split + kg;
     int pk = entry_of(64 * s + 16 * gk), pv = entry_of(64 * s + 16 * h);
     kv8_entry t;
     if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
-    const int col0 = ct * KV8_COLS, ncol = t.cnt * G;
-    if (col0 >= ncol) return;
+    const int ncol = t.cnt * G, tiles = (ncol + COLS - 1) / COLS, at_ = x / c.heads;
+    if (at_ >= tiles) return;
+    const int tile = order == KV8_AS_IS ? at_ : order == KV8_LONG_FIRST || at_ < (tiles + 1) / 2 ? tiles - 1 - at_
+                                                                                                 : at_ - (tiles + 1) / 2;
+    const int col0 = tile * COLS, w0 = col0 + 16 * CT * cg;                // the block's and the wave's first column
     const int full = (t.pos + t.cnt) >> lb << lb;                          // keys in finished blocks
-    const int kend = t.pos + min(t.cnt - 1, (col0 + KV8_COLS - 1) / G) + 1;   // keys the block's last column sees
-    const int ns = (min(full, kend) + 63) >> 6, stride = NWV * gridDim.x;
+    const int wlast = w0 < ncol ? t.pos + min(t.cnt - 1, (w0 + 16 * CT - 1) / G) : -1;   // the last key the wave sees
+    const int wfirst = w0 < ncol ? t.pos + w0 / G : -1;                    // and the last that all its columns see
+    const int ns = (min(full, wlast + 1) + 63) >> 6, stride = KG * nsplit;
 
-    const int col = col0 + cl;
-    const bool in = col < ncol;
-    const int qr = in ? col / G : 0, qg = in ? col % G : 0;
-    const int last = in ? t.pos + qr : -1;                                 // the column's last key
+    int last[CT];                                                          // the column's last key
+    kv8_row<BF> qr_[CT][KS];
+#pragma unroll
+    for (int n = 0; n < CT; n++) {
+        const int col = w0 + 16 * n + cl;
+        const bool in = col < ncol;
+        const int qr = in ? col / G : 0, qg = in ? col % G : 0;
+        last[n] = in ? t.pos + qr : -1;
+#pragma unroll
+        for (int j = 0; j < KS; j++)
+            qr_[n][j].load(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + (D / 4) * h + 8 * j, in);
+    }
     auto page_of = [&](int key, int p) { return key < full && (unsigned)p < (unsigned)c.n_page ? p : -1; };
     uint4 kk[4][D / 64], vv[DT];
     auto load_k = [&](int s, int p) {
@@ -380,79 +413,110 @@ __global__ __launch_bounds__(WAVE *NWV, 2) void k_kv8_few(qm_kv8_t c, void *__re
 #pragma unroll
         for (int i = 0; i < DT; i++) vv[i] = p >= 0 ? *(const uint4 *)(b + (size_t)16 * i * B) : uint4{};
     };
-
-    float m = -INFINITY, l = 0.0f;
-    f32x4 o[DT], s4[4];
-#pragma unroll
-    for (int i = 0; i < DT; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // weights p (times the page's V scale) as B operands of key half s2
-    auto weights = [&](int s2, float vs, bf16x8 (&pf)[NW]) {
-        const f32x4 a = s4[2 * s2] * vs, b = s4[2 * s2 + 1] * vs;
-        kv8_pieces<NW>(f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, pf);
-    };
-
-    kv8_row<BF> qr_[KS];
-#pragma unroll
-    for (int j = 0; j < KS; j++)
-        qr_[j].load(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + (D / 4) * h + 8 * j, in);
     if (s < ns) {
         pk = page_of(64 * s + 16 * gk, pk);
         pv = page_of(64 * s + 16 * h, pv);
         load_k(s, pk);
     }
-    bf16x8 qf[KS][NP];
+    bf16x8 qf[CT][KS][NP];
+    float m[CT], l[CT];
+    f32x4 o[CT][DT], s4[CT][4];
 #pragma unroll
-    for (int j = 0; j < KS; j++) qr_[j].pieces(qf[j]);
+    for (int n = 0; n < CT; n++) {
+#pragma unroll
+        for (int j = 0; j < KS; j++) qr_[n][j].pieces(qf[n][j]);
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DT; i++) o[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // one tile of 16 keys' products
+    auto score = [&](int i, const bf16x8 (&kf)[KS]) {
+#pragma unroll
+        for (int n = 0; n < CT; n++) {
+            s4[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < KS; j++)
+#pragma unroll
+                for (int u = 0; u < NP; u++) s4[n][i] = kv8_mma(kf[j], qf[n][j][u], s4[n][i]);
+        }
+    };
+    auto softmax = [&](float k) {
+#pragma unroll
+        for (int n = 0; n < CT; n++) {
+            const float r = kv8_softmax(s4[n], k, m[n], l[n]);
+            if (__any(r != 1.0f)) {                                        // a maximum grew
+#pragma unroll
+                for (int i = 0; i < DT; i++) o[n][i] *= r;
+            }
+        }
+    };
+    // weights (times the page's V scale) as B operands of key half s2
+    auto weights = [&](int s2, float vs, bf16x8 (&pf)[CT][NW]) {
+#pragma unroll
+        for (int n = 0; n < CT; n++) {
+            const f32x4 a = s4[n][2 * s2] * vs, b = s4[n][2 * s2 + 1] * vs;
+            kv8_pieces<NW>(f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, pf[n]);
+        }
+    };
+    auto add_v = [&](int i, bf16x8 vf, const bf16x8 (&pf)[CT][NW]) {
+#pragma unroll
+        for (int n = 0; n < CT; n++)
+#pragma unroll
+            for (int u = 0; u < NW; u++) o[n][i] = kv8_mma(vf, pf[n][u], o[n][i]);
+    };
+
     for (; s < ns; s += stride) {
         load_v(s, pv);
-        const float ks = pv >= 0 ? c.k_scale[(size_t)pv * c.heads + head] * f : 0.0f;
+        // (a scale of 0, a block of zeros, would make 0 x -inf of a masked key)
+        const float ks = pv >= 0 ? fmaxf(c.k_scale[(size_t)pv * c.heads + head] * f, FLT_MIN) : 1.0f;
         const float vs = pv >= 0 ? c.v_scale[(size_t)pv * c.heads + head] : 0.0f;
-        const int lim = pv >= 0 ? last - (64 * s + 16 * h) : -1;           // the group's last key that is seen
         const int nx = s + stride;
         int pkn = -1, pvn = -1;
         if (nx < ns) {
-            const int kk_ = 64 * nx + 16 * gk, kv_ = 64 * nx + 16 * h;
-            pkn = page_of(kk_, entry_of(kk_));
-            pvn = page_of(kv_, entry_of(kv_));
+            const int ka = 64 * nx + 16 * gk, va = 64 * nx + 16 * h;
+            pkn = page_of(ka, entry_of(ka));
+            pvn = page_of(va, entry_of(va));
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+            bf16x8 kf[KS];
 #pragma unroll
             for (int j = 0; j < KS; j++) {
                 const uint4 w = kk[i][j >> 1];
-                const bf16x8 kf = (j & 1) ? kv8_bf16<FMT>(w.z, w.w) : kv8_bf16<FMT>(w.x, w.y);
-#pragma unroll
-                for (int n = 0; n < NP; n++) a = kv8_mma(kf, qf[j][n], a);
+                kf[j] = (j & 1) ? kv8_bf16<FMT>(w.z, w.w) : kv8_bf16<FMT>(w.x, w.y);
             }
-#pragma unroll
-            for (int r = 0; r < 4; r++) s4[i][r] = 4 * i + r <= lim ? a[r] * ks : -INFINITY;
-            if constexpr (FMT == QM_KV8_INT8) __builtin_amdgcn_sched_barrier(0);   // fp32 halfway: one tile's at a time
+            score(i, kf);
         }
         if (nx < ns) load_k(nx, pkn);
         __builtin_amdgcn_sched_barrier(0);                // V's codes are not converted before they are needed
-        const float rs = kv8_softmax(s4, m, l);
+        if (64 * s + 63 > wfirst || 64 * s + 64 > full || __any(pv < 0)) {
 #pragma unroll
-        for (int i = 0; i < DT; i++) o[i] *= rs;
+            for (int n = 0; n < CT; n++) {
+                const int lim = pv >= 0 ? last[n] - (64 * s + 16 * h) : -1;        // the group's last key that is seen
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s4[n][i][r] = 4 * i + r <= lim ? s4[n][i][r] : -INFINITY;
+            }
+        }
+        softmax(ks);
 #pragma unroll
         for (int s2 = 0; s2 < 2; s2++) {
-            bf16x8 pf[NW];
+            bf16x8 pf[CT][NW];
             weights(s2, vs, pf);
 #pragma unroll
-            for (int i = 0; i < DT; i++) {
-                const bf16x8 vf = s2 ? kv8_bf16<FMT>(vv[i].z, vv[i].w) : kv8_bf16<FMT>(vv[i].x, vv[i].y);
-#pragma unroll
-                for (int n = 0; n < NW; n++) o[i] = kv8_mma(vf, pf[n], o[i]);
-            }
+            for (int i = 0; i < DT; i++)
+                add_v(i, s2 ? kv8_bf16<FMT>(vv[i].z, vv[i].w) : kv8_bf16<FMT>(vv[i].x, vv[i].y), pf);
             __builtin_amdgcn_sched_barrier(0);
         }
         pv = pvn;
     }
 
-    // the unfinished block, as step ns of the turn.  Its rows are read whether
-    // they are there or not (within the tail): scores of keys that are not are
-    // masked, and V is cleared where they lie, as it may hold anything
-    if (kend > full && ns % stride == NWV * (int)blockIdx.x + wave) {
+    // the unfinished block, as one more step of the turn.  Its rows are read
+    // whether they are there or not (within the tail): scores of keys that are
+    // not are masked, and V is cleared where they lie, as it may hold anything
+    if (wlast >= full && (full + 63) / 64 % stride == KG * split + kg) {
         const int nt = t.pos + t.cnt - full;                               // rows it holds, < B <= 64
         const __bf16 *kt = (const __bf16 *)c.k_tail + ((size_t)e * c.heads + head) * ((size_t)B * D);
         const __bf16 *vt = (const __bf16 *)c.v_tail + ((size_t)e * c.heads + head) * ((size_t)B * D);
@@ -469,23 +533,19 @@ __global__ __launch_bounds__(WAVE *NWV, 2) void k_kv8_few(qm_kv8_t c, void *__re
                 tv[s2][i] = *(const bf16x8 *)(vt + (size_t)(16 * i + cl) * B + min(16 * h + 8 * s2, B - 8));
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+            score(i, tk[i]);
 #pragma unroll
-            for (int j = 0; j < KS; j++)
+            for (int n = 0; n < CT; n++)
 #pragma unroll
-                for (int n = 0; n < NP; n++) a = kv8_mma(tk[i][j], qf[j][n], a);
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int k = 16 * h + 4 * i + r;
-                s4[i][r] = k < nt && full + k <= last ? a[r] * f : -INFINITY;
-            }
+                for (int r = 0; r < 4; r++) {
+                    const int k = 16 * h + 4 * i + r;
+                    s4[n][i][r] = k < nt && full + k <= last[n] ? s4[n][i][r] : -INFINITY;
+                }
         }
-        const float rs = kv8_softmax(s4, m, l);
-#pragma unroll
-        for (int i = 0; i < DT; i++) o[i] *= rs;
+        softmax(f);
 #pragma unroll
         for (int s2 = 0; s2 < 2; s2++) {
-            bf16x8 pf[NW];
+            bf16x8 pf[CT][NW];
             weights(s2, 1.0f, pf);
             const int there = nt - (16 * h + 8 * s2);
             // 32 bits, two keys, at a time
@@ -494,53 +554,54 @@ __global__ __launch_bounds__(WAVE *NWV, 2) void k_kv8_few(qm_kv8_t c, void *__re
 #pragma unroll
             for (int n = 0; n < 4; n++) mask[n] = there > 2 * n + 1 ? ~0u : there == 2 * n + 1 ? 0xFFFFu : 0u;
 #pragma unroll
-            for (int i = 0; i < DT; i++) {
-                const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u4, tv[s2][i]) & mask);
-#pragma unroll
-                for (int n = 0; n < NW; n++) o[i] = kv8_mma(vf, pf[n], o[i]);
-            }
+            for (int i = 0; i < DT; i++)
+                add_v(i, __builtin_bit_cast(bf16x8, __builtin_bit_cast(u4, tv[s2][i]) & mask), pf);
         }
     }
 
-    // merge the waves
-    __shared__ __align__(16) float so[NWV][KV8_COLS][LD];
-    __shared__ float sm[NWV][KV8_COLS], sl[NWV][KV8_COLS];
-    l = col_sum(l);
+    // the groups' sums, and the splits' partials
+    __shared__ __align__(16) float so[KG][COLS][LD];
+    __shared__ float sm[KG][COLS], sl[KG][COLS];
 #pragma unroll
-    for (int i = 0; i < DT; i++) *(f32x4 *)&so[wave][cl][16 * i + 4 * h] = o[i];
-    if (h == 0) { sm[wave][cl] = m; sl[wave][cl] = l; }
+    for (int n = 0; n < CT; n++) {
+        const int cc = 16 * (CT * cg + n) + cl;
+        l[n] = col_sum(l[n]);
+#pragma unroll
+        for (int i = 0; i < DT; i++) *(f32x4 *)&so[kg][cc][16 * i + 4 * h] = o[n][i];
+        if (h == 0) { sm[kg][cc] = m[n]; sl[kg][cc] = l[n]; }
+    }
     __syncthreads();
     constexpr int TPC = D / 4;                            // threads of a column
-    for (int i = tid; i < KV8_COLS * TPC; i += WAVE * NWV) {
-        const int cc = i / TPC, d = i % TPC * 4, cg = col0 + cc;
-        if (cg >= ncol) continue;
+    for (int i = tid; i < COLS * TPC; i += NT) {
+        const int cc = i / TPC, d = i % TPC * 4, col = col0 + cc;
+        if (col >= ncol) continue;
         float mx = sm[0][cc];
 #pragma unroll
-        for (int w = 1; w < NWV; w++) mx = fmaxf(mx, sm[w][cc]);
+        for (int g = 1; g < KG; g++) mx = fmaxf(mx, sm[g][cc]);
         const float ref = mx == -INFINITY ? 0.0f : mx;
         float den = 0.0f;
         f32x4 num = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < NWV; w++) {
+        for (int g = 0; g < KG; g++) {
             // a wave without keys weighs 0 (its sums are 0); one whose scores were all NaN keeps its NaN
-            const float g = __builtin_amdgcn_exp2f(sm[w][cc] - ref);
-            den += g * sl[w][cc];
-            num += *(const f32x4 *)&so[w][cc][d] * g;
+            const float w = __builtin_amdgcn_exp2f(sm[g][cc] - ref);
+            den += w * sl[g][cc];
+            num += *(const f32x4 *)&so[g][cc][d] * w;
         }
-        if (gridDim.x == 1) {
+        if (nsplit == 1) {
             num *= kv8_inverse(den);
-            const size_t at = (size_t)(t.r0 + cg / G) * ldo + (size_t)(head * G + cg % G) * D + d;
+            const size_t at = (size_t)(t.r0 + col / G) * ldo + (size_t)(head * G + col % G) * D + d;
             if constexpr (BF) *(uint2 *)((uint16_t *)out + at) = pack4(num);
             else *(f32x4 *)((float *)out + at) = num;
         } else {
-            float *p = part + ((((size_t)e * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * KV8_COLS + cc) * LD;
+            float *p = part + (((size_t)e * gridDim.x + blockIdx.x) * COLS + cc) * LD;
             *(f32x4 *)(p + 4 + d) = num;
             if (d == 0) { p[0] = mx; p[1] = den; }
         }
     }
 }
 
-// the splits' partials of k_kv8_few merged: a wave a column, its D / 4 lanes
+// the splits' partials of k_kv8_attend merged: a wave a column, its D / 4 lanes
 // twice (D = 128) or four times (64) over the splits, so that all are read at
 // once
 template <int D, bool BF>
@@ -598,219 +659,6 @@ __global__ __launch_bounds__(NTH) void k_kv8_merge(qm_kv8_t c, void *__restrict_
     const size_t at = (size_t)(t.r0 + col / G) * ldo + (size_t)(head * G + col % G) * D + d;
     if constexpr (BF) *(uint2 *)((uint16_t *)out + at) = pack4(num);
     else *(f32x4 *)((float *)out + at) = num;
-}
-
-// ---- many columns: a prompt's rows ------------------------------------------
-// Block b: kv head b % heads (each XCD serves a head's pages from its own L2
-// where there are eight), the column tiles with the longest contexts first.
-// Four waves of 32 columns share each step's 64 keys in LDS, converted to bf16
-// once and laid out as the MFMAs' operands (16 bytes a lane, conflict-free);
-// the next step's codes are in flight while this one is computed.
-#define KV8_MANY 128                   // columns of a block
-template <int FMT, int D, bool BF>
-__global__ __launch_bounds__(NTH, 2) void k_kv8_many(qm_kv8_t c, void *__restrict__ out, const void *__restrict__ q,
-                                                    size_t ldo, size_t ldq, const int *__restrict__ row,
-                                                    const int *__restrict__ pos, int rows, int max_rows, int G, float f) {
-    constexpr int NP = BF ? 1 : 3, KS = D / 32, DT = D / 16, CT = 2;
-    constexpr int UN = 64 * D / 16 / NTH;                 // 16-code units of K, and of V, a thread stages
-    const int e = blockIdx.y, head = blockIdx.x % c.heads;
-    kv8_entry t;
-    if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
-    const int ncol = t.cnt * G, tiles = (ncol + KV8_MANY - 1) / KV8_MANY;
-    const int tile = tiles - 1 - (int)(blockIdx.x / c.heads);
-    if (tile < 0) return;
-    const int col0 = tile * KV8_MANY;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int cl = lane & 15, h = lane >> 4;
-    const int B = c.block, lb = __builtin_ctz(B);
-    const int end = t.pos + t.cnt, full = end >> lb << lb;
-    const int kend = t.pos + min(t.cnt - 1, (col0 + KV8_MANY - 1) / G) + 1;
-    const int ns = (kend + 63) >> 6;
-
-    __shared__ __align__(16) bf16x8 lk[2][4 * KS * 64], lv[2][2 * DT * 64];
-
-    // the wave's columns
-    const int w0 = col0 + wave * 16 * CT;
-    int last[CT];
-    bf16x8 qf[CT][KS][NP];
-#pragma unroll
-    for (int n = 0; n < CT; n++) {
-        const int col = w0 + 16 * n + cl;
-        const bool in = col < ncol;
-        const int qr = in ? col / G : 0, qg = in ? col % G : 0;
-        last[n] = in ? t.pos + qr : -1;
-#pragma unroll
-        for (int j = 0; j < KS; j++) {
-            kv8_row<BF> x;
-            x.load(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + 32 * j + 8 * h, in);
-            x.pieces(qf[n][j]);
-        }
-    }
-    const int wfirst = w0 < ncol ? t.pos + w0 / G : -1;                    // keys all the wave's columns see, and any
-    const int wlast = w0 < ncol ? t.pos + min(t.cnt - 1, (w0 + 16 * CT - 1) / G) : -1;
-    const bool whole = w0 + 16 * CT <= ncol;
-
-    const int *table = c.table + (size_t)e * c.max_blocks;
-    auto page_of = [&](int key) {
-        int p = -1;
-        if (key < full) p = table[key >> lb];
-        return (unsigned)p < (unsigned)c.n_page ? p : -1;
-    };
-    // unit u of a step: K 16 dims of key u / (D / 16); V 16 keys of a dim, in
-    // the order they lie in their pages
-    const int sub = B / 16, lsub = lb - 4;
-    auto v_group = [&](int u) { return (u >> lsub) / D * sub + (u & (sub - 1)); };
-    auto v_dim = [&](int u) { return (u >> lsub) & (D - 1); };
-    uint4 ku[UN], vu[UN];
-    auto load = [&](int s) {
-#pragma unroll
-        for (int i = 0; i < UN; i++) {
-            const int u = tid + NTH * i, key = 64 * s + u / (D / 16);
-            const int p = page_of(key);
-            ku[i] = p >= 0 ? *(const uint4 *)(c.k + (((size_t)p * c.heads + head) * B + (key & (B - 1))) * D + u % (D / 16) * 16)
-                           : uint4{};
-            const int kv = 64 * s + 16 * v_group(u), pv = page_of(kv);
-            vu[i] = pv >= 0 ? *(const uint4 *)(c.v + (((size_t)pv * c.heads + head) * D + v_dim(u)) * B + (kv & (B - 1)))
-                            : uint4{};
-        }
-    };
-    auto put_k = [&](int b, int u, bf16x8 x, bf16x8 y) {
-        const int key = u / (D / 16), ds = u % (D / 16);
-        const int at = ((((key >> 2) & 3) * KS + (ds >> 1)) * 64) + (ds & 1) * 32 + ((key >> 4) << 2 | (key & 3));
-        lk[b][at] = x;
-        lk[b][at + 16] = y;
-    };
-    auto put_v = [&](int b, int u, bf16x8 x, bf16x8 y) {
-        const int d = v_dim(u), at = (d >> 4) * 64 + v_group(u) * 16 + (d & 15);
-        lv[b][at] = x;
-        lv[b][DT * 64 + at] = y;
-    };
-    auto put = [&](int b, int s) {
-#pragma unroll
-        for (int i = 0; i < UN; i++) {
-            const int u = tid + NTH * i;
-            put_k(b, u, kv8_bf16<FMT>(ku[i].x, ku[i].y), kv8_bf16<FMT>(ku[i].z, ku[i].w));
-            put_v(b, u, kv8_bf16<FMT>(vu[i].x, vu[i].y), kv8_bf16<FMT>(vu[i].z, vu[i].w));
-        }
-        if (64 * s + 64 <= full) return;
-        // the step reaches into the unfinished block: its groups come from the tail
-        const __bf16 *kt = (const __bf16 *)c.k_tail + ((size_t)e * c.heads + head) * ((size_t)B * D);
-        const __bf16 *vt = (const __bf16 *)c.v_tail + ((size_t)e * c.heads + head) * ((size_t)B * D);
-        for (int i = 0; i < UN; i++) {
-            const int u = tid + NTH * i, key = 64 * s + u / (D / 16), ds = u % (D / 16);
-            if (key >= full && key < end) {
-                const bf16x8 *p = (const bf16x8 *)(kt + (size_t)(key - full) * D + ds * 16);
-                put_k(b, u, p[0], p[1]);
-            }
-            const int kv = 64 * s + 16 * v_group(u);
-            if (kv >= full && kv < end) {
-                const bf16x8 *p = (const bf16x8 *)(vt + (size_t)v_dim(u) * B + (kv - full));
-                bf16x8 x = p[0], y = p[1];
-#pragma unroll
-                for (int n = 0; n < 8; n++) {             // behind the last row: anything
-                    x[n] = kv + n < end ? x[n] : (__bf16)0.0f;
-                    y[n] = kv + 8 + n < end ? y[n] : (__bf16)0.0f;
-                }
-                put_v(b, u, x, y);
-            }
-        }
-    };
-    float ksn = 0.0f, vsn = 0.0f;                          // the next step's scales of this lane's 16 keys
-    int okn = 0;
-    auto scales = [&](int s) {
-        const int key = 64 * s + 16 * h, p = page_of(key);
-        okn = p >= 0 || (key >= full && key < end);
-        ksn = p >= 0 ? c.k_scale[(size_t)p * c.heads + head] * f : f;
-        vsn = p >= 0 ? c.v_scale[(size_t)p * c.heads + head] : 1.0f;
-    };
-
-    float m[CT], l[CT];
-    f32x4 o[DT][CT];
-#pragma unroll
-    for (int n = 0; n < CT; n++) {
-        m[n] = -INFINITY;
-        l[n] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < DT; i++) o[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    load(0);
-    scales(0);
-    for (int s = 0; s < ns; s++) {
-        const int b = s & 1;
-        put(b, s);
-        const float ks = ksn, vs = vsn;
-        const int ok = okn;
-        __syncthreads();                                  // this buffer is full; the other one's readers are done
-        if (s + 1 < ns) {
-            load(s + 1);
-            scales(s + 1);
-        }
-        if (64 * s > wlast) continue;                     // uniform per wave: nothing of it is seen
-        f32x4 s4[CT][4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            f32x4 a[CT];
-#pragma unroll
-            for (int n = 0; n < CT; n++) a[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < KS; j++) {
-                const bf16x8 kf = lk[b][(i * KS + j) * 64 + lane];
-#pragma unroll
-                for (int n = 0; n < CT; n++)
-#pragma unroll
-                    for (int x = 0; x < NP; x++) a[n] = kv8_mma(kf, qf[n][j][x], a[n]);
-            }
-#pragma unroll
-            for (int n = 0; n < CT; n++) s4[n][i] = a[n] * ks;
-        }
-        const bool clear = whole && 64 * s + 63 <= wfirst && __all(ok);
-        if (!clear) {
-#pragma unroll
-            for (int n = 0; n < CT; n++) {
-                const int lim = ok ? last[n] - (64 * s + 16 * h) : -1;
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) s4[n][i][r] = 4 * i + r <= lim ? s4[n][i][r] : -INFINITY;
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < CT; n++) {
-            const float rs = kv8_softmax(s4[n], m[n], l[n]);
-#pragma unroll
-            for (int i = 0; i < DT; i++) o[i][n] *= rs;
-        }
-#pragma unroll
-        for (int s2 = 0; s2 < 2; s2++) {
-            bf16x8 pf[CT][NP];
-#pragma unroll
-            for (int n = 0; n < CT; n++) {
-                const f32x4 x = s4[n][2 * s2] * vs, y = s4[n][2 * s2 + 1] * vs;
-                kv8_pieces<NP>(f32x8{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w}, pf[n]);
-            }
-#pragma unroll
-            for (int i = 0; i < DT; i++) {
-                const bf16x8 vf = lv[b][(s2 * DT + i) * 64 + lane];
-#pragma unroll
-                for (int n = 0; n < CT; n++)
-#pragma unroll
-                    for (int x = 0; x < NP; x++) o[i][n] = kv8_mma(vf, pf[n][x], o[i][n]);
-            }
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < CT; n++) {
-        const int col = w0 + 16 * n + cl;
-        const float inv = kv8_inverse(col_sum(l[n]));
-        if (col >= ncol) continue;
-        const size_t at = (size_t)(t.r0 + col / G) * ldo + (size_t)(head * G + col % G) * D + 4 * h;
-#pragma unroll
-        for (int i = 0; i < DT; i++) {
-            const f32x4 x = o[i][n] * inv;
-            if constexpr (BF) *(uint2 *)((uint16_t *)out + at + 16 * i) = pack4(x);
-            else *(f32x4 *)((float *)out + at + 16 * i) = x;
-        }
-    }
 }
 
 // ---------------------------------------------------------------------------
@@ -906,7 +754,7 @@ extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, si
 }
 
 #define KV8_FEW_COLS 64                // columns up to which the keys are split instead
-// The launch of k_kv8_few: four waves a block where the blocks fill the CUs
+// The launch for few columns: four waves a block where the blocks fill the CUs
 // twice, eight otherwise; the keys split over blocks where a wave would walk
 // more than three steps, as long as each still walks one and CUs are idle.
 struct kv8_plan { int waves, splits; };
@@ -936,21 +784,25 @@ extern "C" int qm_kv8_attention(const qm_kv8_t *c, void *out, const void *q, siz
     if (!rc) rc = kv8_call_check(c, row, pos, n, rows, max_rows);
     if (rc) return rc;
     if (q_heads < 1 || q_heads % c->heads || q_heads / c->heads > QM_KV8_MAX_GROUP) return QH_EINVAL;
-    if (max_ctx < 1 || max_ctx > c->max_blocks * c->block || !(fabsf(scale) < INFINITY)) return QH_EINVAL;
+    if (max_ctx < 1 || max_ctx > c->max_blocks * c->block || !(scale > 0.0f && scale < INFINITY)) return QH_EINVAL;
     if (n == 0 || rows == 0) return QH_OK;
     if (!kv8_rows_ok(q, ldq, q_heads * c->head_dim, bf16) || !kv8_rows_ok(out, ldo, q_heads * c->head_dim, bf16))
         return QH_EINVAL;
     const int G = q_heads / c->heads;
     const long cols = (long)max_rows * G;
     const float f = scale * 1.44269504088896340736f;     // the softmax runs on powers of two
+#define ATTEND(F, D_, BF_, CT_, CG_, KG_)                                                                              \
+    hipLaunchKernelGGL((k_kv8_attend<F, D_, BF_, CT_, CG_, KG_>), grid, dim3(WAVE *CG_ *KG_), 0, stream(), *c, out, q, ldo, \
+                       ldq, row, pos, rows, max_rows, G, f, ns, order, (float *)work)
     if (cols > KV8_FEW_COLS) {
-        const long tiles = (cols + KV8_MANY - 1) / KV8_MANY;
-        if (tiles * c->heads * NTH >= 1L << 32) return QH_ETOOBIG;
+        // fp32 rows take the registers of a second column tile for their pieces
+        const int tcols = bf16 ? 64 : 32, ns = 1;
+        const long blocks = (cols + tcols - 1) / tcols * c->heads;
+        if (blocks * 256 >= 1L << 32) return QH_ETOOBIG;
         if (!stream()) return QH_ESTATE;
-        const dim3 grid((unsigned)(tiles * c->heads), n);
-#define MANY(F, D_, BF_)                                                                                             \
-    hipLaunchKernelGGL((k_kv8_many<F, D_, BF_>), grid, dim3(NTH), 0, stream(), *c, out, q, ldo, ldq, row, pos, rows, \
-                       max_rows, G, f)
+        const int order = blocks * n <= 512 ? KV8_PAIRED : KV8_LONG_FIRST;
+        const dim3 grid((unsigned)blocks, n);
+#define MANY(F, D_, BF_) ATTEND(F, D_, BF_, (BF_ ? 2 : 1), 2, 2)
         KV8_SWITCH(MANY);
 #undef MANY
         return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
@@ -961,18 +813,16 @@ extern "C" int qm_kv8_attention(const qm_kv8_t *c, void *out, const void *q, siz
     if (ns > 1 && (!work || !aligned16(work))) return QH_EINVAL;
     if (work_bytes < qm_kv8_attention_work(c, q_heads, n, max_rows, max_ctx)) return QH_ETOOBIG;
     if (!stream()) return QH_ESTATE;
-    const dim3 grid(ns, c->heads * tiles, n);
-#define FEW_W(F, D_, BF_, W_)                                                                                          \
-    hipLaunchKernelGGL((k_kv8_few<F, D_, BF_, W_>), grid, dim3(WAVE *W_), 0, stream(), *c, out, q, ldo, ldq, row, pos, \
-                       rows, max_rows, G, f, (float *)work)
-#define FEW(F, D_, BF_)                             \
-    do {                                            \
-        if (plan.waves == 4) FEW_W(F, D_, BF_, 4);  \
-        else FEW_W(F, D_, BF_, 8);                  \
+    const dim3 grid(ns * c->heads * tiles, n);
+    const int order = KV8_AS_IS;
+#define FEW(F, D_, BF_)                                     \
+    do {                                                    \
+        if (plan.waves == 4) ATTEND(F, D_, BF_, 1, 1, 4);   \
+        else ATTEND(F, D_, BF_, 1, 1, 8);                   \
     } while (0)
     KV8_SWITCH(FEW);
 #undef FEW
-#undef FEW_W
+#undef ATTEND
     if (hipGetLastError() != hipSuccess) return QH_ELAUNCH;
     if (ns > 1) {
         const int per = NTH / WAVE;

@@ -69,7 +69,7 @@ def test_nothing_to_do():
 
 @pytest.mark.parametrize("bad", [dict(out=None), dict(q=A + 4), dict(ldo=2047), dict(ldq=2044 + 2), dict(heads=12), dict(heads=0),
                                  dict(heads=8 * 65, ldo=1 << 17, ldq=1 << 17), dict(n=5), dict(row=None), dict(ctx=0),
-                                 dict(ctx=513), dict(scale=float("nan")), dict(scale=float("inf")), dict(work=None),
+                                 dict(ctx=513), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=0.0), dict(scale=-0.1), dict(work=None),
                                  dict(work=A + 4), dict(most=513), dict(pos=None)])
 def test_attentions_that_are_refused(bad):
     assert attend() == ESTATE

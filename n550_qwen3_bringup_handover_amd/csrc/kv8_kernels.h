@@ -349,7 +349,6 @@ __device__ __forceinline__ float kv8_softmax(f32x4 (&s)[4], float k, float &m, f
 //   many (a prompt): two groups of keys, two of columns; the column tiles with
 //   the longest contexts first, or, where all blocks fit the CUs at once, so
 //   that the two blocks of a CU are a long and a short one
-#define KV8_COLS 16
 #define KV8_MAX_SPLITS 32
 enum { KV8_AS_IS, KV8_LONG_FIRST, KV8_PAIRED };
 template <int FMT, int D, bool BF, int CT, int CG, int KG>
@@ -608,15 +607,15 @@ template <int D, bool BF>
 __global__ __launch_bounds__(NTH) void k_kv8_merge(qm_kv8_t c, void *__restrict__ out, size_t ldo,
                                                    const int *__restrict__ row, const int *__restrict__ pos, int rows,
                                                    int max_rows, int G, const float *__restrict__ part, int nsplit,
-                                                   int tiles) {
+                                                   int tiles, int cols) {
     constexpr int TPC = D / 4, LD = D + 4, GR = WAVE / TPC, PER = KV8_MAX_SPLITS / GR;
     const int e = blockIdx.z, head = blockIdx.y, lane = threadIdx.x & 63;
     kv8_entry t;
     if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
     const int col = blockIdx.x * (NTH / WAVE) + (threadIdx.x >> 6), d = lane % TPC * 4, gr = lane / TPC;
     if (col >= t.cnt * G) return;
-    const int y = col / KV8_COLS * c.heads + head;
-    const float *p = part + (((size_t)e * (tiles * c.heads) + y) * nsplit * KV8_COLS + col % KV8_COLS) * LD;
+    const int y = col / cols * c.heads + head;
+    const float *p = part + (((size_t)e * (tiles * c.heads) + y) * nsplit * cols + col % cols) * LD;
     float ms[PER], ls[PER];
     f32x4 o[PER];
 #pragma unroll
@@ -626,7 +625,7 @@ __global__ __launch_bounds__(NTH) void k_kv8_merge(qm_kv8_t c, void *__restrict_
         ls[u] = 0.0f;
         o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (u * GR < nsplit && s < nsplit) {
-            const float *ps = p + (size_t)s * KV8_COLS * LD;
+            const float *ps = p + (size_t)s * cols * LD;
             ms[u] = ps[0];
             ls[u] = ps[1];
             o[u] = *(const f32x4 *)(ps + 4 + d);
@@ -753,28 +752,50 @@ extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, si
     return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
 }
 
-#define KV8_FEW_COLS 64                // columns up to which the keys are split instead
-// The launch for few columns: four waves a block where the blocks fill the CUs
-// twice, eight otherwise; the keys split over blocks where a wave would walk
-// more than three steps, as long as each still walks one and CUs are idle.
-struct kv8_plan { int waves, splits; };
-static kv8_plan kv8_few_plan(const qm_kv8_t *c, int n, int tiles, int max_ctx) {
-    const long blocks = (long)n * c->heads * tiles;
-    const int steps = (max_ctx + 63) / 64 + 1;
-    if (blocks >= 512) return kv8_plan{4, 1};
-    if (steps <= 24) return kv8_plan{8, 1};
-    long s = (steps + 15) / 16, room = (320 + blocks - 1) / blocks;
-    if (s > room) s = room;
-    if (s > KV8_MAX_SPLITS) s = KV8_MAX_SPLITS;
-    return kv8_plan{8, (int)s};
+// The launch for max_rows x G columns a kv head and sequence.
+//   CT: two column tiles a wave where rows are bf16 and there are more than 16
+//     columns (fp32 rows take the registers for their pieces).
+//   Blocks that fill the CUs twice (512 of four waves, two a CU): four groups of
+//     keys; for long prompts two of keys and two of columns, which share what
+//     they read (1,999 tokens 43.2 against 45.4 us, 4 x 499 22.0 against 24.6;
+//     500 behind 1,499 37.6 against 22.9 the other way).
+//   Fewer: eight waves on the keys, and the keys split over as many blocks as
+//     leave a wave a step, one block a CU, if a wave would walk more than two:
+//     700 positions 9.7 us on one block a head and 11.2 split, 1,500 14.5 and
+//     11.1, 3,000 18.1 and 11.2; 6 x 8,000 17.9 us on 192 blocks, 25 on 336.
+struct kv8_plan { int ct, cg, kg, splits, order, cols, tiles; };
+static kv8_plan kv8_plan_of(const qm_kv8_t *c, int G, int n, int max_rows, int max_ctx, int bf16) {
+    const long cols = (long)max_rows * G;
+    kv8_plan p = {bf16 && cols > 16 ? 2 : 1, 1, 4, 1, KV8_LONG_FIRST, 0, 0};
+    p.cols = 16 * p.ct;
+    p.tiles = (int)((cols + p.cols - 1) / p.cols);
+    const long blocks = (long)p.tiles * c->heads * n;
+    if (blocks >= 960 && p.tiles >= 16 && c->head_dim == 128) {
+        p.cg = p.kg = 2;
+        p.cols *= 2;
+        p.tiles = (p.tiles + 1) / 2;
+        if ((long)p.tiles * c->heads * n <= 512) p.order = KV8_PAIRED;
+    } else if (blocks < 512) {
+        p.kg = 8;
+        const int steps = (max_ctx + 63) / 64 + 1;
+        const long room = 256 / blocks, want = (steps + 7) / 8;
+        if (steps > 16) p.splits = (int)(want < room ? want : room);
+        if (p.splits > KV8_MAX_SPLITS) p.splits = KV8_MAX_SPLITS;
+        if (p.splits < 1) p.splits = 1;
+        if (p.splits > 1) p.order = KV8_AS_IS;           // the order of k_kv8_merge
+    }
+    return p;
+}
+static size_t kv8_plan_work(const qm_kv8_t *c, int n, const kv8_plan &p) {
+    return p.splits == 1 ? 0 : (size_t)n * c->heads * p.tiles * p.splits * p.cols * (c->head_dim + 4) * sizeof(float);
 }
 
 extern "C" size_t qm_kv8_attention_work(const qm_kv8_t *c, int q_heads, int n, int max_rows, int max_ctx) {
-    if (!c || c->heads < 1 || q_heads < c->heads || n < 1 || max_rows < 1) return 0;
-    const long cols = (long)max_rows * (q_heads / c->heads);
-    if (cols > KV8_FEW_COLS) return 0;
-    const int tiles = (int)((cols + KV8_COLS - 1) / KV8_COLS), s = kv8_few_plan(c, n, tiles, max_ctx).splits;
-    return s == 1 ? 0 : (size_t)n * c->heads * tiles * s * KV8_COLS * (c->head_dim + 4) * sizeof(float);
+    if (!c || kv8_sizes(c) || q_heads < c->heads || n < 1 || max_rows < 1 || max_ctx < 1) return 0;
+    const int G = q_heads / c->heads;
+    const size_t a = kv8_plan_work(c, n, kv8_plan_of(c, G, n, max_rows, max_ctx, 0));
+    const size_t b = kv8_plan_work(c, n, kv8_plan_of(c, G, n, max_rows, max_ctx, 1));
+    return a > b ? a : b;
 }
 
 extern "C" int qm_kv8_attention(const qm_kv8_t *c, void *out, const void *q, size_t ldo, size_t ldq, int bf16, int q_heads,
@@ -789,47 +810,39 @@ extern "C" int qm_kv8_attention(const qm_kv8_t *c, void *out, const void *q, siz
     if (!kv8_rows_ok(q, ldq, q_heads * c->head_dim, bf16) || !kv8_rows_ok(out, ldo, q_heads * c->head_dim, bf16))
         return QH_EINVAL;
     const int G = q_heads / c->heads;
-    const long cols = (long)max_rows * G;
     const float f = scale * 1.44269504088896340736f;     // the softmax runs on powers of two
-#define ATTEND(F, D_, BF_, CT_, CG_, KG_)                                                                              \
-    hipLaunchKernelGGL((k_kv8_attend<F, D_, BF_, CT_, CG_, KG_>), grid, dim3(WAVE *CG_ *KG_), 0, stream(), *c, out, q, ldo, \
-                       ldq, row, pos, rows, max_rows, G, f, ns, order, (float *)work)
-    if (cols > KV8_FEW_COLS) {
-        // fp32 rows take the registers of a second column tile for their pieces
-        const int tcols = bf16 ? 64 : 32, ns = 1;
-        const long blocks = (cols + tcols - 1) / tcols * c->heads;
-        if (blocks * 256 >= 1L << 32) return QH_ETOOBIG;
-        if (!stream()) return QH_ESTATE;
-        const int order = blocks * n <= 512 ? KV8_PAIRED : KV8_LONG_FIRST;
-        const dim3 grid((unsigned)blocks, n);
-#define MANY(F, D_, BF_) ATTEND(F, D_, BF_, (BF_ ? 2 : 1), 2, 2)
-        KV8_SWITCH(MANY);
-#undef MANY
-        return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
-    }
-    const int tiles = (int)((cols + KV8_COLS - 1) / KV8_COLS);
-    const kv8_plan plan = kv8_few_plan(c, n, tiles, max_ctx);
-    const int ns = plan.splits;
-    if (ns > 1 && (!work || !aligned16(work))) return QH_EINVAL;
-    if (work_bytes < qm_kv8_attention_work(c, q_heads, n, max_rows, max_ctx)) return QH_ETOOBIG;
+    const kv8_plan p = kv8_plan_of(c, G, n, max_rows, max_ctx, bf16);
+    if (p.splits > 1 && (!work || !aligned16(work))) return QH_EINVAL;
+    if (work_bytes < kv8_plan_work(c, n, p)) return QH_ETOOBIG;
+    const long blocks = (long)p.tiles * c->heads * p.splits;
+    if (blocks * 512 >= 1L << 32) return QH_ETOOBIG;
     if (!stream()) return QH_ESTATE;
-    const dim3 grid(ns * c->heads * tiles, n);
-    const int order = KV8_AS_IS;
-#define FEW(F, D_, BF_)                                     \
-    do {                                                    \
-        if (plan.waves == 4) ATTEND(F, D_, BF_, 1, 1, 4);   \
-        else ATTEND(F, D_, BF_, 1, 1, 8);                   \
+    const dim3 grid((unsigned)blocks, n);
+#define ATTEND_AS(F, D_, BF_, CT_, CG_, KG_)                                                                           \
+    hipLaunchKernelGGL((k_kv8_attend<F, D_, BF_, CT_, CG_, KG_>), grid, dim3(WAVE *CG_ *KG_), 0, stream(), *c, out, q, ldo, \
+                       ldq, row, pos, rows, max_rows, G, f, p.splits, p.order, (float *)work)
+#define ATTEND_CT(F, D_, BF_, CT_)                                \
+    do {                                                          \
+        if (p.cg == 2) ATTEND_AS(F, D_, BF_, CT_, 2, 2);          \
+        else if (p.kg == 4) ATTEND_AS(F, D_, BF_, CT_, 1, 4);     \
+        else ATTEND_AS(F, D_, BF_, CT_, 1, 8);                    \
     } while (0)
-    KV8_SWITCH(FEW);
-#undef FEW
+#define ATTEND(F, D_, BF_)                              \
+    do {                                                \
+        if (p.ct == 2) ATTEND_CT(F, D_, BF_, (BF_ ? 2 : 1)); \
+        else ATTEND_CT(F, D_, BF_, 1);                  \
+    } while (0)
+    KV8_SWITCH(ATTEND);
 #undef ATTEND
+#undef ATTEND_CT
+#undef ATTEND_AS
     if (hipGetLastError() != hipSuccess) return QH_ELAUNCH;
-    if (ns > 1) {
-        const int per = NTH / WAVE;
-        const dim3 mg((unsigned)((cols + per - 1) / per), c->heads, n);
+    if (p.splits > 1) {
+        const long cols = (long)max_rows * G;
+        const dim3 mg((unsigned)((cols + NTH / WAVE - 1) / (NTH / WAVE)), c->heads, n);
 #define MERGE(D_, BF_)                                                                                               \
     hipLaunchKernelGGL((k_kv8_merge<D_, BF_>), mg, dim3(NTH), 0, stream(), *c, out, ldo, row, pos, rows, max_rows, G, \
-                       (const float *)work, ns, tiles)
+                       (const float *)work, p.splits, p.tiles, p.cols)
         if (c->head_dim == 128) { if (bf16) MERGE(128, true); else MERGE(128, false); }
         else { if (bf16) MERGE(64, true); else MERGE(64, false); }
 #undef MERGE

@@ -18,7 +18,7 @@ class Shim(ctypes.Structure):     # qm_kv8_t has qwen3_hip_kv8's fields in its o
 
 
 def cache(**kw):
-    d = dict(format=0, kv_heads=8, head_dim=128, block=32, n_page=64, n_seq=4, max_blocks=16, k=A, v=A, k_scale=A, v_scale=A,
+    d = dict(format=0, kv_heads=8, head_dim=128, block=32, n_page=64, n_seq=4, max_blocks=64, k=A, v=A, k_scale=A, v_scale=A,
              k_tail=A, v_tail=A, table=A)
     d.update(kw)
     return Shim(*[d[n] for n, _ in Shim._fields_])
@@ -29,7 +29,7 @@ def append(c=None, k=A, v=A, ldk=1024, ldv=1024, bf16=0, row=A, pos=A, n=4, rows
     return f(ctypes.byref(c or cache()), VP(k), VP(v), SZ(ldk), SZ(ldv), bf16, VP(row), VP(pos), n, rows, most)
 
 
-def attend(c=None, out=A, q=A, ldo=2048, ldq=2048, bf16=0, heads=16, row=A, pos=A, n=4, rows=9, most=3, ctx=512, scale=0.1,
+def attend(c=None, out=A, q=A, ldo=2048, ldq=2048, bf16=0, heads=16, row=A, pos=A, n=4, rows=9, most=3, ctx=2048, scale=0.1,
            work=A, bytes=1 << 30):
     f = runtime.lib().qm_kv8_attention
     return f(ctypes.byref(c or cache()), VP(out), VP(q), SZ(ldo), SZ(ldq), bf16, heads, VP(row), VP(pos), n, rows, most, ctx,
@@ -55,7 +55,7 @@ def test_caches_at_their_limits():
 
 
 @pytest.mark.parametrize("bad", [dict(k=None), dict(v=A + 4), dict(ldk=1023), dict(ldv=1026), dict(pos=None), dict(n=5),
-                                 dict(n=-1), dict(rows=-1), dict(most=0), dict(most=513), dict(row=None),
+                                 dict(n=-1), dict(rows=-1), dict(most=0), dict(most=2049), dict(row=None),
                                  dict(ldk=1028, bf16=1)])
 def test_appends_that_are_refused(bad):
     assert append() == ESTATE
@@ -69,8 +69,8 @@ def test_nothing_to_do():
 
 @pytest.mark.parametrize("bad", [dict(out=None), dict(q=A + 4), dict(ldo=2047), dict(ldq=2044 + 2), dict(heads=12), dict(heads=0),
                                  dict(heads=8 * 65, ldo=1 << 17, ldq=1 << 17), dict(n=5), dict(row=None), dict(ctx=0),
-                                 dict(ctx=513), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=0.0), dict(scale=-0.1), dict(work=None),
-                                 dict(work=A + 4), dict(most=513), dict(pos=None)])
+                                 dict(ctx=2049), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=0.0), dict(scale=-0.1), dict(work=None),
+                                 dict(work=A + 4), dict(most=2049), dict(pos=None)])
 def test_attentions_that_are_refused(bad):
     assert attend() == ESTATE
     assert attend(**bad) == EINVAL
@@ -78,12 +78,12 @@ def test_attentions_that_are_refused(bad):
 
 def test_attention_needs_its_workspace():
     c = cache()
-    need = runtime.lib().qwen3_hip_kv8_attention_work(ctypes.cast(ctypes.byref(c), runtime.KV8P), 16, 4, 3, 512)
-    assert need > 0
+    need = runtime.lib().qwen3_hip_kv8_attention_work(ctypes.cast(ctypes.byref(c), runtime.KV8P), 16, 4, 3, 2048)
+    assert need > 0                                   # its keys are split over blocks
     assert attend(c, bytes=need) == ESTATE
     assert attend(c, bytes=need - 1) == ETOOBIG
     # a prompt's launch needs none
-    assert runtime.lib().qwen3_hip_kv8_attention_work(ctypes.cast(ctypes.byref(c), runtime.KV8P), 16, 4, 200, 512) == 0
+    assert runtime.lib().qwen3_hip_kv8_attention_work(ctypes.cast(ctypes.byref(c), runtime.KV8P), 16, 4, 200, 2048) == 0
     assert attend(c, rows=800, most=200, work=None, bytes=0) == ESTATE
 
 

@@ -18,7 +18,7 @@
 #define BEAM_PIECE 2048                // logits of a wave: 32 a lane
 #define BEAM_V (BEAM_PIECE / WAVE)
 #define BEAM_NONE 0x7FFFFFFF           // the index of no candidate
-#define BEAM_E 32                      // list entries a lane of the second launch holds: vocab x W up to 4 M
+#define BEAM_E 8                       // list entries a lane of the second launch has in flight
 
 struct beam_cand { float v; int i; };
 struct beam_sum { float m, s; };
@@ -42,22 +42,29 @@ __device__ __forceinline__ int wave_min_int(int v) {
 
 // a comes before b: larger, or equal with the lower index
 __device__ __forceinline__ bool beam_before(float av, int ai, float bv, int bi) {
-    return av > bv || (av == bv && ai < bi);
+    return (av > bv) | ((av == bv) & (ai < bi));          // no branch: loops over it keep their reads in flight
 }
 
-// A wave's choice of W among what its lanes hold: W times the largest of the
-// lanes' maxima is dropped; what reaches the last of them, T, are at least W
-// values and hardly more, which go to LDS, where each finds its rank by
-// counting who comes before it.  Where more than a lane each reach T (equal
-// values), or fewer than W are finite, the callers choose one at a time.
+// A wave's choice of W among what its lanes hold: a threshold that W of the
+// lanes' maxima reach, so that at least W values do and hardly more; they go to
+// LDS, where each finds its rank by counting who comes before it.  Where more
+// than a lane each reach it (equal values), or fewer than W are finite, the
+// callers choose one at a time.
 #define BEAM_CAP WAVE
+// found bit by bit over the order of floats, until W lanes are left: about
+// twelve rounds of a compare and a count whatever W is, where W rounds of a
+// wave-wide maximum take 200 cycles each
 __device__ __forceinline__ float beam_threshold(float lane_max, int W) {
-    float t = -INFINITY;
-    for (int w = 0; w < W; w++) {
-        t = wave_max(lane_max);
-        lane_max = lane_max == t ? -INFINITY : lane_max;
+    const unsigned b = __float_as_uint(lane_max), key = b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+    unsigned t = 0;
+    for (int bit = 31; bit >= 0; bit--) {
+        const unsigned c = t | 1u << bit;
+        const int n = __popcll(__ballot(key >= c));
+        if (n >= W) t = c;
+        if (n == W) break;
     }
-    return t;
+    if (t <= 0x007FFFFFu) return -INFINITY;               // the place of -inf in that order
+    return __uint_as_float(t & 0x80000000u ? t ^ 0x80000000u : ~t);
 }
 __device__ __forceinline__ void beam_collect(beam_cand *cand, int &n, bool in, float v, int i) {
     const unsigned long long mask = __ballot(in);
@@ -70,7 +77,10 @@ __device__ __forceinline__ void beam_collect(beam_cand *cand, int &n, bool in, f
 __device__ __forceinline__ int beam_rank(const beam_cand *cand, int n, beam_cand t) {
     int rank = 0;
 #pragma unroll 4
-    for (int u = 0; u < n; u++) rank += beam_before(cand[u].v, cand[u].i, t.v, t.i);
+    for (int u = 0; u < n; u++) {
+        const beam_cand o = cand[u];
+        rank += beam_before(o.v, o.i, t.v, t.i);
+    }
     return rank;
 }
 
@@ -164,7 +174,7 @@ __global__ __launch_bounds__(NTH) void k_beam_pieces(const float *__restrict__ l
 }
 
 // Block: one group.  Wave w joins row w's sums and finds the row's best W in
-// its pieces' lists; then one thread for each of the W x W counts its rank.
+// its pieces' lists; then the W x W are ranked.
 __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, int pieces, const float *score,
                                                              const int *done, int end0, int end1,
                                                              const beam_sum *__restrict__ sums,
@@ -175,12 +185,13 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
     __shared__ double cv[BEAM_MAX * BEAM_MAX];
     __shared__ long cid[BEAM_MAX * BEAM_MAX];             // w V + token, BEAM_NOWHERE for no candidate
     __shared__ beam_cand cands[BEAM_MAX][BEAM_CAP];
-    __shared__ int sdone[BEAM_MAX];
+    __shared__ int sdone[BEAM_MAX], ranks[BEAM_MAX * BEAM_MAX];
     constexpr long BEAM_NOWHERE = 0x7FFFFFFFFFFFFFFFL;
     const int r = g * W + w;                              // launched with W waves
     const bool over = done && done[r] != 0;
     const double base = score[r];
     if (lane == 0) sdone[w] = over;
+    for (int i = threadIdx.x; i < W * W; i += W * WAVE) ranks[i] = 0;
     if (over) {
         if (lane < W) {
             cv[w * W + lane] = lane == 0 ? base : -INFINITY;
@@ -190,13 +201,6 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
         const beam_sum *ps = sums + (size_t)r * pieces;
         const beam_cand *pl = lists + (size_t)r * pieces * W;
         const int entries = pieces * W;
-        // the first BEAM_E x 64 entries of the lists in registers, all loads in flight
-        beam_cand t[BEAM_E];
-#pragma unroll
-        for (int k = 0; k < BEAM_E; k++) {
-            t[k] = beam_cand{-INFINITY, BEAM_NONE};
-            if (WAVE * (k / 8 * 8) < entries && WAVE * k + lane < entries) t[k] = pl[WAVE * k + lane];
-        }
         float mx = -INFINITY;
 #pragma unroll 2
         for (int p = lane; p < pieces; p += WAVE) mx = fmaxf(mx, ps[p].m);
@@ -213,17 +217,28 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
             cv[w * W + k] = t == t ? t : -INFINITY;       // no probabilities, no score
             cid[w * W + k] = i == BEAM_NONE ? BEAM_NOWHERE : (long)w * vocab + i;
         };
+        // twice over the lists, eight entries a lane in flight: unrolled over all
+        // of them, in registers, the kernel spends its time fetching instructions
         float lm = -INFINITY;
+        for (int i0 = lane; i0 < entries; i0 += BEAM_E * WAVE) {
+            float v[BEAM_E];
 #pragma unroll
-        for (int k = 0; k < BEAM_E; k++) lm = fmaxf(lm, t[k].v);
-        const float thr = entries <= WAVE * BEAM_E ? beam_threshold(lm, W) : -INFINITY;
+            for (int k = 0; k < BEAM_E; k++) v[k] = i0 + WAVE * k < entries ? pl[i0 + WAVE * k].v : -INFINITY;
+#pragma unroll
+            for (int k = 0; k < BEAM_E; k++) lm = fmaxf(lm, v[k]);
+        }
+        const float thr = beam_threshold(lm, W);
         beam_cand *cand = cands[w];
         int n = 0;
-        if (thr > -INFINITY) {
+        if (thr > -INFINITY)
+            for (int i0 = lane; i0 - lane < entries; i0 += BEAM_E * WAVE) {
+                beam_cand t[BEAM_E];
 #pragma unroll
-            for (int k = 0; k < BEAM_E; k++)
-                if (WAVE * (k / 8 * 8) < entries) beam_collect(cand, n, t[k].v >= thr, t[k].v, t[k].i);
-        }
+                for (int k = 0; k < BEAM_E; k++)
+                    t[k] = i0 + WAVE * k < entries ? pl[i0 + WAVE * k] : beam_cand{-INFINITY, BEAM_NONE};
+#pragma unroll
+                for (int k = 0; k < BEAM_E; k++) beam_collect(cand, n, t[k].v >= thr, t[k].v, t[k].i);
+            }
         if (n > 0 && n <= BEAM_CAP) {
             if (lane < n) {
                 const beam_cand t = cand[lane];
@@ -246,14 +261,29 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
             }
         }
     }
+    __syncthreads();
+    // each of the W x W counts who comes before it: a thread for each of them
+    // and each beam
+    const int n2 = W * W;
+    for (int task = threadIdx.x; task < n2 * W; task += W * WAVE) {
+        const int i = task % n2, from = task / n2 * W;
+        const double v = cv[i];
+        const long id = cid[i];
+        int before = 0;
+#pragma unroll 4
+        for (int u = 0; u < W; u++) {
+            const double a = cv[from + u];
+            const long b = cid[from + u];
+            before += (a > v) | ((a == v) & (b < id));    // no branch: the reads stay in flight
+        }
+        if (before) atomicAdd(&ranks[i], before);
+    }
     __syncthreads();                                      // the group's inputs have been read: outputs may lie there
     const int i = threadIdx.x;
-    if (i >= W * W) return;
+    if (i >= n2) return;
     const double v = cv[i];
     const long id = cid[i];
-    int rank = 0;
-#pragma unroll 8
-    for (int u = 0; u < W * W; u++) rank += cv[u] > v || (cv[u] == v && cid[u] < id);
+    const int rank = ranks[i];
     if (rank < W && id != BEAM_NOWHERE) {
         const int par = i / W, tok = (int)(id - (long)par * vocab);
         score_out[g * W + rank] = (float)v;
@@ -291,7 +321,7 @@ __global__ __launch_bounds__(NTH) void k_beam_reorder(uint8_t *dst, const uint8_
     }
 #pragma unroll
     for (int w = 0; w < WT; w++)
-        if (p[w] >= 0) *(T *)(dst + at + (size_t)w * seq_stride) = v[w];
+        if (p[w] >= 0) __builtin_nontemporal_store(v[w], (T *)(dst + at + (size_t)w * seq_stride));
 }
 
 // ---------------------------------------------------------------------------

@@ -85,38 +85,58 @@ __device__ __forceinline__ __bf16 kv8_held(float x) {
     return (__bf16)fminf(fmaxf(x, -KV8_BF16_MAX), KV8_BF16_MAX);
 }
 
+// A block's scale s = a / qmax and what divides by it: x / s rounded to fp32, as
+// the definition has it, in three instructions for the compiler's ten.  With
+// y = 1 / s rounded, q = x y is off by a last place or two, and q plus its
+// remainder x - q s times y rounds to the quotient -- for every
+// pair of 8-bit significands of x and a, which is all there are (the tests
+// divide each).  Small blocks are scaled up first, so that no remainder
+// underflows.
+struct kv8_div { float s, y, up; };
 template <int FMT>
-__device__ __forceinline__ uint32_t kv8_codes4(float a, float b, float c, float d, float s) {
-    if (s == 0.0f) return 0;
-    a /= s; b /= s; c /= s; d /= s;
+__device__ __forceinline__ kv8_div kv8_scale(float a) {
+    kv8_div d;
+    d.up = a < 0x1p-40f ? 0x1p64f : 1.0f;
+    d.s = a < KV8_TINY ? 0.0f : a / kv8_qmax<FMT>::v;
+    d.y = d.s == 0.0f ? 0.0f : 1.0f / (d.s * d.up);
+    return d;
+}
+__device__ __forceinline__ float kv8_quotient(float x, kv8_div d) {
+    x *= d.up;
+    const float q = x * d.y, s = d.s * d.up;
+    return fmaf(fmaf(-q, s, x), d.y, q);
+}
+
+template <int FMT>
+__device__ __forceinline__ uint32_t kv8_codes4(float a, float b, float c, float d, kv8_div s) {
+    a = kv8_quotient(a, s);
+    b = kv8_quotient(b, s);
+    c = kv8_quotient(c, s);
+    d = kv8_quotient(d, s);
     if constexpr (FMT == QM_KV8_E4M3) {
         int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
         return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
     } else {
-        auto i = [](float x) { return (uint32_t)(int)fminf(fmaxf(rintf(x), -127.0f), 127.0f) & 0xFFu; };
+        // |x / s| is at most 127 (1 + 2^-23): it rounds to a byte
+        auto i = [](float x) { return (uint32_t)(int)rintf(x) & 0xFFu; };
         return i(a) | i(b) << 8 | i(c) << 16 | i(d) << 24;
     }
 }
 
-// sixteen consecutive values, 16-byte aligned (BF) or 16-byte aligned fp32
+// sixteen consecutive values, 16-byte aligned, as they lie and as the cache holds them
 template <bool BF>
-__device__ __forceinline__ void kv8_load16(const void *p, size_t i, __bf16 (&x)[16]) {
-    if constexpr (BF) {
-        const bf16x8 a = *(const bf16x8 *)((const __bf16 *)p + i), b = *(const bf16x8 *)((const __bf16 *)p + i + 8);
+struct kv8_16 {
+    f32x4 v[BF ? 2 : 4];
+    __device__ __forceinline__ void load(const void *p, size_t i) {
+        const f32x4 *q = (const f32x4 *)(BF ? (const void *)((const __bf16 *)p + i) : (const void *)((const float *)p + i));
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            x[j] = kv8_held((float)a[j]);
-            x[8 + j] = kv8_held((float)b[j]);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-            const f32x4 a = *(const f32x4 *)((const float *)p + i + j);
-#pragma unroll
-            for (int u = 0; u < 4; u++) x[j + u] = kv8_held(a[u]);
-        }
+        for (int j = 0; j < (BF ? 2 : 4); j++) v[j] = q[j];
     }
-}
+    __device__ __forceinline__ float at(int j) const {
+        if constexpr (BF) return (float)__builtin_bit_cast(bf16x8, v[j >> 3])[j & 7];
+        else return v[j >> 2][j & 3];
+    }
+};
 
 // Block (h, e, z): kv head h of entry e, the z-th block its rows touch; B D / 16
 // threads, so that a finished block is one unit of 16 values of K (of a row)
@@ -146,20 +166,25 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
         const int p0 = t.r0 + b * B - t.pos;              // row of the block's slot 0 (before r0 where some are in the tail)
         const int kr = tid / (D / 16), kd = tid % (D / 16) * 16;       // K: slot and dims
         const int vd = tid % D, vr = tid / D * 16;                     // V: dim and slots
-        __bf16 x[16], y[16];
-        kv8_load16<BF>(kn, (size_t)(p0 + max(kr, have)) * ldk + h * D + kd, x);
+        // every load first, the tail's too where some of the rows lie there
+        kv8_16<true> kold = {}, vold = {};
+        if (have > 0) {
+            kold.load(kt, kr * D + kd);
+            vold.load(vt, vd * B + vr);
+        }
+        kv8_16<BF> knew;
+        float vnew[16];
+        knew.load(kn, (size_t)(p0 + max(kr, have)) * ldk + h * D + kd);
 #pragma unroll
         for (int j = 0; j < 16; j++) {
             const size_t i = (size_t)(p0 + max(vr + j, have)) * ldv + h * D + vd;
-            y[j] = kv8_held(BF ? (float)((const __bf16 *)vn)[i] : ((const float *)vn)[i]);
+            vnew[j] = BF ? (float)((const __bf16 *)vn)[i] : ((const float *)vn)[i];
         }
-        if (have > 0) {
-            if (kr < have) kv8_load16<true>(kt, kr * D + kd, x);
-            __bf16 o[16];
-            kv8_load16<true>(vt, vd * B + vr, o);
+        __bf16 x[16], y[16];
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (vr + j < have) y[j] = o[j];
+        for (int j = 0; j < 16; j++) {
+            x[j] = kv8_held(kr < have ? kold.at(j) : knew.at(j));
+            y[j] = kv8_held(vr + j < have ? vold.at(j) : vnew[j]);
         }
         float ak = 0.0f, av = 0.0f;
 #pragma unroll
@@ -177,8 +202,7 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
             ak = fmaxf(ak, red[0][w]);
             av = fmaxf(av, red[1][w]);
         }
-        const float ks = ak < KV8_TINY ? 0.0f : ak / kv8_qmax<FMT>::v;
-        const float vs = av < KV8_TINY ? 0.0f : av / kv8_qmax<FMT>::v;
+        const kv8_div ks = kv8_scale<FMT>(ak), vs = kv8_scale<FMT>(av);
         if (page >= 0 && page < c.n_page) {               // the same for the whole block
             const size_t at = (size_t)page * c.heads + h;
             uint32_t u[4], w[4];
@@ -190,8 +214,8 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
             *(uint4 *)(c.k + at * (B * D) + kr * D + kd) = make_uint4(u[0], u[1], u[2], u[3]);
             *(uint4 *)(c.v + at * (B * D) + vd * B + vr) = make_uint4(w[0], w[1], w[2], w[3]);
             if (tid == 0) {
-                c.k_scale[at] = ks;
-                c.v_scale[at] = vs;
+                c.k_scale[at] = ks.s;
+                c.v_scale[at] = vs.s;
             }
         }
     }

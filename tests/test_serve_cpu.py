@@ -136,3 +136,34 @@ def test_reorders_at_their_limits():
     assert reorder(width=1) == 0                      # in place, one beam: nothing moves
     assert reorder(groups=65536, slab=1 << 40) == ETOOBIG
     assert reorder(runs=1, used=1 << 36, seq=1 << 36, slab=1 << 40) == ETOOBIG
+
+
+@pytest.mark.parametrize("qmax", [448, 127])
+def test_the_stores_division_is_exact(qmax):
+    """the kernel's x / s, s = fl(a / qmax): q = fl(x y) with y = fl(1 / s), then fl(q + fl(x - q s) y) equals the
+    rounded quotient for every pair of bf16 significands of x and a, in exact arithmetic (exponents only shift)"""
+    from fractions import Fraction as F
+
+    def fl(x):                                     # nearest fp32 of a rational, ties to even, no underflow
+        if x == 0:
+            return x
+        sign, x = (1, x) if x > 0 else (-1, -x)
+        e = x.numerator.bit_length() - x.denominator.bit_length() - 23
+        if x / F(2) ** e >= 2 ** 24:
+            e += 1
+        elif x / F(2) ** e < 2 ** 23:
+            e -= 1
+        n = x / F(2) ** e
+        k = n.numerator // n.denominator
+        rest = n - k
+        if rest > F(1, 2) or (rest == F(1, 2) and k % 2):
+            k += 1
+        return sign * k * F(2) ** e
+
+    for am in range(128, 256):
+        s = fl(F(am, 128) / qmax)
+        y = fl(1 / s)
+        for xm in range(128, 256):
+            x = F(xm, 256)
+            q = fl(x * y)
+            assert fl(q + fl(x - q * s) * y) == fl(x / s), (am, xm)

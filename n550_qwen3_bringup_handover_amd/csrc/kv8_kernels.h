@@ -366,15 +366,28 @@ __device__ __forceinline__ float kv8_softmax(f32x4 (&s)[4], float k, float &m, f
 // (K of the next step is in flight during this step's V product), so that
 // waves never wait for one another until the groups' sums meet in LDS at the
 // end.  The unfinished block is one more step.  With several splits (blocks on
-// the same columns) each block leaves a partial {m, l, -, -, o[D]} per column
-// for k_kv8_merge.
+// the same columns) each block writes a partial {m, l, -, -, o[D]} per column
+// with agent-scope (write-through) stores, waits for them, and takes a ticket
+// of its columns; the block that draws the last one reads all partials, merges
+// them in split order and resets the counter.  No block waits for another; a
+// launch of its own for the merge cost 4 us.
 //   few columns (decode, a few rows): CT = CG = 1, the keys split over four or
 //   eight waves and over blocks
 //   many (a prompt): two groups of keys, two of columns; the column tiles with
 //   the longest contexts first, or, where all blocks fit the CUs at once, so
 //   that the two blocks of a CU are a long and a short one
 #define KV8_MAX_SPLITS 32
-enum { KV8_AS_IS, KV8_LONG_FIRST, KV8_PAIRED };
+template <bool NT>
+__device__ __forceinline__ uint4 kv8_read(const uint8_t *p) {
+    if constexpr (NT) return __builtin_bit_cast(uint4, __builtin_nontemporal_load((const u32x4 *)p));
+    return *(const uint4 *)p;
+}
+enum { KV8_LONG_FIRST, KV8_PAIRED };
+#define KV8_SC1 16                     // agent scope: past this XCD's L2
+// one per kv head, sequence and column tile of a launch that splits its keys;
+// zero between launches, which run one after the other on the library stream
+#define KV8_TICKETS 128
+__device__ unsigned kv8_tickets[KV8_TICKETS];
 template <int FMT, int D, bool BF, int CT, int CG, int KG>
 __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void *__restrict__ out,
                                                                const void *__restrict__ q, size_t ldo, size_t ldq,
@@ -399,8 +412,7 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
     const int ncol = t.cnt * G, tiles = (ncol + COLS - 1) / COLS, at_ = x / c.heads;
     if (at_ >= tiles) return;
-    const int tile = order == KV8_AS_IS ? at_ : order == KV8_LONG_FIRST || at_ < (tiles + 1) / 2 ? tiles - 1 - at_
-                                                                                                 : at_ - (tiles + 1) / 2;
+    const int tile = order == KV8_LONG_FIRST || at_ < (tiles + 1) / 2 ? tiles - 1 - at_ : at_ - (tiles + 1) / 2;
     const int col0 = tile * COLS, w0 = col0 + 16 * CT * cg;                // the block's and the wave's first column
     const int full = (t.pos + t.cnt) >> lb << lb;                          // keys in finished blocks
     const int wlast = w0 < ncol ? t.pos + min(t.cnt - 1, (w0 + 16 * CT - 1) / G) : -1;   // the last key the wave sees
@@ -428,13 +440,13 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int u = 0; u < D / 64; u++)
-                kk[i][u] = p >= 0 ? *(const uint4 *)(b + (size_t)4 * i * D + 16 * u) : uint4{};
+                kk[i][u] = p >= 0 ? kv8_read<CT == 1 && CG == 1 && KG == 4>(b + (size_t)4 * i * D + 16 * u) : uint4{};
     };
     auto load_v = [&](int s, int p) {
         const int key = 64 * s + 16 * h;
         const uint8_t *b = c.v + (((size_t)p * c.heads + head) * D + cl) * B + (key & (B - 1));
 #pragma unroll
-        for (int i = 0; i < DT; i++) vv[i] = p >= 0 ? *(const uint4 *)(b + (size_t)16 * i * B) : uint4{};
+        for (int i = 0; i < DT; i++) vv[i] = p >= 0 ? kv8_read<CT == 1 && CG == 1 && KG == 4>(b + (size_t)16 * i * B) : uint4{};
     };
     if (s < ns) {
         pk = page_of(64 * s + 16 * gk, pk);
@@ -595,9 +607,21 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     }
     __syncthreads();
     constexpr int TPC = D / 4;                            // threads of a column
-    for (int i = tid; i < COLS * TPC; i += NT) {
-        const int cc = i / TPC, d = i % TPC * 4, col = col0 + cc;
-        if (col >= ncol) continue;
+    constexpr int PER = (COLS * TPC + NT - 1) / NT;       // quads of the block's output a thread
+    auto store = [&](int col, int d, f32x4 num, float den) {
+        num *= kv8_inverse(den);
+        const size_t at = (size_t)(t.r0 + col / G) * ldo + (size_t)(head * G + col % G) * D + d;
+        if constexpr (BF) *(uint2 *)((uint16_t *)out + at) = pack4(num);
+        else *(f32x4 *)((float *)out + at) = num;
+    };
+    // this block's partials, [split][column][LD]
+    constexpr unsigned BYTES = COLS * LD * 4;
+    const unsigned mine = (unsigned)e * (gridDim.x / nsplit) + x;          // of its kv head, sequence and tile
+    const __amdgpu_buffer_rsrc_t rp = buf_rsrc((char *)part + (size_t)mine * nsplit * BYTES, (size_t)nsplit * BYTES);
+#pragma unroll
+    for (int u = 0; u < PER; u++) {
+        const int i = tid + NT * u, cc = i / TPC, d = i % TPC * 4, col = col0 + cc;
+        if (i >= COLS * TPC || col >= ncol) continue;
         float mx = sm[0][cc];
 #pragma unroll
         for (int g = 1; g < KG; g++) mx = fmaxf(mx, sm[g][cc]);
@@ -612,76 +636,54 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
             num += *(const f32x4 *)&so[g][cc][d] * w;
         }
         if (nsplit == 1) {
-            num *= kv8_inverse(den);
-            const size_t at = (size_t)(t.r0 + col / G) * ldo + (size_t)(head * G + col % G) * D + d;
-            if constexpr (BF) *(uint2 *)((uint16_t *)out + at) = pack4(num);
-            else *(f32x4 *)((float *)out + at) = num;
+            store(col, d, num, den);
         } else {
-            float *p = part + (((size_t)e * gridDim.x + blockIdx.x) * COLS + cc) * LD;
-            *(f32x4 *)(p + 4 + d) = num;
-            if (d == 0) { p[0] = mx; p[1] = den; }
+            const unsigned at = split * BYTES + (cc * LD + 4 + d) * 4;
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, num), rp, at, 0, KV8_SC1);
+            if (d == 0)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{mx, den, 0.f, 0.f}), rp, at - 16, 0,
+                                                       KV8_SC1);
         }
     }
-}
-
-// the splits' partials of k_kv8_attend merged: a wave a column, its D / 4 lanes
-// twice (D = 128) or four times (64) over the splits, so that all are read at
-// once
-template <int D, bool BF>
-__global__ __launch_bounds__(NTH) void k_kv8_merge(qm_kv8_t c, void *__restrict__ out, size_t ldo,
-                                                   const int *__restrict__ row, const int *__restrict__ pos, int rows,
-                                                   int max_rows, int G, const float *__restrict__ part, int nsplit,
-                                                   int tiles, int cols) {
-    constexpr int TPC = D / 4, LD = D + 4, GR = WAVE / TPC, PER = KV8_MAX_SPLITS / GR;
-    const int e = blockIdx.z, head = blockIdx.y, lane = threadIdx.x & 63;
-    kv8_entry t;
-    if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
-    const int col = blockIdx.x * (NTH / WAVE) + (threadIdx.x >> 6), d = lane % TPC * 4, gr = lane / TPC;
-    if (col >= t.cnt * G) return;
-    const int y = col / cols * c.heads + head;
-    const float *p = part + (((size_t)e * (tiles * c.heads) + y) * nsplit * cols + col % cols) * LD;
-    float ms[PER], ls[PER];
-    f32x4 o[PER];
+    if (nsplit == 1) return;
+    __shared__ unsigned drawn;
+    __builtin_amdgcn_s_waitcnt(0);                        // this thread's sums have landed
+    __syncthreads();                                      // ... and every thread's
+    if (tid == 0) drawn = __hip_atomic_fetch_add(&kv8_tickets[mine], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (drawn != (unsigned)nsplit - 1u) return;           // uniform over the block
 #pragma unroll
     for (int u = 0; u < PER; u++) {
-        const int s = u * GR + gr;
-        ms[u] = -INFINITY;
-        ls[u] = 0.0f;
-        o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (u * GR < nsplit && s < nsplit) {
-            const float *ps = p + (size_t)s * cols * LD;
-            ms[u] = ps[0];
-            ls[u] = ps[1];
-            o[u] = *(const f32x4 *)(ps + 4 + d);
+        const int i = tid + NT * u, cc = i / TPC, d = i % TPC * 4, col = col0 + cc;
+        if (i >= COLS * TPC || col >= ncol) continue;
+        float mx = -INFINITY, den = 0.0f;
+        f32x4 num = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = 0; s0 < nsplit; s0 += 8) {          // eight splits' reads in flight
+            f32x4 ml[8], o8[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const unsigned at = s0 + k < nsplit ? (s0 + k) * BYTES + cc * LD * 4 : BUF_OOB;
+                ml[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, at, 0, KV8_SC1));
+                o8[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, at + 16 + d * 4, 0, KV8_SC1));
+                if (s0 + k >= nsplit) ml[k].x = -INFINITY;
+            }
+            float nm = mx;
+#pragma unroll
+            for (int k = 0; k < 8; k++) nm = fmaxf(nm, ml[k].x);
+            const float ref = nm == -INFINITY ? 0.0f : nm, r = __builtin_amdgcn_exp2f(mx - ref);
+            den *= r;
+            num *= r;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float w = __builtin_amdgcn_exp2f(ml[k].x - ref);
+                den += w * ml[k].y;
+                num += o8[k] * w;
+            }
+            mx = nm;
         }
+        store(col, d, num, den);
     }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < PER; u++) mx = fmaxf(mx, ms[u]);
-    mx = wave_max(mx);
-    const float ref = mx == -INFINITY ? 0.0f : mx;
-    float den = 0.0f;
-    f32x4 num = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int u = 0; u < PER; u++) {
-        const float g = __builtin_amdgcn_exp2f(ms[u] - ref);
-        den += g * ls[u];
-        num += o[u] * g;
-    }
-    auto join = [](float x) {                             // the groups of lanes
-        f32x2 q;
-        if constexpr (GR == 4) { q = swap16(x); x = q.x + q.y; }
-        q = swap32(x);
-        return q.x + q.y;
-    };
-    den = join(den);
-#pragma unroll
-    for (int i = 0; i < 4; i++) num[i] = join(num[i]);
-    if (gr > 0) return;
-    num *= kv8_inverse(den);
-    const size_t at = (size_t)(t.r0 + col / G) * ldo + (size_t)(head * G + col % G) * D + d;
-    if constexpr (BF) *(uint2 *)((uint16_t *)out + at) = pack4(num);
-    else *(f32x4 *)((float *)out + at) = num;
+    if (tid == 0) __hip_atomic_store(&kv8_tickets[mine], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // ---------------------------------------------------------------------------
@@ -783,10 +785,12 @@ extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, si
 //     keys; for long prompts two of keys and two of columns, which share what
 //     they read (1,999 tokens 43.2 against 45.4 us, 4 x 499 22.0 against 24.6;
 //     500 behind 1,499 37.6 against 22.9 the other way).
-//   Fewer: eight waves on the keys, and the keys split over as many blocks as
-//     leave a wave a step, one block a CU, if a wave would walk more than two:
-//     700 positions 9.7 us on one block a head and 11.2 split, 1,500 14.5 and
-//     11.1, 3,000 18.1 and 11.2; 6 x 8,000 17.9 us on 192 blocks, 25 on 336.
+//   Fewer: the keys split over blocks.  Up to half the CUs, blocks of four waves
+//     with a step each (one head of a kv head's, 700 positions: 8.0 us against
+//     9.7 on one block of eight waves and 9.9 on two, 1,500 8.3 against 10.1);
+//     beyond, blocks of eight waves with a step each as long as there is a CU
+//     for each (6 x 8,000: 17.9 us on 240 blocks, 25 on 336; 4 x 3,000 11.0
+//     against 12.5 with four waves).
 struct kv8_plan { int ct, cg, kg, splits, order, cols, tiles; };
 static kv8_plan kv8_plan_of(const qm_kv8_t *c, int G, int n, int max_rows, int max_ctx, int bf16) {
     const long cols = (long)max_rows * G;
@@ -800,13 +804,17 @@ static kv8_plan kv8_plan_of(const qm_kv8_t *c, int G, int n, int max_rows, int m
         p.tiles = (p.tiles + 1) / 2;
         if ((long)p.tiles * c->heads * n <= 512) p.order = KV8_PAIRED;
     } else if (blocks < 512) {
-        p.kg = 8;
-        const int steps = (max_ctx + 63) / 64 + 1;
-        const long room = 256 / blocks, want = (steps + 7) / 8;
-        if (steps > 16) p.splits = (int)(want < room ? want : room);
+        const int steps = (max_ctx + 63) / 64 + 1;       // the unfinished block's among them
+        static_assert(KV8_TICKETS >= 256 / 2, "a ticket for each block that is split");
+        if (blocks * ((steps + 3) / 4) <= 128) {
+            p.splits = (steps + 3) / 4;
+        } else {
+            p.kg = 8;
+            const long room = 256 / blocks, want = (steps + 7) / 8;
+            if (steps > 16) p.splits = (int)(want < room ? want : room);
+        }
         if (p.splits > KV8_MAX_SPLITS) p.splits = KV8_MAX_SPLITS;
         if (p.splits < 1) p.splits = 1;
-        if (p.splits > 1) p.order = KV8_AS_IS;           // the order of k_kv8_merge
     }
     return p;
 }
@@ -860,16 +868,5 @@ extern "C" int qm_kv8_attention(const qm_kv8_t *c, void *out, const void *q, siz
 #undef ATTEND
 #undef ATTEND_CT
 #undef ATTEND_AS
-    if (hipGetLastError() != hipSuccess) return QH_ELAUNCH;
-    if (p.splits > 1) {
-        const long cols = (long)max_rows * G;
-        const dim3 mg((unsigned)((cols + NTH / WAVE - 1) / (NTH / WAVE)), c->heads, n);
-#define MERGE(D_, BF_)                                                                                               \
-    hipLaunchKernelGGL((k_kv8_merge<D_, BF_>), mg, dim3(NTH), 0, stream(), *c, out, ldo, row, pos, rows, max_rows, G, \
-                       (const float *)work, p.splits, p.tiles, p.cols)
-        if (c->head_dim == 128) { if (bf16) MERGE(128, true); else MERGE(128, false); }
-        else { if (bf16) MERGE(64, true); else MERGE(64, false); }
-#undef MERGE
-    }
     return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
 }

@@ -298,30 +298,46 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
 // ---------------------------------------------------------------------------
 // dst row w of every group = src row parent[w], over `slabs` states of
 // n_group * W rows, each row `runs` stretches of `run_bytes` used bytes.  A
-// thread owns one unit of T at the same place of all W rows: it reads every
-// row it needs before it writes any, so dst may be src, and rows that stay
-// where they are are then not touched.  Bound by the memory's rate.
+// thread owns two units of T, a block's width apart, at the same place of all W
+// rows: it reads every row it needs before it writes any, so dst may be src,
+// and rows that stay where they are are then not touched.  Bound by the
+// memory's rate: the tails of 8 x 8 beams (235 MB, of which a random choice of
+// parents reads two thirds) 81 us, where a copy of as much takes 89; 108 with
+// one unit a thread, 85 with four, 116 with stores through the caches.
+#define REORDER_UNITS 2
 template <typename T, int WT>
 __global__ __launch_bounds__(NTH) void k_beam_reorder(uint8_t *dst, const uint8_t *src, const int *__restrict__ parent,
                                                      int W, unsigned units, unsigned runs, size_t slab_stride,
                                                      size_t seq_stride, size_t run_stride) {
     const int g = blockIdx.y;
-    const unsigned u = blockIdx.x * NTH + threadIdx.x, run = u / units;
-    if (run >= runs) return;
-    const size_t at = (size_t)blockIdx.z * slab_stride + (size_t)g * W * seq_stride + (size_t)run * run_stride +
-                      (size_t)(u - run * units) * sizeof(T);
     const bool same = dst == src;
-    T v[WT];
     int p[WT];
 #pragma unroll
     for (int w = 0; w < WT; w++) {
         p[w] = w < W ? parent[g * W + w] : -1;
         if (p[w] >= W || (same && p[w] == w)) p[w] = -1;
-        if (p[w] >= 0) v[w] = *(const T *)(src + at + (size_t)p[w] * seq_stride);
+    }
+    constexpr int NU = REORDER_UNITS;
+    T v[NU][WT];
+    size_t at[NU];
+    bool in[NU];
+#pragma unroll
+    for (int k = 0; k < NU; k++) {
+        const unsigned u = (blockIdx.x * NU + k) * NTH + threadIdx.x, run = u / units;
+        in[k] = run < runs;
+        at[k] = (size_t)blockIdx.z * slab_stride + (size_t)g * W * seq_stride + (size_t)run * run_stride +
+                (size_t)(u - run * units) * sizeof(T);
     }
 #pragma unroll
-    for (int w = 0; w < WT; w++)
-        if (p[w] >= 0) __builtin_nontemporal_store(v[w], (T *)(dst + at + (size_t)w * seq_stride));
+    for (int k = 0; k < NU; k++)
+#pragma unroll
+        for (int w = 0; w < WT; w++)
+            if (in[k] && p[w] >= 0) v[k][w] = *(const T *)(src + at[k] + (size_t)p[w] * seq_stride);
+#pragma unroll
+    for (int k = 0; k < NU; k++)
+#pragma unroll
+        for (int w = 0; w < WT; w++)
+            if (in[k] && p[w] >= 0) __builtin_nontemporal_store(v[k][w], (T *)(dst + at[k] + (size_t)w * seq_stride));
 }
 
 // ---------------------------------------------------------------------------
@@ -419,7 +435,7 @@ extern "C" int qm_beam_reorder(void *dst, const void *src, const int *parent, in
     const size_t units = run_bytes / (wide ? 16 : 4);
     if (units * runs >= (size_t)1 << 31) return QH_ETOOBIG;
     if (!stream()) return QH_ESTATE;
-    const dim3 grid((unsigned)((units * runs + NTH - 1) / NTH), n_group, slabs);
+    const dim3 grid((unsigned)((units * runs + NTH * REORDER_UNITS - 1) / (NTH * REORDER_UNITS)), n_group, slabs);
 #define REORDER(T, WT)                                                                                               \
     hipLaunchKernelGGL((k_beam_reorder<T, WT>), grid, dim3(NTH), 0, stream(), (uint8_t *)dst, (const uint8_t *)src,  \
                        parent, width, (unsigned)units, (unsigned)runs, slab_stride, seq_stride, run_stride)

@@ -618,7 +618,7 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     constexpr unsigned BYTES = COLS * LD * 4;
     const unsigned mine = (unsigned)e * (gridDim.x / nsplit) + x;          // of its kv head, sequence and tile
     const __amdgpu_buffer_rsrc_t rp = buf_rsrc((char *)part + (size_t)mine * nsplit * BYTES, (size_t)nsplit * BYTES);
-#pragma unroll
+#pragma unroll 1
     for (int u = 0; u < PER; u++) {
         const int i = tid + NT * u, cc = i / TPC, d = i % TPC * 4, col = col0 + cc;
         if (i >= COLS * TPC || col >= ncol) continue;
@@ -652,7 +652,7 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     if (tid == 0) drawn = __hip_atomic_fetch_add(&kv8_tickets[mine], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     if (drawn != (unsigned)nsplit - 1u) return;           // uniform over the block
-#pragma unroll
+#pragma unroll 1
     for (int u = 0; u < PER; u++) {
         const int i = tid + NT * u, cc = i / TPC, d = i % TPC * 4, col = col0 + cc;
         if (i >= COLS * TPC || col >= ncol) continue;

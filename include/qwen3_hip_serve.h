@@ -105,10 +105,11 @@ int qwen3_hip_kv8_attention_dev(const qwen3_hip_kv8 *cache, void *out_d, const v
  * continues (parent, 0 .. width - 1) and whether it is finished (its parent
  * was, or its token is end0 or end1; -1: no such token, which end0 may be only
  * where done_d is NULL).  Equal scores go in
- * the order of width-index and token.  Scores are compared in 64 bits.  A
- * score of -inf (a beam not in use, as all but the first are before the first
- * token; a masked token) or of NaN ranks last: such continuations are taken,
- * in the same order, only where there is nothing else, as -inf.
+ * the order of beam and token.  Scores are compared in 64 bits.  Where fewer
+ * than `width` continuations have a score, the others are taken in the same
+ * order, as -inf: those of beams not in use (a score_d that is not finite; -inf
+ * before the first token for all beams but the first), of tokens whose logit is
+ * -inf or NaN, and of rows with an infinite logit, which have no probabilities.
  * logits_d: fp32 [n_group * width][ld >= vocab]; vocab in width .. 2^21.
  * score_out_d may be score_d and done_out_d done_d.  work_d:
  * qwen3_hip_beam_select_work() bytes, 8-byte aligned. */

@@ -99,25 +99,18 @@ __global__ __launch_bounds__(NTH) void k_beam_pieces(const float *__restrict__ l
     const int base = piece * BEAM_PIECE;
     float v[BEAM_V];
     auto at = [&](int k) { return VEC ? base + (k >> 2) * (4 * WAVE) + 4 * lane + (k & 3) : base + k * WAVE + lane; };
-    // a finished beam's row is not read; a beam that cannot be chosen for its
-    // score offers its first tokens, in case nothing else is left
+    // a finished beam's row is not read; a beam that is not in use offers its
+    // first tokens, in case nothing else is left
     const bool over = done && done[r] != 0;
-    if (over || score[r] == -INFINITY) {
+    if (over || !(fabsf(score[r]) < INFINITY)) {
         if (lane < W) out[(size_t)lane * pieces] = beam_cand{-INFINITY, !over && piece == 0 && lane < vocab ? lane : BEAM_NONE};
         if (lane == 0) sums[(size_t)r * pieces + piece] = beam_sum{-INFINITY, 0.0f};
         return;
     }
-    if constexpr (VEC) {
+    if (VEC && base + BEAM_PIECE <= vocab) {
 #pragma unroll
         for (int k = 0; k < BEAM_V; k += 4) {
-            const int i = at(k);
-            f32x4 t = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (i + 3 < vocab) t = *(const f32x4 *)(x + i);
-            else {
-#pragma unroll
-                for (int u = 0; u < 4; u++)
-                    if (i + u < vocab) t[u] = x[i + u];
-            }
+            const f32x4 t = *(const f32x4 *)(x + at(k));
 #pragma unroll
             for (int u = 0; u < 4; u++) v[k + u] = t[u];
         }
@@ -134,7 +127,7 @@ __global__ __launch_bounds__(NTH) void k_beam_pieces(const float *__restrict__ l
     const float mx = wave_max(lm);
     float sum = 0.0f;
     if (mx > -INFINITY) {
-        // +inf gives NaN: a row without probabilities
+        // +inf gives NaN: a row without probabilities, which the maximum tells
 #pragma unroll
         for (int k = 0; k < BEAM_V; k++) sum += __builtin_amdgcn_exp2f((v[k] - mx) * 1.44269504088896340736f);
     }
@@ -189,7 +182,7 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
     constexpr long BEAM_NOWHERE = 0x7FFFFFFFFFFFFFFFL;
     const int r = g * W + w;                              // launched with W waves
     const bool over = done && done[r] != 0;
-    const double base = score[r];
+    const double base = fabsf(score[r]) < INFINITY ? (double)score[r] : -INFINITY;
     if (lane == 0) sdone[w] = over;
     for (int i = threadIdx.x; i < W * W; i += W * WAVE) ranks[i] = 0;
     if (over) {
@@ -214,7 +207,7 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
         const double lse = (double)mx + log(sum);
         auto put = [&](int k, float v, int i) {
             const double t = base + ((double)v - lse);
-            cv[w * W + k] = t == t ? t : -INFINITY;       // no probabilities, no score
+            cv[w * W + k] = t == t ? t : -INFINITY;       // -inf of a row of -inf
             cid[w * W + k] = i == BEAM_NONE ? BEAM_NOWHERE : (long)w * vocab + i;
         };
         // twice over the lists, eight entries a lane in flight: unrolled over all
@@ -239,7 +232,9 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
 #pragma unroll
                 for (int k = 0; k < BEAM_E; k++) beam_collect(cand, n, t[k].v >= thr, t[k].v, t[k].i);
             }
-        if (n > 0 && n <= BEAM_CAP) {
+        if (mx == INFINITY) {                             // no probabilities: as a beam that is not in use
+            if (lane < W) put(lane, -INFINITY, lane);
+        } else if (n > 0 && n <= BEAM_CAP) {
             if (lane < n) {
                 const beam_cand t = cand[lane];
                 const int rank = beam_rank(cand, n, t);

@@ -28,12 +28,13 @@ def totals(logits, score, done, end0):
     x = np.where(np.isnan(logits), -np.inf, logits).astype(np.float64)
     total = np.full((W, V), np.nan)
     for w in range(W):
+        base = float(score[w]) if np.isfinite(score[w]) else -np.inf
         if done[w]:
-            total[w, end0] = score[w]
+            total[w, end0] = base
             continue
         with np.errstate(all="ignore"):
             m = x[w].max()
-            t = float(score[w]) + (x[w] - (m + np.log(np.exp(x[w] - m).sum())))
+            t = base + (x[w] - (m + np.log(np.exp(x[w] - m).sum())))
         total[w] = np.where(np.isnan(t), -np.inf, t)
     return total
 
@@ -148,6 +149,24 @@ def test_masked_tokens_and_rows_without_probabilities():
     logits[4, 0, 4321] = 1.0
     logits[5] = np.nan
     check(logits, -rng.uniform(0, 1, (6, W)).astype(np.float32), np.zeros((6, W), bool), 1, -1)
+
+
+def test_beams_that_are_not_in_use():
+    """scores that are not finite, of running and of finished beams, and rows without probabilities, as all there is"""
+    rng = np.random.default_rng(7)
+    W, V = 4, 2500
+    logits = rng.standard_normal((5, W, V)).astype(np.float32)
+    score = np.zeros((5, W), np.float32)
+    score[0] = [np.nan, -np.inf, np.inf, -1.0]
+    score[1] = [np.nan, np.inf, -np.inf, np.nan]
+    score[2] = -np.inf
+    logits[3, :, 77] = np.inf
+    logits[4] = -np.inf
+    logits[4, 2, 5] = 0.0
+    done = np.zeros((5, W), bool)
+    done[1, 0] = done[1, 1] = done[2, 3] = True
+    check(logits, score, done, 9, 9)
+    check(logits, score, np.zeros((5, W), bool), -1, -1, in_place=True)
 
 
 def test_select_replayed_from_a_graph(lib):

@@ -177,7 +177,7 @@ int qwen3_hip_batch_open(qwen3_hip_batch **batch, qwen3_hip_model *model, int n_
 
 /* The same with the KV caches in 8 bits (format: QWEN3_HIP_KV8_E4M3 or _INT8
  * of qwen3_hip_serve.h, which says what a cache of blocks of 32 tokens holds):
- * 57,568 bytes per position, rounded up to blocks, and 3.7 MB per sequence for
+ * 57,400 bytes per position, rounded up to blocks, and 3.7 MB per sequence for
  * the unfinished blocks, instead of 229,376 per position.  Every call below
  * takes either kind.  Attention, a prompt's included, reads K and V as the
  * cache holds them, so logits differ from an fp32 batch's by the codes'

@@ -65,6 +65,8 @@ size_t qwen3_hip_kv8_bytes(const qwen3_hip_kv8 *cache);
  * is set, [kv_heads][head_dim] at a stride of ldk / ldv values (a multiple of
  * 16 bytes; 16-byte aligned pointers).  `rows`: rows of k_d and v_d;
  * max_rows: the most rows of an entry.
+ * Where two entries' tables name the same page for a block that this call
+ * finishes, the page holds either's rows or a mix.
  * An entry whose rows do not lie in 0 .. rows, exceed max_rows or max_blocks
  * blocks, or whose pos_d is negative is left out (a negative pos_d leaves a
  * sequence out on purpose); a finished block whose table entry is no page is
@@ -85,9 +87,10 @@ int qwen3_hip_kv8_append_dev(const qwen3_hip_kv8 *cache, const void *k_d, const 
  * page of the pool is left out of the sums, and a row with nothing left is 0.
  * max_ctx: a bound on pos_d[i] + rows of i, which picks the launch (a longer
  * entry is right too).  work_d: qwen3_hip_kv8_attention_work() bytes for the
- * same sizes, 16-byte aligned, written by the call; QWEN3_HIP_ETOOBIG where
+ * same sizes or larger ones (4.4 MB at most; it never shrinks as n, max_rows or
+ * max_ctx grow), 16-byte aligned, written by the call; QWEN3_HIP_ETOOBIG where
  * work_bytes is less.  Calls that share it have to run one after the other, as
- * calls on the library stream do. */
+ * calls on the library stream do.  out_d must not overlap what the call reads. */
 size_t qwen3_hip_kv8_attention_work(const qwen3_hip_kv8 *cache, int q_heads, int n, int max_rows, int max_ctx);
 int qwen3_hip_kv8_attention_dev(const qwen3_hip_kv8 *cache, void *out_d, const void *q_d, size_t ldo, size_t ldq,
                                 int bf16, int q_heads, const int *row_d, const int *pos_d, int n, int rows,

@@ -759,8 +759,8 @@ extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, si
     if (n == 0 || rows == 0) return QH_OK;
     if (!kv8_rows_ok(k, ldk, c->heads * c->head_dim, bf16) || !kv8_rows_ok(v, ldv, c->heads * c->head_dim, bf16))
         return QH_EINVAL;
-    // blocks that max_rows rows touch at most, wherever they start
-    const dim3 grid(c->heads, n, (max_rows + c->block - 2) / c->block + 1);
+    // blocks that an entry's rows touch at most, wherever they start
+    const dim3 grid(c->heads, n, ((max_rows < rows ? max_rows : rows) + c->block - 2) / c->block + 1);
     if (grid.z > 65535) return QH_ETOOBIG;
     if (!stream()) return QH_ESTATE;
 #define APPEND_B(F, D_, B_, BF_) \
@@ -818,16 +818,15 @@ static kv8_plan kv8_plan_of(const qm_kv8_t *c, int G, int n, int max_rows, int m
     }
     return p;
 }
-static size_t kv8_plan_work(const qm_kv8_t *c, int n, const kv8_plan &p) {
-    return p.splits == 1 ? 0 : (size_t)n * c->heads * p.tiles * p.splits * p.cols * (c->head_dim + 4) * sizeof(float);
-}
-
+// Bytes of partials that calls of at most these sizes need: a program asks for
+// its largest once.  Of all launches above that split, with blocks of 16
+// columns, splits <= (steps + 3) / 4 and blocks x splits <= 256; with 32 columns
+// a block, there are as many blocks or fewer.
 extern "C" size_t qm_kv8_attention_work(const qm_kv8_t *c, int q_heads, int n, int max_rows, int max_ctx) {
     if (!c || kv8_sizes(c) || q_heads < c->heads || n < 1 || max_rows < 1 || max_ctx < 1) return 0;
-    const int G = q_heads / c->heads;
-    const size_t a = kv8_plan_work(c, n, kv8_plan_of(c, G, n, max_rows, max_ctx, 0));
-    const size_t b = kv8_plan_work(c, n, kv8_plan_of(c, G, n, max_rows, max_ctx, 1));
-    return a > b ? a : b;
+    const size_t cols = (size_t)max_rows * (q_heads / c->heads), split = ((size_t)(max_ctx - 1) / 64 + 2 + 3) / 4;
+    const size_t most = (size_t)n * c->heads * ((cols + 15) / 16) * split;
+    return split == 1 ? 0 : (most < 256 ? most : 256) * (cols > 16 ? 32 : 16) * (c->head_dim + 4) * sizeof(float);
 }
 
 extern "C" int qm_kv8_attention(const qm_kv8_t *c, void *out, const void *q, size_t ldo, size_t ldq, int bf16, int q_heads,
@@ -843,9 +842,10 @@ extern "C" int qm_kv8_attention(const qm_kv8_t *c, void *out, const void *q, siz
         return QH_EINVAL;
     const int G = q_heads / c->heads;
     const float f = scale * 1.44269504088896340736f;     // the softmax runs on powers of two
-    const kv8_plan p = kv8_plan_of(c, G, n, max_rows, max_ctx, bf16);
-    if (p.splits > 1 && (!work || !aligned16(work))) return QH_EINVAL;
-    if (work_bytes < kv8_plan_work(c, n, p)) return QH_ETOOBIG;
+    const size_t need = qm_kv8_attention_work(c, q_heads, n, max_rows, max_ctx);
+    if (need && (!work || !aligned16(work))) return QH_EINVAL;
+    if (work_bytes < need) return QH_ETOOBIG;
+    const kv8_plan p = kv8_plan_of(c, G, n, max_rows < rows ? max_rows : rows, max_ctx, bf16);
     const long blocks = (long)p.tiles * c->heads * p.splits;
     if (blocks * 512 >= 1L << 32) return QH_ETOOBIG;
     if (!stream()) return QH_ESTATE;

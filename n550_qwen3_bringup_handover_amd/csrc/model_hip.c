@@ -794,13 +794,10 @@ static int open_kv8(qwen3_hip_batch *b, int format) {
     c->v_scale = c->k_scale + NL * b->kv8.scales;
     c->v_tail = c->k_tail + NL * b->kv8.tails;
     c->table = b->table;
-    /* of a step of every sequence, and of the short passes of a prompt that
-     * split the keys */
+    /* of a step of every sequence, and of a prompt's pass */
     b->kv8.work_bytes = qm_kv8_attention_work(c, QW3M_N_HEADS, b->n_seq, 1, b->max_ctx);
-    for (int rows = 1; rows <= QM_MAX_CHUNK; rows++) {
-        const size_t w = qm_kv8_attention_work(c, QW3M_N_HEADS, 1, rows, b->max_ctx);
-        if (w > b->kv8.work_bytes) b->kv8.work_bytes = w;
-    }
+    const size_t pass = qm_kv8_attention_work(c, QW3M_N_HEADS, 1, b->max_ctx, b->max_ctx);
+    if (pass > b->kv8.work_bytes) b->kv8.work_bytes = pass;
     rc = qh_malloc(&b->kv8.work, b->kv8.work_bytes);
     if (!rc) rc = qm_zero_i32(b->kv8.row, 2);
     if (!rc) rc = qm_kv8_own(b->table, NULL, b->n_seq, c->block, c->max_blocks);

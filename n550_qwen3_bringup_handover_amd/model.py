@@ -263,6 +263,10 @@ def main(argv=None):
     ap.add_argument("--kv", choices=("fp32", *KV8_FORMATS), default="fp32", help="how a batch's caches are held")
     ap.add_argument("--beams", type=int, default=0, help="beams of each search of a batch")
     args = ap.parse_args(argv)
+    if (args.beams or args.kv != "fp32") and not args.batch:
+        ap.error("--kv and --beams are a batch's")
+    if args.beams < 0 or (args.beams and args.batch % args.beams):
+        ap.error("--beams must divide --batch")
     blob = qw3m_random(args.seed, LAYOUT_TILE if args.tile else LAYOUT_ROW, threads=16)
     if args.batch:
         return _main_batch(args, blob)

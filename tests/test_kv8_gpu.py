@@ -243,10 +243,10 @@ def test_attention_split_over_blocks(fmt, dim, block, heads, group, bf16, counts
     print(f"splits {fmt} dim {dim} block {block} group {group} bf16 {bf16} {counts}", flush=True)
     rng = np.random.default_rng([dim, block, group])
     before = [3000, 1535, 64, 2047]
-    c = Cache(rng, fmt, heads, dim, block, 4, 3072 // block)
+    c = Cache(rng, fmt, heads, dim, block, 4, 3200 // block)
     c.append(rng, before, bf16)
     pos = c.append(rng, counts, bf16)
-    for ctx in (3072, 1700):
+    for ctx in (3200, 1700):
         assert abi.kv8_attention_work(c.c, heads * group, 4, max(counts), ctx) > 0
         c.check_attention(rng, pos, counts, group, bf16, max_ctx=ctx)
 

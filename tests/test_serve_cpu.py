@@ -82,9 +82,27 @@ def test_attention_needs_its_workspace():
     assert need > 0                                   # its keys are split over blocks
     assert attend(c, bytes=need) == ESTATE
     assert attend(c, bytes=need - 1) == ETOOBIG
-    # a prompt's launch needs none
-    assert runtime.lib().qwen3_hip_kv8_attention_work(ctypes.cast(ctypes.byref(c), runtime.KV8P), 16, 4, 200, 2048) == 0
-    assert attend(c, rows=800, most=200, work=None, bytes=0) == ESTATE
+    # four steps of 64 keys, the unfinished block's among them, are never split
+    assert runtime.lib().qwen3_hip_kv8_attention_work(ctypes.cast(ctypes.byref(c), runtime.KV8P), 16, 4, 200, 192) == 0
+    assert attend(c, rows=800, most=200, ctx=192, work=None, bytes=0) == ESTATE
+
+
+@pytest.mark.parametrize("heads,group", [(8, 2), (1, 1), (3, 16)])
+def test_a_workspace_serves_smaller_calls(heads, group):
+    """asked for once, for the largest call, whatever launch the smaller ones pick"""
+    c = cache(kv_heads=heads, n_seq=64)
+    def work(*a):
+        return runtime.lib().qwen3_hip_kv8_attention_work(ctypes.cast(ctypes.byref(c), runtime.KV8P), heads * group, *a)
+    ns, rows, ctxs = (1, 2, 5, 17, 64), (1, 2, 9, 33, 60, 64, 65, 120, 128, 700), range(64, 2049, 64)
+    for i, n in enumerate(ns):
+        for j, r in enumerate(rows):
+            most = 0
+            for ctx in ctxs:
+                w = work(n, r, ctx)
+                assert w >= most and (not i or w >= work(ns[i - 1], r, ctx)) and (not j or w >= work(n, rows[j - 1], ctx))
+                most = w
+    assert attend(c, heads=heads * group, ldo=1 << 13, ldq=1 << 13, n=64, rows=64, most=64, ctx=448,
+                  bytes=work(64, 700, 2048)) == ESTATE
 
 
 def test_bytes_of_a_cache():
@@ -167,3 +185,10 @@ def test_the_stores_division_is_exact(qmax):
             x = F(xm, 256)
             q = fl(x * y)
             assert fl(q + fl(x - q * s) * y) == fl(x / s), (am, xm)
+
+
+@pytest.mark.parametrize("argv", [["--beams", "4"], ["--kv", "int8"], ["--batch", "6", "--beams", "4"], ["--batch", "4", "--kv", "fp8"]])
+def test_commands_that_are_refused(argv):
+    from n550_qwen3_bringup_handover_amd import model
+    with pytest.raises(SystemExit):
+        model.main(argv)

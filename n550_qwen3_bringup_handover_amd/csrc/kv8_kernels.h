@@ -339,9 +339,12 @@ __device__ __forceinline__ float kv8_inverse(float den) { return den == 0.0f ? 0
 // which k > 0 times each is the score in units of log2, become weights; returns
 // what the sums so far are to be multiplied by
 __device__ __forceinline__ float kv8_softmax(f32x4 (&s)[4], float k, float &m, float &l) {
-    float mx = -INFINITY;
+    auto mx2 = [](float a, float b) { return __builtin_elementwise_maximum(a, b); };
+    float mx = s[0].x;
 #pragma unroll
-    for (int t = 0; t < 4; t++) mx = fmaxf(mx, fmaxf(fmaxf(s[t].x, s[t].y), fmaxf(s[t].z, s[t].w)));
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int i = t ? 0 : 1; i < 4; i++) mx = mx2(mx, s[t][i]);
     const float nm = fmaxf(m, col_max(mx * k));
     const float ref = nm == -INFINITY ? 0.0f : nm;       // nothing seen yet: every weight is 0
     const float r = __builtin_amdgcn_exp2f(m - ref);
@@ -431,22 +434,24 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
         for (int j = 0; j < KS; j++)
             qr_[n][j].load(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + (D / 4) * h + 8 * j, in);
     }
+    // -1: no finished block.  Its lanes read page 0, without a branch, and do not
+    // use what they read
     auto page_of = [&](int key, int p) { return key < full && (unsigned)p < (unsigned)c.n_page ? p : -1; };
     uint4 kk[4][D / 64], vv[DT];
     auto load_k = [&](int s, int p) {
         const int key = 64 * s + 16 * gk;
-        const uint8_t *b = c.k + (((size_t)p * c.heads + head) * B + ((key & (B - 1)) + (lane & 3))) * D + (D / 4) * h;
+        const uint8_t *b = c.k + (((size_t)max(p, 0) * c.heads + head) * B + ((key & (B - 1)) + (lane & 3))) * D + (D / 4) * h;
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int u = 0; u < D / 64; u++)
-                kk[i][u] = p >= 0 ? kv8_read<CT == 1 && CG == 1 && KG == 4>(b + (size_t)4 * i * D + 16 * u) : uint4{};
+                kk[i][u] = kv8_read<CT == 1 && CG == 1 && KG == 4>(b + (size_t)4 * i * D + 16 * u);
     };
     auto load_v = [&](int s, int p) {
         const int key = 64 * s + 16 * h;
-        const uint8_t *b = c.v + (((size_t)p * c.heads + head) * D + cl) * B + (key & (B - 1));
+        const uint8_t *b = c.v + (((size_t)max(p, 0) * c.heads + head) * D + cl) * B + (key & (B - 1));
 #pragma unroll
-        for (int i = 0; i < DT; i++) vv[i] = p >= 0 ? kv8_read<CT == 1 && CG == 1 && KG == 4>(b + (size_t)16 * i * B) : uint4{};
+        for (int i = 0; i < DT; i++) vv[i] = kv8_read<CT == 1 && CG == 1 && KG == 4>(b + (size_t)16 * i * B);
     };
     if (s < ns) {
         pk = page_of(64 * s + 16 * gk, pk);
@@ -504,8 +509,9 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     for (; s < ns; s += stride) {
         load_v(s, pv);
         // (a scale of 0, a block of zeros, would make 0 x -inf of a masked key)
-        const float ks = pv >= 0 ? fmaxf(c.k_scale[(size_t)pv * c.heads + head] * f, FLT_MIN) : 1.0f;
-        const float vs = pv >= 0 ? c.v_scale[(size_t)pv * c.heads + head] : 0.0f;
+        const size_t at = (size_t)max(pv, 0) * c.heads + head;
+        const float ksr = c.k_scale[at], vsr = c.v_scale[at];
+        const float ks = pv >= 0 ? fmaxf(ksr * f, FLT_MIN) : 1.0f, vs = pv >= 0 ? vsr : 0.0f;
         const int nx = s + stride;
         int pkn = -1, pvn = -1;
         if (nx < ns) {
@@ -534,6 +540,8 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
 #pragma unroll
                     for (int r = 0; r < 4; r++) s4[n][i][r] = 4 * i + r <= lim ? s4[n][i][r] : -INFINITY;
             }
+#pragma unroll
+            for (int i = 0; i < DT; i++) vv[i] = pv >= 0 ? vv[i] : uint4{};
         }
         softmax(ks);
 #pragma unroll

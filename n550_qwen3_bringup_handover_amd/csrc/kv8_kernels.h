@@ -407,10 +407,12 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     const int B = c.block, lb = __builtin_ctz(B);
     const int *table = c.table + (size_t)e * c.max_blocks;
     // table entry of a key, and the page it stands for, -1 where there is none.
-    // The first step's are read before anything says how long the sequence is
-    auto entry_of = [&](int key) { return (key >> lb) < c.max_blocks ? table[key >> lb] : -1; };
+    // Entries are read two steps ahead, the first before anything says how long
+    // the sequence is, so that no address waits for one
+    auto entry_of = [&](int key) { return table[min(key >> lb, c.max_blocks - 1)]; };
     int s = KG * split + kg;
     int pk = entry_of(64 * s + 16 * gk), pv = entry_of(64 * s + 16 * h);
+    int ek = entry_of(64 * (s + KG * nsplit) + 16 * gk), ev = entry_of(64 * (s + KG * nsplit) + 16 * h);
     kv8_entry t;
     if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
     const int ncol = t.cnt * G, tiles = (ncol + COLS - 1) / COLS, at_ = x / c.heads;
@@ -422,6 +424,9 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     const int wfirst = w0 < ncol ? t.pos + w0 / G : -1;                    // and the last that all its columns see
     const int ns = (min(full, wlast + 1) + 63) >> 6, stride = KG * nsplit;
 
+    // the lane's dims of the MFMA over the j-th 32: 16 consecutive ones of each 64,
+    // so that the four lanes of a row read 64 consecutive bytes of K
+    auto dim_of = [&](int j) { return 64 * (j >> 1) + 16 * h + 8 * (j & 1); };
     int last[CT];                                                          // the column's last key
     kv8_row<BF> qr_[CT][KS];
 #pragma unroll
@@ -432,7 +437,7 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
         last[n] = in ? t.pos + qr : -1;
 #pragma unroll
         for (int j = 0; j < KS; j++)
-            qr_[n][j].load(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + (D / 4) * h + 8 * j, in);
+            qr_[n][j].load(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + dim_of(j), in);
     }
     // -1: no finished block.  Its lanes read page 0, without a branch, and do not
     // use what they read
@@ -440,12 +445,12 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     uint4 kk[4][D / 64], vv[DT];
     auto load_k = [&](int s, int p) {
         const int key = 64 * s + 16 * gk;
-        const uint8_t *b = c.k + (((size_t)max(p, 0) * c.heads + head) * B + ((key & (B - 1)) + (lane & 3))) * D + (D / 4) * h;
+        const uint8_t *b = c.k + (((size_t)max(p, 0) * c.heads + head) * B + ((key & (B - 1)) + (lane & 3))) * D + 16 * h;
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int u = 0; u < D / 64; u++)
-                kk[i][u] = kv8_read<CT == 1 && CG == 1 && KG == 4>(b + (size_t)4 * i * D + 16 * u);
+                kk[i][u] = kv8_read<CT == 1 && CG == 1 && KG == 4>(b + (size_t)4 * i * D + 64 * u);
     };
     auto load_v = [&](int s, int p) {
         const int key = 64 * s + 16 * h;
@@ -507,18 +512,14 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     };
 
     for (; s < ns; s += stride) {
-        load_v(s, pv);
-        // (a scale of 0, a block of zeros, would make 0 x -inf of a masked key)
+        // In this order, and without a branch, so that nothing below waits for
+        // loads behind those it needs
         const size_t at = (size_t)max(pv, 0) * c.heads + head;
-        const float ksr = c.k_scale[at], vsr = c.v_scale[at];
-        const float ks = pv >= 0 ? fmaxf(ksr * f, FLT_MIN) : 1.0f, vs = pv >= 0 ? vsr : 0.0f;
-        const int nx = s + stride;
-        int pkn = -1, pvn = -1;
-        if (nx < ns) {
-            const int ka = 64 * nx + 16 * gk, va = 64 * nx + 16 * h;
-            pkn = page_of(ka, entry_of(ka));
-            pvn = page_of(va, entry_of(va));
-        }
+        float ks = c.k_scale[at] * f, vs = c.v_scale[at];
+        const int nx = s + stride, pkn = page_of(64 * nx + 16 * gk, ek), pvn = page_of(64 * nx + 16 * h, ev);
+        ek = entry_of(64 * (nx + stride) + 16 * gk);
+        ev = entry_of(64 * (nx + stride) + 16 * h);
+        load_v(s, pv);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             bf16x8 kf[KS];
@@ -529,7 +530,7 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
             }
             score(i, kf);
         }
-        if (nx < ns) load_k(nx, pkn);
+        load_k(nx, pkn);
         __builtin_amdgcn_sched_barrier(0);                // V's codes are not converted before they are needed
         if (64 * s + 63 > wfirst || 64 * s + 64 > full || __any(pv < 0)) {
 #pragma unroll
@@ -542,8 +543,11 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
             }
 #pragma unroll
             for (int i = 0; i < DT; i++) vv[i] = pv >= 0 ? vv[i] : uint4{};
+            ks = pv >= 0 ? ks : 1.0f;
+            vs = pv >= 0 ? vs : 0.0f;
         }
-        softmax(ks);
+        // (a scale of 0, a block of zeros, would make 0 x -inf of a masked key)
+        softmax(fmaxf(ks, FLT_MIN));
 #pragma unroll
         for (int s2 = 0; s2 < 2; s2++) {
             bf16x8 pf[CT][NW];
@@ -568,7 +572,7 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int j = 0; j < KS; j++)
-                tk[i][j] = *(const bf16x8 *)(kt + (size_t)min(16 * gk + 4 * i + (lane & 3), B - 1) * D + (D / 4) * h + 8 * j);
+                tk[i][j] = *(const bf16x8 *)(kt + (size_t)min(16 * gk + 4 * i + (lane & 3), B - 1) * D + dim_of(j));
 #pragma unroll
         for (int s2 = 0; s2 < 2; s2++)
 #pragma unroll

@@ -298,11 +298,10 @@ __device__ __forceinline__ f32x4 kv8_mma(bf16x8 a, bf16x8 b, f32x4 c) {
 template <bool BF>
 struct kv8_row {
     f32x4 a, b;
-    __device__ __forceinline__ void load(const void *q, size_t i, bool in) {
-        a = b = f32x4{0.f, 0.f, 0.f, 0.f};
+    __device__ __forceinline__ void load(const void *q, size_t i) {
         if constexpr (BF) {
-            if (in) a = *(const f32x4 *)((const __bf16 *)q + i);
-        } else if (in) {
+            a = *(const f32x4 *)((const __bf16 *)q + i);
+        } else {
             a = *(const f32x4 *)((const float *)q + i);
             b = *(const f32x4 *)((const float *)q + i + 4);
         }
@@ -395,7 +394,8 @@ template <int FMT, int D, bool BF, int CT, int CG, int KG>
 __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void *__restrict__ out,
                                                                const void *__restrict__ q, size_t ldo, size_t ldq,
                                                                const int *__restrict__ row, const int *__restrict__ pos,
-                                                               int rows, int max_rows, int G, float f, int nsplit,
+                                                               int rows, int max_rows, int G, unsigned inv_G, float f,
+                                                               int nsplit,
                                                                int order, float *__restrict__ part) {
     constexpr int NP = BF ? 1 : 3, NW = !BF ? 3 : CT == 1 ? 2 : 1;         // pieces of q, and of a weight
     constexpr int KS = D / 32, DT = D / 16, LD = D + 4, COLS = 16 * CT * CG, NT = WAVE * CG * KG;
@@ -415,13 +415,15 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     int ek = entry_of(64 * (s + KG * nsplit) + 16 * gk), ev = entry_of(64 * (s + KG * nsplit) + 16 * h);
     kv8_entry t;
     if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
+    // column / G, exact up to 2^26 columns of up to 64 a row
+    auto row_of = [&](int col) { return inv_G ? (int)__umulhi((unsigned)col, inv_G) : col; };
     const int ncol = t.cnt * G, tiles = (ncol + COLS - 1) / COLS, at_ = x / c.heads;
     if (at_ >= tiles) return;
     const int tile = order == KV8_LONG_FIRST || at_ < (tiles + 1) / 2 ? tiles - 1 - at_ : at_ - (tiles + 1) / 2;
     const int col0 = tile * COLS, w0 = col0 + 16 * CT * cg;                // the block's and the wave's first column
     const int full = (t.pos + t.cnt) >> lb << lb;                          // keys in finished blocks
-    const int wlast = w0 < ncol ? t.pos + min(t.cnt - 1, (w0 + 16 * CT - 1) / G) : -1;   // the last key the wave sees
-    const int wfirst = w0 < ncol ? t.pos + w0 / G : -1;                    // and the last that all its columns see
+    const int wlast = w0 < ncol ? t.pos + min(t.cnt - 1, row_of(w0 + 16 * CT - 1)) : -1;   // the last key the wave sees
+    const int wfirst = w0 < ncol ? t.pos + row_of(w0) : -1;                    // and the last that all its columns see
     const int ns = (min(full, wlast + 1) + 63) >> 6, stride = KG * nsplit;
 
     // the lane's dims of the MFMA over the j-th 32: 16 consecutive ones of each 64,
@@ -433,16 +435,17 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     for (int n = 0; n < CT; n++) {
         const int col = w0 + 16 * n + cl;
         const bool in = col < ncol;
-        const int qr = in ? col / G : 0, qg = in ? col % G : 0;
+        const int qr = in ? row_of(col) : 0, qg = in ? col - qr * G : 0;   // a lane without a column reads the first's
         last[n] = in ? t.pos + qr : -1;
 #pragma unroll
         for (int j = 0; j < KS; j++)
-            qr_[n][j].load(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + dim_of(j), in);
+            qr_[n][j].load(q, (size_t)(t.r0 + qr) * ldq + (size_t)(head * G + qg) * D + dim_of(j));
     }
     // -1: no finished block.  Its lanes read page 0, without a branch, and do not
     // use what they read
     auto page_of = [&](int key, int p) { return key < full && (unsigned)p < (unsigned)c.n_page ? p : -1; };
     uint4 kk[4][D / 64], vv[DT];
+    float ksn = 0.0f, vsn = 0.0f;                                          // the next step's scales
     auto load_k = [&](int s, int p) {
         const int key = 64 * s + 16 * gk;
         const uint8_t *b = c.k + (((size_t)max(p, 0) * c.heads + head) * B + ((key & (B - 1)) + (lane & 3))) * D + 16 * h;
@@ -462,6 +465,9 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
         pk = page_of(64 * s + 16 * gk, pk);
         pv = page_of(64 * s + 16 * h, pv);
         load_k(s, pk);
+        const size_t at = (size_t)max(pv, 0) * c.heads + head;
+        ksn = c.k_scale[at];
+        vsn = c.v_scale[at];
     }
     bf16x8 qf[CT][KS][NP];
     float m[CT], l[CT];
@@ -514,12 +520,15 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     for (; s < ns; s += stride) {
         // In this order, and without a branch, so that nothing below waits for
         // loads behind those it needs
-        const size_t at = (size_t)max(pv, 0) * c.heads + head;
-        float ks = c.k_scale[at] * f, vs = c.v_scale[at];
+        load_v(s, pv);
         const int nx = s + stride, pkn = page_of(64 * nx + 16 * gk, ek), pvn = page_of(64 * nx + 16 * h, ev);
         ek = entry_of(64 * (nx + stride) + 16 * gk);
         ev = entry_of(64 * (nx + stride) + 16 * h);
-        load_v(s, pv);
+        float ks = ksn * f, vs = vsn;
+        const size_t at = (size_t)max(pvn, 0) * c.heads + head;
+        ksn = c.k_scale[at];
+        vsn = c.v_scale[at];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             bf16x8 kf[KS];
@@ -622,7 +631,8 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
     constexpr int PER = (COLS * TPC + NT - 1) / NT;       // quads of the block's output a thread
     auto store = [&](int col, int d, f32x4 num, float den) {
         num *= kv8_inverse(den);
-        const size_t at = (size_t)(t.r0 + col / G) * ldo + (size_t)(head * G + col % G) * D + d;
+        const int qr = row_of(col);
+        const size_t at = (size_t)(t.r0 + qr) * ldo + (size_t)(head * G + col - qr * G) * D + d;
         if constexpr (BF) *(uint2 *)((uint16_t *)out + at) = pack4(num);
         else *(f32x4 *)((float *)out + at) = num;
     };
@@ -853,6 +863,7 @@ extern "C" int qm_kv8_attention(const qm_kv8_t *c, void *out, const void *q, siz
     if (!kv8_rows_ok(q, ldq, q_heads * c->head_dim, bf16) || !kv8_rows_ok(out, ldo, q_heads * c->head_dim, bf16))
         return QH_EINVAL;
     const int G = q_heads / c->heads;
+    const unsigned inv_G = G == 1 ? 0 : (unsigned)(((1ull << 32) + G - 1) / G);
     const float f = scale * 1.44269504088896340736f;     // the softmax runs on powers of two
     const size_t need = qm_kv8_attention_work(c, q_heads, n, max_rows, max_ctx);
     if (need && (!work || !aligned16(work))) return QH_EINVAL;
@@ -864,7 +875,7 @@ extern "C" int qm_kv8_attention(const qm_kv8_t *c, void *out, const void *q, siz
     const dim3 grid((unsigned)blocks, n);
 #define ATTEND_AS(F, D_, BF_, CT_, CG_, KG_)                                                                           \
     hipLaunchKernelGGL((k_kv8_attend<F, D_, BF_, CT_, CG_, KG_>), grid, dim3(WAVE *CG_ *KG_), 0, stream(), *c, out, q, ldo, \
-                       ldq, row, pos, rows, max_rows, G, f, p.splits, p.order, (float *)work)
+                       ldq, row, pos, rows, max_rows, G, inv_G, f, p.splits, p.order, (float *)work)
 #define ATTEND_CT(F, D_, BF_, CT_)                                \
     do {                                                          \
         if (p.cg == 2) ATTEND_AS(F, D_, BF_, CT_, 2, 2);          \

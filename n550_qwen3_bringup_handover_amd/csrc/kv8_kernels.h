@@ -803,16 +803,20 @@ extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, si
 // The launch for max_rows x G columns a kv head and sequence.
 //   CT: two column tiles a wave where rows are bf16 and there are more than 16
 //     columns (fp32 rows take the registers for their pieces).
-//   Blocks that fill the CUs twice (512 of four waves, two a CU): four groups of
-//     keys; for long prompts two of keys and two of columns, which share what
-//     they read (1,999 tokens 43.2 against 45.4 us, 4 x 499 22.0 against 24.6;
-//     500 behind 1,499 37.6 against 22.9 the other way).
-//   Fewer: the keys split over blocks.  Up to half the CUs, blocks of four waves
-//     with a step each (one head of a kv head's, 700 positions: 8.0 us against
-//     9.7 on one block of eight waves and 9.9 on two, 1,500 8.3 against 10.1);
-//     beyond, blocks of eight waves with a step each as long as there is a CU
-//     for each (6 x 8,000: 17.9 us on 240 blocks, 25 on 336; 4 x 3,000 11.0
-//     against 12.5 with four waves).
+//   Long prompts: blocks of two groups of keys and two of columns, which share
+//     what they read (1,999 tokens 35.6 against 38.1 us with four groups of keys,
+//     8 x 250 14.9 against 19.2; fp32 58 against 67).
+//   Few blocks: the keys split over blocks of four waves, a step a wave, up to
+//     128 blocks (one head of a kv head's, 700 positions: 8.0 us against 9.7 on
+//     one block of eight waves and 9.9 on two, 1,500 8.3 against 10.1).
+//   Between: four groups of keys where a wave of eight would have a step or two
+//     (32 x 700 positions 10.8 against 11.5 us, 60 x 700 17.6 against 20.1) or
+//     where columns see different numbers of keys and there is a block for each
+//     CU (1,000 tokens 16.1 against 19.6, fp32 500 behind 1,499 28.9 against
+//     33.5); eight elsewhere, which read ahead further (8 x 960 positions 10.0
+//     against 10.5 us, 40 x 2,000 34.4 against 36.7), with the keys of long
+//     contexts split over blocks as long as there is a CU for each (6 x 8,000:
+//     17.9 us on 240 blocks, 25 on 336).
 struct kv8_plan { int ct, cg, kg, splits, order, cols, tiles; };
 static kv8_plan kv8_plan_of(const qm_kv8_t *c, int G, int n, int max_rows, int max_ctx, int bf16) {
     const long cols = (long)max_rows * G;
@@ -828,9 +832,10 @@ static kv8_plan kv8_plan_of(const qm_kv8_t *c, int G, int n, int max_rows, int m
     } else if (blocks < 512) {
         const int steps = (max_ctx + 63) / 64 + 1;       // the unfinished block's among them
         static_assert(KV8_TICKETS >= 256 / 2, "a ticket for each block that is split");
+        const bool cu_each = blocks >= 256;
         if (blocks * ((steps + 3) / 4) <= 128) {
             p.splits = (steps + 3) / 4;
-        } else {
+        } else if (steps > (p.tiles > 1 || cu_each ? 16 : 12) && !(p.tiles > 1 && cu_each)) {
             p.kg = 8;
             const long room = 256 / blocks, want = (steps + 7) / 8;
             if (steps > 16) p.splits = (int)(want < room ? want : room);

@@ -181,6 +181,17 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
     __shared__ int sdone[BEAM_MAX], ranks[BEAM_MAX * BEAM_MAX];
     constexpr long BEAM_NOWHERE = 0x7FFFFFFFFFFFFFFFL;
     const int r = g * W + w;                              // launched with W waves
+    const beam_sum *ps = sums + (size_t)r * pieces;
+    const beam_cand *pl = lists + (size_t)r * pieces * W;
+    const int entries = pieces * W;
+    // the first reads of everything at once: each costs the kernel a microsecond
+    // if it waits for another
+    beam_cand first[BEAM_E];
+    beam_sum sum0[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) sum0[k] = lane + WAVE * k < pieces ? ps[lane + WAVE * k] : beam_sum{-INFINITY, 0.0f};
+#pragma unroll
+    for (int k = 0; k < BEAM_E; k++) first[k] = lane + WAVE * k < entries ? pl[lane + WAVE * k] : beam_cand{-INFINITY, BEAM_NONE};
     const bool over = done && done[r] != 0;
     const double base = fabsf(score[r]) < INFINITY ? (double)score[r] : -INFINITY;
     if (lane == 0) sdone[w] = over;
@@ -191,17 +202,17 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
             cid[w * W + lane] = lane == 0 ? (long)w * vocab + end0 : BEAM_NOWHERE;
         }
     } else {
-        const beam_sum *ps = sums + (size_t)r * pieces;
-        const beam_cand *pl = lists + (size_t)r * pieces * W;
-        const int entries = pieces * W;
-        float mx = -INFINITY;
-#pragma unroll 2
-        for (int p = lane; p < pieces; p += WAVE) mx = fmaxf(mx, ps[p].m);
+        float mx = fmaxf(sum0[0].m, sum0[1].m);
+        for (int p = lane + 2 * WAVE; p < pieces; p += WAVE) mx = fmaxf(mx, ps[p].m);
         mx = wave_max(mx);
         // log of the sum of e^x over the row
         double sum = 0.0;
-        for (int p = lane; p < pieces; p += WAVE)
-            if (ps[p].m > -INFINITY) sum += (double)ps[p].s * exp((double)ps[p].m - (double)mx);
+        auto add = [&](beam_sum t) {
+            if (t.m > -INFINITY) sum += (double)t.s * exp((double)t.m - (double)mx);
+        };
+        add(sum0[0]);
+        add(sum0[1]);
+        for (int p = lane + 2 * WAVE; p < pieces; p += WAVE) add(ps[p]);
 #pragma unroll
         for (int s = 32; s >= 1; s >>= 1) sum += __shfl_xor(sum, s);
         const double lse = (double)mx + log(sum);
@@ -213,7 +224,9 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
         // twice over the lists, eight entries a lane in flight: unrolled over all
         // of them, in registers, the kernel spends its time fetching instructions
         float lm = -INFINITY;
-        for (int i0 = lane; i0 < entries; i0 += BEAM_E * WAVE) {
+#pragma unroll
+        for (int k = 0; k < BEAM_E; k++) lm = fmaxf(lm, first[k].v);
+        for (int i0 = lane + BEAM_E * WAVE; i0 < entries; i0 += BEAM_E * WAVE) {
             float v[BEAM_E];
 #pragma unroll
             for (int k = 0; k < BEAM_E; k++) v[k] = i0 + WAVE * k < entries ? pl[i0 + WAVE * k].v : -INFINITY;
@@ -223,8 +236,10 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
         const float thr = beam_threshold(lm, W);
         beam_cand *cand = cands[w];
         int n = 0;
-        if (thr > -INFINITY)
-            for (int i0 = lane; i0 - lane < entries; i0 += BEAM_E * WAVE) {
+        if (thr > -INFINITY) {
+#pragma unroll
+            for (int k = 0; k < BEAM_E; k++) beam_collect(cand, n, first[k].v >= thr, first[k].v, first[k].i);
+            for (int i0 = lane + BEAM_E * WAVE; i0 - lane < entries; i0 += BEAM_E * WAVE) {
                 beam_cand t[BEAM_E];
 #pragma unroll
                 for (int k = 0; k < BEAM_E; k++)
@@ -232,6 +247,7 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
 #pragma unroll
                 for (int k = 0; k < BEAM_E; k++) beam_collect(cand, n, t[k].v >= thr, t[k].v, t[k].i);
             }
+        }
         if (mx == INFINITY) {                             // no probabilities: as a beam that is not in use
             if (lane < W) put(lane, -INFINITY, lane);
         } else if (n > 0 && n <= BEAM_CAP) {

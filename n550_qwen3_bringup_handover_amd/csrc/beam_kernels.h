@@ -184,16 +184,26 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
     const beam_sum *ps = sums + (size_t)r * pieces;
     const beam_cand *pl = lists + (size_t)r * pieces * W;
     const int entries = pieces * W;
-    // the first reads of everything at once: each costs the kernel a microsecond
-    // if it waits for another
+    // the first reads of everything at once, without branches around them: each
+    // costs the kernel a microsecond if it waits for another
+    const int dn = *(done ? done + r : (const int *)ps);
+    const float sc = score[r];
     beam_cand first[BEAM_E];
     beam_sum sum0[2];
+    auto entry = [&](int i) {
+        const beam_cand t = pl[min(i, entries - 1)];
+        return beam_cand{i < entries ? t.v : -INFINITY, i < entries ? t.i : BEAM_NONE};
+    };
 #pragma unroll
-    for (int k = 0; k < 2; k++) sum0[k] = lane + WAVE * k < pieces ? ps[lane + WAVE * k] : beam_sum{-INFINITY, 0.0f};
+    for (int k = 0; k < 2; k++) sum0[k] = ps[min(lane + WAVE * k, pieces - 1)];
 #pragma unroll
-    for (int k = 0; k < BEAM_E; k++) first[k] = lane + WAVE * k < entries ? pl[lane + WAVE * k] : beam_cand{-INFINITY, BEAM_NONE};
-    const bool over = done && done[r] != 0;
-    const double base = fabsf(score[r]) < INFINITY ? (double)score[r] : -INFINITY;
+    for (int k = 0; k < BEAM_E; k++) first[k] = entry(lane + WAVE * k);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+        if (lane + WAVE * k >= pieces) sum0[k].m = -INFINITY;
+    const bool over = done && dn != 0;
+    const double base = fabsf(sc) < INFINITY ? (double)sc : -INFINITY;
     if (lane == 0) sdone[w] = over;
     for (int i = threadIdx.x; i < W * W; i += W * WAVE) ranks[i] = 0;
     if (over) {
@@ -229,7 +239,7 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
         for (int i0 = lane + BEAM_E * WAVE; i0 < entries; i0 += BEAM_E * WAVE) {
             float v[BEAM_E];
 #pragma unroll
-            for (int k = 0; k < BEAM_E; k++) v[k] = i0 + WAVE * k < entries ? pl[i0 + WAVE * k].v : -INFINITY;
+            for (int k = 0; k < BEAM_E; k++) v[k] = entry(i0 + WAVE * k).v;
 #pragma unroll
             for (int k = 0; k < BEAM_E; k++) lm = fmaxf(lm, v[k]);
         }
@@ -242,8 +252,7 @@ __global__ __launch_bounds__(WAVE *BEAM_MAX) void k_beam_pick(int vocab, int W, 
             for (int i0 = lane + BEAM_E * WAVE; i0 - lane < entries; i0 += BEAM_E * WAVE) {
                 beam_cand t[BEAM_E];
 #pragma unroll
-                for (int k = 0; k < BEAM_E; k++)
-                    t[k] = i0 + WAVE * k < entries ? pl[i0 + WAVE * k] : beam_cand{-INFINITY, BEAM_NONE};
+                for (int k = 0; k < BEAM_E; k++) t[k] = entry(i0 + WAVE * k);
 #pragma unroll
                 for (int k = 0; k < BEAM_E; k++) beam_collect(cand, n, t[k].v >= thr, t[k].v, t[k].i);
             }

@@ -92,7 +92,9 @@ __global__ __launch_bounds__(NTH) void k_beam_pieces(const float *__restrict__ l
                                                     beam_cand *__restrict__ lists) {
     __shared__ beam_cand cands[NTH / WAVE][BEAM_CAP];
     const int lane = threadIdx.x & 63;
-    const int piece = blockIdx.x * (NTH / WAVE) + (threadIdx.x >> 6), r = blockIdx.y;
+    const int r = blockIdx.y, piece = blockIdx.x * (NTH / WAVE) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int dn = *(done ? done + r : (const int *)score);     // both reads at once
+    const float sc = score[r];
     if (piece >= pieces) return;
     beam_cand *out = lists + (size_t)r * pieces * W + piece;             // entry w at w * pieces
     const float *x = logits + (size_t)r * ld;
@@ -101,8 +103,8 @@ __global__ __launch_bounds__(NTH) void k_beam_pieces(const float *__restrict__ l
     auto at = [&](int k) { return VEC ? base + (k >> 2) * (4 * WAVE) + 4 * lane + (k & 3) : base + k * WAVE + lane; };
     // a finished beam's row is not read; a beam that is not in use offers its
     // first tokens, in case nothing else is left
-    const bool over = done && done[r] != 0;
-    if (over || !(fabsf(score[r]) < INFINITY)) {
+    const bool over = done && dn != 0;
+    if (over || !(fabsf(sc) < INFINITY)) {
         if (lane < W) out[(size_t)lane * pieces] = beam_cand{-INFINITY, !over && piece == 0 && lane < vocab ? lane : BEAM_NONE};
         if (lane == 0) sums[(size_t)r * pieces + piece] = beam_sum{-INFINITY, 0.0f};
         return;
@@ -116,7 +118,10 @@ __global__ __launch_bounds__(NTH) void k_beam_pieces(const float *__restrict__ l
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < BEAM_V; k++) v[k] = at(k) < vocab ? x[at(k)] : -INFINITY;
+        for (int k = 0; k < BEAM_V; k++) {
+            const float t = x[min(at(k), vocab - 1)];
+            v[k] = at(k) < vocab ? t : -INFINITY;
+        }
     }
     float lm = -INFINITY;
 #pragma unroll

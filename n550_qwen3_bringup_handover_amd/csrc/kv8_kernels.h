@@ -157,6 +157,8 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
     if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
     const int end = t.pos + t.cnt, b0 = t.pos / B, bl = end / B, b = b0 + z;
     if (b >= bl && z > 0) return;
+    const int kr = tid / (D / 16), kd = tid % (D / 16) * 16;           // the thread's K: slot and dims
+    const int vd = tid % D, vr = tid / D * 16;                         // and V: dim and slots
     __bf16 *kt = (__bf16 *)c.k_tail + ((size_t)e * c.heads + h) * (B * D);
     __bf16 *vt = (__bf16 *)c.v_tail + ((size_t)e * c.heads + h) * (B * D);
 
@@ -164,8 +166,6 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
         const int page = c.table[(size_t)e * c.max_blocks + b];
         const int have = max(t.pos - b * B, 0);           // rows in the tail, < B
         const int p0 = t.r0 + b * B - t.pos;              // row of the block's slot 0 (before r0 where some are in the tail)
-        const int kr = tid / (D / 16), kd = tid % (D / 16) * 16;       // K: slot and dims
-        const int vd = tid % D, vr = tid / D * 16;                     // V: dim and slots
         // every load first, the tail's too where some of the rows lie there
         kv8_16<true> kold = {}, vold = {};
         if (have > 0) {
@@ -180,6 +180,7 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
             const size_t i = (size_t)(p0 + max(vr + j, have)) * ldv + h * D + vd;
             vnew[j] = BF ? (float)((const __bf16 *)vn)[i] : ((const float *)vn)[i];
         }
+        __builtin_amdgcn_sched_barrier(0);                // all in flight before the first is waited for
         __bf16 x[16], y[16];
 #pragma unroll
         for (int j = 0; j < 16; j++) {
@@ -220,15 +221,41 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
         }
     }
     if (z > 0) return;
-    const int from = max(t.pos, bl * B);
-    for (int i = tid; i < (end - from) * D; i += NT) {
-        const int p = from + i / D, d = i % D;
-        const size_t r = t.r0 + p - t.pos;
-        const float a = BF ? (float)((const __bf16 *)kn)[r * ldk + h * D + d] : ((const float *)kn)[r * ldk + h * D + d];
-        const float o = BF ? (float)((const __bf16 *)vn)[r * ldv + h * D + d] : ((const float *)vn)[r * ldv + h * D + d];
-        kt[(p - bl * B) * D + d] = kv8_held(a);
-        vt[d * B + (p - bl * B)] = kv8_held(o);
+    // slots lo .. hi - 1 of the tail, which begin with row p0
+    const int lo = max(t.pos - bl * B, 0), hi = end - bl * B, p0 = t.r0 + bl * B - t.pos;
+    if (hi - lo <= NT / D) {                              // a row or few: a value of K and of V a thread
+        const int slot = lo + tid / D;
+        if (slot >= hi) return;
+        const size_t r = p0 + slot;
+        const float a = BF ? (float)((const __bf16 *)kn)[r * ldk + h * D + vd] : ((const float *)kn)[r * ldk + h * D + vd];
+        const float o = BF ? (float)((const __bf16 *)vn)[r * ldv + h * D + vd] : ((const float *)vn)[r * ldv + h * D + vd];
+        kt[slot * D + vd] = kv8_held(a);
+        vt[vd * B + slot] = kv8_held(o);
+        return;
     }
+    // the units of a block again, all loads first (of the nearest row that is there)
+    kv8_16<BF> kx;
+    float vx[16];
+    kx.load(kn, (size_t)(p0 + min(max(kr, lo), hi - 1)) * ldk + h * D + kd);
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+        const size_t i = (size_t)(p0 + min(max(vr + j, lo), hi - 1)) * ldv + h * D + vd;
+        vx[j] = BF ? (float)((const __bf16 *)vn)[i] : ((const float *)vn)[i];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (kr >= lo && kr < hi) {
+        __bf16 *o = kt + kr * D + kd;
+#pragma unroll
+        for (int j = 0; j < 16; j += 8) {
+            bf16x8 u;
+#pragma unroll
+            for (int n = 0; n < 8; n++) u[n] = kv8_held(kx.at(j + n));
+            *(bf16x8 *)(o + j) = u;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+        if (vr + j >= lo && vr + j < hi) vt[vd * B + vr + j] = kv8_held(vx[j]);
 }
 
 // ---------------------------------------------------------------------------

@@ -146,6 +146,12 @@ struct kv8_16 {
 // tail.  The rows behind the last finished block go to the tail, by z = 0
 // alone and after it has read the tail: two blocks of one launch must not meet
 // there.
+// Bound by latencies: position, rows and tail, exchange, codes.  A row each of
+// 64 sequences (3 % of which finish a block) 5.9 us, 3.1 where none does; 1,999
+// rows (20.5 MB) 7.7 us, 16 x 300 5.9, where a copy of as much takes 3.9 and
+// 1.2.  With the loads in the compiler's order, conversions between them, and
+// the tail's values one a thread and turn, 9.9 and 7.7; in two passes over
+// memory 18.5.
 template <int FMT, int D, int B, bool BF>
 __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void *__restrict__ kn,
                                                          const void *__restrict__ vn, size_t ldk, size_t ldv,
@@ -261,10 +267,10 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
 // ---------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------
-// Both kernels work on S^T = K Q^T and O^T += V^T P^T with 16x16x32 bf16
-// MFMAs, the columns being query rows (row r, query head g of the kv head:
-// column r G + g), 64 keys a step.  8-bit codes are exact in bf16, so the
-// scales stay outside: K's multiplies the scores, V's the weights.
+// S^T = K Q^T and O^T += V^T P^T with 16x16x32 bf16 MFMAs, the columns being
+// query rows (row r, query head g of the kv head: column r G + g), 64 keys a
+// step.  8-bit codes are exact in bf16, so the scales stay outside: K's
+// multiplies the scores, V's the weights.
 // fp32 rows keep fp32 accuracy: q and the weights go through the matrix cores
 // as three bf16 pieces each (8 bits apiece: x - x1 - x2 - x3 < 2^-24 x).  bf16
 // rows are one piece; their weights are two where the bytes bound the kernel
@@ -405,6 +411,15 @@ __device__ __forceinline__ float kv8_softmax(f32x4 (&s)[4], float k, float &m, f
 //   many (a prompt): two groups of keys, two of columns; the column tiles with
 //   the longest contexts first, or, where all blocks fit the CUs at once, so
 //   that the two blocks of a CU are a long and a short one
+// Few columns are bound by the bytes: 64 sequences at 2,048 positions (238 MB)
+// 44.5 us, 5.3 TB/s, where a copy reaches 5.3; with fewer blocks than CUs by
+// the chain of latencies of a block and the merge (700 positions 7.5 us).
+// Prompts are bound by the vector instructions that make operands and weights,
+// behind which the two waves a SIMD has registers for hide the products only in
+// part: of 64 products (19 cycles each) and about 480 others a step of a wave,
+// 128 convert codes (6) and 32 are exponentials (9).  2,048 rows behind 6,000
+// 147 us, 800 TFLOP/s; 1,999 behind nothing 32 us, 506, where the columns with
+// the most keys end alone.
 #define KV8_MAX_SPLITS 32
 template <bool NT>
 __device__ __forceinline__ uint4 kv8_read(const uint8_t *p) {

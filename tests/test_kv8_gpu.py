@@ -237,7 +237,8 @@ def test_attention_of_several_rows(fmt, dim, block, heads, group, bf16, counts, 
 @pytest.mark.parametrize("fmt,dim,block,heads,group,bf16,counts", [
     ("e4m3", 128, 32, 1, 2, False, [1, 1, 1, 1]), ("int8", 128, 64, 1, 8, True, [1, 1, 1, 1]),
     ("e4m3", 64, 16, 2, 1, True, [1, 1, 0, 1]), ("int8", 64, 32, 1, 3, False, [1, 1, 1, 1]),
-    ("e4m3", 128, 32, 1, 2, False, [17, 1, 30, 2]), ("int8", 128, 16, 1, 4, True, [3, 16, 1, 0])])
+    ("e4m3", 128, 32, 1, 2, False, [17, 1, 30, 2]), ("int8", 128, 16, 1, 4, True, [3, 16, 1, 0]),
+    ("e4m3", 128, 32, 2, 4, True, [40, 9, 33, 0]), ("int8", 64, 64, 3, 4, True, [33, 1, 0, 40])])
 def test_attention_split_over_blocks(fmt, dim, block, heads, group, bf16, counts):
     """long and short contexts in one call, the keys of each split over blocks and merged"""
     print(f"splits {fmt} dim {dim} block {block} group {group} bf16 {bf16} {counts}", flush=True)
@@ -249,6 +250,21 @@ def test_attention_split_over_blocks(fmt, dim, block, heads, group, bf16, counts
     for ctx in (3200, 1700):
         assert abi.kv8_attention_work(c.c, heads * group, 4, max(counts), ctx) > 0
         c.check_attention(rng, pos, counts, group, bf16, max_ctx=ctx)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("bf16,counts,before", [
+    (True, [16, 15], [70, 0]),                      # a block for each CU: four groups of keys
+    (True, [64, 63], [0, 70]), (False, [63], [33]),           # two of columns, long and short columns in pairs
+    (True, [64, 1, 50], [31, 0, 200]), (False, [64, 33], [0, 97])])        # ... and the longest first
+def test_attention_of_many_blocks(fmt, bf16, counts, before):
+    """as long prompts are launched, of few rows: 32 kv heads of 8 query heads"""
+    print(f"many blocks {fmt} bf16 {bf16} {counts} at {before}", flush=True)
+    rng = np.random.default_rng([len(counts), counts[0], bf16])
+    c = Cache(rng, fmt, 32, 128, 32, len(counts), 9)
+    c.append(rng, before, bf16)
+    pos = c.append(rng, counts, bf16)
+    c.check_attention(rng, pos, counts, 8, bf16)
 
 
 @pytest.mark.parametrize("bf16", [False, True])

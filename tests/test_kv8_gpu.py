@@ -267,6 +267,29 @@ def test_attention_of_many_blocks(fmt, bf16, counts, before):
     c.check_attention(rng, pos, counts, 8, bf16)
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("bf16,counts", [(False, [1, 1]), (True, [1, 1]), (False, [40, 9]), (True, [70, 33])])
+def test_page_0_is_not_read_into_results(fmt, bf16, counts):
+    """page 0, no sequence's, holds NaN; steps end inside blocks, and blocks in the middle have no page"""
+    print(f"page 0 {fmt} bf16 {bf16} {counts}", flush=True)
+    rng = np.random.default_rng(counts[0])
+    c = Cache(rng, fmt, 2, 128, 16, 2, 24)
+    spare = np.setdiff1d(np.arange(c.n_page), c.table)[-1]
+    c.table[c.table == 0] = spare
+    c.tb.upload(c.table)
+    c.append(rng, [250, 137], bf16)
+    pos = c.append(rng, counts, bf16)
+    c.check_attention(rng, pos, counts, 2, bf16)
+    c.table[0, 3:6] = c.table[1, 2] = c.table[1, 0] = -1
+    c.tb.upload(c.table)
+    q, got, _ = c.attend(rng, pos, counts, 2, bf16)
+    at = 0
+    for s, p, n, skip in zip(c.seqs, pos, counts, ((3, 4, 5), (0, 2))):
+        want, mean, delta = ko.attention(s, q[at:at + n].astype(np.float64), int(p), 1 / np.sqrt(128), skip)
+        assert (np.abs(got[at:at + n] - want) <= ko.tolerance(mean, delta, int(p) + n, bf16, want)).all()
+        at += n
+
+
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("counts", [[1, 1], [40, 70]])
 def test_a_row_that_is_not_finite_stays_alone(bf16, counts):

@@ -39,25 +39,34 @@ __device__ __forceinline__ bool kv8_get(kv8_entry &t, const qm_kv8_t &c, const i
 
 // ---------------------------------------------------------------------------
 // The model's q and k rows before they meet the cache: QK-norm and RoPE
-// (qwen3.c:298-305, ops_scalar.c:21-35) of row i at position pos[i] (each) or
-// *pos + i.  k in place; q in place or, where qb is set, as bf16 [nt][2048].
-// grid = (nt, 6): wave w of block (i, b) takes head 4 b + w of q's 16 and k's 8.
+// (qwen3.c:298-305, ops_scalar.c:21-35) of one head's 128 values, two a lane
 // ---------------------------------------------------------------------------
-__global__ __launch_bounds__(NTH) void k_qk_rope(float *__restrict__ qkv, uint16_t *__restrict__ qb,
-                                                const uint16_t *__restrict__ qn, const uint16_t *__restrict__ kn,
-                                                const float *__restrict__ rcos, const float *__restrict__ rsin,
-                                                const int *__restrict__ pos_d, int each, int max_seq, float eps) {
+typedef struct {
+    float *qkv;                        // rows of QKV_LD: 16 query heads, 8 key heads, 8 value heads
+    const uint16_t *qn, *kn;           // norm weights
+    const float *rcos, *rsin;          // [max_seq][64]
+    int max_seq;
+    float eps;
+} kv8_rope;
+__device__ __forceinline__ void kv8_rope_head(const kv8_rope &a, const float *x, const uint16_t *w, int pos, int lane,
+                                              float &o0, float &o1) {
+    const float x0 = x[lane], x1 = x[lane + 64];
+    const float c = a.rcos[(size_t)pos * (HD / 2) + lane], sn = a.rsin[(size_t)pos * (HD / 2) + lane];
+    const float sc = 1.0f / sqrtf(wave_sum(sumsq2(x0, x1)) / (float)HD + a.eps);
+    rope_pair((x0 * sc) * bf16f(w[lane]), (x1 * sc) * bf16f(w[lane + 64]), c, sn, o0, o1);
+}
+
+// A prompt's pass: row i at position *pos + i.  k in place; q in place or, where
+// qb is set, as bf16 [nt][2048].  grid = (nt, 6): wave w of block (i, b) takes
+// head 4 b + w of q's 16 and k's 8.  (A decode step's rows: k_kv8_append.)
+__global__ __launch_bounds__(NTH) void k_qk_rope(kv8_rope a, uint16_t *__restrict__ qb, const int *__restrict__ pos_d) {
     constexpr int QH = NKV * GRP;
     const int i = blockIdx.x, lane = threadIdx.x & 63, hd = blockIdx.y * 4 + (threadIdx.x >> 6);
-    const int pos = each ? pos_d[i] : *pos_d + i;
-    if (pos < 0 || pos >= max_seq) return;
-    float *x = qkv + (size_t)i * QKV_LD + hd * HD;           // k's heads lie behind q's
-    const uint16_t *w = hd < QH ? qn : kn;
-    const float x0 = x[lane], x1 = x[lane + 64];
-    const float c = rcos[(size_t)pos * (HD / 2) + lane], sn = rsin[(size_t)pos * (HD / 2) + lane];
-    const float sc = 1.0f / sqrtf(wave_sum(sumsq2(x0, x1)) / (float)HD + eps);
+    const int pos = *pos_d + i;
+    if (pos < 0 || pos >= a.max_seq) return;
+    float *x = a.qkv + (size_t)i * QKV_LD + hd * HD;         // k's heads lie behind q's
     float o0, o1;
-    rope_pair((x0 * sc) * bf16f(w[lane]), (x1 * sc) * bf16f(w[lane + 64]), c, sn, o0, o1);
+    kv8_rope_head(a, x, hd < QH ? a.qn : a.kn, pos, lane, o0, o1);
     if (qb && hd < QH) {
         __bf16 *o = (__bf16 *)qb + (size_t)i * (QH * HD) + hd * HD;
         o[lane] = (__bf16)o0;
@@ -152,15 +161,34 @@ struct kv8_16 {
 // 1.2.  With the loads in the compiler's order, conversions between them, and
 // the tail's values one a thread and turn, 9.9 and 7.7; in two passes over
 // memory 18.5.
-template <int FMT, int D, int B, bool BF>
-__global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void *__restrict__ kn,
-                                                         const void *__restrict__ vn, size_t ldk, size_t ldv,
+// ROPE: a row of each of the model's sequences, as its product left them (kn and
+// vn point into rope.qkv).  The block's waves normalise and rotate its key head,
+// handed on in LDS, and its query heads, in place; a launch of its own for that
+// cost a layer 2 us.
+template <int FMT, int D, int B, bool BF, bool ROPE>
+__global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void *kn, const void *vn, size_t ldk, size_t ldv,
                                                          const int *__restrict__ row, const int *__restrict__ pos, int rows,
-                                                         int max_rows) {
+                                                         int max_rows, kv8_rope rope) {
     constexpr int NT = B * D / 16, NWV = NT / WAVE;
     const int h = blockIdx.x, e = blockIdx.y, z = blockIdx.z, tid = threadIdx.x;
     kv8_entry t;
     if (!kv8_get(t, c, row, pos, e, rows, max_rows)) return;
+    if (ROPE && t.pos >= rope.max_seq) return;
+    __shared__ __align__(16) float krow[ROPE ? D : 4];
+    auto rotate = [&] {
+        if constexpr (ROPE) {
+            const int lane = tid & 63;
+            float *x = rope.qkv + (size_t)e * QKV_LD;
+            for (int hd = tid >> 6; hd < 1 + GRP; hd += NWV) {
+                float *q = x + (h * GRP + hd - 1) * HD, o0, o1;
+                kv8_rope_head(rope, hd == 0 ? x + (NKV * GRP + h) * HD : q, hd == 0 ? rope.kn : rope.qn, t.pos, lane, o0, o1);
+                float *o = hd == 0 ? krow : q;
+                o[lane] = o0;
+                o[lane + 64] = o1;
+            }
+            __syncthreads();
+        }
+    };
     const int end = t.pos + t.cnt, b0 = t.pos / B, bl = end / B, b = b0 + z;
     if (b >= bl && z > 0) return;
     const int kr = tid / (D / 16), kd = tid % (D / 16) * 16;           // the thread's K: slot and dims
@@ -180,13 +208,17 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
         }
         kv8_16<BF> knew;
         float vnew[16];
-        knew.load(kn, (size_t)(p0 + max(kr, have)) * ldk + h * D + kd);
+        if constexpr (!ROPE) knew.load(kn, (size_t)(p0 + max(kr, have)) * ldk + h * D + kd);
 #pragma unroll
         for (int j = 0; j < 16; j++) {
             const size_t i = (size_t)(p0 + max(vr + j, have)) * ldv + h * D + vd;
             vnew[j] = BF ? (float)((const __bf16 *)vn)[i] : ((const float *)vn)[i];
         }
         __builtin_amdgcn_sched_barrier(0);                // all in flight before the first is waited for
+        if constexpr (ROPE) {
+            rotate();
+            knew.load(krow, kd);
+        }
         __bf16 x[16], y[16];
 #pragma unroll
         for (int j = 0; j < 16; j++) {
@@ -226,15 +258,22 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
             }
         }
     }
-    if (z > 0) return;
+    if (z > 0 || (ROPE && b < bl)) return;                // (a row alone finishes its block or is in the tail)
     // slots lo .. hi - 1 of the tail, which begin with row p0
     const int lo = max(t.pos - bl * B, 0), hi = end - bl * B, p0 = t.r0 + bl * B - t.pos;
-    if (hi - lo <= NT / D) {                              // a row or few: a value of K and of V a thread
+    if (ROPE || hi - lo <= NT / D) {                      // a row or few: a value of K and of V a thread
         const int slot = lo + tid / D;
-        if (slot >= hi) return;
-        const size_t r = p0 + slot;
-        const float a = BF ? (float)((const __bf16 *)kn)[r * ldk + h * D + vd] : ((const float *)kn)[r * ldk + h * D + vd];
+        const bool in = slot < hi;
+        const size_t r = p0 + (in ? slot : lo);
+        float a = 0.0f;
+        if constexpr (!ROPE) a = BF ? (float)((const __bf16 *)kn)[r * ldk + h * D + vd] : ((const float *)kn)[r * ldk + h * D + vd];
         const float o = BF ? (float)((const __bf16 *)vn)[r * ldv + h * D + vd] : ((const float *)vn)[r * ldv + h * D + vd];
+        if constexpr (ROPE) {
+            __builtin_amdgcn_sched_barrier(0);            // V's values on their way meanwhile
+            rotate();
+            a = krow[vd];
+        }
+        if (!in) return;
         kt[slot * D + vd] = kv8_held(a);
         vt[vd * B + slot] = kv8_held(o);
         return;
@@ -799,11 +838,31 @@ extern "C" size_t qm_kv8_bytes(const qm_kv8_t *c) {
 }
 
 extern "C" int qm_qk_rope(float *qkv, uint16_t *qb, const uint16_t *qn, const uint16_t *kn, const float *rcos,
-                          const float *rsin, const int *pos, int each, int nt, int max_seq, float eps) {
+                          const float *rsin, const int *pos, int nt, int max_seq, float eps) {
     if (!qkv || !qn || !kn || !rcos || !rsin || !pos || nt <= 0 || max_seq <= 0) return QH_EINVAL;
     if (!stream()) return QH_ESTATE;
-    hipLaunchKernelGGL(k_qk_rope, dim3(nt, (NKV * GRP + NKV) / 4), dim3(NTH), 0, stream(), qkv, qb, qn, kn, rcos, rsin, pos,
-                       each, max_seq, eps);
+    const kv8_rope a = {qkv, qn, kn, rcos, rsin, max_seq, eps};
+    hipLaunchKernelGGL(k_qk_rope, dim3(nt, (NKV * GRP + NKV) / 4), dim3(NTH), 0, stream(), a, qb, pos);
+    return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
+}
+
+extern "C" int qm_kv8_rope_append(const qm_kv8_t *c, float *qkv, const uint16_t *qn, const uint16_t *kn, const float *rcos,
+                                  const float *rsin, const int *pos, int n, int max_seq, float eps) {
+    int rc = kv8_check(c);
+    if (!rc) rc = kv8_call_check(c, NULL, pos, n, n, 1);
+    if (rc) return rc;
+    if (c->heads != NKV || c->head_dim != HD || c->block != 32) return QH_EINVAL;
+    if (n == 0) return QH_OK;
+    if (!qkv || !aligned16(qkv) || !qn || !kn || !rcos || !rsin || max_seq <= 0) return QH_EINVAL;
+    if (!stream()) return QH_ESTATE;
+    const kv8_rope a = {qkv, qn, kn, rcos, rsin, max_seq, eps};
+    const float *k = qkv + NKV * GRP * HD, *v = k + NKV * HD;
+    if (c->format == QM_KV8_E4M3)
+        hipLaunchKernelGGL((k_kv8_append<QM_KV8_E4M3, HD, 32, false, true>), dim3(NKV, n), dim3(2 * HD), 0, stream(), *c, k, v,
+                           QKV_LD, QKV_LD, NULL, pos, n, 1, a);
+    else
+        hipLaunchKernelGGL((k_kv8_append<QM_KV8_INT8, HD, 32, false, true>), dim3(NKV, n), dim3(2 * HD), 0, stream(), *c, k, v,
+                           QKV_LD, QKV_LD, NULL, pos, n, 1, a);
     return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
 }
 
@@ -828,8 +887,8 @@ extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, si
     if (grid.z > 65535) return QH_ETOOBIG;
     if (!stream()) return QH_ESTATE;
 #define APPEND_B(F, D_, B_, BF_) \
-    hipLaunchKernelGGL((k_kv8_append<F, D_, B_, BF_>), grid, dim3(B_ *D_ / 16), 0, stream(), *c, k, v, ldk, ldv, row, pos, rows, \
-                       max_rows)
+    hipLaunchKernelGGL((k_kv8_append<F, D_, B_, BF_, false>), grid, dim3(B_ *D_ / 16), 0, stream(), *c, k, v, ldk, ldv, row, \
+                       pos, rows, max_rows, kv8_rope{})
 #define APPEND(F, D_, BF_)                                  \
     do {                                                    \
         if (c->block == 16) APPEND_B(F, D_, 16, BF_);       \

@@ -394,9 +394,14 @@ static int attend_kv8(qwen3_hip_model *m, const kv8_t *k, int l, const layer_t *
     const int each = n == nt;          /* a row of each sequence */
     /* bf16 rows: the output takes the first half of the buffer, q the second */
     uint16_t *qb = bf16 ? (uint16_t *)m->att + (size_t)nt * QW3M_Q_DIM : NULL;
-    int rc = qm_qk_rope(m->qkv, qb, L->qn, L->kn, m->rcos, m->rsin, pos, each, nt, m->max_seq, QW3M_RMS_EPS);
-    if (!rc) rc = qm_kv8_append(&c, m->qkv + QW3M_Q_DIM, m->qkv + QW3M_Q_DIM + QW3M_KV_DIM, QKV_N, QKV_N, 0,
-                                each ? NULL : k->row, pos, n, nt, each ? 1 : nt);
+    int rc;
+    if (each) {
+        rc = qm_kv8_rope_append(&c, m->qkv, L->qn, L->kn, m->rcos, m->rsin, pos, n, m->max_seq, QW3M_RMS_EPS);
+    } else {
+        rc = qm_qk_rope(m->qkv, qb, L->qn, L->kn, m->rcos, m->rsin, pos, nt, m->max_seq, QW3M_RMS_EPS);
+        if (!rc) rc = qm_kv8_append(&c, m->qkv + QW3M_Q_DIM, m->qkv + QW3M_Q_DIM + QW3M_KV_DIM, QKV_N, QKV_N, 0, k->row,
+                                    pos, n, nt, nt);
+    }
     if (!rc) rc = qm_kv8_attention(&c, m->att, bf16 ? (const void *)qb : m->qkv, QW3M_Q_DIM, bf16 ? QW3M_Q_DIM : QKV_N,
                                    bf16, QW3M_N_HEADS, each ? NULL : k->row, pos, n, nt, each ? 1 : nt, ctx,
                                    ATT_SCALE, k->work, k->work_bytes);

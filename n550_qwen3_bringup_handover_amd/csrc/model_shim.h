@@ -132,10 +132,15 @@ int qm_kv8_attention(const qm_kv8_t *c, void *out_d, const void *q_d, size_t ldo
                      const int *row_d, const int *pos_d, int n, int rows, int max_rows, int max_ctx, float scale,
                      void *work_d, size_t work_bytes);
 
-/* QK-norm + RoPE of qkv rows ([nt][4096]) at positions pos_d[i] (each) or
- * *pos_d + i: k in place, q in place or as bf16 [nt][2048] into qb_d */
+/* QK-norm + RoPE of qkv rows ([nt][4096]) at positions *pos_d + i: k in place,
+ * q in place or as bf16 [nt][2048] into qb_d */
 int qm_qk_rope(float *qkv_d, uint16_t *qb_d, const uint16_t *qn_d, const uint16_t *kn_d, const float *rcos_d,
-               const float *rsin_d, const int *pos_d, int each, int nt, int max_seq, float eps);
+               const float *rsin_d, const int *pos_d, int nt, int max_seq, float eps);
+/* the same of one row of each of n sequences, at pos_d[i], q in place, and k and
+ * v into their caches (the model's heads, blocks of 32); k's place keeps its row
+ * as it was */
+int qm_kv8_rope_append(const qm_kv8_t *c, float *qkv_d, const uint16_t *qn_d, const uint16_t *kn_d, const float *rcos_d,
+                       const float *rsin_d, const int *pos_d, int n, int max_seq, float eps);
 /* table entries of unfinished blocks (all where pos_d is NULL) = the
  * sequence's own pages, s * max_blocks + block index */
 int qm_kv8_own(int *table_d, const int *pos_d, int n_seq, int block, int max_blocks);

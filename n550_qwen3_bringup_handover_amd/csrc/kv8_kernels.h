@@ -452,7 +452,8 @@ __device__ __forceinline__ float kv8_softmax(f32x4 (&s)[4], float k, float &m, f
 //   that the two blocks of a CU are a long and a short one
 // Few columns are bound by the bytes: 64 sequences at 2,048 positions (238 MB)
 // 44.5 us, 5.3 TB/s, where a copy reaches 5.3; with fewer blocks than CUs by
-// the chain of latencies of a block and the merge (700 positions 7.5 us).
+// the chain of latencies of a block and the merge (700 positions 7.5 us, 6 x
+// 8,000 of int8, 48 MB, 15).
 // Prompts are bound by the vector instructions that make operands and weights,
 // behind which the two waves a SIMD has registers for hide the products only in
 // part: of 64 products (19 cycles each) and about 480 others a step of a wave,
@@ -909,15 +910,19 @@ extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, si
 //     8 x 250 14.9 against 19.2; fp32 58 against 67).
 //   Few blocks: the keys split over blocks of four waves, a step a wave, up to
 //     128 blocks (one head of a kv head's, 700 positions: 8.0 us against 9.7 on
-//     one block of eight waves and 9.9 on two, 1,500 8.3 against 10.1).
+//     one block of eight waves and 9.9 on two, 1,500 8.3 against 10.1); with 17
+//     to 64 blocks up to 192 to 256 (5 x 960 positions 8.1 us against 9.8 on
+//     blocks of eight waves, 17 rows behind 6,000 14.2 against 16.2, 6 x 8,000
+//     15.0 against 16.4; 24 blocks by ten are slower than by eight, 15.7, since
+//     a multiple of eight keeps the tiles of the same keys on one XCD).
 //   Between: four groups of keys where a wave of eight would have a step or two
 //     (32 x 700 positions 10.8 against 11.5 us, 60 x 700 17.6 against 20.1) or
 //     where columns see different numbers of keys and there is a block for each
 //     CU (1,000 tokens 16.1 against 19.6, fp32 500 behind 1,499 28.9 against
-//     33.5); eight elsewhere, which read ahead further (8 x 960 positions 10.0
-//     against 10.5 us, 40 x 2,000 34.4 against 36.7), with the keys of long
-//     contexts split over blocks as long as there is a CU for each (6 x 8,000:
-//     17.9 us on 240 blocks, 25 on 336).
+//     33.5); eight elsewhere, which read ahead further (16 x 700 positions 9.1
+//     us against 10.2, 40 x 2,000 34.4 against 36.7), with the keys of long
+//     contexts split over blocks as long as there is a CU for each (8 heads at
+//     8,000: 11.5 us on 128 blocks).
 struct kv8_plan { int ct, cg, kg, splits, order, cols, tiles; };
 static kv8_plan kv8_plan_of(const qm_kv8_t *c, int G, int n, int max_rows, int max_ctx, int bf16) {
     const long cols = (long)max_rows * G;
@@ -936,6 +941,9 @@ static kv8_plan kv8_plan_of(const qm_kv8_t *c, int G, int n, int max_rows, int m
         const bool cu_each = blocks >= 256;
         if (blocks * ((steps + 3) / 4) <= 128) {
             p.splits = (steps + 3) / 4;
+        } else if (blocks > 16 && blocks <= 64) {
+            p.splits = blocks <= 21 ? 12 : blocks <= 32 ? 8 : blocks <= 42 ? 6 : 4;
+            if (p.splits > (steps + 3) / 4) p.splits = (steps + 3) / 4;
         } else if (steps > (p.tiles > 1 || cu_each ? 16 : 12) && !(p.tiles > 1 && cu_each)) {
             p.kg = 8;
             const long room = 256 / blocks, want = (steps + 7) / 8;

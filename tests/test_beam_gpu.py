@@ -97,7 +97,8 @@ def check(logits, score, done, end0, end1, **kw):
 
 @pytest.mark.parametrize("G,W,V,ld,offset", [(1, 1, 1, 1, 0), (1, 4, 151936, 151936, 0), (3, 8, 5001, 5001, 0), (2, 16, 2048, 2052, 0),
                                              (2, 3, 2049, 2050, 1), (5, 2, 17, 33, 3), (1, 16, 16, 16, 0), (2, 5, 70001, 70004, 0),
-                                             (7, 7, 4096, 4096, 2), (1, 16, 151936, 151936, 0)])
+                                             (7, 7, 4096, 4096, 2), (1, 16, 151936, 151936, 0),
+                                             (2, 2, 300001, 300004, 0), (1, 3, 1 << 21, 1 << 21, 0), (1, 2, 1000003, 1000003, 0)])
 def test_choice(G, W, V, ld, offset):
     print(f"select {G} x {W} of {V}, stride {ld}, offset {offset}", flush=True)
     rng = np.random.default_rng([G, W, V])

@@ -267,6 +267,56 @@ def test_attention_of_many_blocks(fmt, bf16, counts, before):
     c.check_attention(rng, pos, counts, 8, bf16)
 
 
+@pytest.mark.parametrize("heads,group,dim,bf16", [(256, 1, 64, False), (1, 64, 64, True), (2, 64, 128, False)])
+def test_heads_and_groups_at_their_limits(heads, group, dim, bf16):
+    print(f"limits heads {heads} group {group} dim {dim} bf16 {bf16}", flush=True)
+    rng = np.random.default_rng([heads, group])
+    c = Cache(rng, "e4m3", heads, dim, 16, 2, 5)
+    c.append(rng, [33, 15], bf16)
+    for counts in ([1, 1], [3, 2]):
+        pos = c.append(rng, counts, bf16)
+        c.check_stored()
+        c.check_attention(rng, pos, counts, group, bf16)
+
+
+@pytest.mark.parametrize("rows_bf16,q_bf16", [(False, True), (True, False)])
+def test_rows_queries_and_results_of_different_strides_and_types(rows_bf16, q_bf16):
+    """K, V, q and out as parts of wider rows, each with a stride of its own; rows in one type, queries in the other"""
+    rng = np.random.default_rng(17)
+    heads, group, dim = 2, 2, 128
+    c = Cache(rng, "int8", heads, dim, 32, 2, 4)
+    counts, ldk, ldv, ldq, ldo = [40, 31], 320, 264, 528, 1024
+    total = sum(counts)
+    kv = rng.standard_normal((2, total, heads, dim)).astype(np.float32)
+    kv = ko.bf16_value(ko.bf16_bits(kv)) if rows_bf16 else kv
+    q = rng.standard_normal((total, heads * group, dim)).astype(np.float32)
+    q = ko.bf16_value(ko.bf16_bits(q)) if q_bf16 else q
+
+    def rows(x, ld, bf16):
+        full = np.full((total, ld), 9.0, np.float32)
+        full[:, :x[0].size] = x.reshape(total, -1)
+        return abi.DeviceBuffer.from_array(ko.bf16_bits(full) if bf16 else full)
+
+    kd, vd, qd = rows(kv[0], ldk, rows_bf16), rows(kv[1], ldv, rows_bf16), rows(q, ldq, q_bf16)
+    od = rows(np.full((total, 1), 9.0, np.float32), ldo, q_bf16)
+    rd = abi.DeviceBuffer.from_array(np.array([0, 40, 71], np.int32))
+    pd = abi.DeviceBuffer.from_array(np.zeros(2, np.int32))
+    abi.kv8_append_dev(c.c, kd.ptr, vd.ptr, ldk, ldv, rows_bf16, rd.ptr, pd.ptr, 2, total, 40)
+    for s, a, b in zip(c.seqs, (0, 40), (40, 71)):
+        s.append(kv[0, a:b], kv[1, a:b])
+    work = abi.kv8_attention_work(c.c, heads * group, 2, 40, 128)
+    wd = abi.DeviceBuffer(max(work, 16))
+    abi.kv8_attention_dev(c.c, od.ptr, qd.ptr, ldo, ldq, q_bf16, heads * group, rd.ptr, pd.ptr, 2, total, 40, 128, 0.09, wd.ptr, work)
+    abi.sync()
+    raw = od.download(np.uint16 if q_bf16 else np.float32, total * ldo).reshape(total, ldo)
+    got = ko.bf16_value(raw) if q_bf16 else raw
+    assert np.all(got[:, heads * group * dim:] == 9.0)
+    got = got[:, :heads * group * dim].reshape(q.shape)
+    for s, a, b in zip(c.seqs, (0, 40), (40, 71)):
+        want, mean, delta = ko.attention(s, q[a:b].astype(np.float64), 0, 0.09)
+        assert (np.abs(got[a:b] - want) <= ko.tolerance(mean, delta, b - a, q_bf16, want)).all()
+
+
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("bf16,counts", [(False, [1, 1]), (True, [1, 1]), (False, [40, 9]), (True, [70, 33])])
 def test_page_0_is_not_read_into_results(fmt, bf16, counts):

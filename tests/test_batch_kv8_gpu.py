@@ -83,6 +83,26 @@ def test_logits_are_near_those_of_fp32_caches(plain, kv):
         assert 0 < off <= LIMIT[kv]
 
 
+def test_prompts_of_several_passes(blob):
+    """2,100 tokens: two passes that meet inside a block, the second over the first's codes and tail"""
+    ps = prompts(2, [2100, 2049], 10)
+    with M.Model(blob, max_seq=2200) as m:
+        got = []
+        for kind in ("fp32", "e4m3", "int8"):
+            with M.Batch(m, 2, 2200, kind) as b:
+                for s, p in enumerate(ps):
+                    b.prefill(s, p)
+                got.append((b.decode(1)[:, 0], b.logits()))
+    for kind, (fed, logits) in zip(("e4m3", "int8"), got[1:]):
+        same = got[0][0] == fed
+        assert same.any()
+        for s in np.flatnonzero(same):
+            x, y = got[0][1][s].astype(np.float64), logits[s].astype(np.float64)
+            off = np.sqrt(((y - x) ** 2).mean()) / x.std()
+            print(f"{kind}, sequence {s}: {off:.4f}", flush=True)
+            assert 0 < off <= LIMIT[kind]
+
+
 @pytest.mark.parametrize("kv", ["fp32", "e4m3"])
 def test_graph_and_eager_steps_agree(sharp, kv):
     ps = prompts(4, [17, 62, 95], 3)

@@ -82,8 +82,8 @@ int qwen3_hip_kv8_append_dev(const qwen3_hip_kv8 *cache, const void *k_d, const 
  * q_d and out_d: [q_heads][head_dim] per row, both fp32 or, where bf16 is set,
  * both bf16; query head h reads kv head h / (q_heads / kv_heads), at most 64
  * query heads a kv head.  fp32 rows are computed with fp32 accuracy
- * throughout; bf16 rows with weights of at least bf16.  Strides and alignment
- * as above.  A row that is left out keeps what out_d held; a page that is no
+ * throughout; bf16 rows with weights of 16 bits, so that the rounding of the
+ * results is all that shows.  Strides and alignment as above.  A row that is left out keeps what out_d held; a page that is no
  * page of the pool is left out of the sums, and a row with nothing left is 0.
  * max_ctx: a bound on pos_d[i] + rows of i, which picks the launch (a longer
  * entry is right too).  work_d: qwen3_hip_kv8_attention_work() bytes for the

@@ -312,9 +312,9 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
 // multiplies the scores, V's the weights.
 // fp32 rows keep fp32 accuracy: q and the weights go through the matrix cores
 // as three bf16 pieces each (8 bits apiece: x - x1 - x2 - x3 < 2^-24 x).  bf16
-// rows are one piece; their weights are two where the bytes bound the kernel
-// and one in a prompt, whose results are rounded to bf16 anyway (the weights'
-// roundings, each its own, then add as much as that one does).
+// rows are one piece, and their weights two: in one, 15 % faster in a prompt,
+// the weights' roundings would add as much error as the results' own, or more
+// where few keys weigh (1.5 times the results' alone over short prompts).
 //   S^T tile t, row m <-> key 16 (m / 4) + 4 t + m % 4 of the step, so that
 //   lane (c, h) = (lane % 16, lane / 16) ends up with keys 16 h + 4 t + i of
 //   column c: four tiles are 16 consecutive keys, which lie in one page (one
@@ -456,10 +456,10 @@ __device__ __forceinline__ float kv8_softmax(f32x4 (&s)[4], float k, float &m, f
 // 8,000 of int8, 48 MB, 15).
 // Prompts are bound by the vector instructions that make operands and weights,
 // behind which the two waves a SIMD has registers for hide the products only in
-// part: of 64 products (19 cycles each) and about 480 others a step of a wave,
-// 128 convert codes (6) and 32 are exponentials (9).  2,048 rows behind 6,000
-// 147 us, 800 TFLOP/s; 1,999 behind nothing 32 us, 506, where the columns with
-// the most keys end alone.
+// part: of 96 products (19 cycles each) and about 570 others a step of a wave,
+// 128 convert codes (6), 32 are exponentials (9) and 96 split the weights.  2,048
+// rows behind 6,000 187 us, 630 TFLOP/s; 1,999 behind nothing 39 us, 420, where
+// the columns with the most keys end alone.
 #define KV8_MAX_SPLITS 32
 template <bool NT>
 __device__ __forceinline__ uint4 kv8_read(const uint8_t *p) {
@@ -479,7 +479,7 @@ __global__ __launch_bounds__(WAVE *CG *KG, 2) void k_kv8_attend(qm_kv8_t c, void
                                                                int rows, int max_rows, int G, unsigned inv_G, float f,
                                                                int nsplit,
                                                                int order, float *__restrict__ part) {
-    constexpr int NP = BF ? 1 : 3, NW = !BF ? 3 : CT == 1 ? 2 : 1;         // pieces of q, and of a weight
+    constexpr int NP = BF ? 1 : 3, NW = BF ? 2 : 3;         // pieces of q, and of a weight
     constexpr int KS = D / 32, DT = D / 16, LD = D + 4, COLS = 16 * CT * CG, NT = WAVE * CG * KG;
     const int e = blockIdx.y, split = blockIdx.x % nsplit, x = blockIdx.x / nsplit, head = x % c.heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -906,8 +906,8 @@ extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, si
 //   CT: two column tiles a wave where rows are bf16 and there are more than 16
 //     columns (fp32 rows take the registers for their pieces).
 //   Long prompts: blocks of two groups of keys and two of columns, which share
-//     what they read (1,999 tokens 35.6 against 38.1 us with four groups of keys,
-//     8 x 250 14.9 against 19.2; fp32 58 against 67).
+//     what they read (1,999 tokens 42.6 against 45.6 us with four groups of keys,
+//     8 x 250 16.1 against 20.1; fp32 61 against 70).
 //   Few blocks: the keys split over blocks of four waves, a step a wave, up to
 //     128 blocks (one head of a kv head's, 700 positions: 8.0 us against 9.7 on
 //     one block of eight waves and 9.9 on two, 1,500 8.3 against 10.1); with 17
@@ -918,7 +918,7 @@ extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, si
 //   Between: four groups of keys where a wave of eight would have a step or two
 //     (32 x 700 positions 10.8 against 11.5 us, 60 x 700 17.6 against 20.1) or
 //     where columns see different numbers of keys and there is a block for each
-//     CU (1,000 tokens 16.1 against 19.6, fp32 500 behind 1,499 28.9 against
+//     CU (1,000 tokens 18.0 against 20.5, fp32 500 behind 1,499 28.9 against
 //     33.5); eight elsewhere, which read ahead further (16 x 700 positions 9.1
 //     us against 10.2, 40 x 2,000 34.4 against 36.7), with the keys of long
 //     contexts split over blocks as long as there is a CU for each (8 heads at

@@ -130,10 +130,12 @@ def tolerance(mean, delta, ctx, bf16, out):
     """Every weight is off by delta U at most, relative, so numerator and denominator by that each; the sums of
     weights and of weights times v go through 3 x 2 matrix instructions a step of 64 keys, 4 roundings each, rescaled
     once a step, then merged (32 splits, 4 waves): a rounding each of what the sum went through, sum p|v|.  bf16:
-    weights are rounded to bf16 in the numerator, and the result is."""
+    weights are two pieces in the numerator, the second the first's remainder rounded to bf16, and the result is
+    rounded."""
     steps = ctx / 64 + 2
     rel = (2 * delta + 2 * (24 + 1) * steps + 2 * 36 + 8) * U
     tol = rel * mean
     if bf16:
-        tol = tol + UB * mean + UB * (np.abs(out) + tol + UB * mean)
+        tol = tol + UB * UB * mean
+        tol = tol + UB * (np.abs(out) + tol)
     return tol + 1e-37

@@ -330,22 +330,15 @@ __device__ __forceinline__ bf16x8 kv8_bf16(uint32_t a, uint32_t b) {      // eig
         r.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
         r.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
     } else {
-        // three instructions for two codes, and two registers halfway: left to
-        // the scheduler the fp32 values of many codes are made first, and spill
-#define KV8_I8(R, X, B0, B1)                                                                                    \
-    do {                                                                                                        \
-        float t0, t1;                                                                                           \
-        asm("v_cvt_f32_i32_sdwa %1, sext(%3) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:" B0 "\n\t"           \
-            "v_cvt_f32_i32_sdwa %2, sext(%3) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:" B1 "\n\t"           \
-            "v_cvt_pk_bf16_f32 %0, %1, %2"                                                                      \
-            : "=v"(R), "=&v"(t0), "=&v"(t1)                                                                     \
-            : "v"(X));                                                                                          \
-    } while (0)
-        KV8_I8(r.p[0], a, "BYTE_0", "BYTE_1");
-        KV8_I8(r.p[1], a, "BYTE_2", "BYTE_3");
-        KV8_I8(r.p[2], b, "BYTE_0", "BYTE_1");
-        KV8_I8(r.p[3], b, "BYTE_2", "BYTE_3");
-#undef KV8_I8
+        // a code's byte is sign-extended by the conversion itself: three instructions for two codes
+        auto pair = [](uint32_t x, int n) {
+            const f32x2 t = {(float)(int)(signed char)(x >> n), (float)(int)(signed char)(x >> (n + 8))};
+            return __builtin_convertvector(t, bf16x2);
+        };
+        r.p[0] = pair(a, 0);
+        r.p[1] = pair(a, 16);
+        r.p[2] = pair(b, 0);
+        r.p[3] = pair(b, 16);
     }
     return r.v;
 }

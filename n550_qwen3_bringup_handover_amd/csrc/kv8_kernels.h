@@ -258,9 +258,10 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
             }
         }
     }
-    if (z > 0 || (ROPE && b < bl)) return;                // (a row alone finishes its block or is in the tail)
-    // slots lo .. hi - 1 of the tail, which begin with row p0
+    // slots lo .. hi - 1 of the tail, which begin with row p0 + lo.  None where the
+    // rows end with a block: p0 + lo is then the row behind them
     const int lo = max(t.pos - bl * B, 0), hi = end - bl * B, p0 = t.r0 + bl * B - t.pos;
+    if (z > 0 || hi <= lo) return;
     if (ROPE || hi - lo <= NT / D) {                      // a row or few: a value of K and of V a thread
         const int slot = lo + tid / D;
         const bool in = slot < hi;

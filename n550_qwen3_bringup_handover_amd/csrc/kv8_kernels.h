@@ -984,20 +984,21 @@ extern "C" int qm_kv8_attention(const qm_kv8_t *c, void *out, const void *q, siz
 #define ATTEND_AS(F, D_, BF_, CT_, CG_, KG_)                                                                           \
     hipLaunchKernelGGL((k_kv8_attend<F, D_, BF_, CT_, CG_, KG_>), grid, dim3(WAVE *CG_ *KG_), 0, stream(), *c, out, q, ldo, \
                        ldq, row, pos, rows, max_rows, G, inv_G, f, p.splits, p.order, (float *)work)
-#define ATTEND_CT(F, D_, BF_, CT_)                                \
-    do {                                                          \
-        if (p.cg == 2) ATTEND_AS(F, D_, BF_, CT_, 2, 2);          \
-        else if (p.kg == 4) ATTEND_AS(F, D_, BF_, CT_, 1, 4);     \
-        else ATTEND_AS(F, D_, BF_, CT_, 1, 8);                    \
+#define ATTEND_KG(F, D_, BF_, CT_)                            \
+    do {                                                      \
+        if (p.kg == 4) ATTEND_AS(F, D_, BF_, CT_, 1, 4);      \
+        else ATTEND_AS(F, D_, BF_, CT_, 1, 8);                \
     } while (0)
-#define ATTEND(F, D_, BF_)                              \
-    do {                                                \
-        if (p.ct == 2) ATTEND_CT(F, D_, BF_, (BF_ ? 2 : 1)); \
-        else ATTEND_CT(F, D_, BF_, 1);                  \
+    // (two groups of columns only at head_dim 128, and with bf16 rows only two tiles a wave)
+#define ATTEND(F, D_, BF_)                                    \
+    do {                                                      \
+        if (p.cg == 2) ATTEND_AS(F, 128, BF_, (BF_ ? 2 : 1), 2, 2); \
+        else if (p.ct == 2) ATTEND_KG(F, D_, BF_, (BF_ ? 2 : 1)); \
+        else ATTEND_KG(F, D_, BF_, 1);                        \
     } while (0)
     KV8_SWITCH(ATTEND);
 #undef ATTEND
-#undef ATTEND_CT
+#undef ATTEND_KG
 #undef ATTEND_AS
     return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
 }

@@ -180,8 +180,10 @@ int qwen3_hip_batch_open(qwen3_hip_batch **batch, qwen3_hip_model *model, int n_
  * 57,400 bytes per position, rounded up to blocks, and 3.7 MB per sequence for
  * the unfinished blocks, instead of 229,376 per position.  Every call below
  * takes either kind.  Attention, a prompt's included, reads K and V as the
- * cache holds them, so logits differ from an fp32 batch's by the codes'
- * roundings. */
+ * cache holds them, so logits differ from an fp32 batch's by the roundings of
+ * finished blocks to codes and of unfinished ones to bf16; in passes of more
+ * than 64 prompt tokens also by those of q to bf16 and of attention's weights
+ * to 16 bits. */
 int qwen3_hip_batch_open_kv8(qwen3_hip_batch **batch, qwen3_hip_model *model, int n_seq, int max_ctx, int format);
 
 void qwen3_hip_batch_close(qwen3_hip_batch *batch);

@@ -82,9 +82,11 @@ int qwen3_hip_kv8_append_dev(const qwen3_hip_kv8 *cache, const void *k_d, const 
  * q_d and out_d: [q_heads][head_dim] per row, both fp32 or, where bf16 is set,
  * both bf16; query head h reads kv head h / (q_heads / kv_heads), at most 64
  * query heads a kv head.  fp32 rows are computed with fp32 accuracy
- * throughout; bf16 rows with weights of 16 bits, so that the rounding of the
- * results is all that shows.  Strides and alignment as above.  A row that is left out keeps what out_d held; a page that is no
- * page of the pool is left out of the sums, and a row with nothing left is 0.
+ * throughout; bf16 rows with weights of 16 bits: results are off by their own
+ * rounding to bf16 and by little else (about one in 400 is a neighbour of the
+ * value that rounding alone would give).  Strides and alignment as above.  A row
+ * that is left out keeps what out_d held; a page that is no page of the pool is
+ * left out of the sums, and a row with nothing left is 0.
  * max_ctx: a bound on pos_d[i] + rows of i, which picks the launch (a longer
  * entry is right too).  work_d: qwen3_hip_kv8_attention_work() bytes for the
  * same sizes or larger ones (4.4 MB at most; it never shrinks as n, max_rows or
@@ -107,8 +109,12 @@ int qwen3_hip_kv8_attention_dev(const qwen3_hip_kv8 *cache, void *out_d, const v
  * Output row k of a group is its k-th best: its score, token, the beam it
  * continues (parent, 0 .. width - 1) and whether it is finished (its parent
  * was, or its token is end0 or end1; -1: no such token, which end0 may be only
- * where done_d is NULL).  Equal scores go in
- * the order of beam and token.  Scores are compared in 64 bits.  Where fewer
+ * where done_d is NULL).  Of one beam the tokens with the largest logits are
+ * taken, ties to the lowest; those of all beams are compared by their scores in
+ * 64 bits, equal ones in the order of beam and token.  A row's log sum is formed
+ * from fp32 exponentials and fp32 sums of 2,048 of them and is off by 2^-18 at
+ * most, so continuations of two beams whose scores are closer than 2^-17 may
+ * come in either order; score_out_d is the score rounded to fp32.  Where fewer
  * than `width` continuations have a score, the others are taken in the same
  * order, as -inf: those of beams not in use (a score_d that is not finite; -inf
  * before the first token for all beams but the first), of tokens whose logit is

@@ -313,7 +313,7 @@ __global__ __launch_bounds__(B *D / 16) void k_kv8_append(qm_kv8_t c, const void
 // multiplies the scores, V's the weights.
 // fp32 rows keep fp32 accuracy: q and the weights go through the matrix cores
 // as three bf16 pieces each (8 bits apiece: x - x1 - x2 - x3 < 2^-24 x).  bf16
-// rows are one piece, and their weights two: in one, 15 % faster in a prompt,
+// rows are one piece, and their weights two: in one, 16 to 21 % faster in a prompt,
 // the weights' roundings would add as much error as the results' own, or more
 // where few keys weigh (1.5 times the results' alone over short prompts).
 //   S^T tile t, row m <-> key 16 (m / 4) + 4 t + m % 4 of the step, so that
@@ -452,8 +452,10 @@ __device__ __forceinline__ float kv8_softmax(f32x4 (&s)[4], float k, float &m, f
 // behind which the two waves a SIMD has registers for hide the products only in
 // part: of 96 products (19 cycles each) and about 570 others a step of a wave,
 // 128 convert codes (6), 32 are exponentials (9) and 96 split the weights.  2,048
-// rows behind 6,000 187 us, 630 TFLOP/s; 1,999 behind nothing 39 us, 420, where
-// the columns with the most keys end alone.
+// rows behind 6,000 186 us, 630 TFLOP/s; 1,999 behind nothing 38 us, 425, where
+// the columns with the most keys end alone.  int8, whose conversions are three
+// instructions for two codes, 226 and 44; fp32 rows, three products for one, 57
+// (e4m3) and 68 (1,999 rows: 42.6 at a large product's rate).
 #define KV8_MAX_SPLITS 32
 template <bool NT>
 __device__ __forceinline__ uint4 kv8_read(const uint8_t *p) {
@@ -899,16 +901,26 @@ extern "C" int qm_kv8_append(const qm_kv8_t *c, const void *k, const void *v, si
 // The launch for max_rows x G columns a kv head and sequence.
 //   CT: two column tiles a wave where rows are bf16 and there are more than 16
 //     columns (fp32 rows take the registers for their pieces).
-//   Long prompts: blocks of two groups of keys and two of columns, which share
-//     what they read (1,999 tokens 42.6 against 45.6 us with four groups of keys,
-//     8 x 250 16.1 against 20.1; fp32 61 against 70).
+//   Prompts that fill the CUs: blocks of two groups of keys and two of columns,
+//     which share what they read, against four groups of keys.  From 960 blocks
+//     of the latter, where they come even: a prompt of 1,700 bf16 rows (856
+//     blocks) 34.9 us against 32.8, of 1,999 (1,000) 38.2 against 40.5; fp32 700
+//     rows (704) 18.6 against 17.1, 1,000 (1,008) 21.1 against 25.7.  From four
+//     tiles a sequence: 30 x 61 rows 13.0 against 17.5, behind 2,048 positions
+//     64.7 against 65.6; 8 x 250 16.7 against 20.8; with three tiles, the fourth
+//     a block's half that is idle, 40 x 45 behind 2,048 81.6 against 66.9.  At
+//     head_dim 64, whose steps are half the products, only many short prompts
+//     would gain (16 x 120 9.5 against 11.1) and long ones lose (1,999 26.5
+//     against 25.1, 2,500 41.8 against 34.5): never.
 //   Few blocks: the keys split over blocks of four waves, a step a wave, up to
 //     128 blocks (one head of a kv head's, 700 positions: 8.0 us against 9.7 on
 //     one block of eight waves and 9.9 on two, 1,500 8.3 against 10.1); with 17
 //     to 64 blocks up to 192 to 256 (5 x 960 positions 8.1 us against 9.8 on
 //     blocks of eight waves, 17 rows behind 6,000 14.2 against 16.2, 6 x 8,000
 //     15.0 against 16.4; 24 blocks by ten are slower than by eight, 15.7, since
-//     a multiple of eight keeps the tiles of the same keys on one XCD).
+//     a multiple of eight keeps the tiles of the same keys on one XCD).  Two
+//     blocks a CU, by 16, are slower still: 24 blocks at 8,000 18.7, 20 17.1
+//     against 14.1, 32 19.8 against 16.3.
 //   Between: four groups of keys where a wave of eight would have a step or two
 //     (32 x 700 positions 10.8 against 11.5 us, 60 x 700 17.6 against 20.1) or
 //     where columns see different numbers of keys and there is a block for each
@@ -924,7 +936,7 @@ static kv8_plan kv8_plan_of(const qm_kv8_t *c, int G, int n, int max_rows, int m
     p.cols = 16 * p.ct;
     p.tiles = (int)((cols + p.cols - 1) / p.cols);
     const long blocks = (long)p.tiles * c->heads * n;
-    if (blocks >= 960 && p.tiles >= 16 && c->head_dim == 128) {
+    if (blocks >= 960 && p.tiles >= 4 && c->head_dim == 128) {
         p.cg = p.kg = 2;
         p.cols *= 2;
         p.tiles = (p.tiles + 1) / 2;

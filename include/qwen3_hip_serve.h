@@ -79,6 +79,8 @@ int qwen3_hip_kv8_append_dev(const qwen3_hip_kv8 *cache, const void *k_d, const 
  * entry's rows have been appended (qwen3_hip_kv8_append_dev with the same
  * row_d and pos_d):
  *   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j),  scale > 0
+ * (p_j up to 1, as the largest is divided out; sums of p_j v_j, which precede the
+ * division, have to stay within fp32's range)
  * q_d and out_d: [q_heads][head_dim] per row, both fp32 or, where bf16 is set,
  * both bf16; query head h reads kv head h / (q_heads / kv_heads), at most 64
  * query heads a kv head.  fp32 rows are computed with fp32 accuracy

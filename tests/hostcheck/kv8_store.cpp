@@ -7,21 +7,6 @@
 // conversion is the device's own).
 #include "kv8_host.h"
 
-// ---- buffers against an unreadable page
-static bool g_front;                                  // the page before the start, not behind the end
-static std::vector<std::pair<void *, size_t>> g_maps;
-static void *guarded(size_t bytes) {
-    const size_t page = 4096, n = (bytes + page - 1) / page * page;
-    char *p = (char *)mmap(nullptr, n + 2 * page, PROT_NONE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0);
-    if (p == MAP_FAILED || mprotect(p + page, n, PROT_READ | PROT_WRITE)) abort();
-    g_maps.push_back({p, n + 2 * page});
-    return g_front ? p + page : p + page + (n - bytes);
-}
-static void release() {
-    for (auto &m : g_maps) munmap(m.first, m.second);
-    g_maps.clear();
-}
-
 struct Case {
     qm_kv8_t c;
     const void *k, *v;

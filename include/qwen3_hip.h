@@ -141,6 +141,37 @@ int qwen3_hip_gemm_bf16a_dev(float *c_d, const uint16_t *a_d, const uint16_t *b_
 int qwen3_hip_gemm_gate_up_silu_bf16a_dev(float *h_d, const uint16_t *x_d,
                                           const uint16_t *wg_d, const uint16_t *wu_d,
                                           int M, int K, int N);
+/* ---- 8-bit integers --------------------------------------------------------
+ * No counterpart in the reference, whose weights are bf16 (SRC/kernels.h:44-57).
+ * Rows of codes with a scale each: row r stands for scale[r] * code[r][k].
+ *
+ * Rows of fp32 values, or of bf16 where bf16 is set, as such codes; a step's
+ * activations, or a weight matrix once (a row an output channel).  With a NaN
+ * taken as 0 and magnitudes beyond fp32's range as its largest value,
+ *   a = max |x| over the row, scale = a / 127 as fp32,
+ *   code = x / scale (fp32) rounded to the nearest integer, ties to even
+ * and scale = 0 and codes of 0 where a < 2^-100 (or K = 0).  x_d: rows ldx >= K
+ * values apart; q_d: ldq >= K bytes apart, what lies between K and ldq is left
+ * as it was.  Any alignment of the elements' own size; 16 bytes (x_d, ldx in
+ * bytes) and 8 (q_d, ldq) are faster.  K <= 131,071. */
+int qwen3_hip_rows_int8_dev(int8_t *q_d, size_t ldq, float *scale_d, const void *x_d, size_t ldx, int bf16, int rows,
+                            int K);
+/* C[m][n] = a_scale[m] b_scale[n] sum_k A[m][k] B[n][k]: A [M] and B [N] rows of
+ * codes lda and ldb bytes apart, all 256 values allowed; C fp32, or bf16 where
+ * bf16 is set, rows ldc values apart, columns behind N left as they were.  The
+ * sum is exact (int32: K <= 131,071, QWEN3_HIP_ETOOBIG beyond); it is rounded
+ * to fp32 and multiplied by the fp32 product of the scales.  K = 0 is a sum of
+ * 0.  Any addresses and strides; codes 16-byte aligned in rows of a multiple of
+ * 16 bytes are read many times faster, and then all of a row's lda (ldb) bytes
+ * may be read, the last row's too: what lies behind K does not matter.  c_d must
+ * not overlap what the call reads. */
+int qwen3_hip_gemm_int8_dev(void *c_d, size_t ldc, int bf16, const int8_t *a_d, size_t lda, const float *a_scale_d,
+                            const int8_t *b_d, size_t ldb, const float *b_scale_d, int M, int K, int N);
+/* h = silu(g) * u with g and u such products of the same rows x_d, in fp32 up to
+ * the store (silu as in qwen3_gemm_gate_up_silu); both weights ldw bytes a row. */
+int qwen3_hip_gemm_int8_gate_up_silu_dev(void *h_d, size_t ldh, int bf16, const int8_t *x_d, size_t ldx,
+                                         const float *x_scale_d, const int8_t *wg_d, const float *g_scale_d,
+                                         const int8_t *wu_d, const float *u_scale_d, size_t ldw, int M, int K, int N);
 /* qwen3_hip_gemm_dev that allocates nothing: no counterpart in the
  * reference ABI; for callers that cannot allocate device memory (code under
  * HIP graph capture, tight serving loops, harnesses that forbid hipMalloc).

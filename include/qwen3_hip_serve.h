@@ -140,6 +140,46 @@ int qwen3_hip_beam_select_dev(const float *logits_d, size_t ld, int vocab, int n
 int qwen3_hip_beam_reorder_dev(void *dst_d, const void *src_d, const int *parent_d, int n_group, int width, int slabs,
                                size_t slab_stride, size_t seq_stride, int runs, size_t run_stride, size_t run_bytes);
 
+/* ---- rules on logits --------------------------------------------------------
+ *
+ * What a user asks of the tokens, applied to the logits before they are chosen
+ * from (qwen3_hip_argmax_dev, qwen3_hip_beam_select_dev).  Every pointer is
+ * device memory, and every one but n_token beside token may be NULL. */
+typedef struct {
+    const int *token;           /* [n][ld_token]: the row's tokens so far, prompt first; others than 0 .. vocab - 1
+                                 * are passed over.  NULL: no penalties */
+    int ld_token;               /* at most 2^24 */
+    const int *n_prompt;        /* [n]: how many of them are the prompt (NULL: none) */
+    const int *n_token;         /* [n]: how many there are; a row whose number is not in 0 .. ld_token has none */
+    const float *repetition;    /* [n], above 0; NULL: 1 */
+    const float *presence;      /* [n]; NULL: 0 */
+    const float *frequency;     /* [n]; NULL: 0 */
+    const int *bias_row;        /* [n + 1]: row i's biases are entries bias_row[i] .. bias_row[i + 1] - 1; a row whose
+                                 * entries do not lie in 0 .. n_bias has none */
+    const int *bias_token;      /* [n_bias] */
+    const float *bias;          /* [n_bias] */
+    int n_bias;
+    const uint32_t *mask;       /* [n_mask][ld_mask]: bit t % 32 of word t / 32 set: token t is allowed */
+    size_t ld_mask;             /* words a row, at least (vocab + 31) / 32 */
+    int n_mask;
+    const int *mask_of;         /* [n]: which of the masks a row is under; any that is not one: none.  NULL: row i
+                                 * under mask i */
+} qwen3_hip_rules;
+
+/* out[i][v] = y of x = logits[i][v], v < vocab, each step rounded to fp32:
+ *   y = x;  the token is among the row's:           y = x > 0 ? x / repetition : x * repetition
+ *   c times behind the prompt, c > 0:               y = y - frequency * c, then y = y - presence
+ *   a bias names the token:                         y = y + bias (of several, the last entry's)
+ *   the row's mask does not allow the token:        y = -inf, whatever it was
+ * So a row whose mask allows nothing is -inf throughout (qwen3_hip_argmax_dev
+ * gives 0 for it), and a NaN stays one where it is allowed.  out_d may be
+ * logits_d, with ldo = ld: then only what changes is written, and without a mask
+ * only that is read.  Otherwise the two must not overlap.  Rows ld and ldo
+ * values apart, what lies behind vocab is left as it was; vocab <= 2^24, n <=
+ * 65,535.  The structure is read before the call returns; no workspace. */
+int qwen3_hip_logits_rules_dev(float *out_d, size_t ldo, const float *logits_d, size_t ld, int vocab, int n,
+                               const qwen3_hip_rules *rules);
+
 #ifdef __cplusplus
 }
 #endif

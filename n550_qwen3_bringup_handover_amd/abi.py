@@ -155,6 +155,24 @@ def gemm_gate_up_silu_bf16a_dev(h_d, x_d, wg_d, wu_d, M, K, N):
           "qwen3_hip_gemm_gate_up_silu_bf16a_dev")
 
 
+def rows_int8_dev(q_d, ldq, scale_d, x_d, ldx, bf16, rows, K):
+    """Rows of fp32 (or bf16) values as int8 codes, ldq bytes a row, with a scale each."""
+    check(runtime.lib().qwen3_hip_rows_int8_dev(q_d, ldq, scale_d, x_d, ldx, bf16, rows, K), "qwen3_hip_rows_int8_dev")
+
+
+def gemm_int8_dev(c_d, ldc, bf16, a_d, lda, a_scale_d, b_d, ldb, b_scale_d, M, K, N):
+    """C[m][n] = a_scale[m] b_scale[n] sum_k A[m][k] B[n][k] of int8 codes, as fp32 (or bf16)."""
+    check(runtime.lib().qwen3_hip_gemm_int8_dev(c_d, ldc, bf16, a_d, lda, a_scale_d, b_d, ldb, b_scale_d, M, K, N),
+          "qwen3_hip_gemm_int8_dev")
+
+
+def gemm_int8_gate_up_silu_dev(h_d, ldh, bf16, x_d, ldx, x_scale_d, wg_d, g_scale_d, wu_d, u_scale_d, ldw, M, K, N):
+    """h = silu(X.Wg^T) * (X.Wu^T) of int8 codes."""
+    check(runtime.lib().qwen3_hip_gemm_int8_gate_up_silu_dev(h_d, ldh, bf16, x_d, ldx, x_scale_d, wg_d, g_scale_d, wu_d,
+                                                             u_scale_d, ldw, M, K, N),
+          "qwen3_hip_gemm_int8_gate_up_silu_dev")
+
+
 def argmax_dev(out_d, v_d, n):
     check(runtime.lib().qwen3_hip_argmax_dev(VP(out_d), VP(v_d), n), "qwen3_hip_argmax_dev")
 
@@ -209,6 +227,19 @@ def beam_reorder_dev(dst_d, src_d, parent_d, n_group, width, slabs, slab_stride,
     """The beams' states after their parents (dst_d may be src_d)."""
     check(runtime.lib().qwen3_hip_beam_reorder_dev(dst_d, src_d, parent_d, n_group, width, slabs, slab_stride, seq_stride,
                                                    runs, run_stride, run_bytes), "qwen3_hip_beam_reorder_dev")
+
+
+def logits_rules(token=None, ld_token=0, n_prompt=None, n_token=None, repetition=None, presence=None, frequency=None,
+                 bias_row=None, bias_token=None, bias=None, n_bias=0, mask=None, ld_mask=0, n_mask=0, mask_of=None):
+    """A description of the rules on n rows of logits (qwen3_hip_rules) for the call below."""
+    return runtime.Rules(token, ld_token, n_prompt, n_token, repetition, presence, frequency, bias_row, bias_token, bias,
+                         n_bias, mask, ld_mask, n_mask, mask_of)
+
+
+def logits_rules_dev(out_d, ldo, logits_d, ld, vocab, n, rules):
+    """Penalties for repeated tokens, biases and masks on n rows of logits (out_d may be logits_d)."""
+    check(runtime.lib().qwen3_hip_logits_rules_dev(out_d, ldo, logits_d, ld, vocab, n, ctypes.byref(rules)),
+          "qwen3_hip_logits_rules_dev")
 
 
 def sync():

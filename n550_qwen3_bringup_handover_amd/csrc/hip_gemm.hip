@@ -16,6 +16,8 @@
 //   misc_kernels.h     weight re-layout, A rounding, argmax, copies
 //   small_m_kernels.h  decode-batch GEMMs, 5 <= M <= 64: weight-streaming,
 //                      skinny, narrow, wide (lm_head), 16-row
+//   int8_kernels.h     products of 8-bit integers with scales, the rows'
+//                      quantisation, and their launchers
 #include "gemm_common.h"
 #include "gemv_kernels.h"
 #include "tile_kernels.h"
@@ -1936,3 +1938,4 @@ extern "C" int qh_gemv_pro(float *c, const qh_gemv_pro_t *p, const uint16_t *b, 
     return launch_gemv1_t<true>(c, nullptr, b, b2, K, N, gated != 0, pro);
 }
 
+#include "int8_kernels.h"

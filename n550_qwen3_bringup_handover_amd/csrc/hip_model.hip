@@ -853,6 +853,7 @@ static inline hipStream_t stream() { return (hipStream_t)qh_stream(); }
 // the operators of a serving program: their kernels and launchers
 #include "kv8_kernels.h"
 #include "beam_kernels.h"
+#include "rules_kernels.h"
 
 template <bool BF>
 static int rows_norm(float *x, const float *r, const uint16_t *emb, const int *tok, int emb_rows, const uint16_t *nw,

@@ -97,6 +97,14 @@ int qh_gemm_gate_up_silu_bf16ac(uint16_t *h_d, const uint16_t *x_d, const uint16
 /* qh_gemm_bf16a that may leave K slices unadded, as qh_gemm_split */
 int qh_gemm_split_bf16a(float *c_d, const uint16_t *a_d, const uint16_t *b_d, int M, int K, int N,
                         const float **part_d, int *ks);
+/* 8-bit integer rows and their products (int8_kernels.h); what they compute and
+ * what they refuse: include/qwen3_hip.h */
+int qh_rows_int8(int8_t *q_d, size_t ldq, float *scale_d, const void *x_d, size_t ldx, int bf16, int rows, int K);
+int qh_gemm_int8(void *c_d, size_t ldc, int bf16, const int8_t *a_d, size_t lda, const float *as_d, const int8_t *b_d,
+                 size_t ldb, const float *bs_d, int M, int K, int N);
+int qh_gemm_int8_gate_up_silu(void *h_d, size_t ldh, int bf16, const int8_t *x_d, size_t ldx, const float *xs_d,
+                              const int8_t *wg_d, const float *gs_d, const int8_t *wu_d, const float *us_d, size_t ldw,
+                              int M, int K, int N);
 /* tile-major [N/tn][K/tk][tn][tk] -> row-major [N][K] */
 int qh_tile_to_row(uint16_t *dst_d, const uint16_t *src_d, int N, int K,
                    int tile_n, int tile_k);

@@ -584,6 +584,24 @@ int qwen3_hip_gemm_gate_up_silu_bf16a_dev(float *h, const uint16_t *x, const uin
     return note(qh_gemm_gate_up_silu_bf16a(h, x, wg, wu, M, K, N));
 }
 
+int qwen3_hip_rows_int8_dev(int8_t *q, size_t ldq, float *scale, const void *x, size_t ldx, int bf16, int rows, int K) {
+    READY_OR_RETURN();
+    return note(qh_rows_int8(q, ldq, scale, x, ldx, bf16, rows, K));
+}
+
+int qwen3_hip_gemm_int8_dev(void *c, size_t ldc, int bf16, const int8_t *a, size_t lda, const float *a_scale,
+                            const int8_t *b, size_t ldb, const float *b_scale, int M, int K, int N) {
+    READY_OR_RETURN();
+    return note(qh_gemm_int8(c, ldc, bf16, a, lda, a_scale, b, ldb, b_scale, M, K, N));
+}
+
+int qwen3_hip_gemm_int8_gate_up_silu_dev(void *h, size_t ldh, int bf16, const int8_t *x, size_t ldx,
+                                         const float *x_scale, const int8_t *wg, const float *g_scale, const int8_t *wu,
+                                         const float *u_scale, size_t ldw, int M, int K, int N) {
+    READY_OR_RETURN();
+    return note(qh_gemm_int8_gate_up_silu(h, ldh, bf16, x, ldx, x_scale, wg, g_scale, wu, u_scale, ldw, M, K, N));
+}
+
 int qwen3_hip_decode_set_dev(const uint16_t *const *w, const float *x0, float *out, int layers) {
     READY_OR_RETURN();
     return note(qh_decode_persist(w, x0, out, layers));
@@ -669,6 +687,15 @@ int qwen3_hip_beam_reorder_dev(void *dst, const void *src, const int *parent, in
     READY_OR_RETURN();
     return note(qm_beam_reorder(dst, src, parent, n_group, width, slabs, slab_stride, seq_stride, runs, run_stride,
                                 run_bytes));
+}
+
+int qwen3_hip_logits_rules_dev(float *out, size_t ldo, const float *logits, size_t ld, int vocab, int n,
+                               const qwen3_hip_rules *r) {
+    if (!r) return note(QWEN3_HIP_EINVAL);
+    READY_OR_RETURN();
+    const qm_rules_t t = {r->token, r->ld_token, r->n_prompt, r->n_token, r->repetition, r->presence, r->frequency,
+                          r->bias_row, r->bias_token, r->bias, r->n_bias, r->mask, r->ld_mask, r->n_mask, r->mask_of};
+    return note(qm_logits_rules(out, ldo, logits, ld, vocab, n, &t));
 }
 
 int qwen3_hip_capture_begin(void) { READY_OR_RETURN(); return note(qh_capture_begin()); }

@@ -158,6 +158,26 @@ int qm_beam_record(int *hist_d, const int *token_d, const int *parent_d, int *po
 int qm_beam_reorder(void *dst_d, const void *src_d, const int *parent_d, int n_group, int width, int slabs,
                     size_t slab_stride, size_t seq_stride, int runs, size_t run_stride, size_t run_bytes);
 
+/* ---- rules on logits (rules_kernels.h); what the fields hold and what the call
+ * does: include/qwen3_hip_serve.h */
+#define QM_RULES_MAX_ROWS 65535
+#define QM_RULES_MAX_VOCAB (1 << 24)
+#define QM_RULES_MAX_TOKENS (1 << 24)  /* a count is exact as fp32 */
+typedef struct {
+    const int *token;
+    int ld_token;
+    const int *n_prompt, *n_token;
+    const float *repetition, *presence, *frequency;
+    const int *bias_row, *bias_token;
+    const float *bias;
+    int n_bias;
+    const uint32_t *mask;
+    size_t ld_mask;
+    int n_mask;
+    const int *mask_of;
+} qm_rules_t;
+int qm_logits_rules(float *out_d, size_t ldo, const float *logits_d, size_t ld, int vocab, int n, const qm_rules_t *rules);
+
 /* tok[0 .. n) = the host's tokens (n <= QM_MAX_CHUNK) and *pos = pos0, both
  * passed as kernel arguments: the caller's buffer is read before the return */
 int qm_set_tokens(int *tok_d, const int *tokens, int n, int *pos_d, int pos0);

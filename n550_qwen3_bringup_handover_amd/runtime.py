@@ -35,6 +35,17 @@ class Kv8(ctypes.Structure):
 KV8P = ctypes.POINTER(Kv8)
 
 
+class Rules(ctypes.Structure):
+    """qwen3_hip_rules (include/qwen3_hip_serve.h): what is asked of the tokens of n rows of logits"""
+    _fields_ = [("token", VP), ("ld_token", ctypes.c_int), ("n_prompt", VP), ("n_token", VP), ("repetition", VP),
+                ("presence", VP), ("frequency", VP), ("bias_row", VP), ("bias_token", VP), ("bias", VP),
+                ("n_bias", ctypes.c_int), ("mask", VP), ("ld_mask", ctypes.c_size_t), ("n_mask", ctypes.c_int),
+                ("mask_of", VP)]
+
+
+RULESP = ctypes.POINTER(Rules)
+
+
 class Qwen3HipError(RuntimeError):
     pass
 
@@ -72,6 +83,13 @@ _PROTOS = {
     "qwen3_hip_scratch_bytes": (ctypes.c_size_t, []),
     "qwen3_hip_gemm_bf16a_dev": (ctypes.c_int, [VP, VP, VP, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "qwen3_hip_gemm_gate_up_silu_bf16a_dev": (ctypes.c_int, [VP, VP, VP, VP, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "qwen3_hip_rows_int8_dev": (ctypes.c_int, [VP, ctypes.c_size_t, VP, VP, ctypes.c_size_t, ctypes.c_int, ctypes.c_int,
+                                               ctypes.c_int]),
+    "qwen3_hip_gemm_int8_dev": (ctypes.c_int, [VP, ctypes.c_size_t, ctypes.c_int, VP, ctypes.c_size_t, VP, VP,
+                                               ctypes.c_size_t, VP, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "qwen3_hip_gemm_int8_gate_up_silu_dev": (ctypes.c_int, [VP, ctypes.c_size_t, ctypes.c_int, VP, ctypes.c_size_t, VP,
+                                                            VP, VP, VP, VP, ctypes.c_size_t, ctypes.c_int, ctypes.c_int,
+                                                            ctypes.c_int]),
     "qwen3_hip_decode_set_dev": (ctypes.c_int, [ctypes.POINTER(VP), VP, VP, ctypes.c_int]),
     "qwen3_hip_decode_set_supported": (ctypes.c_int, []),
     "qwen3_hip_decode_set_out_ld": (ctypes.c_int, []),
@@ -134,6 +152,8 @@ _PROTOS = {
                                                  ctypes.c_int, ctypes.c_int, VP, VP, VP, VP, VP, ctypes.c_size_t]),
     "qwen3_hip_beam_reorder_dev": (ctypes.c_int, [VP, VP, VP, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_size_t,
                                                   ctypes.c_size_t, ctypes.c_int, ctypes.c_size_t, ctypes.c_size_t]),
+    "qwen3_hip_logits_rules_dev": (ctypes.c_int, [VP, ctypes.c_size_t, VP, ctypes.c_size_t, ctypes.c_int, ctypes.c_int,
+                                                  RULESP]),
 }
 
 # qwen3_hip_dump_fn

@@ -1,0 +1,221 @@
+"""Rules on logits on the GPU, against their definition (tests/int8_oracle.py) bit for bit, and a run of 8-bit rows, the
+head's product, rules and choices together."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from n550_qwen3_bringup_handover_amd import abi, runtime
+from tests import int8_oracle as io
+
+pytestmark = pytest.mark.gpu
+F32 = np.float32
+UP = abi.DeviceBuffer.from_array
+
+
+@pytest.fixture(scope="module", autouse=True)
+def lib():
+    return runtime.init()
+
+
+def made(rng, n, vocab, history=0, biases=0, masks=0, allowed=0.5, mask_of=True, prompt=True):
+    r = {}
+    if history:
+        r["token"] = (vocab ** rng.random((n, history)) - 1).astype(np.int32)
+        r["token"][rng.random((n, history)) < 0.02] = -1          # no tokens: passed over
+        r["token"][rng.random((n, history)) < 0.02] = vocab
+        r["n_token"] = rng.integers(0, history + 1, n).astype(np.int32)
+        r["n_token"][0] = history
+        if prompt:
+            r["n_prompt"] = (r["n_token"] * rng.random(n)).astype(np.int32)
+        r["repetition"] = rng.uniform(0.7, 1.6, n).astype(F32)
+        r["presence"] = rng.uniform(-1, 1, n).astype(F32)
+        r["frequency"] = rng.uniform(-0.5, 0.5, n).astype(F32)
+    if biases:
+        count = rng.integers(0, biases + 1, n)
+        count[-1] = biases
+        r["bias_row"] = np.concatenate([[0], np.cumsum(count)]).astype(np.int32)
+        r["n_bias"] = int(count.sum())
+        r["bias_token"] = rng.integers(-1, min(vocab, 3 * biases) + 1, r["n_bias"]).astype(np.int32)   # some twice, some none
+        r["bias"] = rng.standard_normal(r["n_bias"]).astype(F32) * 5
+    if masks:
+        bits = rng.random((masks, (vocab + 31) // 32 + 2, 32)) < allowed
+        r["mask"] = np.packbits(bits, axis=-1, bitorder="little").reshape(masks, -1).view(np.uint32)
+        r["n_mask"] = masks
+        if mask_of:
+            r["mask_of"] = rng.integers(-1, masks + 1, n).astype(np.int32)
+    return r
+
+
+def on_device(r):
+    """(what keeps the memory, the description)"""
+    keep = {k: UP(v) for k, v in r.items() if isinstance(v, np.ndarray) and v.size}
+    kw = {k: b.ptr for k, b in keep.items()}
+    kw.update({k: v for k, v in r.items() if isinstance(v, int)})
+    if "token" in r:
+        kw["ld_token"] = r["token"].shape[1]
+    if "mask" in r:
+        kw["ld_mask"] = r["mask"].shape[1]
+    return keep, abi.logits_rules(**kw)
+
+
+def apply(x, vocab, r, ld=None, ldo=None, in_place=False):
+    n = x.shape[0]
+    ld, ldo = ld or vocab, ldo or vocab
+    if in_place:
+        ldo = ld
+    full = np.full((n, ld), np.nan, F32)
+    full[:, :vocab] = x
+    xd = UP(full)
+    od = xd if in_place else UP(np.full((n, ldo), 7.25, F32))
+    keep, rules = on_device(r)
+    abi.logits_rules_dev(od.ptr, ldo, xd.ptr, ld, vocab, n, rules)
+    abi.sync()
+    out = od.download(F32, n * ldo).reshape(n, ldo)
+    if in_place:
+        assert np.isnan(out[:, vocab:]).all()
+    else:
+        assert (out[:, vocab:] == 7.25).all()
+        assert np.array_equal(xd.download(F32, n * ld).reshape(n, ld), full, equal_nan=True)
+    return out[:, :vocab]
+
+
+def same(got, want):
+    bad = np.argwhere(~((got == want) | (np.isnan(got) & np.isnan(want))))
+    assert not len(bad), (len(bad), bad[:5], got[tuple(bad[0])], want[tuple(bad[0])])
+
+
+CASES = [(1, 1, dict(history=1)), (1, 31, dict(masks=1)), (2, 33, dict(history=5, biases=3, masks=2)),
+         (3, 1000, dict(history=100)), (5, 4095, dict(biases=50)), (4, 4096, dict(masks=3)), (4, 4097, dict(history=3000, masks=3)),
+         (2, 8192, dict(history=9000, biases=500, masks=2)), (3, 12001, dict(history=70, prompt=False)),
+         (1, 151936, dict(history=700, biases=10)), (64, 151936, dict(history=600, biases=30, masks=8, allowed=0.3)),
+         (9, 151936, dict(masks=9, allowed=0.001, mask_of=False)), (128, 2000, dict(history=200, masks=5, allowed=0.99)),
+         (2, 300001, dict(history=20000, biases=7)), (3, 500, dict())]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("n,vocab,kw", CASES)
+def test_rules(n, vocab, kw, in_place):
+    print("rules", n, vocab, kw, in_place, flush=True)
+    rng = np.random.default_rng(n * 7 + vocab)
+    x = (2.5 * rng.standard_normal((n, vocab))).astype(F32)
+    r = made(rng, n, vocab, **kw)
+    same(apply(x, vocab, r, in_place=in_place), io.rules(x, vocab, **r))
+    for pad in (1, 4):
+        same(apply(x, vocab, r, ld=vocab + pad, ldo=vocab + 2 * pad + 1, in_place=in_place), io.rules(x, vocab, **r))
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("leave", ["repetition", "presence", "frequency", "n_prompt"])
+def test_rules_left_out(leave, in_place):
+    rng = np.random.default_rng(1)
+    x = rng.standard_normal((6, 5000)).astype(F32)
+    r = made(rng, 6, 5000, history=400, biases=20, masks=4)
+    del r[leave]
+    same(apply(x, 5000, r, in_place=in_place), io.rules(x, 5000, **r))
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_odd_values(in_place):
+    """infinities, NaN and the type's lowest value, in allowed and in masked places; masks that leave nothing"""
+    rng = np.random.default_rng(2)
+    n, vocab = 4, 6000
+    x = rng.standard_normal((n, vocab)).astype(F32)
+    odd = np.array([np.nan, np.inf, -np.inf, np.finfo(F32).min, np.finfo(F32).max, 0.0, -0.0, 1e-42], F32)
+    x[:, :2000] = odd[rng.integers(0, 8, (n, 2000))]
+    r = made(rng, n, vocab, history=3000, biases=300, masks=3)
+    r["token"][:, ::2] %= 2000
+    r["mask"][2] = 0
+    r["mask_of"][:] = [0, 1, 2, 2]
+    r["bias"][::5] = -np.inf
+    r["bias"][1::5] = np.inf
+    got = apply(x, vocab, r, in_place=in_place)
+    same(got, io.rules(x, vocab, **r))
+    assert (got[2:] == -np.inf).all() and np.isnan(got[0]).any()
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rows_whose_numbers_do_not_fit_have_no_such_rule(in_place):
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((6, 900)).astype(F32)
+    r = made(rng, 6, 900, history=50, biases=9, masks=2)
+    r["n_token"][:] = [-1, 51, 50, 0, 2 ** 31 - 1, -2 ** 31]
+    r["n_prompt"][:] = [0, 0, -5, 7, 0, 0]
+    r["mask_of"][:] = [2, -1, 2 ** 31 - 1, -2 ** 31, 0, 1]
+    r["bias_row"][:] = [0, 3, r["n_bias"] + 1, 2, -4, 5, 1]         # too far, backwards, before the first
+    same(apply(x, 900, r, in_place=in_place), io.rules(x, 900, **r))
+
+
+def test_one_token_many_times():
+    """counts are exact: 2^20 occurrences, every thread's on one word"""
+    x = np.ones((1, 40), F32)
+    r = dict(token=np.full((1, 1 << 20), 7, np.int32), n_token=np.array([1 << 20], np.int32), n_prompt=np.array([5], np.int32),
+             frequency=np.array([2.0 ** -10], F32))
+    got = apply(x, 40, r)
+    assert got[0, 7] == 1 - ((1 << 20) - 5) / 1024 and (np.delete(got[0], 7) == 1).all()
+
+
+def test_the_same_bias_twice():
+    """the last entry counts, in every order of a block's threads"""
+    rng = np.random.default_rng(4)
+    x = np.zeros((1, 64), F32)
+    tok = rng.integers(0, 64, 5000).astype(np.int32)
+    val = np.arange(5000, dtype=F32)
+    r = dict(bias_row=np.array([0, 5000], np.int32), bias_token=tok, bias=val, n_bias=5000)
+    for _ in range(3):
+        got = apply(x, 64, r)
+        assert all(got[0, v] == val[np.flatnonzero(tok == v)[-1]] for v in range(64))
+
+
+def test_a_decode_steps_end_together():
+    """hidden rows -> codes -> the head's product -> rules -> the choice, greedy and of beams, recorded in one graph whose
+    history grows between the replays"""
+    L = runtime.lib()
+    rng = np.random.default_rng(6)
+    n, k, vocab, hist = 6, 1024, 20000, 40
+    w = rng.standard_normal((vocab, k)).astype(F32)
+    x = rng.standard_normal((n, k)).astype(F32)
+    wd, xd = UP(w), UP(x)
+    wq, ws, xq, xs = UP(np.zeros((vocab, k), np.int8)), UP(np.zeros(vocab, F32)), UP(np.zeros((n, k), np.int8)), UP(np.zeros(n, F32))
+    logits, out, choice = UP(np.zeros((n, vocab), F32)), UP(np.zeros((n, vocab), F32)), UP(np.zeros(n, np.int32))
+    r = made(rng, n, vocab, history=hist, biases=8, masks=3, allowed=0.7)
+    r["n_token"][:], r["n_prompt"][:] = 10, 4
+    keep, rules = on_device(r)
+    work = UP(np.zeros(abi.beam_select_work(vocab, 2, 3), np.uint8))
+    score, done = UP(np.zeros(n, F32)), UP(np.zeros(n, np.int32))
+    score2, done2, tok2, par2 = UP(np.zeros(n, F32)), *(UP(np.zeros(n, np.int32)) for _ in range(3))
+    abi.rows_int8_dev(wq.ptr, k, ws.ptr, wd.ptr, k, False, vocab, k)
+
+    def step():
+        abi.rows_int8_dev(xq.ptr, k, xs.ptr, xd.ptr, k, False, n, k)
+        abi.gemm_int8_dev(logits.ptr, vocab, False, xq.ptr, k, xs.ptr, wq.ptr, k, ws.ptr, n, k, vocab)
+        abi.logits_rules_dev(out.ptr, vocab, logits.ptr, vocab, vocab, n, rules)
+        for i in range(n):
+            abi.argmax_dev(choice.ptr + 4 * i, out.ptr + 4 * i * vocab, vocab)
+        abi.beam_select_dev(out.ptr, vocab, vocab, 2, 3, score.ptr, done.ptr, 0, -1, score2.ptr, done2.ptr, tok2.ptr, par2.ptr,
+                            work.ptr, work.nbytes)
+
+    g = ctypes.c_int()
+    runtime.check(L.qwen3_hip_capture_begin())
+    step()
+    runtime.check(L.qwen3_hip_capture_end(ctypes.byref(g)))
+    qw, sw = io.rows(w)
+    for t in range(4):
+        x = rng.standard_normal((n, k)).astype(F32)
+        xd.upload(x)
+        runtime.check(L.qwen3_hip_graph_launch(g.value))
+        abi.sync()
+        qx, sx = io.rows(x)
+        want = io.rules(io.product(qx, sx, qw, sw), vocab, **r)
+        same(out.download(F32, n * vocab).reshape(n, vocab), want)
+        got = choice.download(np.int32, n)
+        assert np.array_equal(got, want.argmax(1))
+        # the beams' choice, of all but ties: the best continuation of each group in 64 bits
+        logp = want - np.log(np.exp(want.astype(np.float64) - want.max(1, keepdims=True)).sum(1, keepdims=True)) - want.max(1, keepdims=True)
+        best = [divmod(int(logp[3 * i:3 * i + 3].argmax()), vocab) for i in range(2)]
+        assert [tuple(b) for b in zip(par2.download(np.int32, n)[::3], tok2.download(np.int32, n)[::3])] == best
+        r["token"][np.arange(n), r["n_token"]] = got
+        r["n_token"] += 1
+        keep["token"].upload(r["token"])
+        keep["n_token"].upload(r["n_token"])
+    runtime.check(L.qwen3_hip_graph_destroy(g.value))

@@ -124,11 +124,402 @@ __global__ __launch_bounds__(NTHREADS) void k_i8_any(I8Args p) {
     }
 }
 
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+// What the kernels below take: 16-byte aligned codes in rows of a multiple of
+// 16 bytes, so that a row's last piece of 16 may be read whole.  What lies in it
+// behind K may be anything: A's bytes there are cleared, and B's then count for
+// nothing.  Rows behind M and columns behind N repeat the last ones and are not
+// stored.
+__device__ __forceinline__ i32x4 i8_keep(i32x4 v, int left) {     // the first `left` of 16 codes, the others 0
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int n = left - 4 * j;
+        v[j] = n >= 4 ? v[j] : n <= 0 ? 0 : (int)((uint32_t)v[j] & ((1u << (8 * n)) - 1));
+    }
+    return v;
+}
+__device__ __forceinline__ i32x4 i8_load(const int8_t *p) { return *(const i32x4 *)p; }
+
+// ---------------------------------------------------------------------------
+// Few rows, few columns: 16 columns and 16 MT rows a block, K split over its W
+// waves
+// ---------------------------------------------------------------------------
+// D = W X^T with 16x16x64 MFMAs: lane (r, g) = (lane % 16, lane / 16) holds codes
+// 16 g .. 16 g + 15 of weight row r (A operand) and of row r of x (B operand),
+// and gets rows 4 g + i (columns of C) of column r (a row of C).  Operands come
+// straight from memory, a wave's pieces of 128 bytes of each row.  Sums are
+// integers, so the waves' may be added in any order.
+template <int MT, int W, bool GATED, bool CBF>
+__global__ __launch_bounds__(WAVE *W) void k_i8_narrow(I8Args p) {
+    constexpr int G = GATED ? 2 : 1;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
+    const int8_t *wp[G], *xp[MT];
+    wp[0] = p.b + (size_t)min(n0 + r, p.N - 1) * p.ldb;
+    if constexpr (GATED) wp[G - 1] = p.b2 + (size_t)min(n0 + r, p.N - 1) * p.ldb;
+#pragma unroll
+    for (int t = 0; t < MT; t++) xp[t] = p.a + (size_t)min(m0 + 16 * t + r, p.M - 1) * p.lda;
+    struct Set { i32x4 w[2][G], x[2][MT]; };
+    auto load = [&](Set &s, int c) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int k = 128 * c + 64 * u + 16 * g, at = k < p.K ? k : 0;
+#pragma unroll
+            for (int q = 0; q < G; q++) s.w[u][q] = i8_load(wp[q] + at);
+#pragma unroll
+            for (int t = 0; t < MT; t++) s.x[u][t] = i8_load(xp[t] + at);
+        }
+    };
+    i32x4 acc[G][MT] = {};
+    auto multiply = [&](Set &s, int c) {
+        if (128 * c + 128 > p.K) {                        // the last piece, not whole
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int t = 0; t < MT; t++) s.x[u][t] = i8_keep(s.x[u][t], p.K - (128 * c + 64 * u + 16 * g));
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+#pragma unroll
+                for (int q = 0; q < G; q++)
+                    acc[q][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.w[u][q], s.x[u][t], acc[q][t], 0, 0, 0);
+    };
+    const int pieces = (p.K + 127) / 128;
+    Set s0, s1;
+    int c = wave;
+    if (c < pieces) load(s0, c);
+    for (; c < pieces; c += 2 * W) {
+        if (c + W < pieces) load(s1, c + W);
+        multiply(s0, c);
+        if (c + W >= pieces) break;
+        if (c + 2 * W < pieces) load(s0, c + 2 * W);
+        multiply(s1, c + W);
+    }
+    __shared__ i32x4 red[W][G][MT][WAVE];
+#pragma unroll
+    for (int q = 0; q < G; q++)
+#pragma unroll
+        for (int t = 0; t < MT; t++) red[wave][q][t][lane] = acc[q][t];
+    __syncthreads();
+    const int *flat = (const int *)red;
+    constexpr int OUT = MT * WAVE * 4;                    // sums of one product
+    for (int o = tid; o < OUT; o += W * WAVE) {
+        const int m = m0 + o / (WAVE * 4) * 16 + (o >> 2 & 15), n = n0 + (o >> 6 & 3) * 4 + (o & 3);
+        int v[G] = {};
+#pragma unroll
+        for (int w = 0; w < W; w++)
+#pragma unroll
+            for (int q = 0; q < G; q++) v[q] += flat[(w * G + q) * OUT + o];
+        if (m >= p.M || n >= p.N) continue;
+        const float sm = p.as[m];
+        float y = (float)v[0] * (sm * p.bs[n]);
+        if constexpr (GATED) y = silu_mul(y, (float)v[G - 1] * (sm * p.bs2[n]));
+        i8_store<CBF>(p.c, (size_t)m * p.ldc + n, y);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows, many columns: the rows stay in LDS, every wave streams weights
+// ---------------------------------------------------------------------------
+// The operands' roles and layouts are those above.  A block's 8 waves take 16
+// columns each at a time, U steps of 64 codes in flight ahead of the U being
+// multiplied.  x lies in LDS with K rounded up to 256 and zeros behind K; piece
+// c of 16 codes of row r at place c ^ (r % 16), so that the 16 rows of a read
+// meet different banks.
+#define I8_WIDE_WAVES 8
+template <int MT, int LDS, bool GATED, bool CBF>
+__global__ __launch_bounds__(WAVE *I8_WIDE_WAVES, 4) void k_i8_wide(I8Args p, int vec) {
+    constexpr int G = GATED ? 2 : 1, U = GATED ? 4 : 8, NT = WAVE * I8_WIDE_WAVES;
+    __shared__ i32x4 sx[LDS / 16];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int per = (p.K + 255) / 256 * 16;               // pieces of a row in LDS
+    for (int i = tid; i < 16 * MT * per; i += NT) {
+        const int row = i / per, c = i % per;
+        i32x4 v = {};
+        if (16 * c < p.K) v = i8_keep(i8_load(p.a + (size_t)min(row, p.M - 1) * p.lda + 16 * c), p.K - 16 * c);
+        sx[row * per + (c ^ (row & 15))] = v;
+    }
+    float sm[MT];
+#pragma unroll
+    for (int t = 0; t < MT; t++) sm[t] = p.as[min(16 * t + r, p.M - 1)];
+    __syncthreads();
+
+    const int steps = (p.K + 63) / 64, sets = (steps + U - 1) / U;
+    const int tiles = (p.N + 15) / 16, stride = gridDim.x * I8_WIDE_WAVES;
+    struct Set { i32x4 w[U][G]; };
+    auto load = [&](Set &s, int tile, int set) {
+        const size_t row = (size_t)min(tile * 16 + r, p.N - 1) * p.ldb;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int k = 64 * (set * U + u) + 16 * g, at = k < p.K ? k : 0;
+            s.w[u][0] = i8_load(p.b + row + at);
+            if constexpr (GATED) s.w[u][G - 1] = i8_load(p.b2 + row + at);
+        }
+    };
+    i32x4 acc[G][MT] = {};
+    auto step = [&](const Set &s, int set, int u) {
+#pragma unroll
+        for (int t = 0; t < MT; t++) {
+            const i32x4 x = sx[(16 * t + r) * per + ((4 * (set * U + u) + g) ^ r)];
+#pragma unroll
+            for (int q = 0; q < G; q++) acc[q][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.w[u][q], x, acc[q][t], 0, 0, 0);
+        }
+    };
+    auto multiply = [&](const Set &s, int set) {
+        if ((set + 1) * U <= steps) {
+#pragma unroll
+            for (int u = 0; u < U; u++) step(s, set, u);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (set * U + u < steps) step(s, set, u);
+        }
+    };
+    auto finish = [&](int tile) {
+        const int n = tile * 16 + 4 * g;
+        float sn[G][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            sn[0][i] = p.bs[min(n + i, p.N - 1)];
+            if constexpr (GATED) sn[G - 1][i] = p.bs2[min(n + i, p.N - 1)];
+        }
+#pragma unroll
+        for (int t = 0; t < MT; t++) {
+            const int m = 16 * t + r;
+            f32x4 y;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                y[i] = (float)acc[0][t][i] * (sm[t] * sn[0][i]);
+                if constexpr (GATED) y[i] = silu_mul(y[i], (float)acc[G - 1][t][i] * (sm[t] * sn[G - 1][i]));
+            }
+#pragma unroll
+            for (int q = 0; q < G; q++) acc[q][t] = i32x4{};
+            if (m >= p.M) continue;
+            const size_t at = (size_t)m * p.ldc + n;
+            if (vec && n + 4 <= p.N) {
+                if constexpr (CBF)
+                    *(uint2 *)((uint16_t *)p.c + at) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+                else
+                    *(f32x4 *)((float *)p.c + at) = y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (n + i < p.N) i8_store<CBF>(p.c, at + i, y[i]);
+            }
+        }
+    };
+    int tile = blockIdx.x * I8_WIDE_WAVES + wave, set = 0;
+    if (tile >= tiles) return;
+    auto next = [&](int &t, int &s) {
+        if (++s == sets) {
+            s = 0;
+            t += stride;
+        }
+    };
+    Set s0, s1;
+    load(s0, tile, 0);
+    for (;;) {
+        int t1 = tile, k1 = set;
+        next(t1, k1);
+        if (t1 < tiles) load(s1, t1, k1);
+        multiply(s0, set);
+        if (k1 == 0) finish(tile);
+        if (t1 >= tiles) break;
+        tile = t1;
+        set = k1;
+        next(tile, set);
+        if (tile < tiles) load(s0, tile, set);
+        multiply(s1, k1);
+        if (set == 0) finish(t1);
+        if (tile >= tiles) break;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: tiles through LDS
+// ---------------------------------------------------------------------------
+// BM x BN outputs a block of WM x WN waves, 32x32x32 MFMAs: lane (c, h) = (lane %
+// 32, lane / 32) gives codes 16 h .. 16 h + 15 of row c of either operand and
+// holds rows 8 (e / 4) + 4 h + e % 4 of column c of the result.  Stages of BK codes
+// of each row are copied from memory straight into one of ST places in LDS, 1,024
+// bytes an instruction; piece c of 16 codes of row r lies at place c ^ f(r) of its
+// row, f such that the rows of a fragment meet different banks, and with a period
+// of 32 rows so that a wave's fragments differ by constants.
+template <int BM_, int BN_, int WM_, int WN_, int BK_, int ST_>
+struct I8Tile {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = BK_, ST = ST_;
+    static constexpr int NW = WM * WN, CPR = BK / 16, RPI = 64 / CPR;    // rows that a copy instruction fills
+    static constexpr int TM = BM / WM / 32, TN = BN / WN / 32, KS = BK / 32;
+    static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE = A_BYTES + B_BYTES;
+    static constexpr int A_DMA = A_BYTES / 1024 / NW, B_DMA = B_BYTES / 1024 / NW, DMA = A_DMA + B_DMA;
+    static_assert(A_DMA * NW * 1024 == A_BYTES && B_DMA * NW * 1024 == B_BYTES, "whole copies a wave");
+    static_assert(TM >= 1 && TN >= 1 && ST >= 2 && ST * STAGE <= 160 * 1024, "tile");
+    static_assert(STAGE >= 12 * 256, "the scales of a tile in a stage's place");
+};
+template <int CPR>
+__device__ __forceinline__ int i8_swz(int row) {
+    if constexpr (CPR == 8) return (row ^ (row >> 3 & 3)) & 7;
+    else return (row ^ (row >> 2)) & 3;
+}
+// 16 bytes a lane from byte at + k0 of a buffer to 1,024 of LDS.  (The host's pass
+// knows the builtin, but not the size, and would drop the kernels that use it.)
+typedef __attribute__((address_space(3))) void i8_lds;
+__device__ __forceinline__ void i8_copy(__amdgpu_buffer_rsrc_t from, unsigned char *to, int at, int k0) {
+#ifdef __HIP_DEVICE_COMPILE__
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (i8_lds *)to, 16, at, k0, 0, 0);
+#endif
+}
+#define I8_VMCNT(n) (0x0070 | ((n) & 15) | ((n) >> 4 << 14))      // s_waitcnt vmcnt(n) lgkmcnt(0)
+
+template <typename T, bool GATED, bool CBF>
+__global__ __launch_bounds__(WAVE *T::NW, T::NW == 8 ? 2 : 1) void k_i8_tile(I8Args p, int MT, int NT, int per) {
+    constexpr int BNO = GATED ? T::BN / 2 : T::BN, ES = CBF ? 2 : 4;
+    __shared__ __align__(1024) unsigned char smem[T::ST * T::STAGE];
+    // tiles in the order of the XCDs, which get workgroups in turn: each a run of
+    // `per` tiles, walked in groups of 8 tile rows, so that what runs together on
+    // an XCD shares its L2
+    const int local = blockIdx.x >> 3, idx = (blockIdx.x & 7) * per + local;
+    if (idx >= MT * NT) return;
+    const int first = idx / (8 * NT) * 8, gs = min(MT - first, 8), in = idx - first * NT;
+    const int m0 = (first + in % gs) * T::BM, n0 = in / gs * BNO;
+
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int wm = wave / T::WN, wn = wave % T::WN;
+    const int rows = min(p.M - m0, T::BM), cols = min(p.N - n0, BNO);
+    const auto ra = buf_rsrc(p.a + (size_t)m0 * p.lda, (size_t)rows * p.lda);
+    const auto rb = buf_rsrc(p.b + (size_t)n0 * p.ldb, (size_t)cols * p.ldb);
+    const auto rb2 = buf_rsrc((GATED ? p.b2 : p.b) + (size_t)n0 * p.ldb, (size_t)cols * p.ldb);
+    // row and piece that copy instruction i of the wave brings to this lane's place
+    auto a_row = [&](int i) { return (wave * T::A_DMA + i) * T::RPI + lane / T::CPR; };
+    auto b_row = [&](int i) { return (wave * T::B_DMA + i) * T::RPI + lane / T::CPR; };
+    auto piece = [&](int row) { return ((lane % T::CPR) ^ i8_swz<T::CPR>(row)) * 16; };
+    auto a_at = [&](int i) { return min(a_row(i), rows - 1) * (int)p.lda; };
+    auto b_at = [&](int i) { return min(GATED && b_row(i) >= BNO ? b_row(i) - BNO : b_row(i), cols - 1) * (int)p.ldb; };
+    int va[T::A_DMA], vb[T::B_DMA];
+#pragma unroll
+    for (int i = 0; i < T::A_DMA; i++) va[i] = a_at(i) + piece(a_row(i));
+#pragma unroll
+    for (int i = 0; i < T::B_DMA; i++) vb[i] = b_at(i) + piece(b_row(i));
+    // WHOLE 0: the last stage, of fewer than BK codes.  A's come through registers, those
+    // behind K cleared; of pieces that lie behind K the stage's first is read instead
+    auto issue = [&](int kt, auto WHOLE) {
+        unsigned char *slot = smem + kt % T::ST * T::STAGE;
+        const int k0 = kt * T::BK, room = p.K - k0;
+#pragma unroll
+        for (int i = 0; i < T::A_DMA; i++) {
+            unsigned char *to = slot + (wave * T::A_DMA + i) * 1024;
+            if constexpr (decltype(WHOLE)::value) {
+                i8_copy(ra, to, va[i], k0);
+            } else {
+                const int pc = piece(a_row(i)), at = a_at(i) + (pc < room ? pc : 0);
+                const i32x4 v = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(ra, at, k0, 0));
+                *(i32x4 *)(to + lane * 16) = i8_keep(v, room - pc);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < T::B_DMA; i++) {
+            const bool up = GATED && (wave * T::B_DMA + i) * T::RPI >= BNO;
+            const int at = decltype(WHOLE)::value || piece(b_row(i)) < room ? vb[i] : b_at(i);
+            i8_copy(up ? rb2 : rb, slot + T::A_BYTES + (wave * T::B_DMA + i) * 1024, at, k0);
+        }
+    };
+    // this lane's first fragment of A and of B in each step of a stage; the others lie 32 rows on
+    const int fr = lane & 31, fh = lane >> 5;
+    constexpr int NEXT = 32 * T::BK, UP = (BNO - 32 * (T::TN / 2)) * T::BK;
+    int fa_at[T::KS], fb_at[T::KS];
+#pragma unroll
+    for (int s = 0; s < T::KS; s++) {
+        const int pc = ((2 * s + fh) ^ i8_swz<T::CPR>(fr)) * 16;
+        fa_at[s] = (wm * (T::BM / T::WM) + fr) * T::BK + pc;
+        fb_at[s] = T::A_BYTES + (wn * (BNO / T::WN) + fr) * T::BK + pc;
+    }
+    i32x16 acc[T::TM][T::TN] = {};
+    auto multiply = [&](int kt) {
+        const unsigned char *slot = smem + kt % T::ST * T::STAGE;
+#pragma unroll
+        for (int s = 0; s < T::KS; s++) {
+            i32x4 fa[T::TM], fb[T::TN];
+#pragma unroll
+            for (int i = 0; i < T::TM; i++) fa[i] = *(const i32x4 *)(slot + fa_at[s] + i * NEXT);
+#pragma unroll
+            for (int j = 0; j < T::TN; j++)
+                fb[j] = *(const i32x4 *)(slot + fb_at[s] + j * NEXT + (GATED && j >= T::TN / 2 ? UP : 0));
+#pragma unroll
+            for (int i = 0; i < T::TM; i++)
+#pragma unroll
+                for (int j = 0; j < T::TN; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
+        }
+    };
+    const int nk = (p.K + T::BK - 1) / T::BK, whole = p.K / T::BK;
+    auto issue_any = [&](int kt) {
+        if (kt < whole) issue(kt, IC<1>{});
+        else issue(kt, IC<0>{});
+    };
+    for (int t = 0; t < T::ST - 1; t++)
+        if (t < nk) issue_any(t);
+    int kt = 0;
+    for (; kt + T::ST - 1 < whole; kt++) {
+        // this wave's copies of stage kt are there, later ones may be on their way; every
+        // wave has read stage kt - 1, whose place is next
+        __builtin_amdgcn_s_waitcnt(I8_VMCNT((T::ST - 2) * T::DMA));
+        __builtin_amdgcn_s_barrier();
+        issue(kt + T::ST - 1, IC<1>{});
+        multiply(kt);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    for (; kt < nk; kt++) {
+        __builtin_amdgcn_s_waitcnt(I8_VMCNT(0));
+        __builtin_amdgcn_s_barrier();
+        if (kt + T::ST - 1 < nk) issue_any(kt + T::ST - 1);
+        multiply(kt);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+
+    // the tile's scales through LDS; stores behind M and N fall out of the buffer's range
+    __syncthreads();
+    float *sm = (float *)smem, *sn = sm + T::BM, *su = sn + BNO;
+    for (int i = tid; i < T::BM; i += WAVE * T::NW) sm[i] = p.as[min(m0 + i, p.M - 1)];
+    for (int i = tid; i < BNO; i += WAVE * T::NW) {
+        sn[i] = p.bs[min(n0 + i, p.N - 1)];
+        if constexpr (GATED) su[i] = p.bs2[min(n0 + i, p.N - 1)];
+    }
+    __syncthreads();
+    constexpr int TNO = GATED ? T::TN / 2 : T::TN;
+    const auto rc = buf_rsrc((char *)p.c + ((size_t)m0 * p.ldc + n0) * ES, ((size_t)(rows - 1) * p.ldc + cols) * ES);
+    const int ldc = (int)p.ldc * ES;
+#pragma unroll
+    for (int j = 0; j < TNO; j++) {
+        const int n = wn * (BNO / T::WN) + 32 * j + fr;
+        const float s = sn[n], s2 = GATED ? su[n] : 0.0f;
+        const unsigned at = n < cols ? n * ES : BUF_OOB;
+#pragma unroll
+        for (int i = 0; i < T::TM; i++)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; e4++) {
+                const int m = wm * (T::BM / T::WM) + 32 * i + 8 * e4 + 4 * fh;
+                const f32x4 r = *(const f32x4 *)(sm + m);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float y = (float)acc[i][j][4 * e4 + e] * (r[e] * s);
+                    if constexpr (GATED) y = silu_mul(y, (float)acc[i][j + TNO][4 * e4 + e] * (r[e] * s2));
+                    const unsigned to = at + (unsigned)((m + e) * ldc);
+                    if constexpr (CBF) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (__bf16)y), rc, to, 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y), rc, to, 0, 0);
+                }
+            }
+    }
+}
+
 // ---------------------------------------------------------------------------
 // launchers
 // ---------------------------------------------------------------------------
 static inline bool aligned(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 #define I8_MAX_LD ((size_t)1 << 40)
+#define I8_MAX_NEAR ((size_t)1 << 22)     // 256 rows within 2^31 bytes
 
 extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, size_t ldx, int bf16, int rows, int K) {
     if (rows < 0 || K < 0 || ldq < (size_t)K || ldx < (size_t)K) return QH_EINVAL;
@@ -142,11 +533,62 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
     return QH_OK;
 }
 
+enum { I8_ANY_PLAN, I8_NARROW1_8, I8_NARROW1_16, I8_NARROW2_8, I8_NARROW4_8, I8_WIDE1, I8_WIDE4, I8_TILE64, I8_TILE128, I8_TILE256 };
+
+static int i8_plan_of(const I8Args &p, bool gated) {
+    if (!p.K || !aligned16(p.a) || !aligned16(p.b) || !aligned16(p.b2) || p.lda % 16 || p.ldb % 16 || p.lda > I8_MAX_NEAR ||
+        p.ldb > I8_MAX_NEAR)
+        return I8_ANY_PLAN;
+    if (p.ldc > I8_MAX_NEAR / 4) return I8_NARROW4_8;
+    const long cols = (p.N + 15) / 16;
+    if (p.M <= 64) {
+        if (cols >= 4096 && p.M <= 16 && (p.K + 255) / 256 * 256 * 16 <= 65536) return I8_WIDE1;
+        if (cols >= 4096 && (p.K + 255) / 256 * 256 * 64 <= 65536) return I8_WIDE4;
+        if (p.M <= 16) return p.K > 2048 ? I8_NARROW1_16 : I8_NARROW1_8;
+        return p.M <= 32 ? I8_NARROW2_8 : I8_NARROW4_8;
+    }
+    const long t = (gated ? 2 : 1) * (long)p.N;
+    if (((p.M + 255) / 256) * ((t + 255) / 256) >= 256) return I8_TILE256;
+    if (((p.M + 127) / 128) * ((t + 127) / 128) >= 256) return I8_TILE128;
+    return I8_TILE64;
+}
+
+template <int MT, int W, bool GATED, bool CBF>
+static void i8_narrow(const I8Args &p) {
+    hipLaunchKernelGGL((k_i8_narrow<MT, W, GATED, CBF>), dim3((p.N + 15) / 16, (p.M + 16 * MT - 1) / (16 * MT)), dim3(WAVE *W), 0,
+                       g_stream, p);
+}
+template <int MT, int KB, bool GATED, bool CBF>
+static void i8_wide(const I8Args &p) {
+    const int vec = p.ldc % 4 == 0 && aligned(p.c, CBF ? 8 : 16);
+    hipLaunchKernelGGL((k_i8_wide<MT, KB * 1024, GATED, CBF>), dim3(512), dim3(WAVE *I8_WIDE_WAVES), 0, g_stream, p, vec);
+}
+template <typename T, bool GATED, bool CBF>
+static void i8_tile(const I8Args &p) {
+    const long mt = (p.M + T::BM - 1) / T::BM, bno = GATED ? T::BN / 2 : T::BN, nt = (p.N + bno - 1) / bno;
+    const int per = (int)((mt * nt + 7) / 8);
+    hipLaunchKernelGGL((k_i8_tile<T, GATED, CBF>), dim3(8 * per), dim3(WAVE *T::NW), 0, g_stream, p, (int)mt, (int)nt, per);
+}
+
 template <bool GATED, bool CBF>
 static int i8_launch(const I8Args &p) {
-    const dim3 any((p.N + I8_ANY - 1) / I8_ANY, (p.M + I8_ANY - 1) / I8_ANY);
-    if (any.y > 65535) return QH_ETOOBIG;
-    hipLaunchKernelGGL((k_i8_any<GATED, CBF>), any, dim3(NTHREADS), 0, g_stream, p);
+    switch (i8_plan_of(p, GATED)) {
+    case I8_ANY_PLAN: {
+        const dim3 any((p.N + I8_ANY - 1) / I8_ANY, (p.M + I8_ANY - 1) / I8_ANY);
+        if (any.y > 65535) return QH_ETOOBIG;
+        hipLaunchKernelGGL((k_i8_any<GATED, CBF>), any, dim3(NTHREADS), 0, g_stream, p);
+        break;
+    }
+    case I8_NARROW1_8: i8_narrow<1, 8, GATED, CBF>(p); break;
+    case I8_NARROW1_16: i8_narrow<1, 16, GATED, CBF>(p); break;
+    case I8_NARROW2_8: i8_narrow<2, 8, GATED, CBF>(p); break;
+    case I8_NARROW4_8: i8_narrow<4, 8, GATED, CBF>(p); break;
+    case I8_WIDE1: i8_wide<1, 64, GATED, CBF>(p); break;
+    case I8_WIDE4: i8_wide<4, 64, GATED, CBF>(p); break;
+    case I8_TILE64: i8_tile<I8Tile<64, 64, 2, 2 - GATED, 128, 4>, GATED, CBF>(p); break;
+    case I8_TILE128: i8_tile<I8Tile<128, 128, 2, 2, 128, 2>, GATED, CBF>(p); break;
+    case I8_TILE256: i8_tile<I8Tile<256, 256, 2, 4, 128, 2>, GATED, CBF>(p); break;
+    }
     HCHECK(hipGetLastError(), QH_ELAUNCH);
     return QH_OK;
 }

@@ -30,30 +30,112 @@ __device__ __forceinline__ float i8_held(float x) {
     return fminf(fmaxf(x, -FLT_MAX), FLT_MAX);
 }
 
-template <bool BF>
-__device__ __forceinline__ float i8_value(const void *x, size_t i) {
-    return BF ? bf16_lo(((const uint16_t *)x)[i]) : ((const float *)x)[i];
+// rint(x / s), both rounded to fp32 first as the definition has it, without the
+// division where it cannot matter: with y = 1 / s rounded (2^-107 <= s < 2^122),
+// x y is off x / s by 2^-23 of it, 2^-16 at most, and the quotient's own rounding
+// moves it by half of that.  Only a product within 2^-14 of n + 1/2 is divided.
+__device__ __forceinline__ int i8_code(float x, float s, float y) {
+    float q = x * y, n = rintf(q);
+    if (fabsf(fabsf(q - n) - 0.5f) < 0x1p-14f) n = rintf(x / s);
+    return (int)n;
 }
 
-template <bool BF>
-__global__ __launch_bounds__(NTHREADS) void k_rows_int8(int8_t *__restrict__ q, size_t ldq, float *__restrict__ scale,
-                                                       const void *__restrict__ x, size_t ldx, int K) {
-    const size_t row = blockIdx.x;
-    const int tid = threadIdx.x;
-    float a = 0.0f;
-    for (int k = tid; k < K; k += NTHREADS) a = fmaxf(a, fabsf(i8_held(i8_value<BF>(x, row * ldx + k))));
-    __shared__ float red[NTHREADS / WAVE];
+// eight values from x on, `left` of them there
+template <bool BF, bool VEC>
+__device__ __forceinline__ void i8_eight(float *v, const void *x, size_t i, int left) {
+    if (VEC && left >= 8) {
+        if constexpr (BF) {
+            const u32x4 w = *(const u32x4 *)((const uint16_t *)x + i);
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) a = fmaxf(a, __shfl_xor(a, m));
-    if ((tid & 63) == 0) red[tid >> 6] = a;
-    __syncthreads();
+            for (int j = 0; j < 4; j++) {
+                v[2 * j] = bf16_lo(w[j]);
+                v[2 * j + 1] = bf16_hi(w[j]);
+            }
+        } else {
+            const f32x4 lo = *(const f32x4 *)((const float *)x + i), hi = *(const f32x4 *)((const float *)x + i + 4);
 #pragma unroll
-    for (int w = 0; w < NTHREADS / WAVE; w++) a = fmaxf(a, red[w]);
+            for (int j = 0; j < 4; j++) {
+                v[j] = lo[j];
+                v[4 + j] = hi[j];
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        v[j] = j >= left ? 0.0f : BF ? bf16_lo(((const uint16_t *)x)[i + j]) : ((const float *)x)[i + j];
+}
+
+// TPR threads a row, in turns of 8 values each.  The first KEEP turns' values stay
+// in registers between the maximum and the codes; a longer row's others are read
+// again.
+template <bool BF, bool VEC, int TPR, int KEEP>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__restrict__ q, size_t ldq, float *__restrict__ scale,
+                                                                   const void *__restrict__ x, size_t ldx, int K, int rows) {
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+    const size_t row = (size_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    const int t = threadIdx.x % TPR;
+    if (TPR <= WAVE && row >= (size_t)rows) return;       // whole waves
+    const size_t from = row * ldx;
+    float v[KEEP][8], a = 0.0f;
+#pragma unroll
+    for (int u = 0; u < KEEP; u++) {
+        const int k = 8 * (t + u * TPR);
+        i8_eight<BF, VEC>(v[u], x, from + k, K - k);
+    }
+    for (int k = 8 * (t + KEEP * TPR); k < K; k += 8 * TPR) {
+        float w[8];
+        i8_eight<BF, VEC>(w, x, from + k, K - k);
+#pragma unroll
+        for (int j = 0; j < 8; j++) a = fmaxf(a, fabsf(i8_held(w[j])));
+    }
+#pragma unroll
+    for (int u = 0; u < KEEP; u++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            v[u][j] = i8_held(v[u][j]);
+            a = fmaxf(a, fabsf(v[u][j]));
+        }
+#pragma unroll
+    for (int m = WAVE / 2; m >= 1; m >>= 1) a = fmaxf(a, __shfl_xor(a, m));
+    if constexpr (TPR > WAVE) {
+        __shared__ float red[TPR / WAVE];
+        if ((t & 63) == 0) red[t >> 6] = a;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < TPR / WAVE; w++) a = fmaxf(a, red[w]);
+    }
     const float s = a < I8_TINY ? 0.0f : a / 127.0f;
-    if (tid == 0) scale[row] = s;
-    for (int k = tid; k < K; k += NTHREADS) {
-        const float v = i8_held(i8_value<BF>(x, row * ldx + k));
-        q[row * ldq + k] = s == 0.0f ? 0 : (int8_t)(int)rintf(v / s);
+    const float y = s == 0.0f ? 0.0f : 1.0f / s;
+    if (t == 0) scale[row] = s;
+    auto store = [&](const float *w, int k) {
+        if (k >= K) return;
+        int8_t *to = q + row * ldq + k;
+        int c[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) c[j] = s == 0.0f ? 0 : i8_code(w[j], s, y);
+        if (VEC && k + 8 <= K) {
+            uint32_t lo = 0, hi = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                lo |= (uint32_t)(c[j] & 0xFF) << (8 * j);
+                hi |= (uint32_t)(c[4 + j] & 0xFF) << (8 * j);
+            }
+            *(uint2 *)to = make_uint2(lo, hi);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (k + j < K) to[j] = (int8_t)c[j];
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < KEEP; u++) store(v[u], 8 * (t + u * TPR));
+    for (int k = 8 * (t + KEEP * TPR); k < K; k += 8 * TPR) {
+        float w[8];
+        i8_eight<BF, VEC>(w, x, from + k, K - k);
+#pragma unroll
+        for (int j = 0; j < 8; j++) w[j] = i8_held(w[j]);
+        store(w, k);
     }
 }
 
@@ -527,8 +609,26 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
     if (!scale || !aligned(scale, 4) || (K > 0 && (!q || !x)) || !aligned(x, bf16 ? 2 : 4)) return QH_EINVAL;
     if (K > I8_MAX_K || ldq > I8_MAX_LD || ldx > I8_MAX_LD) return QH_ETOOBIG;
     if (!g_inited) return QH_ESTATE;
-    if (bf16) hipLaunchKernelGGL(k_rows_int8<true>, dim3(rows), dim3(NTHREADS), 0, g_stream, q, ldq, scale, x, ldx, K);
-    else hipLaunchKernelGGL(k_rows_int8<false>, dim3(rows), dim3(NTHREADS), 0, g_stream, q, ldq, scale, x, ldx, K);
+    const bool vec = aligned16(x) && ldx * (bf16 ? 2 : 4) % 16 == 0 && aligned(q, 8) && ldq % 8 == 0;
+    const unsigned four = (unsigned)(((size_t)rows + 3) / 4);
+#define ROWS_AS(BF, V, TPR, KEEP)                                                                             \
+    hipLaunchKernelGGL((k_rows_int8<BF, V, TPR, KEEP>), dim3(TPR == 64 ? four : rows), dim3(TPR < 256 ? 256 : TPR), 0, \
+                       g_stream, q, ldq, scale, x, ldx, K, rows)
+#define ROWS(BF, V)                                        \
+    do {                                                   \
+        if (K <= 1024) ROWS_AS(BF, V, 64, 2);              \
+        else if (K <= 4096) ROWS_AS(BF, V, 256, 2);        \
+        else ROWS_AS(BF, V, 1024, 2);                      \
+    } while (0)
+    if (bf16) {
+        if (vec) ROWS(true, true);
+        else ROWS(true, false);
+    } else {
+        if (vec) ROWS(false, true);
+        else ROWS(false, false);
+    }
+#undef ROWS
+#undef ROWS_AS
     HCHECK(hipGetLastError(), QH_ELAUNCH);
     return QH_OK;
 }

@@ -14,9 +14,10 @@
 // nothing to clear between calls.
 
 #define RULES_PIECE 4096
+#define RULES_GROUPS (RULES_PIECE / 4 / NTH)  // of four tokens a thread: tid, tid + NTH, ...
 #define RULES_SEEN 0x80000000u
 
-// e: a token's word of `tab`
+// e: a token's word of the table
 __device__ __forceinline__ float rules_penalised(float x, uint32_t e, float r, float f, float p) {
 #pragma clang fp contract(off)
     if (e & RULES_SEEN) x = x > 0.0f ? x / r : x * r;
@@ -28,50 +29,119 @@ __device__ __forceinline__ float rules_penalised(float x, uint32_t e, float r, f
     return x;
 }
 
-__global__ __launch_bounds__(NTH) void k_logits_rules(float *out, size_t ldo, const float *x, size_t ldx, int vocab,
+// four tokens from x on, `left` of them there
+template <bool VEC>
+__device__ __forceinline__ f32x4 rules_load(const float *x, int left) {
+    if (VEC && left >= 4) return *(const f32x4 *)x;
+    f32x4 v = {};
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (e < left) v[e] = x[e];
+    return v;
+}
+template <bool VEC>
+__device__ __forceinline__ void rules_store(float *x, f32x4 v, int left) {
+    if (VEC && left >= 4) {
+        *(f32x4 *)x = v;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (e < left) x[e] = v[e];
+}
+
+// INPLACE: what a rule does not touch is neither read nor written.
+// Every load that does not wait for another one goes out first: the logits, the
+// first tokens of the history (whose number is then not known yet), the row's
+// numbers.
+template <bool VEC, bool INPLACE, bool BIAS>
+__global__ __launch_bounds__(NTH) void k_logits_rules(float *out, size_t ldo, const float *in, size_t ldx, int vocab,
                                                      qm_rules_t t) {
-    __shared__ uint32_t tab[RULES_PIECE];     // occurrences behind the prompt, RULES_SEEN
-    __shared__ int last[RULES_PIECE];         // 1 + the last bias entry that names the token
+    __shared__ __align__(16) uint32_t tab[RULES_PIECE];          // occurrences behind the prompt, RULES_SEEN
+    __shared__ __align__(16) int last[BIAS ? RULES_PIECE : 4];   // 1 + the last bias entry that names the token
     const int i = blockIdx.y, tid = threadIdx.x;
     const int v0 = blockIdx.x * RULES_PIECE, nv = min(vocab - v0, RULES_PIECE);
-    for (int v = tid; v < RULES_PIECE; v += NTH) {
-        tab[v] = 0;
-        last[v] = 0;
+    const float *x = in + (size_t)i * ldx + v0;
+    float *o = out + (size_t)i * ldo + v0;
+    f32x4 y[RULES_GROUPS];
+    if constexpr (!INPLACE) {
+#pragma unroll
+        for (int u = 0; u < RULES_GROUPS; u++) y[u] = rules_load<VEC>(x + 4 * (tid + u * NTH), nv - 4 * (tid + u * NTH));
     }
-    __syncthreads();
-    if (t.token) {
-        const int len = t.n_token[i], prompt = t.n_prompt ? t.n_prompt[i] : 0;
-        const int *h = t.token + (size_t)i * t.ld_token;
-        if (len >= 0 && len <= t.ld_token)
-            for (int j = tid; j < len; j += NTH) {
-                const unsigned v = (unsigned)h[j] - (unsigned)v0;
-                if (v < (unsigned)nv) {
-                    atomicOr(&tab[v], RULES_SEEN);
-                    if (j >= prompt) atomicAdd(&tab[v], 1u);
-                }
-            }
+    const int *h = t.token + (size_t)i * t.ld_token;
+    int early[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) early[u] = tid + u * NTH < t.ld_token && t.token ? h[tid + u * NTH] : -1;
+    int len = t.token ? t.n_token[i] : 0;
+    if (len > t.ld_token) len = 0;
+    const int prompt = t.n_prompt ? t.n_prompt[i] : 0;
+    int b0 = 0, b1 = 0;
+    if constexpr (BIAS) {
+        b0 = t.bias_row[i];
+        b1 = t.bias_row[i + 1];
+        if (b0 < 0 || b1 > t.n_bias) b1 = b0;
     }
-    if (t.bias_row) {
-        const int b0 = t.bias_row[i], b1 = t.bias_row[i + 1];
-        if (b0 >= 0 && b1 <= t.n_bias)
-            for (int j = b0 + tid; j < b1; j += NTH) {
-                const unsigned v = (unsigned)t.bias_token[j] - (unsigned)v0;
-                if (v < (unsigned)nv) atomicMax(&last[v], j + 1);
-            }
-    }
-    __syncthreads();
     const float r = t.repetition ? t.repetition[i] : 1.0f, f = t.frequency ? t.frequency[i] : 0.0f;
     const float p = t.presence ? t.presence[i] : 0.0f;
-    const uint32_t *mask = nullptr;
-    if (t.mask) {
-        const int m = t.mask_of ? t.mask_of[i] : i;
-        if (m >= 0 && m < t.n_mask) mask = t.mask + (size_t)m * t.ld_mask;
+    const int mi = !t.mask ? -1 : t.mask_of ? t.mask_of[i] : i;
+    const uint32_t *mask = mi >= 0 && mi < t.n_mask ? t.mask + (size_t)mi * t.ld_mask + v0 / 32 : nullptr;
+
+#pragma unroll
+    for (int u = 0; u < RULES_GROUPS; u++) {
+        ((uint4 *)tab)[tid + u * NTH] = make_uint4(0, 0, 0, 0);
+        if constexpr (BIAS) ((uint4 *)last)[tid + u * NTH] = make_uint4(0, 0, 0, 0);
     }
-    for (int v = tid; v < nv; v += NTH) {
-        float y = rules_penalised(x[(size_t)i * ldx + v0 + v], tab[v], r, f, p);
-        if (last[v]) y += t.bias[last[v] - 1];
-        if (mask && !(mask[(v0 + v) >> 5] >> ((v0 + v) & 31) & 1)) y = -INFINITY;
-        out[(size_t)i * ldo + v0 + v] = y;
+    uint32_t words[RULES_GROUPS];
+#pragma unroll
+    for (int u = 0; u < RULES_GROUPS; u++)
+        words[u] = mask && 4 * (tid + u * NTH) < nv ? mask[(tid + u * NTH) / 8] >> (tid % 8 * 4) & 15 : 15;
+    __syncthreads();
+    auto count = [&](int token, int j) {
+        const unsigned v = (unsigned)token - (unsigned)v0;
+        if (v >= (unsigned)nv) return;
+        atomicOr(&tab[v], RULES_SEEN);
+        if (j >= prompt) atomicAdd(&tab[v], 1u);
+    };
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+        if (tid + u * NTH < len) count(early[u], tid + u * NTH);
+    for (int j = tid + 4 * NTH; j < len; j += 4 * NTH) {
+        int v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) v[u] = h[min(j + u * NTH, len - 1)];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (j + u * NTH < len) count(v[u], j + u * NTH);
+    }
+    if constexpr (BIAS)
+        for (int j = b0 + tid; j < b1; j += NTH) {
+            const unsigned v = (unsigned)t.bias_token[j] - (unsigned)v0;
+            if (v < (unsigned)nv) atomicMax(&last[v], j + 1);
+        }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < RULES_GROUPS; u++) {
+        const int g = tid + u * NTH, left = nv - 4 * g;
+        if (left <= 0) continue;
+        const uint4 e = ((const uint4 *)tab)[g];
+        const uint4 l = BIAS ? ((const uint4 *)last)[g] : make_uint4(0, 0, 0, 0);
+        const bool touched = (e.x | e.y | e.z | e.w | l.x | l.y | l.z | l.w) != 0;
+        if constexpr (INPLACE) {
+            if (!touched && words[u] == 15) continue;
+            if (words[u]) y[u] = rules_load<VEC>(x + 4 * g, left);
+        }
+        if (touched) {
+            const uint32_t ee[4] = {e.x, e.y, e.z, e.w}, ll[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                y[u][k] = rules_penalised(y[u][k], ee[k], r, f, p);
+                if (BIAS && ll[k]) y[u][k] += t.bias[ll[k] - 1];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (!(words[u] >> k & 1)) y[u][k] = -INFINITY;
+        rules_store<VEC>(o + 4 * g, y[u], left);
     }
 }
 
@@ -97,7 +167,23 @@ extern "C" int qm_logits_rules(float *out, size_t ldo, const float *logits, size
     if (t->mask && !t->mask_of && t->n_mask < n) return QH_EINVAL;
     if (t->mask_of && !t->mask) return QH_EINVAL;
     if (!stream()) return QH_ESTATE;
-    hipLaunchKernelGGL(k_logits_rules, dim3((vocab + RULES_PIECE - 1) / RULES_PIECE, n), dim3(NTH), 0, stream(), out, ldo,
-                       logits, ld, vocab, *t);
+    const dim3 grid((vocab + RULES_PIECE - 1) / RULES_PIECE, n);
+    const bool vec = aligned16(out) && aligned16(logits) && ldo % 4 == 0 && ld % 4 == 0;
+#define RULES_AS(V, I, B) \
+    hipLaunchKernelGGL((k_logits_rules<V, I, B>), grid, dim3(NTH), 0, stream(), out, ldo, logits, ld, vocab, *t)
+#define RULES(V, I)                           \
+    do {                                      \
+        if (t->n_bias > 0) RULES_AS(V, I, true); \
+        else RULES_AS(V, I, false);           \
+    } while (0)
+    if (out == logits) {
+        if (vec) RULES(true, true);
+        else RULES(false, true);
+    } else {
+        if (vec) RULES(true, false);
+        else RULES(false, false);
+    }
+#undef RULES
+#undef RULES_AS
     return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
 }

@@ -160,14 +160,32 @@ __device__ __forceinline__ void i8_store(void *c, size_t i, float v) {
     else ((float *)c)[i] = v;
 }
 
+// silu(g) u = g / (1 + exp(-g)) u in a third of the instructions that the library's
+// exponential and division take, of which a block has as much as of a product of
+// K = 1,024: a power of two of -g log2 e, and a reciprocal.  That product's
+// remainder is put back for fp32 results, which are then within 9 half steps; bf16
+// ones are off by up to |g| 2^-24 more, at most 2^-17.5, where a half step is 2^-9.
+template <bool CBF>
+__device__ __forceinline__ float i8_silu_mul(float g, float u) {
+    float e;
+    if constexpr (CBF) {
+        e = __builtin_amdgcn_exp2f(g * -1.44269504e+00f);
+    } else {
+        const float x = -fminf(fmaxf(g, -104.0f), 104.0f);
+        const float hi = x * 1.44269504e+00f, lo = fmaf(x, 1.92596299e-08f, fmaf(x, 1.44269504e+00f, -hi));
+        e = __builtin_amdgcn_exp2f(hi) * fmaf(lo, 6.93147182e-01f, 1.0f);
+    }
+    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+}
+
 // Any K, strides and addresses: 64 x 64 outputs a block, 64 bytes of K a step
 // through LDS, read byte by byte, 4 x 4 outputs a thread by v_dot4.
 #define I8_ANY 64
 template <bool GATED, bool CBF>
-__global__ __launch_bounds__(NTHREADS) void k_i8_any(I8Args p) {
+__global__ __launch_bounds__(NTHREADS) void k_i8_any(I8Args p, unsigned nt) {
     __shared__ int sa[I8_ANY][I8_ANY / 4 + 1], sb[GATED ? 2 : 1][I8_ANY][I8_ANY / 4 + 1];
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const size_t m0 = (size_t)blockIdx.y * I8_ANY, n0 = (size_t)blockIdx.x * I8_ANY;
+    const size_t m0 = (size_t)(blockIdx.x / nt) * I8_ANY, n0 = (size_t)(blockIdx.x % nt) * I8_ANY;
     auto four = [&](const int8_t *x, size_t ld, size_t row, int rows, int k) {
         int w = 0;
         for (int j = 0; j < 4; j++)
@@ -200,7 +218,7 @@ __global__ __launch_bounds__(NTHREADS) void k_i8_any(I8Args p) {
             const size_t n = n0 + tx + 16 * j;
             if (n >= (size_t)p.N) continue;
             float v = (float)acc[0][i][j] * (p.as[m] * p.bs[n]);
-            if constexpr (GATED) v = silu_mul(v, (float)acc[GATED][i][j] * (p.as[m] * p.bs2[n]));
+            if constexpr (GATED) v = i8_silu_mul<CBF>(v, (float)acc[GATED][i][j] * (p.as[m] * p.bs2[n]));
             i8_store<CBF>(p.c, m * p.ldc + n, v);
         }
     }
@@ -236,12 +254,12 @@ template <int MT, int W, bool GATED, bool CBF>
 __global__ __launch_bounds__(WAVE *W) void k_i8_narrow(I8Args p) {
     constexpr int G = GATED ? 2 : 1;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
+    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT), cols = p.N - n0, rows = p.M - m0;
     const int8_t *wp[G], *xp[MT];
-    wp[0] = p.b + (size_t)min(n0 + r, p.N - 1) * p.ldb;
-    if constexpr (GATED) wp[G - 1] = p.b2 + (size_t)min(n0 + r, p.N - 1) * p.ldb;
+    wp[0] = p.b + (size_t)(n0 + min(r, cols - 1)) * p.ldb;
+    if constexpr (GATED) wp[G - 1] = p.b2 + (size_t)(n0 + min(r, cols - 1)) * p.ldb;
 #pragma unroll
-    for (int t = 0; t < MT; t++) xp[t] = p.a + (size_t)min(m0 + 16 * t + r, p.M - 1) * p.lda;
+    for (int t = 0; t < MT; t++) xp[t] = p.a + (size_t)(m0 + min(16 * t + r, rows - 1)) * p.lda;
     struct Set { i32x4 w[2][G], x[2][MT]; };
     auto load = [&](Set &s, int c) {
 #pragma unroll
@@ -289,134 +307,18 @@ __global__ __launch_bounds__(WAVE *W) void k_i8_narrow(I8Args p) {
     const int *flat = (const int *)red;
     constexpr int OUT = MT * WAVE * 4;                    // sums of one product
     for (int o = tid; o < OUT; o += W * WAVE) {
-        const int m = m0 + o / (WAVE * 4) * 16 + (o >> 2 & 15), n = n0 + (o >> 6 & 3) * 4 + (o & 3);
+        const int mo = o / (WAVE * 4) * 16 + (o >> 2 & 15), no = (o >> 6 & 3) * 4 + (o & 3);
         int v[G] = {};
 #pragma unroll
         for (int w = 0; w < W; w++)
 #pragma unroll
             for (int q = 0; q < G; q++) v[q] += flat[(w * G + q) * OUT + o];
-        if (m >= p.M || n >= p.N) continue;
+        if (mo >= rows || no >= cols) continue;
+        const int m = m0 + mo, n = n0 + no;
         const float sm = p.as[m];
         float y = (float)v[0] * (sm * p.bs[n]);
-        if constexpr (GATED) y = silu_mul(y, (float)v[G - 1] * (sm * p.bs2[n]));
+        if constexpr (GATED) y = i8_silu_mul<CBF>(y, (float)v[G - 1] * (sm * p.bs2[n]));
         i8_store<CBF>(p.c, (size_t)m * p.ldc + n, y);
-    }
-}
-
-// ---------------------------------------------------------------------------
-// Few rows, many columns: the rows stay in LDS, every wave streams weights
-// ---------------------------------------------------------------------------
-// The operands' roles and layouts are those above.  A block's 8 waves take 16
-// columns each at a time, U steps of 64 codes in flight ahead of the U being
-// multiplied.  x lies in LDS with K rounded up to 256 and zeros behind K; piece
-// c of 16 codes of row r at place c ^ (r % 16), so that the 16 rows of a read
-// meet different banks.
-#define I8_WIDE_WAVES 8
-template <int MT, int LDS, bool GATED, bool CBF>
-__global__ __launch_bounds__(WAVE *I8_WIDE_WAVES, 4) void k_i8_wide(I8Args p, int vec) {
-    constexpr int G = GATED ? 2 : 1, U = GATED ? 4 : 8, NT = WAVE * I8_WIDE_WAVES;
-    __shared__ i32x4 sx[LDS / 16];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, g = lane >> 4;
-    const int per = (p.K + 255) / 256 * 16;               // pieces of a row in LDS
-    for (int i = tid; i < 16 * MT * per; i += NT) {
-        const int row = i / per, c = i % per;
-        i32x4 v = {};
-        if (16 * c < p.K) v = i8_keep(i8_load(p.a + (size_t)min(row, p.M - 1) * p.lda + 16 * c), p.K - 16 * c);
-        sx[row * per + (c ^ (row & 15))] = v;
-    }
-    float sm[MT];
-#pragma unroll
-    for (int t = 0; t < MT; t++) sm[t] = p.as[min(16 * t + r, p.M - 1)];
-    __syncthreads();
-
-    const int steps = (p.K + 63) / 64, sets = (steps + U - 1) / U;
-    const int tiles = (p.N + 15) / 16, stride = gridDim.x * I8_WIDE_WAVES;
-    struct Set { i32x4 w[U][G]; };
-    auto load = [&](Set &s, int tile, int set) {
-        const size_t row = (size_t)min(tile * 16 + r, p.N - 1) * p.ldb;
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int k = 64 * (set * U + u) + 16 * g, at = k < p.K ? k : 0;
-            s.w[u][0] = i8_load(p.b + row + at);
-            if constexpr (GATED) s.w[u][G - 1] = i8_load(p.b2 + row + at);
-        }
-    };
-    i32x4 acc[G][MT] = {};
-    auto step = [&](const Set &s, int set, int u) {
-#pragma unroll
-        for (int t = 0; t < MT; t++) {
-            const i32x4 x = sx[(16 * t + r) * per + ((4 * (set * U + u) + g) ^ r)];
-#pragma unroll
-            for (int q = 0; q < G; q++) acc[q][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.w[u][q], x, acc[q][t], 0, 0, 0);
-        }
-    };
-    auto multiply = [&](const Set &s, int set) {
-        if ((set + 1) * U <= steps) {
-#pragma unroll
-            for (int u = 0; u < U; u++) step(s, set, u);
-        } else {
-#pragma unroll
-            for (int u = 0; u < U; u++)
-                if (set * U + u < steps) step(s, set, u);
-        }
-    };
-    auto finish = [&](int tile) {
-        const int n = tile * 16 + 4 * g;
-        float sn[G][4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            sn[0][i] = p.bs[min(n + i, p.N - 1)];
-            if constexpr (GATED) sn[G - 1][i] = p.bs2[min(n + i, p.N - 1)];
-        }
-#pragma unroll
-        for (int t = 0; t < MT; t++) {
-            const int m = 16 * t + r;
-            f32x4 y;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                y[i] = (float)acc[0][t][i] * (sm[t] * sn[0][i]);
-                if constexpr (GATED) y[i] = silu_mul(y[i], (float)acc[G - 1][t][i] * (sm[t] * sn[G - 1][i]));
-            }
-#pragma unroll
-            for (int q = 0; q < G; q++) acc[q][t] = i32x4{};
-            if (m >= p.M) continue;
-            const size_t at = (size_t)m * p.ldc + n;
-            if (vec && n + 4 <= p.N) {
-                if constexpr (CBF)
-                    *(uint2 *)((uint16_t *)p.c + at) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
-                else
-                    *(f32x4 *)((float *)p.c + at) = y;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (n + i < p.N) i8_store<CBF>(p.c, at + i, y[i]);
-            }
-        }
-    };
-    int tile = blockIdx.x * I8_WIDE_WAVES + wave, set = 0;
-    if (tile >= tiles) return;
-    auto next = [&](int &t, int &s) {
-        if (++s == sets) {
-            s = 0;
-            t += stride;
-        }
-    };
-    Set s0, s1;
-    load(s0, tile, 0);
-    for (;;) {
-        int t1 = tile, k1 = set;
-        next(t1, k1);
-        if (t1 < tiles) load(s1, t1, k1);
-        multiply(s0, set);
-        if (k1 == 0) finish(tile);
-        if (t1 >= tiles) break;
-        tile = t1;
-        set = k1;
-        next(tile, set);
-        if (tile < tiles) load(s0, tile, set);
-        multiply(s1, k1);
-        if (set == 0) finish(t1);
-        if (tile >= tiles) break;
     }
 }
 
@@ -425,15 +327,28 @@ __global__ __launch_bounds__(WAVE *I8_WIDE_WAVES, 4) void k_i8_wide(I8Args p, in
 // ---------------------------------------------------------------------------
 // BM x BN outputs a block of WM x WN waves, 32x32x32 MFMAs: lane (c, h) = (lane %
 // 32, lane / 32) gives codes 16 h .. 16 h + 15 of row c of either operand and
-// holds rows 8 (e / 4) + 4 h + e % 4 of column c of the result.  Stages of BK codes
-// of each row are copied from memory straight into one of ST places in LDS, 1,024
-// bytes an instruction; piece c of 16 codes of row r lies at place c ^ f(r) of its
-// row, f such that the rows of a fragment meet different banks, and with a period
-// of 32 rows so that a wave's fragments differ by constants.
-template <int BM_, int BN_, int WM_, int WN_, int BK_, int ST_>
+// holds rows 8 (e / 4) + 4 h + e % 4 of column c of the result.  Stages of 128
+// codes of each row are copied from memory straight into one of ST places in LDS,
+// 1,024 bytes an instruction; piece c of 16 codes of row r lies at place c ^ f(r)
+// of its row, f such that the rows of a fragment meet different banks (the
+// conflict counter reads 0), and with a period of 32 rows so that a wave's
+// fragments differ by constants.
+// A stage is four steps of 32 codes; a step's MFMAs run while the next step's
+// fragments are read.  A stage's last step runs behind the barrier: its fragments
+// are in registers by then, so the copies of stage kt + ST may start into the same
+// place and the first fragments of stage kt + 1 be read while the matrix cores
+// still have work (4096 x 4096 x 8192 132 us with the barrier between stages, 124
+// so).
+// What bounds it: 4096 x 4096 x 8192, bf16 results, 124 us on 256 x 256 tiles, 2.2
+// POP/s; without the copies 109, the copies alone 75 to 105.  The matrix cores
+// alone reach 3.3 POP/s on such data (the clock falls to two thirds under it; on
+// zeros 4.9).  64 x 64 tiles take in 16 KB a stage and are bound by that: 2048 x
+// 8192 x 1024 34.3 us, the copies alone 35.  Splitting a stage's codes over waves,
+// which halves what is read from LDS, and more stages in flight gained nothing.
+template <int BM_, int BN_, int WM_, int WN_, int ST_>
 struct I8Tile {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = BK_, ST = ST_;
-    static constexpr int NW = WM * WN, CPR = BK / 16, RPI = 64 / CPR;    // rows that a copy instruction fills
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = 128, ST = ST_;
+    static constexpr int NW = WM * WN, CPR = BK / 16, RPI = 64 / CPR;    // pieces of a row; rows that a copy instruction fills
     static constexpr int TM = BM / WM / 32, TN = BN / WN / 32, KS = BK / 32;
     static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE = A_BYTES + B_BYTES;
     static constexpr int A_DMA = A_BYTES / 1024 / NW, B_DMA = B_BYTES / 1024 / NW, DMA = A_DMA + B_DMA;
@@ -441,11 +356,7 @@ struct I8Tile {
     static_assert(TM >= 1 && TN >= 1 && ST >= 2 && ST * STAGE <= 160 * 1024, "tile");
     static_assert(STAGE >= 12 * 256, "the scales of a tile in a stage's place");
 };
-template <int CPR>
-__device__ __forceinline__ int i8_swz(int row) {
-    if constexpr (CPR == 8) return (row ^ (row >> 3 & 3)) & 7;
-    else return (row ^ (row >> 2)) & 3;
-}
+__device__ __forceinline__ int i8_swz(int row) { return (row ^ (row >> 3 & 3)) & 7; }
 // 16 bytes a lane from byte at + k0 of a buffer to 1,024 of LDS.  (The host's pass
 // knows the builtin, but not the size, and would drop the kernels that use it.)
 typedef __attribute__((address_space(3))) void i8_lds;
@@ -454,10 +365,31 @@ __device__ __forceinline__ void i8_copy(__amdgpu_buffer_rsrc_t from, unsigned ch
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (i8_lds *)to, 16, at, k0, 0, 0);
 #endif
 }
+// The compiler moves no LDS access across a barrier.
+__device__ __forceinline__ void i8_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 #define I8_VMCNT(n) (0x0070 | ((n) & 15) | ((n) >> 4 << 14))      // s_waitcnt vmcnt(n) lgkmcnt(0)
 
+// The order of a step's instructions in a wave: MFMAs with the next step's
+// fragments, and the copies, between them.
+template <int I, int PER, int FR, int DMA>
+struct I8Order {
+    static __device__ __forceinline__ void run() {
+        if constexpr (I < PER) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                           // an MFMA
+            constexpr int n = (I + 1) * FR / PER - I * FR / PER, m = (I + 1) * DMA / PER - I * DMA / PER;
+            if constexpr (n > 0) __builtin_amdgcn_sched_group_barrier(0x100, n, 0);      // LDS reads
+            if constexpr (m > 0) __builtin_amdgcn_sched_group_barrier(0x020, m, 0);      // copies
+            I8Order<I + 1, PER, FR, DMA>::run();
+        }
+    }
+};
+
 template <typename T, bool GATED, bool CBF>
-__global__ __launch_bounds__(WAVE *T::NW, T::NW == 8 ? 2 : 1) void k_i8_tile(I8Args p, int MT, int NT, int per) {
+__global__ __launch_bounds__(WAVE *T::NW, T::NW / 4) void k_i8_tile(I8Args p, int MT, int NT, int per) {
     constexpr int BNO = GATED ? T::BN / 2 : T::BN, ES = CBF ? 2 : 4;
     __shared__ __align__(1024) unsigned char smem[T::ST * T::STAGE];
     // tiles in the order of the XCDs, which get workgroups in turn: each a run of
@@ -468,7 +400,7 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW == 8 ? 2 : 1) void k_i8_tile(I8A
     const int first = idx / (8 * NT) * 8, gs = min(MT - first, 8), in = idx - first * NT;
     const int m0 = (first + in % gs) * T::BM, n0 = in / gs * BNO;
 
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int wm = wave / T::WN, wn = wave % T::WN;
     const int rows = min(p.M - m0, T::BM), cols = min(p.N - n0, BNO);
     const auto ra = buf_rsrc(p.a + (size_t)m0 * p.lda, (size_t)rows * p.lda);
@@ -477,7 +409,7 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW == 8 ? 2 : 1) void k_i8_tile(I8A
     // row and piece that copy instruction i of the wave brings to this lane's place
     auto a_row = [&](int i) { return (wave * T::A_DMA + i) * T::RPI + lane / T::CPR; };
     auto b_row = [&](int i) { return (wave * T::B_DMA + i) * T::RPI + lane / T::CPR; };
-    auto piece = [&](int row) { return ((lane % T::CPR) ^ i8_swz<T::CPR>(row)) * 16; };
+    auto piece = [&](int row) { return ((lane % T::CPR) ^ i8_swz(row)) * 16; };
     auto a_at = [&](int i) { return min(a_row(i), rows - 1) * (int)p.lda; };
     auto b_at = [&](int i) { return min(GATED && b_row(i) >= BNO ? b_row(i) - BNO : b_row(i), cols - 1) * (int)p.ldb; };
     int va[T::A_DMA], vb[T::B_DMA];
@@ -514,26 +446,35 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW == 8 ? 2 : 1) void k_i8_tile(I8A
     int fa_at[T::KS], fb_at[T::KS];
 #pragma unroll
     for (int s = 0; s < T::KS; s++) {
-        const int pc = ((2 * s + fh) ^ i8_swz<T::CPR>(fr)) * 16;
+        const int pc = ((2 * s + fh) ^ i8_swz(fr)) * 16;
         fa_at[s] = (wm * (T::BM / T::WM) + fr) * T::BK + pc;
         fb_at[s] = T::A_BYTES + (wn * (BNO / T::WN) + fr) * T::BK + pc;
     }
     i32x16 acc[T::TM][T::TN] = {};
-    auto multiply = [&](int kt) {
+    i32x4 fa[2][T::TM], fb[2][T::TN];
+    auto read = [&](int kt, int s) {
         const unsigned char *slot = smem + kt % T::ST * T::STAGE;
 #pragma unroll
-        for (int s = 0; s < T::KS; s++) {
-            i32x4 fa[T::TM], fb[T::TN];
+        for (int j = 0; j < T::TN; j++)
+            fb[s & 1][j] = *(const i32x4 *)(slot + fb_at[s] + j * NEXT + (GATED && j >= T::TN / 2 ? UP : 0));
 #pragma unroll
-            for (int i = 0; i < T::TM; i++) fa[i] = *(const i32x4 *)(slot + fa_at[s] + i * NEXT);
+        for (int i = 0; i < T::TM; i++) fa[s & 1][i] = *(const i32x4 *)(slot + fa_at[s] + i * NEXT);
+    };
+    auto multiply = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < T::TM; i++)
 #pragma unroll
             for (int j = 0; j < T::TN; j++)
-                fb[j] = *(const i32x4 *)(slot + fb_at[s] + j * NEXT + (GATED && j >= T::TN / 2 ? UP : 0));
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[s & 1][i], fb[s & 1][j], acc[i][j], 0, 0, 0);
+    };
+    constexpr int PER = T::TM * T::TN, FR = T::TM + T::TN;
+    // all but the last step of stage kt, each with the next one's fragments on their way
+    auto most = [&](int kt) {
 #pragma unroll
-            for (int i = 0; i < T::TM; i++)
-#pragma unroll
-                for (int j = 0; j < T::TN; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
+        for (int s = 0; s + 1 < T::KS; s++) {
+            read(kt, s + 1);
+            multiply(s);
+            I8Order<0, PER, FR, 0>::run();
         }
     };
     const int nk = (p.K + T::BK - 1) / T::BK, whole = p.K / T::BK;
@@ -541,33 +482,42 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW == 8 ? 2 : 1) void k_i8_tile(I8A
         if (kt < whole) issue(kt, IC<1>{});
         else issue(kt, IC<0>{});
     };
-    for (int t = 0; t < T::ST - 1; t++)
+    for (int t = 0; t < T::ST; t++)
         if (t < nk) issue_any(t);
     int kt = 0;
-    for (; kt + T::ST - 1 < whole; kt++) {
-        // this wave's copies of stage kt are there, later ones may be on their way; every
-        // wave has read stage kt - 1, whose place is next
+    if (whole >= T::ST) __builtin_amdgcn_s_waitcnt(I8_VMCNT((T::ST - 1) * T::DMA));
+    else __builtin_amdgcn_s_waitcnt(I8_VMCNT(0));
+    i8_barrier();
+    read(0, 0);
+    for (; kt + T::ST < whole; kt++) {
+        most(kt);
+        // this wave has read all of stage kt and its copies of the next are there: after the
+        // barrier every wave's
         __builtin_amdgcn_s_waitcnt(I8_VMCNT((T::ST - 2) * T::DMA));
-        __builtin_amdgcn_s_barrier();
-        issue(kt + T::ST - 1, IC<1>{});
-        multiply(kt);
+        i8_barrier();
+        issue(kt + T::ST, IC<1>{});
+        read(kt + 1, 0);
+        multiply(T::KS - 1);
+        I8Order<0, PER, FR, T::DMA>::run();
         __builtin_amdgcn_sched_barrier(0);
     }
     for (; kt < nk; kt++) {
+        most(kt);
         __builtin_amdgcn_s_waitcnt(I8_VMCNT(0));
-        __builtin_amdgcn_s_barrier();
-        if (kt + T::ST - 1 < nk) issue_any(kt + T::ST - 1);
-        multiply(kt);
+        i8_barrier();
+        if (kt + T::ST < nk) issue_any(kt + T::ST);
+        if (kt + 1 < nk) read(kt + 1, 0);
+        multiply(T::KS - 1);
         __builtin_amdgcn_sched_barrier(0);
     }
 
     // the tile's scales through LDS; stores behind M and N fall out of the buffer's range
     __syncthreads();
     float *sm = (float *)smem, *sn = sm + T::BM, *su = sn + BNO;
-    for (int i = tid; i < T::BM; i += WAVE * T::NW) sm[i] = p.as[min(m0 + i, p.M - 1)];
+    for (int i = tid; i < T::BM; i += WAVE * T::NW) sm[i] = p.as[m0 + min(i, rows - 1)];
     for (int i = tid; i < BNO; i += WAVE * T::NW) {
-        sn[i] = p.bs[min(n0 + i, p.N - 1)];
-        if constexpr (GATED) su[i] = p.bs2[min(n0 + i, p.N - 1)];
+        sn[i] = p.bs[n0 + min(i, cols - 1)];
+        if constexpr (GATED) su[i] = p.bs2[n0 + min(i, cols - 1)];
     }
     __syncthreads();
     constexpr int TNO = GATED ? T::TN / 2 : T::TN;
@@ -577,20 +527,28 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW == 8 ? 2 : 1) void k_i8_tile(I8A
     for (int j = 0; j < TNO; j++) {
         const int n = wn * (BNO / T::WN) + 32 * j + fr;
         const float s = sn[n], s2 = GATED ? su[n] : 0.0f;
-        const unsigned at = n < cols ? n * ES : BUF_OOB;
+        const unsigned at = (n < cols ? n * ES : BUF_OOB) + 4 * fh * ldc;
 #pragma unroll
         for (int i = 0; i < T::TM; i++)
 #pragma unroll
             for (int e4 = 0; e4 < 4; e4++) {
-                const int m = wm * (T::BM / T::WM) + 32 * i + 8 * e4 + 4 * fh;
-                const f32x4 r = *(const f32x4 *)(sm + m);
+                const int m = wm * (T::BM / T::WM) + 32 * i + 8 * e4;
+                const f32x4 r = *(const f32x4 *)(sm + m + 4 * fh);
+                float y[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    float y = (float)acc[i][j][4 * e4 + e] * (r[e] * s);
-                    if constexpr (GATED) y = silu_mul(y, (float)acc[i][j + TNO][4 * e4 + e] * (r[e] * s2));
-                    const unsigned to = at + (unsigned)((m + e) * ldc);
-                    if constexpr (CBF) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (__bf16)y), rc, to, 0, 0);
-                    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y), rc, to, 0, 0);
+                    y[e] = (float)acc[i][j][4 * e4 + e] * (r[e] * s);
+                    if constexpr (GATED) y[e] = i8_silu_mul<CBF>(y[e], (float)acc[i][j + TNO][4 * e4 + e] * (r[e] * s2));
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const unsigned to = at + (m + e) * ldc;
+                    if constexpr (CBF) {
+                        const uint32_t two = pack_bf16x2(y[e & ~1], y[e | 1]);
+                        __builtin_amdgcn_raw_buffer_store_b16((short)(e & 1 ? two >> 16 : two), rc, to, 0, 0);
+                    } else {
+                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y[e]), rc, to, 0, 0);
+                    }
                 }
             }
     }
@@ -633,39 +591,51 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
     return QH_OK;
 }
 
-enum { I8_ANY_PLAN, I8_NARROW1_8, I8_NARROW1_16, I8_NARROW2_8, I8_NARROW4_8, I8_WIDE1, I8_WIDE4, I8_TILE64, I8_TILE128, I8_TILE256 };
+enum { I8_ANY_PLAN, I8_NARROW1, I8_NARROW2, I8_TILE64, I8_TILE64X128, I8_TILE128, I8_TILE192X256, I8_TILE256 };
 
+// Few blocks of 16 columns: as long as there is at most one on each of the 256
+// CUs (two of 16 rows), against tiles: 64 x 1024 x 1024 3.2 us and 4.8, 128 x 4096 x
+// 1024 7.8 and 9.7; with 512 blocks 64 x 1024 x 4096 5.3 and 4.9.  Rows are read
+// by every block, so blocks of 16 rows until 256 of them, then of 32.  Up to four
+// rows always: they are read once a block, 1 x 4096 x 20000 18.2 and 21.1 us.
+// Tiles: the least of an estimate, us = fixed + rounds of 256 * a tile's start and
+// end + stages * tiles a CU * a stage, fitted to 1,142 measurements (M 16 to
+// 4,096, N 512 to 20,000, K 512 to 4,096; it takes 1.3% longer than the best of
+// them on average).  A gated product has two weights' columns.
 static int i8_plan_of(const I8Args &p, bool gated) {
     if (!p.K || !aligned16(p.a) || !aligned16(p.b) || !aligned16(p.b2) || p.lda % 16 || p.ldb % 16 || p.lda > I8_MAX_NEAR ||
         p.ldb > I8_MAX_NEAR)
         return I8_ANY_PLAN;
-    if (p.ldc > I8_MAX_NEAR / 4) return I8_NARROW4_8;
-    const long cols = (p.N + 15) / 16;
-    if (p.M <= 64) {
-        if (cols >= 4096 && p.M <= 16 && (p.K + 255) / 256 * 256 * 16 <= 65536) return I8_WIDE1;
-        if (cols >= 4096 && (p.K + 255) / 256 * 256 * 64 <= 65536) return I8_WIDE4;
-        if (p.M <= 16) return p.K > 2048 ? I8_NARROW1_16 : I8_NARROW1_8;
-        return p.M <= 32 ? I8_NARROW2_8 : I8_NARROW4_8;
+    if (p.ldc > I8_MAX_NEAR / 4) return p.M <= 65535 * 32 ? I8_NARROW2 : I8_ANY_PLAN;   // tiles' stores have 32-bit offsets
+    const long cols = ((long)p.N + 15) / 16;
+    if (p.M <= 4 || cols * ((p.M + 15l) / 16) <= (p.M <= 16 ? 512 : 256)) return I8_NARROW1;
+    if (cols * ((p.M + 31l) / 32) <= 256) return I8_NARROW2;
+    static const struct { int plan, bm, bn; float fixed, tile, stage; } T[] = {
+        {I8_TILE64, 64, 64, 2.35f, 0.82f, 0.223f},      {I8_TILE64X128, 64, 128, 2.19f, 1.34f, 0.343f},
+        {I8_TILE128, 128, 128, 1.99f, 1.89f, 0.566f},   {I8_TILE192X256, 192, 256, 0.0f, 5.55f, 0.956f},
+        {I8_TILE256, 256, 256, 0.0f, 6.40f, 1.153f}};
+    const double stages = (p.K + 127) / 128;
+    double best = 1e30;
+    int plan = I8_TILE64;
+    for (const auto &t : T) {
+        const double tiles = ceil(p.M / (double)t.bm) * ceil(p.N * (gated ? 2.0 : 1.0) / t.bn);
+        const double us = t.fixed + ceil(tiles / 256) * t.tile + stages * fmax(tiles / 256, 1.0) * t.stage;
+        if (us < best) {
+            best = us;
+            plan = t.plan;
+        }
     }
-    const long t = (gated ? 2 : 1) * (long)p.N;
-    if (((p.M + 255) / 256) * ((t + 255) / 256) >= 256) return I8_TILE256;
-    if (((p.M + 127) / 128) * ((t + 127) / 128) >= 256) return I8_TILE128;
-    return I8_TILE64;
+    return plan;
 }
 
 template <int MT, int W, bool GATED, bool CBF>
 static void i8_narrow(const I8Args &p) {
-    hipLaunchKernelGGL((k_i8_narrow<MT, W, GATED, CBF>), dim3((p.N + 15) / 16, (p.M + 16 * MT - 1) / (16 * MT)), dim3(WAVE *W), 0,
-                       g_stream, p);
-}
-template <int MT, int KB, bool GATED, bool CBF>
-static void i8_wide(const I8Args &p) {
-    const int vec = p.ldc % 4 == 0 && aligned(p.c, CBF ? 8 : 16);
-    hipLaunchKernelGGL((k_i8_wide<MT, KB * 1024, GATED, CBF>), dim3(512), dim3(WAVE *I8_WIDE_WAVES), 0, g_stream, p, vec);
+    hipLaunchKernelGGL((k_i8_narrow<MT, W, GATED, CBF>), dim3((p.N + 15l) / 16, (p.M + 16 * MT - 1l) / (16 * MT)),
+                       dim3(WAVE *W), 0, g_stream, p);
 }
 template <typename T, bool GATED, bool CBF>
 static void i8_tile(const I8Args &p) {
-    const long mt = (p.M + T::BM - 1) / T::BM, bno = GATED ? T::BN / 2 : T::BN, nt = (p.N + bno - 1) / bno;
+    const long bno = GATED ? T::BN / 2 : T::BN, mt = (p.M + T::BM - 1l) / T::BM, nt = (p.N + bno - 1) / bno;
     const int per = (int)((mt * nt + 7) / 8);
     hipLaunchKernelGGL((k_i8_tile<T, GATED, CBF>), dim3(8 * per), dim3(WAVE *T::NW), 0, g_stream, p, (int)mt, (int)nt, per);
 }
@@ -674,20 +644,18 @@ template <bool GATED, bool CBF>
 static int i8_launch(const I8Args &p) {
     switch (i8_plan_of(p, GATED)) {
     case I8_ANY_PLAN: {
-        const dim3 any((p.N + I8_ANY - 1) / I8_ANY, (p.M + I8_ANY - 1) / I8_ANY);
-        if (any.y > 65535) return QH_ETOOBIG;
-        hipLaunchKernelGGL((k_i8_any<GATED, CBF>), any, dim3(NTHREADS), 0, g_stream, p);
+        const long mt = (p.M + I8_ANY - 1l) / I8_ANY, nt = (p.N + I8_ANY - 1l) / I8_ANY;
+        if (mt * nt >= 1l << 31) return QH_ETOOBIG;
+        hipLaunchKernelGGL((k_i8_any<GATED, CBF>), dim3((unsigned)(mt * nt)), dim3(NTHREADS), 0, g_stream, p, (unsigned)nt);
         break;
     }
-    case I8_NARROW1_8: i8_narrow<1, 8, GATED, CBF>(p); break;
-    case I8_NARROW1_16: i8_narrow<1, 16, GATED, CBF>(p); break;
-    case I8_NARROW2_8: i8_narrow<2, 8, GATED, CBF>(p); break;
-    case I8_NARROW4_8: i8_narrow<4, 8, GATED, CBF>(p); break;
-    case I8_WIDE1: i8_wide<1, 64, GATED, CBF>(p); break;
-    case I8_WIDE4: i8_wide<4, 64, GATED, CBF>(p); break;
-    case I8_TILE64: i8_tile<I8Tile<64, 64, 2, 2 - GATED, 128, 4>, GATED, CBF>(p); break;
-    case I8_TILE128: i8_tile<I8Tile<128, 128, 2, 2, 128, 2>, GATED, CBF>(p); break;
-    case I8_TILE256: i8_tile<I8Tile<256, 256, 2, 4, 128, 2>, GATED, CBF>(p); break;
+    case I8_NARROW1: i8_narrow<1, 8, GATED, CBF>(p); break;
+    case I8_NARROW2: i8_narrow<2, 8, GATED, CBF>(p); break;
+    case I8_TILE64: i8_tile<I8Tile<64, 64, 2, 2 - GATED, 4>, GATED, CBF>(p); break;
+    case I8_TILE64X128: i8_tile<I8Tile<64, 128, 2, 2, 3>, GATED, CBF>(p); break;
+    case I8_TILE128: i8_tile<I8Tile<128, 128, 2, 2, 2>, GATED, CBF>(p); break;
+    case I8_TILE192X256: i8_tile<I8Tile<192, 256, 2, 4, 2>, GATED, CBF>(p); break;
+    case I8_TILE256: i8_tile<I8Tile<256, 256, 2, 4, 2>, GATED, CBF>(p); break;
     }
     HCHECK(hipGetLastError(), QH_ELAUNCH);
     return QH_OK;

@@ -68,14 +68,18 @@ __device__ __forceinline__ void i8_eight(float *v, const void *x, size_t i, int 
 
 // TPR threads a row, in turns of 8 values each.  The first KEEP turns' values stay
 // in registers between the maximum and the codes; a longer row's others are read
-// again.
+// again.  Bound by memory: 65,536 x 1,024 fp32 60.8 us (5.5 TB/s), 4,096 x 4,096
+// 18.2; below some MB by the launch and two latencies: one row 2.9, 1,999 x 2,048
+// bf16 6.3.  As few threads a row as hold it in registers: 30,000 x 64 5.6 us on 16
+// threads and 13.8 on 64, 8,000 x 5,000 39 on 256 with four turns and 52 on 1,024;
+// four turns where two do (64 x 1,024) 3.7 and 3.2.
 template <bool BF, bool VEC, int TPR, int KEEP>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__restrict__ q, size_t ldq, float *__restrict__ scale,
                                                                    const void *__restrict__ x, size_t ldx, int K, int rows) {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
     const size_t row = (size_t)blockIdx.x * RPB + threadIdx.x / TPR;
     const int t = threadIdx.x % TPR;
-    if (TPR <= WAVE && row >= (size_t)rows) return;       // whole waves
+    if (TPR <= WAVE && row >= (size_t)rows) return;       // all lanes of a row
     const size_t from = row * ldx;
     float v[KEEP][8], a = 0.0f;
 #pragma unroll
@@ -97,7 +101,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__r
             a = fmaxf(a, fabsf(v[u][j]));
         }
 #pragma unroll
-    for (int m = WAVE / 2; m >= 1; m >>= 1) a = fmaxf(a, __shfl_xor(a, m));
+    for (int m = (TPR < WAVE ? TPR : WAVE) / 2; m >= 1; m >>= 1) a = fmaxf(a, __shfl_xor(a, m));
     if constexpr (TPR > WAVE) {
         __shared__ float red[TPR / WAVE];
         if ((t & 63) == 0) red[t >> 6] = a;
@@ -568,14 +572,15 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
     if (K > I8_MAX_K || ldq > I8_MAX_LD || ldx > I8_MAX_LD) return QH_ETOOBIG;
     if (!g_inited) return QH_ESTATE;
     const bool vec = aligned16(x) && ldx * (bf16 ? 2 : 4) % 16 == 0 && aligned(q, 8) && ldq % 8 == 0;
-    const unsigned four = (unsigned)(((size_t)rows + 3) / 4);
-#define ROWS_AS(BF, V, TPR, KEEP)                                                                             \
-    hipLaunchKernelGGL((k_rows_int8<BF, V, TPR, KEEP>), dim3(TPR == 64 ? four : rows), dim3(TPR < 256 ? 256 : TPR), 0, \
-                       g_stream, q, ldq, scale, x, ldx, K, rows)
+#define ROWS_AS(BF, V, TPR, KEEP)                                                                            \
+    hipLaunchKernelGGL((k_rows_int8<BF, V, TPR, KEEP>), dim3((unsigned)(((size_t)rows * TPR + 255) / (TPR < 256 ? 256 : TPR))), \
+                       dim3(TPR < 256 ? 256 : TPR), 0, g_stream, q, ldq, scale, x, ldx, K, rows)
 #define ROWS(BF, V)                                        \
     do {                                                   \
-        if (K <= 1024) ROWS_AS(BF, V, 64, 2);              \
+        if (K <= 256) ROWS_AS(BF, V, 16, 2);               \
+        else if (K <= 1024) ROWS_AS(BF, V, 64, 2);         \
         else if (K <= 4096) ROWS_AS(BF, V, 256, 2);        \
+        else if (K <= 8192) ROWS_AS(BF, V, 256, 4);        \
         else ROWS_AS(BF, V, 1024, 2);                      \
     } while (0)
     if (bf16) {

@@ -13,8 +13,9 @@
 // no bound on the history's length, no table of n x vocab counts in memory and
 // nothing to clear between calls.
 
-#define RULES_PIECE 4096
-#define RULES_GROUPS (RULES_PIECE / 4 / NTH)  // of four tokens a thread: tid, tid + NTH, ...
+#define RULES_NT 512
+#define RULES_PIECE 8192
+#define RULES_GROUPS (RULES_PIECE / 4 / RULES_NT)  // of four tokens a thread: tid, tid + NT, ...
 #define RULES_SEEN 0x80000000u
 
 // e: a token's word of the table
@@ -50,15 +51,26 @@ __device__ __forceinline__ void rules_store(float *x, f32x4 v, int left) {
         if (e < left) x[e] = v[e];
 }
 
+// four tokens of the history from j on, below n
+__device__ __forceinline__ uint4 rules_tokens(const int *h, int j, int n, bool vec) {
+    if (vec && j + 4 <= n) return *(const uint4 *)(h + j);
+    uint4 v = make_uint4(~0u, ~0u, ~0u, ~0u);
+    if (j < n) v.x = h[j];
+    if (j + 1 < n) v.y = h[j + 1];
+    if (j + 2 < n) v.z = h[j + 2];
+    if (j + 3 < n) v.w = h[j + 3];
+    return v;
+}
+
 // INPLACE: what a rule does not touch is neither read nor written.
 // Every load that does not wait for another one goes out first: the logits, the
 // first tokens of the history (whose number is then not known yet), the row's
-// numbers.
-template <bool VEC, bool INPLACE, bool BIAS>
-__global__ __launch_bounds__(NTH) void k_logits_rules(float *out, size_t ldo, const float *in, size_t ldx, int vocab,
-                                                     qm_rules_t t) {
-    __shared__ __align__(16) uint32_t tab[RULES_PIECE];          // occurrences behind the prompt, RULES_SEEN
-    __shared__ __align__(16) int last[BIAS ? RULES_PIECE : 4];   // 1 + the last bias entry that names the token
+// numbers.  The biases take the table's place once the penalties are done with it.
+template <bool VEC, bool INPLACE>
+__global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ldo, const float *in, size_t ldx, int vocab,
+                                                          qm_rules_t t, bool hvec) {
+    constexpr int NT = RULES_NT;
+    __shared__ __align__(16) uint32_t tab[RULES_PIECE];   // occurrences behind the prompt, RULES_SEEN; then 1 + a bias entry
     const int i = blockIdx.y, tid = threadIdx.x;
     const int v0 = blockIdx.x * RULES_PIECE, nv = min(vocab - v0, RULES_PIECE);
     const float *x = in + (size_t)i * ldx + v0;
@@ -66,17 +78,15 @@ __global__ __launch_bounds__(NTH) void k_logits_rules(float *out, size_t ldo, co
     f32x4 y[RULES_GROUPS];
     if constexpr (!INPLACE) {
 #pragma unroll
-        for (int u = 0; u < RULES_GROUPS; u++) y[u] = rules_load<VEC>(x + 4 * (tid + u * NTH), nv - 4 * (tid + u * NTH));
+        for (int u = 0; u < RULES_GROUPS; u++) y[u] = rules_load<VEC>(x + 4 * (tid + u * NT), nv - 4 * (tid + u * NT));
     }
     const int *h = t.token + (size_t)i * t.ld_token;
-    int early[4];
-#pragma unroll
-    for (int u = 0; u < 4; u++) early[u] = tid + u * NTH < t.ld_token && t.token ? h[tid + u * NTH] : -1;
+    const uint4 early = rules_tokens(h, 4 * tid, t.token ? t.ld_token : 0, hvec);
     int len = t.token ? t.n_token[i] : 0;
     if (len > t.ld_token) len = 0;
     const int prompt = t.n_prompt ? t.n_prompt[i] : 0;
     int b0 = 0, b1 = 0;
-    if constexpr (BIAS) {
+    if (t.bias_row) {
         b0 = t.bias_row[i];
         b1 = t.bias_row[i + 1];
         if (b0 < 0 || b1 > t.n_bias) b1 = b0;
@@ -86,57 +96,76 @@ __global__ __launch_bounds__(NTH) void k_logits_rules(float *out, size_t ldo, co
     const int mi = !t.mask ? -1 : t.mask_of ? t.mask_of[i] : i;
     const uint32_t *mask = mi >= 0 && mi < t.n_mask ? t.mask + (size_t)mi * t.ld_mask + v0 / 32 : nullptr;
 
+    auto clear = [&] {
 #pragma unroll
-    for (int u = 0; u < RULES_GROUPS; u++) {
-        ((uint4 *)tab)[tid + u * NTH] = make_uint4(0, 0, 0, 0);
-        if constexpr (BIAS) ((uint4 *)last)[tid + u * NTH] = make_uint4(0, 0, 0, 0);
-    }
+        for (int u = 0; u < RULES_GROUPS; u++) ((uint4 *)tab)[tid + u * NT] = make_uint4(0, 0, 0, 0);
+    };
+    clear();
     uint32_t words[RULES_GROUPS];
 #pragma unroll
     for (int u = 0; u < RULES_GROUPS; u++)
-        words[u] = mask && 4 * (tid + u * NTH) < nv ? mask[(tid + u * NTH) / 8] >> (tid % 8 * 4) & 15 : 15;
+        words[u] = mask && 4 * (tid + u * NT) < nv ? mask[(tid + u * NT) / 8] >> (tid % 8 * 4) & 15 : 15;
     __syncthreads();
-    auto count = [&](int token, int j) {
-        const unsigned v = (unsigned)token - (unsigned)v0;
-        if (v >= (unsigned)nv) return;
+    auto count = [&](uint32_t token, int j) {
+        const uint32_t v = token - (uint32_t)v0;
+        if (j >= len || v >= (uint32_t)nv) return;
         atomicOr(&tab[v], RULES_SEEN);
         if (j >= prompt) atomicAdd(&tab[v], 1u);
     };
-#pragma unroll
-    for (int u = 0; u < 4; u++)
-        if (tid + u * NTH < len) count(early[u], tid + u * NTH);
-    for (int j = tid + 4 * NTH; j < len; j += 4 * NTH) {
-        int v[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++) v[u] = h[min(j + u * NTH, len - 1)];
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-            if (j + u * NTH < len) count(v[u], j + u * NTH);
+    auto count4 = [&](uint4 v, int j) {
+        count(v.x, j);
+        count(v.y, j + 1);
+        count(v.z, j + 2);
+        count(v.w, j + 3);
+    };
+    count4(early, 4 * tid);
+    for (int j = 4 * (tid + NT); j < len; j += 8 * NT) {
+        const uint4 one = rules_tokens(h, j, len, hvec), two = rules_tokens(h, j + 4 * NT, len, hvec);
+        count4(one, j);
+        count4(two, j + 4 * NT);
     }
-    if constexpr (BIAS)
-        for (int j = b0 + tid; j < b1; j += NTH) {
-            const unsigned v = (unsigned)t.bias_token[j] - (unsigned)v0;
-            if (v < (unsigned)nv) atomicMax(&last[v], j + 1);
-        }
     __syncthreads();
+    uint32_t have = 0;                                    // groups whose values are in y
 #pragma unroll
     for (int u = 0; u < RULES_GROUPS; u++) {
-        const int g = tid + u * NTH, left = nv - 4 * g;
-        if (left <= 0) continue;
+        const int g = tid + u * NT, left = nv - 4 * g;
         const uint4 e = ((const uint4 *)tab)[g];
-        const uint4 l = BIAS ? ((const uint4 *)last)[g] : make_uint4(0, 0, 0, 0);
-        const bool touched = (e.x | e.y | e.z | e.w | l.x | l.y | l.z | l.w) != 0;
-        if constexpr (INPLACE) {
-            if (!touched && words[u] == 15) continue;
-            if (words[u]) y[u] = rules_load<VEC>(x + 4 * g, left);
-        }
-        if (touched) {
-            const uint32_t ee[4] = {e.x, e.y, e.z, e.w}, ll[4] = {l.x, l.y, l.z, l.w};
+        if ((e.x | e.y | e.z | e.w) == 0) continue;
+        if constexpr (INPLACE) y[u] = rules_load<VEC>(x + 4 * g, left);
+        have |= 1u << u;
+        const uint32_t ee[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                y[u][k] = rules_penalised(y[u][k], ee[k], r, f, p);
-                if (BIAS && ll[k]) y[u][k] += t.bias[ll[k] - 1];
-            }
+        for (int k = 0; k < 4; k++) y[u][k] = rules_penalised(y[u][k], ee[k], r, f, p);
+    }
+    if (b0 < b1) {                                        // the same for the whole block
+        __syncthreads();
+        clear();
+        __syncthreads();
+        for (int j = b0 + tid; j < b1; j += NT) {
+            const uint32_t v = (uint32_t)t.bias_token[j] - (uint32_t)v0;
+            if (v < (uint32_t)nv) atomicMax(&tab[v], (uint32_t)j + 1);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < RULES_GROUPS; u++) {
+            const int g = tid + u * NT, left = nv - 4 * g;
+            const uint4 e = ((const uint4 *)tab)[g];
+            if ((e.x | e.y | e.z | e.w) == 0) continue;
+            if (INPLACE && !(have >> u & 1)) y[u] = rules_load<VEC>(x + 4 * g, left);
+            have |= 1u << u;
+            const uint32_t ee[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (ee[k]) y[u][k] += t.bias[ee[k] - 1];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < RULES_GROUPS; u++) {
+        const int g = tid + u * NT, left = nv - 4 * g;
+        if (left <= 0) continue;
+        if constexpr (INPLACE) {
+            if (!(have >> u & 1) && words[u] == 15) continue;
+            if (!(have >> u & 1) && words[u]) y[u] = rules_load<VEC>(x + 4 * g, left);
         }
 #pragma unroll
         for (int k = 0; k < 4; k++)
@@ -169,13 +198,9 @@ extern "C" int qm_logits_rules(float *out, size_t ldo, const float *logits, size
     if (!stream()) return QH_ESTATE;
     const dim3 grid((vocab + RULES_PIECE - 1) / RULES_PIECE, n);
     const bool vec = aligned16(out) && aligned16(logits) && ldo % 4 == 0 && ld % 4 == 0;
-#define RULES_AS(V, I, B) \
-    hipLaunchKernelGGL((k_logits_rules<V, I, B>), grid, dim3(NTH), 0, stream(), out, ldo, logits, ld, vocab, *t)
-#define RULES(V, I)                           \
-    do {                                      \
-        if (t->n_bias > 0) RULES_AS(V, I, true); \
-        else RULES_AS(V, I, false);           \
-    } while (0)
+    const bool hvec = t->token && aligned16(t->token) && t->ld_token % 4 == 0;
+#define RULES(V, I) \
+    hipLaunchKernelGGL((k_logits_rules<V, I>), grid, dim3(RULES_NT), 0, stream(), out, ldo, logits, ld, vocab, *t, hvec)
     if (out == logits) {
         if (vec) RULES(true, true);
         else RULES(false, true);
@@ -184,6 +209,5 @@ extern "C" int qm_logits_rules(float *out, size_t ldo, const float *logits, size
         else RULES(false, false);
     }
 #undef RULES
-#undef RULES_AS
     return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
 }

@@ -217,7 +217,38 @@ int qwen3_hip_batch_decode(qwen3_hip_batch *batch, int n_decode, int *out);
 int qwen3_hip_batch_beam(qwen3_hip_batch *batch, int width, const int *prompts, const int *n_prompt, int n_tokens,
                          int stop_at_eos, int *out, float *scores);
 
-/* Logits of the last decode step, n_seq x vocab floats (synchronous copy). */
+/* Rules on the tokens of sequence seq, from its next choice on, its prefill's
+ * included: penalties for the tokens of its prompt and answer, biases, and a
+ * mask of the tokens that are allowed, as qwen3_hip_logits_rules_dev applies
+ * them (qwen3_hip_serve.h).  rules NULL takes the sequence's rules away.  Host
+ * memory, read before the call returns; a grammar's mask is set anew between
+ * decodes of one step each.  A sequence whose mask allows nothing gets token 0.
+ * Rules stay through prefills.  QWEN3_HIP_EINVAL for a repetition that is not
+ * above 0, numbers that are not finite (a bias may be infinite) and tokens
+ * outside the vocabulary.  While a sequence has rules qwen3_hip_batch_beam
+ * returns QWEN3_HIP_ESTATE. */
+#define QWEN3_HIP_BATCH_MAX_BIAS 151936
+typedef struct {
+    float repetition;            /* 1: none */
+    float presence, frequency;   /* 0: none */
+    int n_bias;                  /* at most QWEN3_HIP_BATCH_MAX_BIAS (QWEN3_HIP_ETOOBIG) */
+    const int *bias_token;       /* of a token named twice the last entry counts */
+    const float *bias;
+    const uint32_t *mask;        /* 4,748 words, bit t % 32 of word t / 32 set: token t is allowed; NULL: every one */
+} qwen3_hip_batch_rules;
+int qwen3_hip_batch_set_rules(qwen3_hip_batch *batch, int seq, const qwen3_hip_batch_rules *rules);
+
+/* The logits of this batch's decode steps, greedy and of searches, from 8-bit
+ * products (1) or bf16 weights (0, the default): the last rows and the tied head
+ * as int8 codes with a scale for each row and each token (qwen3_hip_rows_int8_dev,
+ * qwen3_hip_gemm_int8_dev).  The first 1 makes the head's codes, 156 MB that the
+ * model keeps until it is closed.  Logits are off by the codes' roundings, 1.1% of
+ * their deviation where values are distributed normally.  A prompt's own logits,
+ * which choose its first token, stay those of the bf16 weights. */
+int qwen3_hip_batch_set_int8_head(qwen3_hip_batch *batch, int on);
+
+/* Logits of the last decode step, after the sequences' rules, n_seq x vocab
+ * floats (synchronous copy). */
 int qwen3_hip_batch_logits(qwen3_hip_batch *batch, float *out);
 
 /* Decode steps as one graph replay each (1, the default; the first step of

@@ -63,6 +63,9 @@ struct qwen3_hip_model {
     float *dump_host;                  /* staging for dumps */
     int have_logits;
     double t_prefill_ms, t_decode_ms;
+    /* the head's weights as int8 rows, and a step's rows before it; NULL until a batch asks for them */
+    int8_t *embed8, *row8;
+    float *embed8_scale, *row8_scale;
     struct qwen3_hip_batch *batches;   /* open batches on this model (linked by next) */
 };
 
@@ -144,7 +147,8 @@ void qwen3_hip_model_close(qwen3_hip_model *m) {
     for (int g = 0; g < 2; g++)
         if (m->graph_id[g] >= 0) (void)qh_graph_destroy(m->graph_id[g]);
     void *bufs[] = {m->wbuf, m->kc, m->vc, m->rcos, m->rsin, m->x, m->x0, m->x1, m->xb, m->qkv,
-                    m->att, m->ob, m->hb, m->dn, m->logits, m->apart, m->cpart, m->tok_in, m->state, m->out_tok};
+                    m->att, m->ob, m->hb, m->dn, m->logits, m->apart, m->cpart, m->tok_in, m->state, m->out_tok,
+                    m->embed8, m->row8, m->embed8_scale, m->row8_scale};
     for (size_t i = 0; i < sizeof bufs / sizeof bufs[0]; i++) (void)qh_free(bufs[i]);
     free(m->dump_host);
     free(m);
@@ -708,6 +712,15 @@ int qwen3_hip_model_timing(const qwen3_hip_model *m, double *prefill_ms, double 
 
 /* ---- multi-sequence batched decode ------------------------------------------ */
 
+#define MASK_WORDS ((V + 31) / 32)
+/* what is asked of a sequence's tokens */
+typedef struct {
+    int on, masked, n_bias;
+    float repetition, presence, frequency;
+    int *bias_token;
+    float *bias;
+} seq_rules_t;
+
 struct qwen3_hip_batch {
     qwen3_hip_model *m;
     int n_seq, max_ctx, out_ld;
@@ -723,9 +736,20 @@ struct qwen3_hip_batch {
     int *h_plen;                       /* host: prompt length of each sequence */
     int *h_out;                        /* host staging of out */
     int use_graph;
-    int graph_id[2];                   /* the greedy step and the beams' forward, -1 until captured */
+    int graph_id[3];                   /* the greedy step, the beams' forward, the step under rules; -1 until captured */
     int have_logits;
+    int head8;                         /* the head's product in 8-bit integers */
     double t_decode_ms;
+    /* rules on logits, allocated by the first: the texts [n_seq][out_ld] and their
+     * lengths, kept up while a sequence is under rules; penalties [3][n_seq]; the
+     * sequences' biases one after another, room for bias_room; a mask each */
+    int *h_text;                       /* host: every prefilled sequence's prompt */
+    seq_rules_t *h_rules;
+    int n_rules;                       /* sequences under rules */
+    int *text, *n_text, *bias_row, *bias_token, *mask_of;
+    float *penalty, *bias;
+    uint32_t *mask;
+    int bias_room;
     /* beam search, allocated by the first: per sequence score, finished, parent;
      * {token, parent} of every step; the choice's workspace */
     float *score;
@@ -739,7 +763,7 @@ struct qwen3_hip_batch {
  * first, its batches lose the graphs and the model, and later calls on them
  * return QWEN3_HIP_ESTATE instead of touching freed memory. */
 static void drop_graphs(qwen3_hip_batch *b) {
-    for (int g = 0; g < 2; g++) {
+    for (int g = 0; g < 3; g++) {
         if (b->graph_id[g] >= 0) (void)qh_graph_destroy(b->graph_id[g]);
         b->graph_id[g] = -1;
     }
@@ -763,8 +787,15 @@ void qwen3_hip_batch_close(qwen3_hip_batch *b) {
     }
     drop_graphs(b);
     void *bufs[] = {b->kc, b->vc, b->logits, b->part, b->tok, b->pos, b->plen, b->out, b->kv8.c.k, b->kv8.c.k_scale,
-                    b->kv8.c.k_tail, b->table, b->kv8.row, b->kv8.work, b->score, b->done, b->parent, b->hist, b->swork};
+                    b->kv8.c.k_tail, b->table, b->kv8.row, b->kv8.work, b->score, b->done, b->parent, b->hist, b->swork,
+                    b->text, b->n_text, b->bias_row, b->bias_token, b->mask_of, b->penalty, b->bias, b->mask};
     for (size_t i = 0; i < sizeof bufs / sizeof bufs[0]; i++) (void)qh_free(bufs[i]);
+    for (int s = 0; b->h_rules && s < b->n_seq; s++) {
+        free(b->h_rules[s].bias_token);
+        free(b->h_rules[s].bias);
+    }
+    free(b->h_rules);
+    free(b->h_text);
     free(b->h_next);
     free(b->h_plen);
     free(b->h_out);
@@ -822,12 +853,14 @@ static int batch_open(qwen3_hip_batch **out, qwen3_hip_model *m, int n_seq, int 
     b->out_ld = max_ctx + 1;
     b->kv_seq = (size_t)QW3M_N_KV_HEADS * max_ctx * QW3M_HEAD_DIM;
     b->use_graph = 1;
-    b->graph_id[0] = b->graph_id[1] = -1;
+    b->graph_id[0] = b->graph_id[1] = b->graph_id[2] = -1;
     int rc = QWEN3_HIP_ENOMEM;
     b->h_next = (int *)malloc((size_t)n_seq * sizeof(int));
     b->h_plen = (int *)calloc((size_t)n_seq, sizeof(int));
     b->h_out = (int *)malloc((size_t)n_seq * b->out_ld * sizeof(int));
-    if (!b->h_next || !b->h_plen || !b->h_out) goto fail;
+    b->h_text = (int *)malloc((size_t)n_seq * b->out_ld * sizeof(int));
+    b->h_rules = (seq_rules_t *)calloc((size_t)n_seq, sizeof *b->h_rules);
+    if (!b->h_next || !b->h_plen || !b->h_out || !b->h_text || !b->h_rules) goto fail;
     for (int s = 0; s < n_seq; s++) b->h_next[s] = -1;
 #define DEV(ptr, bytes)                                                   \
     do {                                                                  \
@@ -891,6 +924,180 @@ static int batch_prompt(qwen3_hip_batch *b, int seq, const int *prompt, int n_pr
     return prefill(b->m, &kv, prompt, n_prompt, &nt);
 }
 
+/* the rules on the rows of logits of sequences seq .. */
+static qm_rules_t rules_from(const qwen3_hip_batch *b, int seq) {
+    const int n = b->n_seq;
+    const qm_rules_t r = {b->text + (size_t)seq * b->out_ld, b->out_ld, b->plen + seq, b->n_text + seq, b->penalty + seq,
+                          b->penalty + n + seq, b->penalty + 2 * n + seq, b->bias_row + seq, b->bias_token, b->bias,
+                          b->bias_room, b->mask, MASK_WORDS, n, b->mask_of + seq};
+    return r;
+}
+
+/* the texts of all sequences as they stand, from the prompts and what the steps
+ * have put out: kept up by the steps from here on while there are rules */
+static int rules_texts(qwen3_hip_batch *b) {
+    const size_t all = (size_t)b->n_seq * b->out_ld;
+    int rc = qh_d2h(b->h_out, b->out, all * sizeof(int));
+    if (!rc) rc = qh_sync();
+    int *n = (int *)malloc((size_t)b->n_seq * sizeof(int));
+    if (!n) return QWEN3_HIP_ENOMEM;
+    for (int s = 0; s < b->n_seq && !rc; s++) {
+        const size_t row = (size_t)s * b->out_ld;
+        n[s] = b->h_next[s] < 0 ? 0 : b->h_next[s] + 1;       /* the token that is fed next is the last */
+        for (int i = b->h_plen[s]; i < n[s]; i++) b->h_text[row + i] = b->h_out[row + i - b->h_plen[s]];
+    }
+    if (!rc) rc = qh_h2d(b->text, b->h_text, all * sizeof(int));
+    if (!rc) rc = qh_h2d(b->n_text, n, (size_t)b->n_seq * sizeof(int));
+    if (!rc) rc = qh_sync();
+    free(n);
+    return rc;
+}
+
+/* device room for the rules, `biases` in all */
+static int rules_room(qwen3_hip_batch *b, int biases) {
+    const size_t n = (size_t)b->n_seq;
+    int rc = QWEN3_HIP_OK;
+    if (!b->text) rc = qh_malloc((void **)&b->text, n * b->out_ld * sizeof(int));
+    if (!rc && !b->n_text) rc = qh_malloc((void **)&b->n_text, n * sizeof(int));
+    if (!rc && !b->penalty) rc = qh_malloc((void **)&b->penalty, 3 * n * sizeof(float));
+    if (!rc && !b->bias_row) rc = qh_malloc((void **)&b->bias_row, (n + 1) * sizeof(int));
+    if (!rc && !b->mask_of) rc = qh_malloc((void **)&b->mask_of, n * sizeof(int));
+    if (!rc && !b->mask) rc = qh_malloc((void **)&b->mask, n * MASK_WORDS * sizeof(uint32_t));
+    if (rc || (b->bias_room && biases <= b->bias_room)) return rc;
+    const int room = biases < 512 ? 1024 : 2 * biases;
+    int *tok = NULL;
+    float *val = NULL;
+    rc = qh_malloc((void **)&tok, (size_t)room * sizeof(int));
+    if (!rc) rc = qh_malloc((void **)&val, (size_t)room * sizeof(float));
+    if (!rc) rc = qh_sync();           /* steps that read the old ones */
+    if (rc) {
+        (void)qh_free(tok);
+        (void)qh_free(val);
+        return rc;
+    }
+    if (b->graph_id[2] >= 0) (void)qh_graph_destroy(b->graph_id[2]);
+    b->graph_id[2] = -1;
+    (void)qh_free(b->bias_token);
+    (void)qh_free(b->bias);
+    b->bias_token = tok;
+    b->bias = val;
+    b->bias_room = room;
+    return rc;
+}
+
+/* penalties, biases and which sequences have masks, from the host's copies */
+static int rules_upload(qwen3_hip_batch *b, int biases) {
+    const int n = b->n_seq;
+    float *pen = (float *)malloc(3 * (size_t)n * sizeof(float));
+    int *row = (int *)malloc(((size_t)n + 1) * sizeof(int)), *of = (int *)malloc((size_t)n * sizeof(int));
+    int *tok = (int *)malloc(((size_t)biases + 1) * sizeof(int));
+    float *val = (float *)malloc(((size_t)biases + 1) * sizeof(float));
+    int rc = QWEN3_HIP_ENOMEM;
+    if (pen && row && of && tok && val) {
+        row[0] = 0;
+        for (int s = 0; s < n; s++) {
+            const seq_rules_t *r = &b->h_rules[s];
+            pen[s] = r->on ? r->repetition : 1.0f;
+            pen[n + s] = r->on ? r->presence : 0.0f;
+            pen[2 * n + s] = r->on ? r->frequency : 0.0f;
+            of[s] = r->on && r->masked ? s : -1;
+            const int k = r->on ? r->n_bias : 0;
+            if (k) {
+                memcpy(tok + row[s], r->bias_token, (size_t)k * sizeof(int));
+                memcpy(val + row[s], r->bias, (size_t)k * sizeof(float));
+            }
+            row[s + 1] = row[s] + k;
+        }
+        rc = qh_h2d(b->penalty, pen, 3 * (size_t)n * sizeof(float));
+        if (!rc) rc = qh_h2d(b->bias_row, row, ((size_t)n + 1) * sizeof(int));
+        if (!rc) rc = qh_h2d(b->mask_of, of, (size_t)n * sizeof(int));
+        if (!rc && biases) rc = qh_h2d(b->bias_token, tok, (size_t)biases * sizeof(int));
+        if (!rc && biases) rc = qh_h2d(b->bias, val, (size_t)biases * sizeof(float));
+        if (!rc) rc = qh_sync();
+    }
+    free(pen);
+    free(row);
+    free(of);
+    free(tok);
+    free(val);
+    return rc;
+}
+
+int qwen3_hip_batch_set_rules(qwen3_hip_batch *b, int seq, const qwen3_hip_batch_rules *r) {
+    if (!b || seq < 0 || seq >= b->n_seq) return QWEN3_HIP_EINVAL;
+    if (!b->m) return QWEN3_HIP_ESTATE;
+    seq_rules_t *now = &b->h_rules[seq];
+    if (!r && !now->on) return QWEN3_HIP_OK;
+    if (r) {
+        if (!(r->repetition > 0.0f) || !isfinite(r->repetition) || !isfinite(r->presence) || !isfinite(r->frequency))
+            return QWEN3_HIP_EINVAL;
+        if (r->n_bias < 0 || (r->n_bias && (!r->bias_token || !r->bias))) return QWEN3_HIP_EINVAL;
+        if (r->n_bias > QWEN3_HIP_BATCH_MAX_BIAS) return QWEN3_HIP_ETOOBIG;
+        for (int i = 0; i < r->n_bias; i++)
+            if (r->bias_token[i] < 0 || r->bias_token[i] >= V || isnan(r->bias[i])) return QWEN3_HIP_EINVAL;
+    }
+    if (qh_capturing()) return QWEN3_HIP_ERUNTIME;   /* rules come from the host */
+
+    seq_rules_t next = {0};
+    int biases = r ? r->n_bias : 0, rc = QWEN3_HIP_OK;
+    for (int s = 0; s < b->n_seq; s++)
+        if (s != seq && b->h_rules[s].on) biases += b->h_rules[s].n_bias;
+    if (r) {
+        next = (seq_rules_t){1, r->mask != NULL, r->n_bias, r->repetition, r->presence, r->frequency, NULL, NULL};
+        if (r->n_bias) {
+            next.bias_token = (int *)malloc((size_t)r->n_bias * sizeof(int));
+            next.bias = (float *)malloc((size_t)r->n_bias * sizeof(float));
+            if (!next.bias_token || !next.bias) rc = QWEN3_HIP_ENOMEM;
+            else {
+                memcpy(next.bias_token, r->bias_token, (size_t)r->n_bias * sizeof(int));
+                memcpy(next.bias, r->bias, (size_t)r->n_bias * sizeof(float));
+            }
+        }
+        if (!rc) rc = rules_room(b, biases);
+        if (!rc && b->n_rules == 0) rc = rules_texts(b);
+        if (!rc && r->mask) rc = qh_h2d(b->mask + (size_t)seq * MASK_WORDS, r->mask, MASK_WORDS * sizeof(uint32_t));
+    }
+    if (rc) {                          /* the rules stay as they were, but a mask may be half of each */
+        free(next.bias_token);
+        free(next.bias);
+        return rc;
+    }
+    b->n_rules += next.on - now->on;
+    free(now->bias_token);
+    free(now->bias);
+    *now = next;
+    return rules_upload(b, biases);
+}
+
+int qwen3_hip_batch_set_int8_head(qwen3_hip_batch *b, int on) {
+    if (!b) return QWEN3_HIP_EINVAL;
+    if (!b->m) return QWEN3_HIP_ESTATE;
+    on = on ? 1 : 0;
+    if (on == b->head8) return QWEN3_HIP_OK;
+    if (qh_capturing()) return QWEN3_HIP_ERUNTIME;   /* allocates, and drops graphs */
+    qwen3_hip_model *m = b->m;
+    if (on && !m->embed8) {
+        int8_t *w = NULL;
+        int rc = QWEN3_HIP_OK;
+        if (!m->embed8_scale) rc = qh_malloc((void **)&m->embed8_scale, (size_t)V * sizeof(float));
+        if (!rc && !m->row8) rc = qh_malloc((void **)&m->row8, (size_t)QM_MAX_CHUNK * H);
+        if (!rc && !m->row8_scale) rc = qh_malloc((void **)&m->row8_scale, (size_t)QM_MAX_CHUNK * sizeof(float));
+        if (!rc) rc = qh_malloc((void **)&w, (size_t)V * H);
+        if (!rc) rc = qh_rows_int8(w, H, m->embed8_scale, m->embed, H, 1, V, H);
+        if (!rc) rc = qh_sync();
+        if (rc) {
+            (void)qh_free(w);
+            return rc;
+        }
+        m->embed8 = w;
+    }
+    const int rc = qh_sync();          /* steps of the graphs that go */
+    if (rc) return rc;
+    drop_graphs(b);
+    b->head8 = on;
+    return QWEN3_HIP_OK;
+}
+
 int qwen3_hip_batch_prefill(qwen3_hip_batch *b, int seq, const int *prompt, int n_prompt) {
     if (!b || !prompt || seq < 0 || seq >= b->n_seq || n_prompt < 1 || n_prompt >= b->max_ctx)
         return QWEN3_HIP_EINVAL;
@@ -903,8 +1110,18 @@ int qwen3_hip_batch_prefill(qwen3_hip_batch *b, int seq, const int *prompt, int 
     /* first token: out[seq][0] at pos - plen + 1 = 0, then pos = n_prompt */
     if (!rc) rc = qm_set_i32(b->pos + seq, n_prompt - 1);
     if (!rc) rc = qm_set_i32(b->plen + seq, n_prompt);
+    int *text = b->h_text + (size_t)seq * b->out_ld;
+    memcpy(text, prompt, (size_t)n_prompt * sizeof(int));
+    if (!rc && b->n_rules) rc = qh_h2d(b->text + (size_t)seq * b->out_ld, text, (size_t)n_prompt * sizeof(int));
+    if (!rc && b->n_rules) rc = qm_set_i32(b->n_text + seq, n_prompt);
+    if (!rc && b->h_rules[seq].on) {
+        const qm_rules_t r = rules_from(b, seq);
+        rc = qm_logits_rules(m->logits, V, m->logits, V, V, 1, &r);
+    }
     if (!rc) rc = qm_argmax_rows(m->logits, V, 1, b->tok + seq, b->pos + seq, b->plen + seq,
                                  b->out + (size_t)seq * b->out_ld, b->out_ld);
+    if (!rc && b->n_rules)
+        rc = qm_rules_note(b->text + (size_t)seq * b->out_ld, b->out_ld, b->n_text + seq, b->tok + seq, b->pos + seq, 1);
     if (!rc) rc = qh_sync();
     if (!rc) {
         b->h_next[seq] = n_prompt;
@@ -944,15 +1161,22 @@ static int batch_forward(qwen3_hip_batch *b) {
     }
     if (!rc) rc = qm_rows_norm_split(m->x, dks ? NULL : m->dn, NULL, NULL, 0, m->final_norm, m->xb, n, H, eps,
                                      dpart, dks);
-    if (!rc) rc = qh_gemm(b->logits, m->xb, m->embed, n, H, V);
+    if (!b->head8) return rc ? rc : qh_gemm(b->logits, m->xb, m->embed, n, H, V);
+    if (!rc) rc = qh_rows_int8(m->row8, H, m->row8_scale, m->xb, H, 0, n, H);
+    if (!rc) rc = qh_gemm_int8(b->logits, V, 0, m->row8, H, m->row8_scale, m->embed8, H, m->embed8_scale, n, H, V);
     return rc;
 }
 
-/* the forward and the greedy choice of every sequence's next token (0), or the
- * forward alone (1) */
+/* the forward and the greedy choice of every sequence's next token, without
+ * rules (0) or under them (2), or the forward alone (1) */
 static int batch_step(qwen3_hip_batch *b, int which) {
     int rc = batch_forward(b);
-    if (!rc && which == 0) rc = qm_argmax_rows(b->logits, V, b->n_seq, b->tok, b->pos, b->plen, b->out, b->out_ld);
+    if (!rc && which == 2) {
+        const qm_rules_t r = rules_from(b, 0);
+        rc = qm_logits_rules(b->logits, V, b->logits, V, V, b->n_seq, &r);
+    }
+    if (!rc && which != 1) rc = qm_argmax_rows(b->logits, V, b->n_seq, b->tok, b->pos, b->plen, b->out, b->out_ld);
+    if (!rc && which == 2) rc = qm_rules_note(b->text, b->out_ld, b->n_text, b->tok, b->pos, b->n_seq);
     return rc;
 }
 
@@ -985,7 +1209,7 @@ int qwen3_hip_batch_decode(qwen3_hip_batch *b, int n_decode, int *out) {
         if (b->h_next[s] < 0 || (long)b->h_next[s] + n_decode > b->max_ctx) return QWEN3_HIP_EINVAL;
     int rc = QWEN3_HIP_OK;
     const double t0 = now_ms();
-    for (int i = 0; i < n_decode && !rc; i++) rc = batch_run(b, i, 0);
+    for (int i = 0; i < n_decode && !rc; i++) rc = batch_run(b, i, b->n_rules ? 2 : 0);
     if (!rc) rc = qh_sync();
     b->t_decode_ms = now_ms() - t0;
     if (rc) return rc;
@@ -1050,6 +1274,7 @@ int qwen3_hip_batch_beam(qwen3_hip_batch *b, int width, const int *prompts, cons
     if (!b || !prompts || !n_prompt || !out || !scores || n_tokens < 1) return QWEN3_HIP_EINVAL;
     if (!b->m) return QWEN3_HIP_ESTATE;
     if (width < 1 || width > QM_BEAM_MAX_WIDTH || b->n_seq % width) return QWEN3_HIP_EINVAL;
+    if (b->n_rules) return QWEN3_HIP_ESTATE;
     const int n = b->n_seq, groups = n / width;
     int longest = 0, rc = QWEN3_HIP_OK;
     size_t total = 0;

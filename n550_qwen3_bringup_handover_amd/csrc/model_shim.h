@@ -177,6 +177,8 @@ typedef struct {
     const int *mask_of;
 } qm_rules_t;
 int qm_logits_rules(float *out_d, size_t ldo, const float *logits_d, size_t ld, int vocab, int n, const qm_rules_t *rules);
+/* text_d[i][pos_d[i]] = tok_d[i], n_text_d[i] = pos_d[i] + 1 for n rows of ld tokens; positions outside a row are left out */
+int qm_rules_note(int *text_d, int ld, int *n_text_d, const int *tok_d, const int *pos_d, int n);
 
 /* tok[0 .. n) = the host's tokens (n <= QM_MAX_CHUNK) and *pos = pos0, both
  * passed as kernel arguments: the caller's buffer is read before the return */

@@ -174,9 +174,25 @@ __global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ld
     }
 }
 
+// a sequence's text after a step: the token that is fed next, at its position
+__global__ __launch_bounds__(NTH) void k_rules_note(int *__restrict__ text, int ld, int *__restrict__ n_text,
+                                                   const int *__restrict__ tok, const int *__restrict__ pos, int n) {
+    const int i = blockIdx.x * NTH + threadIdx.x;
+    if (i >= n || pos[i] < 0 || pos[i] >= ld) return;
+    text[(size_t)i * ld + pos[i]] = tok[i];
+    n_text[i] = pos[i] + 1;
+}
+
 // ---------------------------------------------------------------------------
-// launcher
+// launchers
 // ---------------------------------------------------------------------------
+extern "C" int qm_rules_note(int *text, int ld, int *n_text, const int *tok, const int *pos, int n) {
+    if (!text || !n_text || !tok || !pos || ld <= 0 || n <= 0) return QH_EINVAL;
+    if (!stream()) return QH_ESTATE;
+    hipLaunchKernelGGL(k_rules_note, dim3((n + NTH - 1) / NTH), dim3(NTH), 0, stream(), text, ld, n_text, tok, pos, n);
+    return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
+}
+
 extern "C" int qm_logits_rules(float *out, size_t ldo, const float *logits, size_t ld, int vocab, int n, const qm_rules_t *t) {
     if (!t || n < 0 || vocab < 1 || ldo < (size_t)vocab || ld < (size_t)vocab) return QH_EINVAL;
     if (n == 0) return QH_OK;

@@ -226,6 +226,38 @@ class Batch:
                                                scores.ctypes.data_as(F32P)), "qwen3_hip_batch_beam")
         return out, scores
 
+    def set_rules(self, seq, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None):
+        """Rules on sequence seq's tokens from its next choice on: penalties
+        for those of its text, biases {token: value} (or [(token, value), ...],
+        the last of a token's counting), and the tokens that are allowed: a bool
+        array of the vocabulary, or token numbers."""
+        pairs = list(bias.items() if isinstance(bias, dict) else bias or [])
+        tok, val = _i32([t for t, _ in pairs]), np.array([v for _, v in pairs], np.float32)
+        mask = None
+        if allowed is not None:
+            bits = np.asarray(allowed)
+            if bits.dtype != bool:
+                tokens = bits.astype(np.int64).reshape(-1)
+                if tokens.size and not (0 <= tokens.min() and tokens.max() < VOCAB):
+                    raise ValueError("allowed tokens lie outside the vocabulary")
+                bits = np.zeros(VOCAB, bool)
+                bits[tokens] = True
+            if bits.shape != (VOCAB,):
+                raise ValueError(f"a mask has {VOCAB} values")
+            mask = np.zeros((VOCAB + 31) // 32 * 4, np.uint8)
+            packed = np.packbits(bits, bitorder="little")
+            mask[:packed.size] = packed
+        r = runtime.BatchRules(repetition, presence, frequency, tok.size, tok.ctypes.data, val.ctypes.data,
+                               None if mask is None else mask.ctypes.data)
+        _rc(runtime.lib().qwen3_hip_batch_set_rules(self._h, seq, ctypes.byref(r)), "qwen3_hip_batch_set_rules")
+
+    def clear_rules(self, seq):
+        _rc(runtime.lib().qwen3_hip_batch_set_rules(self._h, seq, None), "qwen3_hip_batch_set_rules")
+
+    def set_int8_head(self, on):
+        """Decode steps' logits from 8-bit products of the last rows and the head."""
+        _rc(runtime.lib().qwen3_hip_batch_set_int8_head(self._h, 1 if on else 0), "qwen3_hip_batch_set_int8_head")
+
     def logits(self):
         out = np.empty((self.n_seq, VOCAB), dtype=np.float32)
         _rc(runtime.lib().qwen3_hip_batch_logits(self._h, out.ctypes.data_as(F32P)), "qwen3_hip_batch_logits")
@@ -244,10 +276,13 @@ def main(argv=None):
     """Greedy generation on a seeded random-init blob:
     python -m n550_qwen3_bringup_handover_amd.model [--seed S] [--prompt N] [--decode N]
                                                      [--repeat R] [--eager] [--tile]
-                                                     [--batch B [--kv fp32|e4m3|int8] [--beams W]]
+                                                     [--batch B [--kv fp32|e4m3|int8] [--int8-head]
+                                                                [--beams W | --repetition R --presence P]]
     With --batch B, B sequences with their own random prompts of --prompt
     tokens are decoded together (--repeat calls of --decode steps each), their
-    caches held as --kv says; with --beams W they are B / W beam searches."""
+    caches held as --kv says, their logits from 8-bit products with --int8-head,
+    repeated tokens penalised as --repetition and --presence say; with --beams W
+    they are B / W beam searches."""
     import argparse
     ap = argparse.ArgumentParser(description=main.__doc__)
     ap.add_argument("--seed", type=lambda v: int(v, 0), default=0x03550040)
@@ -262,9 +297,17 @@ def main(argv=None):
                     help="decode this many sequences together (each with its own random prompt)")
     ap.add_argument("--kv", choices=("fp32", *KV8_FORMATS), default="fp32", help="how a batch's caches are held")
     ap.add_argument("--beams", type=int, default=0, help="beams of each search of a batch")
+    ap.add_argument("--int8-head", action="store_true", help="a batch's logits from 8-bit products")
+    ap.add_argument("--repetition", type=float, default=1.0, help="what a batch's repeated tokens' logits are divided by")
+    ap.add_argument("--presence", type=float, default=0.0, help="what is taken from a batch's repeated tokens' logits")
     args = ap.parse_args(argv)
     if (args.beams or args.kv != "fp32") and not args.batch:
         ap.error("--kv and --beams are a batch's")
+    ruled = args.repetition != 1.0 or args.presence != 0.0
+    if (args.int8_head or ruled) and not args.batch:
+        ap.error("--int8-head, --repetition and --presence are a batch's")
+    if ruled and args.beams:
+        ap.error("searches take no rules")
     if args.beams < 0 or (args.beams and args.batch % args.beams):
         ap.error("--beams must divide --batch")
     blob = qw3m_random(args.seed, LAYOUT_TILE if args.tile else LAYOUT_ROW, threads=16)
@@ -293,6 +336,10 @@ def _main_batch(args, blob):
     with Model(blob, max_seq=ctx) as m, Batch(m, args.batch, ctx, args.kv) as b:
         del blob
         b.set_graph(not args.eager)
+        b.set_int8_head(args.int8_head)
+        if args.repetition != 1.0 or args.presence != 0.0:
+            for s in range(args.batch):
+                b.set_rules(s, args.repetition, args.presence)
         if args.beams:
             prompts = [rng.integers(0, VOCAB, args.prompt).astype(np.int32) for _ in range(args.batch // args.beams)]
             for r in range(args.repeat):

@@ -46,6 +46,12 @@ class Rules(ctypes.Structure):
 RULESP = ctypes.POINTER(Rules)
 
 
+class BatchRules(ctypes.Structure):
+    """qwen3_hip_batch_rules (include/qwen3_hip_model.h): what is asked of one sequence's tokens"""
+    _fields_ = [("repetition", ctypes.c_float), ("presence", ctypes.c_float), ("frequency", ctypes.c_float),
+                ("n_bias", ctypes.c_int), ("bias_token", VP), ("bias", VP), ("mask", VP)]
+
+
 class Qwen3HipError(RuntimeError):
     pass
 
@@ -136,6 +142,8 @@ _PROTOS = {
     "qwen3_hip_batch_prefill": (ctypes.c_int, [VP, ctypes.c_int, I32P, ctypes.c_int]),
     "qwen3_hip_batch_decode": (ctypes.c_int, [VP, ctypes.c_int, I32P]),
     "qwen3_hip_batch_beam": (ctypes.c_int, [VP, ctypes.c_int, I32P, I32P, ctypes.c_int, ctypes.c_int, I32P, F32P]),
+    "qwen3_hip_batch_set_rules": (ctypes.c_int, [VP, ctypes.c_int, ctypes.POINTER(BatchRules)]),
+    "qwen3_hip_batch_set_int8_head": (ctypes.c_int, [VP, ctypes.c_int]),
     "qwen3_hip_batch_logits": (ctypes.c_int, [VP, F32P]),
     "qwen3_hip_batch_set_graph": (ctypes.c_int, [VP, ctypes.c_int]),
     "qwen3_hip_batch_timing": (ctypes.c_int, [VP, ctypes.POINTER(ctypes.c_double)]),

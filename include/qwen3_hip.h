@@ -172,6 +172,9 @@ int qwen3_hip_gemm_int8_dev(void *c_d, size_t ldc, int bf16, const int8_t *a_d, 
 int qwen3_hip_gemm_int8_gate_up_silu_dev(void *h_d, size_t ldh, int bf16, const int8_t *x_d, size_t ldx,
                                          const float *x_scale_d, const int8_t *wg_d, const float *g_scale_d,
                                          const int8_t *wu_d, const float *u_scale_d, size_t ldw, int M, int K, int N);
+/* which kernel an 8-bit product of aligned codes and adjoining rows of C goes to
+ * ("narrow16", "tile64", ..., "any" for K = 0, "none" for what is refused) */
+const char *qwen3_hip_int8_plan(int M, int K, int N, int gated);
 /* qwen3_hip_gemm_dev that allocates nothing: no counterpart in the
  * reference ABI; for callers that cannot allocate device memory (code under
  * HIP graph capture, tight serving loops, harnesses that forbid hipMalloc).

@@ -173,6 +173,10 @@ def gemm_int8_gate_up_silu_dev(h_d, ldh, bf16, x_d, ldx, x_scale_d, wg_d, g_scal
           "qwen3_hip_gemm_int8_gate_up_silu_dev")
 
 
+def int8_plan(M, K, N, gated=False):
+    return runtime.lib().qwen3_hip_int8_plan(M, K, N, int(gated)).decode()
+
+
 def argmax_dev(out_d, v_d, n):
     check(runtime.lib().qwen3_hip_argmax_dev(VP(out_d), VP(v_d), n), "qwen3_hip_argmax_dev")
 

@@ -105,6 +105,7 @@ int qh_gemm_int8(void *c_d, size_t ldc, int bf16, const int8_t *a_d, size_t lda,
 int qh_gemm_int8_gate_up_silu(void *h_d, size_t ldh, int bf16, const int8_t *x_d, size_t ldx, const float *xs_d,
                               const int8_t *wg_d, const float *gs_d, const int8_t *wu_d, const float *us_d, size_t ldw,
                               int M, int K, int N);
+const char *qh_int8_plan(int M, int K, int N, int gated);
 /* tile-major [N/tn][K/tk][tn][tk] -> row-major [N][K] */
 int qh_tile_to_row(uint16_t *dst_d, const uint16_t *src_d, int N, int K,
                    int tile_n, int tile_k);

@@ -603,34 +603,44 @@ enum { I8_ANY_PLAN, I8_NARROW1, I8_NARROW2, I8_TILE64, I8_TILE64X128, I8_TILE128
 // 1024 7.8 and 9.7; with 512 blocks 64 x 1024 x 4096 5.3 and 4.9.  Rows are read
 // by every block, so blocks of 16 rows until 256 of them, then of 32.  Up to four
 // rows always: they are read once a block, 1 x 4096 x 20000 18.2 and 21.1 us.
-// Tiles: the least of an estimate, us = fixed + rounds of 256 * a tile's start and
-// end + stages * tiles a CU * a stage, fitted to 1,142 measurements (M 16 to
-// 4,096, N 512 to 20,000, K 512 to 4,096; it takes 1.3% longer than the best of
-// them on average).  A gated product has two weights' columns.
+// Tiles: the least of an estimate, us = fixed + rounds * tile + stages * (rounds *
+// stage + tiles / 256 * shared), rounds = tiles / 256 rounded up: what a CU does one
+// after the other, and what all of them share.  Fitted to 1,142 measurements (M 16
+// to 4,096, N 512 to 20,000, K 512 to 4,096), of whose best it takes 1.1% longer on
+// average.  A gated product has two weights' columns.
 static int i8_plan_of(const I8Args &p, bool gated) {
     if (!p.K || !aligned16(p.a) || !aligned16(p.b) || !aligned16(p.b2) || p.lda % 16 || p.ldb % 16 || p.lda > I8_MAX_NEAR ||
         p.ldb > I8_MAX_NEAR)
         return I8_ANY_PLAN;
-    if (p.ldc > I8_MAX_NEAR / 4) return p.M <= 65535 * 32 ? I8_NARROW2 : I8_ANY_PLAN;   // tiles' stores have 32-bit offsets
     const long cols = ((long)p.N + 15) / 16;
     if (p.M <= 4 || cols * ((p.M + 15l) / 16) <= (p.M <= 16 ? 512 : 256)) return I8_NARROW1;
     if (cols * ((p.M + 31l) / 32) <= 256) return I8_NARROW2;
-    static const struct { int plan, bm, bn; float fixed, tile, stage; } T[] = {
-        {I8_TILE64, 64, 64, 2.35f, 0.82f, 0.223f},      {I8_TILE64X128, 64, 128, 2.19f, 1.34f, 0.343f},
-        {I8_TILE128, 128, 128, 1.99f, 1.89f, 0.566f},   {I8_TILE192X256, 192, 256, 0.0f, 5.55f, 0.956f},
-        {I8_TILE256, 256, 256, 0.0f, 6.40f, 1.153f}};
+    if (p.ldc > I8_MAX_NEAR / 4) return p.M <= 65535 * 32 ? I8_NARROW2 : I8_ANY_PLAN;   // tiles' stores have 32-bit offsets
+    static const struct { int plan, bm, bn; float fixed, tile, stage, shared; } T[] = {
+        {I8_TILE64, 64, 64, 2.44f, 0.73f, 0.206f, 0.014f},      {I8_TILE64X128, 64, 128, 2.75f, 0.90f, 0.298f, 0.079f},
+        {I8_TILE128, 128, 128, 3.03f, 1.05f, 0.490f, 0.138f},   {I8_TILE192X256, 192, 256, 0.10f, 5.28f, 0.818f, 0.675f},
+        {I8_TILE256, 256, 256, 0.0f, 6.26f, 0.994f, 0.928f}};
     const double stages = (p.K + 127) / 128;
     double best = 1e30;
     int plan = I8_TILE64;
     for (const auto &t : T) {
         const double tiles = ceil(p.M / (double)t.bm) * ceil(p.N * (gated ? 2.0 : 1.0) / t.bn);
-        const double us = t.fixed + ceil(tiles / 256) * t.tile + stages * fmax(tiles / 256, 1.0) * t.stage;
+        const double rounds = ceil(tiles / 256);
+        const double us = t.fixed + rounds * t.tile + stages * (rounds * t.stage + tiles / 256 * t.shared);
         if (us < best) {
             best = us;
             plan = t.plan;
         }
     }
     return plan;
+}
+
+// the plan of codes that are aligned as the fast kernels want them
+extern "C" const char *qh_int8_plan(int M, int K, int N, int gated) {
+    static const char *const names[] = {"any", "narrow16", "narrow32", "tile64", "tile64x128", "tile128", "tile192x256", "tile256"};
+    if (M <= 0 || N <= 0 || K < 0 || K > I8_MAX_K) return "none";
+    const size_t ld = ((size_t)K + 15) / 16 * 16;
+    return names[i8_plan_of(I8Args{nullptr, (size_t)N, nullptr, ld, nullptr, nullptr, nullptr, ld, nullptr, nullptr, M, K, N}, gated)];
 }
 
 template <int MT, int W, bool GATED, bool CBF>

@@ -602,6 +602,8 @@ int qwen3_hip_gemm_int8_gate_up_silu_dev(void *h, size_t ldh, int bf16, const in
     return note(qh_gemm_int8_gate_up_silu(h, ldh, bf16, x, ldx, x_scale, wg, g_scale, wu, u_scale, ldw, M, K, N));
 }
 
+const char *qwen3_hip_int8_plan(int M, int K, int N, int gated) { return qh_int8_plan(M, K, N, gated); }
+
 int qwen3_hip_decode_set_dev(const uint16_t *const *w, const float *x0, float *out, int layers) {
     READY_OR_RETURN();
     return note(qh_decode_persist(w, x0, out, layers));

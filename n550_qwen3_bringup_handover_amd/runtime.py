@@ -96,6 +96,7 @@ _PROTOS = {
     "qwen3_hip_gemm_int8_gate_up_silu_dev": (ctypes.c_int, [VP, ctypes.c_size_t, ctypes.c_int, VP, ctypes.c_size_t, VP,
                                                             VP, VP, VP, VP, ctypes.c_size_t, ctypes.c_int, ctypes.c_int,
                                                             ctypes.c_int]),
+    "qwen3_hip_int8_plan": (ctypes.c_char_p, [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "qwen3_hip_decode_set_dev": (ctypes.c_int, [ctypes.POINTER(VP), VP, VP, ctypes.c_int]),
     "qwen3_hip_decode_set_supported": (ctypes.c_int, []),
     "qwen3_hip_decode_set_out_ld": (ctypes.c_int, []),

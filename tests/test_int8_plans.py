@@ -1,0 +1,47 @@
+"""Every kernel of the 8-bit products, gated and not, over lengths that end in the middle of a stage, a piece and a ring of
+stages, and over sizes that end in the middle of a tile.  Which kernel a size goes to is host logic, checked without a GPU."""
+import pytest
+
+from n550_qwen3_bringup_handover_amd import abi, runtime
+from tests.test_int8_gpu import Product
+
+# (kernel, gated, M, N): a size of the kernel at each length below, whose last tiles are not full
+SIZES = [("narrow16", 0, 3, 1001), ("narrow16", 1, 50, 333), ("narrow32", 0, 100, 1001), ("narrow32", 1, 70, 1203),
+         ("tile64", 0, 130, 4003), ("tile64", 1, 130, 2001), ("tile64x128", 0, 60, 20011), ("tile64x128", 1, 60, 10007),
+         ("tile128", 0, 1001, 4001), ("tile128", 1, 1001, 2003), ("tile192x256", 0, 1905, 5600), ("tile192x256", 1, 1905, 2800),
+         ("tile256", 0, 2030, 8101), ("tile256", 1, 2030, 4003)]
+# fewer stages than any ring, a ring, one more; ends behind 1, 16, 17, 127 codes of a stage
+LENGTHS = [129, 256, 384, 500, 511, 513, 528, 640, 1024, 1041]
+OTHERS = {"tile128", "tile192x256", "tile256", "tile64x128", "tile64", "narrow32", "narrow16"}
+
+
+@pytest.mark.parametrize("plan,gated,m,n", SIZES)
+def test_sizes_reach_their_kernels(plan, gated, m, n):
+    for k in LENGTHS:
+        assert abi.int8_plan(m, k, n, gated) == plan, k
+
+
+def test_plans_at_the_ends():
+    assert {s[0] for s in SIZES} == OTHERS
+    assert abi.int8_plan(5, 0, 5) == "any" and abi.int8_plan(0, 16, 5) == "none" and abi.int8_plan(5, 131072, 5) == "none"
+    assert abi.int8_plan(1, 1024, 151936) == "narrow16" and abi.int8_plan(64, 1024, 151936) == "tile64x128"
+    assert abi.int8_plan(4096, 4096, 8192) == "tile256" and abi.int8_plan(2 ** 31 - 1, 16, 1) in OTHERS
+    assert abi.int8_plan(1, 16, 2 ** 31 - 1) == "narrow16" and abi.int8_plan(5, 16, 2 ** 31 - 1) in OTHERS
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("plan,gated,m,n", SIZES)
+def test_kernels(plan, gated, m, n, bf16):
+    runtime.init()
+    for k in LENGTHS if m * n < 4e6 else LENGTHS[::3]:
+        Product(m, k, n, gated=bool(gated), bf16=bf16, ldc=n + 3, seed=k).run()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("plan,gated,m,n", SIZES)
+def test_short_lengths(plan, gated, m, n):
+    """K below one stage; whichever kernel it is then"""
+    runtime.init()
+    for k in (1, 15, 16, 33, 127, 128):
+        Product(m, k, min(n, 3000), gated=bool(gated), seed=k).run()

@@ -515,7 +515,10 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW / 4) void k_i8_tile(I8Args p, in
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // the tile's scales through LDS; stores behind M and N fall out of the buffer's range
+    // the tile's scales through LDS; stores behind M and N fall out of the buffer's range.
+    // They go through the L2 at once: kept there they are written back when the launch
+    // ends (2048 x 1024 x 4096 16.6 -> 14.0 us, 4096 x 1024 x 8192 44.6 -> 42.7; past the
+    // caches altogether 52)
     __syncthreads();
     float *sm = (float *)smem, *sn = sm + T::BM, *su = sn + BNO;
     for (int i = tid; i < T::BM; i += WAVE * T::NW) sm[i] = p.as[m0 + min(i, rows - 1)];
@@ -527,35 +530,43 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW / 4) void k_i8_tile(I8Args p, in
     constexpr int TNO = GATED ? T::TN / 2 : T::TN;
     const auto rc = buf_rsrc((char *)p.c + ((size_t)m0 * p.ldc + n0) * ES, ((size_t)(rows - 1) * p.ldc + cols) * ES);
     const int ldc = (int)p.ldc * ES;
+    // a row's columns one after another, so that its lines fill up at once
+    float s[TNO], s2[TNO];
+    unsigned at[TNO];
 #pragma unroll
     for (int j = 0; j < TNO; j++) {
         const int n = wn * (BNO / T::WN) + 32 * j + fr;
-        const float s = sn[n], s2 = GATED ? su[n] : 0.0f;
-        const unsigned at = (n < cols ? n * ES : BUF_OOB) + 4 * fh * ldc;
+        s[j] = sn[n];
+        s2[j] = GATED ? su[n] : 0.0f;
+        at[j] = (n < cols ? n * ES : BUF_OOB) + 4 * fh * ldc;
+    }
 #pragma unroll
-        for (int i = 0; i < T::TM; i++)
+    for (int i = 0; i < T::TM; i++)
 #pragma unroll
-            for (int e4 = 0; e4 < 4; e4++) {
-                const int m = wm * (T::BM / T::WM) + 32 * i + 8 * e4;
-                const f32x4 r = *(const f32x4 *)(sm + m + 4 * fh);
-                float y[4];
+        for (int e4 = 0; e4 < 4; e4++) {
+            const int m = wm * (T::BM / T::WM) + 32 * i + 8 * e4;
+            const f32x4 r = *(const f32x4 *)(sm + m + 4 * fh);
+            float y[TNO][4];
+#pragma unroll
+            for (int j = 0; j < TNO; j++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    y[e] = (float)acc[i][j][4 * e4 + e] * (r[e] * s);
-                    if constexpr (GATED) y[e] = i8_silu_mul<CBF>(y[e], (float)acc[i][j + TNO][4 * e4 + e] * (r[e] * s2));
+                    y[j][e] = (float)acc[i][j][4 * e4 + e] * (r[e] * s[j]);
+                    if constexpr (GATED) y[j][e] = i8_silu_mul<CBF>(y[j][e], (float)acc[i][j + TNO][4 * e4 + e] * (r[e] * s2[j]));
                 }
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const unsigned to = at + (m + e) * ldc;
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int j = 0; j < TNO; j++) {
+                    const unsigned to = at[j] + (m + e) * ldc;
                     if constexpr (CBF) {
-                        const uint32_t two = pack_bf16x2(y[e & ~1], y[e | 1]);
-                        __builtin_amdgcn_raw_buffer_store_b16((short)(e & 1 ? two >> 16 : two), rc, to, 0, 0);
+                        const uint32_t two = pack_bf16x2(y[j][e & ~1], y[j][e | 1]);
+                        __builtin_amdgcn_raw_buffer_store_b16((short)(e & 1 ? two >> 16 : two), rc, to, 0, AUX_SC1);
                     } else {
-                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y[e]), rc, to, 0, 0);
+                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y[j][e]), rc, to, 0, AUX_SC1);
                     }
                 }
-            }
-    }
+        }
 }
 
 // ---------------------------------------------------------------------------
@@ -596,7 +607,7 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
     return QH_OK;
 }
 
-enum { I8_ANY_PLAN, I8_NARROW1, I8_NARROW2, I8_TILE64, I8_TILE64X128, I8_TILE128, I8_TILE192X256, I8_TILE256 };
+enum { I8_ANY_PLAN, I8_NARROW1, I8_NARROW2, I8_TILE64, I8_TILE64X128, I8_TILE128, I8_TILE128_ALONE, I8_TILE192X256, I8_TILE256 };
 
 // Few blocks of 16 columns: as long as there is at most one on each of the 256
 // CUs (two of 16 rows), against tiles: 64 x 1024 x 1024 3.2 us and 4.8, 128 x 4096 x
@@ -605,9 +616,13 @@ enum { I8_ANY_PLAN, I8_NARROW1, I8_NARROW2, I8_TILE64, I8_TILE64X128, I8_TILE128
 // rows always: they are read once a block, 1 x 4096 x 20000 18.2 and 21.1 us.
 // Tiles: the least of an estimate, us = fixed + rounds * tile + stages * (rounds *
 // stage + tiles / 256 * shared), rounds = tiles / 256 rounded up: what a CU does one
-// after the other, and what all of them share.  Fitted to 1,142 measurements (M 16
-// to 4,096, N 512 to 20,000, K 512 to 4,096), of whose best it takes 1.1% longer on
-// average.  A gated product has two weights' columns.
+// after the other, and what all of them share.  Fitted to 1,497 measurements (M 16
+// to 4,096, N 512 to 20,000, K 512 to 4,096), of whose best it takes 0.3% longer on
+// average.  A gated product has two weights' columns.  128 x 128 tiles that have a
+// CU each take three places for stages instead of two: operands that are in no
+// cache 1000 x 4096 x 2816 30.2 -> 22.5 us (in a cache 23.1 and 20.6), 2048 x 1024 x
+// 2048 11.7 -> 10.8 (10.0 and 10.4); with two tiles a CU 2048 x 1024 x 4096 15.2 and
+// 18.7.
 static int i8_plan_of(const I8Args &p, bool gated) {
     if (!p.K || !aligned16(p.a) || !aligned16(p.b) || !aligned16(p.b2) || p.lda % 16 || p.ldb % 16 || p.lda > I8_MAX_NEAR ||
         p.ldb > I8_MAX_NEAR)
@@ -617,14 +632,15 @@ static int i8_plan_of(const I8Args &p, bool gated) {
     if (cols * ((p.M + 31l) / 32) <= 256) return I8_NARROW2;
     if (p.ldc > I8_MAX_NEAR / 4) return p.M <= 65535 * 32 ? I8_NARROW2 : I8_ANY_PLAN;   // tiles' stores have 32-bit offsets
     static const struct { int plan, bm, bn; float fixed, tile, stage, shared; } T[] = {
-        {I8_TILE64, 64, 64, 2.44f, 0.73f, 0.206f, 0.014f},      {I8_TILE64X128, 64, 128, 2.75f, 0.90f, 0.298f, 0.079f},
-        {I8_TILE128, 128, 128, 3.03f, 1.05f, 0.490f, 0.138f},   {I8_TILE192X256, 192, 256, 0.10f, 5.28f, 0.818f, 0.675f},
-        {I8_TILE256, 256, 256, 0.0f, 6.26f, 0.994f, 0.928f}};
+        {I8_TILE64, 64, 64, 2.41f, 0.67f, 0.201f, 0.012f},      {I8_TILE64X128, 64, 128, 2.59f, 0.79f, 0.300f, 0.062f},
+        {I8_TILE128, 128, 128, 0.72f, 1.88f, 0.345f, 0.190f},   {I8_TILE128_ALONE, 128, 128, 4.0f, 0.0f, 0.404f, 0.210f},
+        {I8_TILE192X256, 192, 256, 0.76f, 4.33f, 0.821f, 0.591f}, {I8_TILE256, 256, 256, 0.31f, 5.63f, 1.004f, 0.753f}};
     const double stages = (p.K + 127) / 128;
     double best = 1e30;
     int plan = I8_TILE64;
     for (const auto &t : T) {
         const double tiles = ceil(p.M / (double)t.bm) * ceil(p.N * (gated ? 2.0 : 1.0) / t.bn);
+        if (t.plan == (tiles > 256 ? I8_TILE128_ALONE : I8_TILE128)) continue;
         const double rounds = ceil(tiles / 256);
         const double us = t.fixed + rounds * t.tile + stages * (rounds * t.stage + tiles / 256 * t.shared);
         if (us < best) {
@@ -637,7 +653,8 @@ static int i8_plan_of(const I8Args &p, bool gated) {
 
 // the plan of codes that are aligned as the fast kernels want them
 extern "C" const char *qh_int8_plan(int M, int K, int N, int gated) {
-    static const char *const names[] = {"any", "narrow16", "narrow32", "tile64", "tile64x128", "tile128", "tile192x256", "tile256"};
+    static const char *const names[] = {"any", "narrow16", "narrow32", "tile64", "tile64x128", "tile128", "tile128-alone",
+                                        "tile192x256", "tile256"};
     if (M <= 0 || N <= 0 || K < 0 || K > I8_MAX_K) return "none";
     const size_t ld = ((size_t)K + 15) / 16 * 16;
     return names[i8_plan_of(I8Args{nullptr, (size_t)N, nullptr, ld, nullptr, nullptr, nullptr, ld, nullptr, nullptr, M, K, N}, gated)];
@@ -669,6 +686,7 @@ static int i8_launch(const I8Args &p) {
     case I8_TILE64: i8_tile<I8Tile<64, 64, 2, 2 - GATED, 4>, GATED, CBF>(p); break;
     case I8_TILE64X128: i8_tile<I8Tile<64, 128, 2, 2, 3>, GATED, CBF>(p); break;
     case I8_TILE128: i8_tile<I8Tile<128, 128, 2, 2, 2>, GATED, CBF>(p); break;
+    case I8_TILE128_ALONE: i8_tile<I8Tile<128, 128, 2, 2, 3>, GATED, CBF>(p); break;
     case I8_TILE192X256: i8_tile<I8Tile<192, 256, 2, 4, 2>, GATED, CBF>(p); break;
     case I8_TILE256: i8_tile<I8Tile<256, 256, 2, 4, 2>, GATED, CBF>(p); break;
     }

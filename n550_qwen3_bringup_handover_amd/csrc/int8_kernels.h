@@ -349,8 +349,10 @@ __global__ __launch_bounds__(WAVE *W) void k_i8_narrow(I8Args p) {
 // zeros 4.9).  64 x 64 tiles take in 16 KB a stage and are bound by that: 2048 x
 // 8192 x 1024 34.3 us, the copies alone 35.  Splitting a stage's codes over waves,
 // which halves what is read from LDS, and more stages in flight gained nothing.
-template <int BM_, int BN_, int WM_, int WN_, int ST_>
+// B_AUX: how B is read (2: past the caches)
+template <int BM_, int BN_, int WM_, int WN_, int ST_, int B_AUX_ = 0>
 struct I8Tile {
+    static constexpr int B_AUX = B_AUX_;
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = 128, ST = ST_;
     static constexpr int NW = WM * WN, CPR = BK / 16, RPI = 64 / CPR;    // pieces of a row; rows that a copy instruction fills
     static constexpr int TM = BM / WM / 32, TN = BN / WN / 32, KS = BK / 32;
@@ -364,9 +366,10 @@ __device__ __forceinline__ int i8_swz(int row) { return (row ^ (row >> 3 & 3)) &
 // 16 bytes a lane from byte at + k0 of a buffer to 1,024 of LDS.  (The host's pass
 // knows the builtin, but not the size, and would drop the kernels that use it.)
 typedef __attribute__((address_space(3))) void i8_lds;
+template <int AUX>
 __device__ __forceinline__ void i8_copy(__amdgpu_buffer_rsrc_t from, unsigned char *to, int at, int k0) {
 #ifdef __HIP_DEVICE_COMPILE__
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (i8_lds *)to, 16, at, k0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (i8_lds *)to, 16, at, k0, 0, AUX);
 #endif
 }
 // The compiler moves no LDS access across a barrier.
@@ -430,7 +433,7 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW / 4) void k_i8_tile(I8Args p, in
         for (int i = 0; i < T::A_DMA; i++) {
             unsigned char *to = slot + (wave * T::A_DMA + i) * 1024;
             if constexpr (decltype(WHOLE)::value) {
-                i8_copy(ra, to, va[i], k0);
+                i8_copy<0>(ra, to, va[i], k0);
             } else {
                 const int pc = piece(a_row(i)), at = a_at(i) + (pc < room ? pc : 0);
                 const i32x4 v = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(ra, at, k0, 0));
@@ -441,7 +444,7 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW / 4) void k_i8_tile(I8Args p, in
         for (int i = 0; i < T::B_DMA; i++) {
             const bool up = GATED && (wave * T::B_DMA + i) * T::RPI >= BNO;
             const int at = decltype(WHOLE)::value || piece(b_row(i)) < room ? vb[i] : b_at(i);
-            i8_copy(up ? rb2 : rb, slot + T::A_BYTES + (wave * T::B_DMA + i) * 1024, at, k0);
+            i8_copy<T::B_AUX>(up ? rb2 : rb, slot + T::A_BYTES + (wave * T::B_DMA + i) * 1024, at, k0);
         }
     };
     // this lane's first fragment of A and of B in each step of a stage; the others lie 32 rows on
@@ -607,7 +610,7 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
     return QH_OK;
 }
 
-enum { I8_ANY_PLAN, I8_NARROW1, I8_NARROW2, I8_TILE64, I8_TILE64X128, I8_TILE128, I8_TILE128_ALONE, I8_TILE192X256, I8_TILE256 };
+enum { I8_ANY_PLAN, I8_NARROW1, I8_NARROW2, I8_TILE64, I8_TILE64X128, I8_TILE64X128_ONCE, I8_TILE128, I8_TILE128_ALONE, I8_TILE192X256, I8_TILE256 };
 
 // Few blocks of 16 columns: as long as there is at most one on each of the 256
 // CUs (two of 16 rows), against tiles: 64 x 1024 x 1024 3.2 us and 4.8, 128 x 4096 x
@@ -623,6 +626,10 @@ enum { I8_ANY_PLAN, I8_NARROW1, I8_NARROW2, I8_TILE64, I8_TILE64X128, I8_TILE128
 // cache 1000 x 4096 x 2816 30.2 -> 22.5 us (in a cache 23.1 and 20.6), 2048 x 1024 x
 // 2048 11.7 -> 10.8 (10.0 and 10.4); with two tiles a CU 2048 x 1024 x 4096 15.2 and
 // 18.7.
+// Weights of 64 MB and more that every tile reads for itself are read past the
+// caches, which they would empty, on three blocks a CU: 64 x 1024 x 151936 38.2 ->
+// 35.8 us, 16 rows 33.4 -> 31.2 (the other way 32.0 and 35.4 where nothing else is
+// read between two calls, so that 155 MB stay in the last cache).
 static int i8_plan_of(const I8Args &p, bool gated) {
     if (!p.K || !aligned16(p.a) || !aligned16(p.b) || !aligned16(p.b2) || p.lda % 16 || p.ldb % 16 || p.lda > I8_MAX_NEAR ||
         p.ldb > I8_MAX_NEAR)
@@ -648,12 +655,13 @@ static int i8_plan_of(const I8Args &p, bool gated) {
             plan = t.plan;
         }
     }
+    if (plan == I8_TILE64X128 && p.M <= 64 && p.ldb * p.N * (gated ? 2 : 1) >= (size_t)64 << 20) plan = I8_TILE64X128_ONCE;
     return plan;
 }
 
 // the plan of codes that are aligned as the fast kernels want them
 extern "C" const char *qh_int8_plan(int M, int K, int N, int gated) {
-    static const char *const names[] = {"any", "narrow16", "narrow32", "tile64", "tile64x128", "tile128", "tile128-alone",
+    static const char *const names[] = {"any", "narrow16", "narrow32", "tile64", "tile64x128", "tile64x128-once", "tile128", "tile128-alone",
                                         "tile192x256", "tile256"};
     if (M <= 0 || N <= 0 || K < 0 || K > I8_MAX_K) return "none";
     const size_t ld = ((size_t)K + 15) / 16 * 16;
@@ -685,6 +693,7 @@ static int i8_launch(const I8Args &p) {
     case I8_NARROW2: i8_narrow<2, 8, GATED, CBF>(p); break;
     case I8_TILE64: i8_tile<I8Tile<64, 64, 2, 2 - GATED, 4>, GATED, CBF>(p); break;
     case I8_TILE64X128: i8_tile<I8Tile<64, 128, 2, 2, 3>, GATED, CBF>(p); break;
+    case I8_TILE64X128_ONCE: i8_tile<I8Tile<64, 128, 2, 2, 2, 2>, GATED, CBF>(p); break;
     case I8_TILE128: i8_tile<I8Tile<128, 128, 2, 2, 2>, GATED, CBF>(p); break;
     case I8_TILE128_ALONE: i8_tile<I8Tile<128, 128, 2, 2, 3>, GATED, CBF>(p); break;
     case I8_TILE192X256: i8_tile<I8Tile<192, 256, 2, 4, 2>, GATED, CBF>(p); break;

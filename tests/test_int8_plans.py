@@ -8,11 +8,12 @@ from tests.test_int8_gpu import Product
 # (kernel, gated, M, N): a size of the kernel at each length below, whose last tiles are not full
 SIZES = [("narrow16", 0, 3, 1001), ("narrow16", 1, 50, 333), ("narrow32", 0, 60, 2003), ("narrow32", 1, 60, 1400),
          ("tile64", 0, 60, 4010), ("tile64", 1, 60, 2150), ("tile64x128", 0, 130, 5603), ("tile64x128", 1, 130, 2801),
+         ("tile64x128-once", 0, 20, 530001), ("tile64x128-once", 1, 20, 265001),
          ("tile128-alone", 0, 700, 3301), ("tile128-alone", 1, 700, 1650), ("tile128", 0, 1001, 4301), ("tile128", 1, 1001, 2150),
          ("tile192x256", 0, 1300, 7003), ("tile192x256", 1, 1300, 3501), ("tile256", 0, 1905, 7001), ("tile256", 1, 1905, 3501)]
 # fewer stages than any ring, a ring, one more; ends behind 1, 16, 17, 127 codes of a stage
 LENGTHS = [129, 256, 384, 500, 511, 513, 528, 640, 1024, 1041]
-OTHERS = {"tile128", "tile128-alone", "tile192x256", "tile256", "tile64x128", "tile64", "narrow32", "narrow16"}
+OTHERS = {"tile64x128-once", "tile128", "tile128-alone", "tile192x256", "tile256", "tile64x128", "tile64", "narrow32", "narrow16"}
 
 
 @pytest.mark.parametrize("plan,gated,m,n", SIZES)
@@ -24,7 +25,7 @@ def test_sizes_reach_their_kernels(plan, gated, m, n):
 def test_plans_at_the_ends():
     assert {s[0] for s in SIZES} == OTHERS
     assert abi.int8_plan(5, 0, 5) == "any" and abi.int8_plan(0, 16, 5) == "none" and abi.int8_plan(5, 131072, 5) == "none"
-    assert abi.int8_plan(1, 1024, 151936) == "narrow16" and abi.int8_plan(64, 1024, 151936) == "tile64x128"
+    assert abi.int8_plan(1, 1024, 151936) == "narrow16" and abi.int8_plan(64, 1024, 151936) == "tile64x128-once"
     assert abi.int8_plan(4096, 4096, 8192) == "tile256" and abi.int8_plan(2 ** 31 - 1, 16, 1) in OTHERS
     assert abi.int8_plan(1, 16, 2 ** 31 - 1) == "narrow16" and abi.int8_plan(5, 16, 2 ** 31 - 1) in OTHERS
 
@@ -34,7 +35,7 @@ def test_plans_at_the_ends():
 @pytest.mark.parametrize("plan,gated,m,n", SIZES)
 def test_kernels(plan, gated, m, n, bf16):
     runtime.init()
-    for k in LENGTHS if m * n < 4e6 else LENGTHS[::3]:
+    for k in LENGTHS if m * n < 4e6 else LENGTHS[::4]:
         Product(m, k, n, gated=bool(gated), bf16=bf16, ldc=n + 3, seed=k).run()
 
 

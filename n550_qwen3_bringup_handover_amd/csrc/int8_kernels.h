@@ -40,19 +40,25 @@ __device__ __forceinline__ int i8_code(float x, float s, float y) {
     return (int)n;
 }
 
+template <bool ONCE, typename T>
+__device__ __forceinline__ T i8_get(const T *p) {         // ONCE: past the caches
+    return ONCE ? __builtin_nontemporal_load(p) : *p;
+}
+
 // eight values from x on, `left` of them there
-template <bool BF, bool VEC>
+template <bool BF, bool VEC, bool ONCE>
 __device__ __forceinline__ void i8_eight(float *v, const void *x, size_t i, int left) {
     if (VEC && left >= 8) {
         if constexpr (BF) {
-            const u32x4 w = *(const u32x4 *)((const uint16_t *)x + i);
+            const u32x4 w = i8_get<ONCE>((const u32x4 *)((const uint16_t *)x + i));
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 v[2 * j] = bf16_lo(w[j]);
                 v[2 * j + 1] = bf16_hi(w[j]);
             }
         } else {
-            const f32x4 lo = *(const f32x4 *)((const float *)x + i), hi = *(const f32x4 *)((const float *)x + i + 4);
+            const f32x4 lo = i8_get<ONCE>((const f32x4 *)((const float *)x + i));
+            const f32x4 hi = i8_get<ONCE>((const f32x4 *)((const float *)x + i + 4));
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 v[j] = lo[j];
@@ -68,12 +74,12 @@ __device__ __forceinline__ void i8_eight(float *v, const void *x, size_t i, int 
 
 // TPR threads a row, in turns of 8 values each.  The first KEEP turns' values stay
 // in registers between the maximum and the codes; a longer row's others are read
-// again.  Bound by memory: 65,536 x 1,024 fp32 60.8 us (5.5 TB/s), 4,096 x 4,096
-// 18.2; below some MB by the launch and two latencies: one row 2.9, 1,999 x 2,048
+// again.  Bound by memory: 65,536 x 1,024 fp32 57.4 us (5.8 TB/s; 60.9 through the
+// caches), 4,096 x 4,096 16.8 (18.3), bf16 12.8 (15.2); below some MB by the launch and two latencies: one row 2.9, 1,999 x 2,048
 // bf16 6.3.  As few threads a row as hold it in registers: 30,000 x 64 5.6 us on 16
 // threads and 13.8 on 64, 8,000 x 5,000 39 on 256 with four turns and 52 on 1,024;
 // four turns where two do (64 x 1,024) 3.7 and 3.2.
-template <bool BF, bool VEC, int TPR, int KEEP>
+template <bool BF, bool VEC, int TPR, int KEEP, bool ONCE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__restrict__ q, size_t ldq, float *__restrict__ scale,
                                                                    const void *__restrict__ x, size_t ldx, int K, int rows) {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
@@ -85,11 +91,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__r
 #pragma unroll
     for (int u = 0; u < KEEP; u++) {
         const int k = 8 * (t + u * TPR);
-        i8_eight<BF, VEC>(v[u], x, from + k, K - k);
+        i8_eight<BF, VEC, ONCE>(v[u], x, from + k, K - k);
     }
     for (int k = 8 * (t + KEEP * TPR); k < K; k += 8 * TPR) {
         float w[8];
-        i8_eight<BF, VEC>(w, x, from + k, K - k);
+        i8_eight<BF, VEC, ONCE>(w, x, from + k, K - k);
 #pragma unroll
         for (int j = 0; j < 8; j++) a = fmaxf(a, fabsf(i8_held(w[j])));
     }
@@ -125,7 +131,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__r
                 lo |= (uint32_t)(c[j] & 0xFF) << (8 * j);
                 hi |= (uint32_t)(c[4 + j] & 0xFF) << (8 * j);
             }
-            *(uint2 *)to = make_uint2(lo, hi);
+            const uint64_t w8 = lo | (uint64_t)hi << 32;
+            if constexpr (ONCE) __builtin_nontemporal_store(w8, (uint64_t *)to);
+            else *(uint64_t *)to = w8;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)
@@ -136,7 +144,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__r
     for (int u = 0; u < KEEP; u++) store(v[u], 8 * (t + u * TPR));
     for (int k = 8 * (t + KEEP * TPR); k < K; k += 8 * TPR) {
         float w[8];
-        i8_eight<BF, VEC>(w, x, from + k, K - k);
+        i8_eight<BF, VEC, ONCE>(w, x, from + k, K - k);
 #pragma unroll
         for (int j = 0; j < 8; j++) w[j] = i8_held(w[j]);
         store(w, k);
@@ -586,23 +594,27 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
     if (K > I8_MAX_K || ldq > I8_MAX_LD || ldx > I8_MAX_LD) return QH_ETOOBIG;
     if (!g_inited) return QH_ESTATE;
     const bool vec = aligned16(x) && ldx * (bf16 ? 2 : 4) % 16 == 0 && aligned(q, 8) && ldq % 8 == 0;
-#define ROWS_AS(BF, V, TPR, KEEP)                                                                            \
-    hipLaunchKernelGGL((k_rows_int8<BF, V, TPR, KEEP>), dim3((unsigned)(((size_t)rows * TPR + 255) / (TPR < 256 ? 256 : TPR))), \
+    // more than the L2s hold is read and written past them
+    const bool once = vec && (size_t)rows * K * (bf16 ? 2 : 4) >= (size_t)32 << 20;
+#define ROWS_AS(BF, V, TPR, KEEP, O)                                                                         \
+    hipLaunchKernelGGL((k_rows_int8<BF, V, TPR, KEEP, O>), dim3((unsigned)(((size_t)rows * TPR + 255) / (TPR < 256 ? 256 : TPR))), \
                        dim3(TPR < 256 ? 256 : TPR), 0, g_stream, q, ldq, scale, x, ldx, K, rows)
-#define ROWS(BF, V)                                        \
+#define ROWS(BF, V, O)                                     \
     do {                                                   \
-        if (K <= 256) ROWS_AS(BF, V, 16, 2);               \
-        else if (K <= 1024) ROWS_AS(BF, V, 64, 2);         \
-        else if (K <= 4096) ROWS_AS(BF, V, 256, 2);        \
-        else if (K <= 8192) ROWS_AS(BF, V, 256, 4);        \
-        else ROWS_AS(BF, V, 1024, 2);                      \
+        if (K <= 256) ROWS_AS(BF, V, 16, 2, O);            \
+        else if (K <= 1024) ROWS_AS(BF, V, 64, 2, O);      \
+        else if (K <= 4096) ROWS_AS(BF, V, 256, 2, O);     \
+        else if (K <= 8192) ROWS_AS(BF, V, 256, 4, O);     \
+        else ROWS_AS(BF, V, 1024, 2, O);                   \
     } while (0)
     if (bf16) {
-        if (vec) ROWS(true, true);
-        else ROWS(true, false);
+        if (once) ROWS(true, true, true);
+        else if (vec) ROWS(true, true, false);
+        else ROWS(true, false, false);
     } else {
-        if (vec) ROWS(false, true);
-        else ROWS(false, false);
+        if (once) ROWS(false, true, true);
+        else if (vec) ROWS(false, true, false);
+        else ROWS(false, false, false);
     }
 #undef ROWS
 #undef ROWS_AS

@@ -106,6 +106,31 @@ def test_rows_of_odd_values():
     assert q[2, 5] == 127 and q[2, 6] == -127 and (q[8] == -127).all() and (q[5] == 127).all()
 
 
+def test_bf16_rows_of_odd_values():
+    x = np.zeros((4, 200), F32)
+    x[0, :4] = [np.inf, -np.inf, np.nan, 3e38]
+    x[1] = np.nan
+    x[2, :3] = [1.0, np.nan, -2.0]
+    x[3] = io.bf16_value(np.array([1], np.uint16))[0]            # the smallest subnormal
+    q, s = quantise(x, True)
+    want_q, want_s = io.rows(x)
+    assert np.array_equal(s, want_s) and np.array_equal(q, want_q) and s[1] == s[3] == 0
+
+
+@pytest.mark.parametrize("rows,k,bf16", [(9000, 1001, False), (70000, 130, False), (2300, 4000, False), (1100, 8191, False),
+                                         (700, 13000, False), (17000, 1000, True), (4200, 4096, True)])
+def test_more_rows_than_the_caches_hold(rows, k, bf16):
+    """rows of other strides, too: those that are read past the caches, and those that are not aligned for it"""
+    print("rows", rows, k, bf16, flush=True)
+    x = np.random.default_rng(k).standard_normal((rows, k), dtype=F32)
+    if bf16:
+        x = io.bf16_value(io.bf16_bits(x))
+    want_q, want_s = io.rows(x)
+    for ldx in (-(-k // 8) * 8, k):
+        q, s = quantise(x, bf16, ldx, -(-k // 8) * 8 + 8)
+        assert np.array_equal(s, want_s) and np.array_equal(q, want_q)
+
+
 def test_no_rows_and_rows_of_nothing():
     abi.rows_int8_dev(None, 0, None, None, 0, False, 0, 0)
     sd = At(np.full(3, np.nan, F32))

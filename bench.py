@@ -658,9 +658,9 @@ DECODE_PROFILE = "decode_gemv_set_kernel_trace.txt"
 
 
 # the headers hip_gemm.hip includes (its kernel families)
-GEMM_KERNEL_HEADERS = ("gemm_common.h", "gemv_kernels.h", "tile_kernels.h", "misc_kernels.h", "small_m_kernels.h")
+GEMM_KERNEL_HEADERS = ("gemm_common.h", "gemv_kernels.h", "tile_kernels.h", "misc_kernels.h", "small_m_kernels.h", "int8_kernels.h")
 # the device headers of the model and persistent kernels
-MODEL_KERNEL_HEADERS = ("persist_common.h", "fp_pinned.h", "model_shim.h", "kv8_kernels.h", "beam_kernels.h")
+MODEL_KERNEL_HEADERS = ("persist_common.h", "fp_pinned.h", "model_shim.h", "kv8_kernels.h", "beam_kernels.h", "rules_kernels.h")
 
 
 def kernel_sources_digest():

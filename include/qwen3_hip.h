@@ -164,7 +164,8 @@ int qwen3_hip_rows_int8_dev(int8_t *q_d, size_t ldq, float *scale_d, const void 
  * 0.  Any addresses and strides; codes 16-byte aligned in rows of a multiple of
  * 16 bytes are read many times faster, and then all of a row's lda (ldb) bytes
  * may be read, the last row's too: what lies behind K does not matter.  c_d must
- * not overlap what the call reads. */
+ * not overlap what the call reads.  QWEN3_HIP_ETOOBIG where a launch would have
+ * 2^32 threads: from 2^27 columns with up to four rows, from 2^36 results. */
 int qwen3_hip_gemm_int8_dev(void *c_d, size_t ldc, int bf16, const int8_t *a_d, size_t lda, const float *a_scale_d,
                             const int8_t *b_d, size_t ldb, const float *b_scale_d, int M, int K, int N);
 /* h = silu(g) * u with g and u such products of the same rows x_d, in fp32 up to

@@ -597,8 +597,8 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
     // more than the L2s hold is read and written past them
     const bool once = vec && (size_t)rows * K * (bf16 ? 2 : 4) >= (size_t)32 << 20;
 #define ROWS_AS(BF, V, TPR, KEEP, O)                                                                         \
-    hipLaunchKernelGGL((k_rows_int8<BF, V, TPR, KEEP, O>), dim3((unsigned)(((size_t)rows * TPR + 255) / (TPR < 256 ? 256 : TPR))), \
-                       dim3(TPR < 256 ? 256 : TPR), 0, g_stream, q, ldq, scale, x, ldx, K, rows)
+    hipLaunchKernelGGL((k_rows_int8<BF, V, TPR, KEEP, O>), dim3((unsigned)(((size_t)some * TPR + 255) / (TPR < 256 ? 256 : TPR))), \
+                       dim3(TPR < 256 ? 256 : TPR), 0, g_stream, q, ldq, scale, x, ldx, K, some)
 #define ROWS(BF, V, O)                                     \
     do {                                                   \
         if (K <= 256) ROWS_AS(BF, V, 16, 2, O);            \
@@ -607,19 +607,26 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
         else if (K <= 8192) ROWS_AS(BF, V, 256, 4, O);     \
         else ROWS_AS(BF, V, 1024, 2, O);                   \
     } while (0)
-    if (bf16) {
-        if (once) ROWS(true, true, true);
-        else if (vec) ROWS(true, true, false);
-        else ROWS(true, false, false);
-    } else {
-        if (once) ROWS(false, true, true);
-        else if (vec) ROWS(false, true, false);
-        else ROWS(false, false, false);
+    // 2^31 threads a launch at most
+    for (int done = 0;;) {
+        const int some = rows - done < 1 << 21 ? rows - done : 1 << 21;
+        if (bf16) {
+            if (once) ROWS(true, true, true);
+            else if (vec) ROWS(true, true, false);
+            else ROWS(true, false, false);
+        } else {
+            if (once) ROWS(false, true, true);
+            else if (vec) ROWS(false, true, false);
+            else ROWS(false, false, false);
+        }
+        HCHECK(hipGetLastError(), QH_ELAUNCH);
+        if ((done += some) >= rows) return QH_OK;
+        q += (size_t)some * ldq;
+        scale += some;
+        x = (const char *)x + (size_t)some * ldx * (bf16 ? 2 : 4);
     }
 #undef ROWS
 #undef ROWS_AS
-    HCHECK(hipGetLastError(), QH_ELAUNCH);
-    return QH_OK;
 }
 
 enum { I8_ANY_PLAN, I8_NARROW1, I8_NARROW2, I8_TILE64, I8_TILE64X128, I8_TILE64X128_ONCE, I8_TILE128, I8_TILE128_ALONE, I8_TILE192X256, I8_TILE256 };
@@ -680,39 +687,47 @@ extern "C" const char *qh_int8_plan(int M, int K, int N, int gated) {
     return names[i8_plan_of(I8Args{nullptr, (size_t)N, nullptr, ld, nullptr, nullptr, nullptr, ld, nullptr, nullptr, M, K, N}, gated)];
 }
 
+// a launch has fewer than 2^32 threads along x
+#define I8_GO(KERNEL, X, Y, THREADS, ...)                                                     \
+    do {                                                                                      \
+        const unsigned long x_ = (X);                                                         \
+        if (x_ * (THREADS) >= 1ul << 32) return QH_ETOOBIG;                                   \
+        if (!g_inited) return QH_ESTATE;                                                      \
+        hipLaunchKernelGGL(KERNEL, dim3((unsigned)x_, Y), dim3(THREADS), 0, g_stream, __VA_ARGS__); \
+        HCHECK(hipGetLastError(), QH_ELAUNCH);                                                \
+        return QH_OK;                                                                         \
+    } while (0)
+
 template <int MT, int W, bool GATED, bool CBF>
-static void i8_narrow(const I8Args &p) {
-    hipLaunchKernelGGL((k_i8_narrow<MT, W, GATED, CBF>), dim3((p.N + 15l) / 16, (p.M + 16 * MT - 1l) / (16 * MT)),
-                       dim3(WAVE *W), 0, g_stream, p);
+static int i8_narrow(const I8Args &p) {
+    I8_GO((k_i8_narrow<MT, W, GATED, CBF>), (p.N + 15l) / 16, (unsigned)((p.M + 16 * MT - 1l) / (16 * MT)), WAVE *W, p);
 }
 template <typename T, bool GATED, bool CBF>
-static void i8_tile(const I8Args &p) {
+static int i8_tile(const I8Args &p) {
     const long bno = GATED ? T::BN / 2 : T::BN, mt = (p.M + T::BM - 1l) / T::BM, nt = (p.N + bno - 1) / bno;
-    const int per = (int)((mt * nt + 7) / 8);
-    hipLaunchKernelGGL((k_i8_tile<T, GATED, CBF>), dim3(8 * per), dim3(WAVE *T::NW), 0, g_stream, p, (int)mt, (int)nt, per);
+    const long per = (mt * nt + 7) / 8;
+    I8_GO((k_i8_tile<T, GATED, CBF>), 8 * per, 1, WAVE *T::NW, p, (int)mt, (int)nt, (int)per);
+}
+template <bool GATED, bool CBF>
+static int i8_any(const I8Args &p) {
+    const long mt = (p.M + I8_ANY - 1l) / I8_ANY, nt = (p.N + I8_ANY - 1l) / I8_ANY;
+    I8_GO((k_i8_any<GATED, CBF>), mt * nt, 1, NTHREADS, p, (unsigned)nt);
 }
 
 template <bool GATED, bool CBF>
 static int i8_launch(const I8Args &p) {
     switch (i8_plan_of(p, GATED)) {
-    case I8_ANY_PLAN: {
-        const long mt = (p.M + I8_ANY - 1l) / I8_ANY, nt = (p.N + I8_ANY - 1l) / I8_ANY;
-        if (mt * nt >= 1l << 31) return QH_ETOOBIG;
-        hipLaunchKernelGGL((k_i8_any<GATED, CBF>), dim3((unsigned)(mt * nt)), dim3(NTHREADS), 0, g_stream, p, (unsigned)nt);
-        break;
+    case I8_NARROW1: return i8_narrow<1, 8, GATED, CBF>(p);
+    case I8_NARROW2: return i8_narrow<2, 8, GATED, CBF>(p);
+    case I8_TILE64: return i8_tile<I8Tile<64, 64, 2, 2 - GATED, 4>, GATED, CBF>(p);
+    case I8_TILE64X128: return i8_tile<I8Tile<64, 128, 2, 2, 3>, GATED, CBF>(p);
+    case I8_TILE64X128_ONCE: return i8_tile<I8Tile<64, 128, 2, 2, 2, 2>, GATED, CBF>(p);
+    case I8_TILE128: return i8_tile<I8Tile<128, 128, 2, 2, 2>, GATED, CBF>(p);
+    case I8_TILE128_ALONE: return i8_tile<I8Tile<128, 128, 2, 2, 3>, GATED, CBF>(p);
+    case I8_TILE192X256: return i8_tile<I8Tile<192, 256, 2, 4, 2>, GATED, CBF>(p);
+    case I8_TILE256: return i8_tile<I8Tile<256, 256, 2, 4, 2>, GATED, CBF>(p);
+    default: return i8_any<GATED, CBF>(p);
     }
-    case I8_NARROW1: i8_narrow<1, 8, GATED, CBF>(p); break;
-    case I8_NARROW2: i8_narrow<2, 8, GATED, CBF>(p); break;
-    case I8_TILE64: i8_tile<I8Tile<64, 64, 2, 2 - GATED, 4>, GATED, CBF>(p); break;
-    case I8_TILE64X128: i8_tile<I8Tile<64, 128, 2, 2, 3>, GATED, CBF>(p); break;
-    case I8_TILE64X128_ONCE: i8_tile<I8Tile<64, 128, 2, 2, 2, 2>, GATED, CBF>(p); break;
-    case I8_TILE128: i8_tile<I8Tile<128, 128, 2, 2, 2>, GATED, CBF>(p); break;
-    case I8_TILE128_ALONE: i8_tile<I8Tile<128, 128, 2, 2, 3>, GATED, CBF>(p); break;
-    case I8_TILE192X256: i8_tile<I8Tile<192, 256, 2, 4, 2>, GATED, CBF>(p); break;
-    case I8_TILE256: i8_tile<I8Tile<256, 256, 2, 4, 2>, GATED, CBF>(p); break;
-    }
-    HCHECK(hipGetLastError(), QH_ELAUNCH);
-    return QH_OK;
 }
 
 static int i8_common(const I8Args &p, bool gated, int bf16) {
@@ -723,7 +738,6 @@ static int i8_common(const I8Args &p, bool gated, int bf16) {
     if (p.K > 0 && (!p.a || !p.b || (gated && !p.b2))) return QH_EINVAL;
     if (!aligned(p.c, bf16 ? 2 : 4) || !aligned(p.as, 4) || !aligned(p.bs, 4) || !aligned(p.bs2, 4)) return QH_EINVAL;
     if (p.K > I8_MAX_K || p.lda > I8_MAX_LD || p.ldb > I8_MAX_LD || p.ldc > I8_MAX_LD) return QH_ETOOBIG;
-    if (!g_inited) return QH_ESTATE;
     if (gated) return bf16 ? i8_launch<true, true>(p) : i8_launch<true, false>(p);
     return bf16 ? i8_launch<false, true>(p) : i8_launch<false, false>(p);
 }

@@ -58,6 +58,12 @@ def test_products_at_their_limits():
     long = dict(lda=1 << 17, ldb=1 << 17)
     assert product(k=131071, **long) == ESTATE and product(k=131072, **long) == ETOOBIG
     assert product(lda=(1 << 40) + 1) == ETOOBIG and product(ldc=(1 << 40) + 1) == ETOOBIG
+    # launches of 2^32 threads and more
+    most = 2 ** 31 - 1
+    assert product(m=1, n=1 << 27, ldc=1 << 27) == ETOOBIG and product(m=1, n=(1 << 27) - 16, ldc=1 << 27) == ESTATE
+    assert product(m=most, n=16) == ETOOBIG and product(m=most // 8, n=16) == ESTATE
+    assert product(m=most, n=most, ldc=most) == ETOOBIG and product(m=most, n=1 << 20, ldc=1 << 20, lda=65) == ETOOBIG
+    assert rows(rows=most) == ESTATE
 
 
 class Rules(ctypes.Structure):             # qm_rules_t has qwen3_hip_rules' fields in its order

@@ -40,25 +40,26 @@ __device__ __forceinline__ int i8_code(float x, float s, float y) {
     return (int)n;
 }
 
-template <bool ONCE, typename T>
-__device__ __forceinline__ T i8_get(const T *p) {         // ONCE: past the caches
-    return ONCE ? __builtin_nontemporal_load(p) : *p;
-}
-
-// eight values from x on, `left` of them there
-template <bool BF, bool VEC, bool ONCE>
+// eight values from x on, `left` of them there: 16 bytes a load, wherever they
+// begin.  ONCE: past the caches
+typedef unsigned int i8_u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float i8_f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint64_t i8_u64 __attribute__((aligned(1)));
+template <bool BF, bool ONCE>
 __device__ __forceinline__ void i8_eight(float *v, const void *x, size_t i, int left) {
-    if (VEC && left >= 8) {
+    if (left >= 8) {
         if constexpr (BF) {
-            const u32x4 w = i8_get<ONCE>((const u32x4 *)((const uint16_t *)x + i));
+            const i8_u32x4 *p = (const i8_u32x4 *)((const uint16_t *)x + i);
+            const u32x4 w = ONCE ? __builtin_nontemporal_load(p) : *p;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 v[2 * j] = bf16_lo(w[j]);
                 v[2 * j + 1] = bf16_hi(w[j]);
             }
         } else {
-            const f32x4 lo = i8_get<ONCE>((const f32x4 *)((const float *)x + i));
-            const f32x4 hi = i8_get<ONCE>((const f32x4 *)((const float *)x + i + 4));
+            const i8_f32x4 *p = (const i8_f32x4 *)((const float *)x + i);
+            const f32x4 lo = ONCE ? __builtin_nontemporal_load(p) : *p;
+            const f32x4 hi = ONCE ? __builtin_nontemporal_load(p + 1) : p[1];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 v[j] = lo[j];
@@ -79,7 +80,7 @@ __device__ __forceinline__ void i8_eight(float *v, const void *x, size_t i, int 
 // bf16 6.3.  As few threads a row as hold it in registers: 30,000 x 64 5.6 us on 16
 // threads and 13.8 on 64, 8,000 x 5,000 39 on 256 with four turns and 52 on 1,024;
 // four turns where two do (64 x 1,024) 3.7 and 3.2.
-template <bool BF, bool VEC, int TPR, int KEEP, bool ONCE>
+template <bool BF, int TPR, int KEEP, bool ONCE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__restrict__ q, size_t ldq, float *__restrict__ scale,
                                                                    const void *__restrict__ x, size_t ldx, int K, int rows) {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
@@ -91,11 +92,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__r
 #pragma unroll
     for (int u = 0; u < KEEP; u++) {
         const int k = 8 * (t + u * TPR);
-        i8_eight<BF, VEC, ONCE>(v[u], x, from + k, K - k);
+        i8_eight<BF, ONCE>(v[u], x, from + k, K - k);
     }
     for (int k = 8 * (t + KEEP * TPR); k < K; k += 8 * TPR) {
         float w[8];
-        i8_eight<BF, VEC, ONCE>(w, x, from + k, K - k);
+        i8_eight<BF, ONCE>(w, x, from + k, K - k);
 #pragma unroll
         for (int j = 0; j < 8; j++) a = fmaxf(a, fabsf(i8_held(w[j])));
     }
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__r
         int c[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) c[j] = s == 0.0f ? 0 : i8_code(w[j], s, y);
-        if (VEC && k + 8 <= K) {
+        if (k + 8 <= K) {
             uint32_t lo = 0, hi = 0;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -132,8 +133,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__r
                 hi |= (uint32_t)(c[4 + j] & 0xFF) << (8 * j);
             }
             const uint64_t w8 = lo | (uint64_t)hi << 32;
-            if constexpr (ONCE) __builtin_nontemporal_store(w8, (uint64_t *)to);
-            else *(uint64_t *)to = w8;
+            if constexpr (ONCE) __builtin_nontemporal_store(w8, (i8_u64 *)to);
+            else *(i8_u64 *)to = w8;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__r
     for (int u = 0; u < KEEP; u++) store(v[u], 8 * (t + u * TPR));
     for (int k = 8 * (t + KEEP * TPR); k < K; k += 8 * TPR) {
         float w[8];
-        i8_eight<BF, VEC, ONCE>(w, x, from + k, K - k);
+        i8_eight<BF, ONCE>(w, x, from + k, K - k);
 #pragma unroll
         for (int j = 0; j < 8; j++) w[j] = i8_held(w[j]);
         store(w, k);
@@ -164,6 +165,7 @@ struct I8Args {
     size_t ldb;
     const float *bs, *bs2;
     int M, K, N;
+    int whole;                         // pieces of 32 of a row of C are whole lines
 };
 
 template <bool CBF>
@@ -527,9 +529,10 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW / 4) void k_i8_tile(I8Args p, in
     }
 
     // the tile's scales through LDS; stores behind M and N fall out of the buffer's range.
-    // They go through the L2 at once: kept there they are written back when the launch
-    // ends (2048 x 1024 x 4096 16.6 -> 14.0 us, 4096 x 1024 x 8192 44.6 -> 42.7; past the
-    // caches altogether 52)
+    // Whole lines go through the L2 at once: kept there they are written back when the
+    // launch ends (2048 x 1024 x 4096 16.6 -> 14.0 us, 4096 x 1024 x 8192 44.6 -> 42.7;
+    // past the caches altogether 52).  Rows of C whose pieces of 32 are not whole lines
+    // are left to the L2, which joins them (597 x 413 x 100827 91 us, through it 136).
     __syncthreads();
     float *sm = (float *)smem, *sn = sm + T::BM, *su = sn + BNO;
     for (int i = tid; i < T::BM; i += WAVE * T::NW) sm[i] = p.as[m0 + min(i, rows - 1)];
@@ -551,33 +554,37 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW / 4) void k_i8_tile(I8Args p, in
         s2[j] = GATED ? su[n] : 0.0f;
         at[j] = (n < cols ? n * ES : BUF_OOB) + 4 * fh * ldc;
     }
+    auto finish = [&](auto AUX) {
 #pragma unroll
-    for (int i = 0; i < T::TM; i++)
+        for (int i = 0; i < T::TM; i++)
 #pragma unroll
-        for (int e4 = 0; e4 < 4; e4++) {
-            const int m = wm * (T::BM / T::WM) + 32 * i + 8 * e4;
-            const f32x4 r = *(const f32x4 *)(sm + m + 4 * fh);
-            float y[TNO][4];
+            for (int e4 = 0; e4 < 4; e4++) {
+                const int m = wm * (T::BM / T::WM) + 32 * i + 8 * e4;
+                const f32x4 r = *(const f32x4 *)(sm + m + 4 * fh);
+                float y[TNO][4];
 #pragma unroll
-            for (int j = 0; j < TNO; j++)
+                for (int j = 0; j < TNO; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    y[j][e] = (float)acc[i][j][4 * e4 + e] * (r[e] * s[j]);
-                    if constexpr (GATED) y[j][e] = i8_silu_mul<CBF>(y[j][e], (float)acc[i][j + TNO][4 * e4 + e] * (r[e] * s2[j]));
-                }
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-                for (int j = 0; j < TNO; j++) {
-                    const unsigned to = at[j] + (m + e) * ldc;
-                    if constexpr (CBF) {
-                        const uint32_t two = pack_bf16x2(y[j][e & ~1], y[j][e | 1]);
-                        __builtin_amdgcn_raw_buffer_store_b16((short)(e & 1 ? two >> 16 : two), rc, to, 0, AUX_SC1);
-                    } else {
-                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y[j][e]), rc, to, 0, AUX_SC1);
+                    for (int e = 0; e < 4; e++) {
+                        y[j][e] = (float)acc[i][j][4 * e4 + e] * (r[e] * s[j]);
+                        if constexpr (GATED) y[j][e] = i8_silu_mul<CBF>(y[j][e], (float)acc[i][j + TNO][4 * e4 + e] * (r[e] * s2[j]));
                     }
-                }
-        }
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int j = 0; j < TNO; j++) {
+                        const unsigned to = at[j] + (m + e) * ldc;
+                        if constexpr (CBF) {
+                            const uint32_t two = pack_bf16x2(y[j][e & ~1], y[j][e | 1]);
+                            __builtin_amdgcn_raw_buffer_store_b16((short)(e & 1 ? two >> 16 : two), rc, to, 0, decltype(AUX)::value);
+                        } else {
+                            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y[j][e]), rc, to, 0, decltype(AUX)::value);
+                        }
+                    }
+            }
+    };
+    if (p.whole) finish(IC<AUX_SC1>{});
+    else finish(IC<0>{});
 }
 
 // ---------------------------------------------------------------------------
@@ -593,31 +600,28 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
     if (!scale || !aligned(scale, 4) || (K > 0 && (!q || !x)) || !aligned(x, bf16 ? 2 : 4)) return QH_EINVAL;
     if (K > I8_MAX_K || ldq > I8_MAX_LD || ldx > I8_MAX_LD) return QH_ETOOBIG;
     if (!g_inited) return QH_ESTATE;
-    const bool vec = aligned16(x) && ldx * (bf16 ? 2 : 4) % 16 == 0 && aligned(q, 8) && ldq % 8 == 0;
     // more than the L2s hold is read and written past them
-    const bool once = vec && (size_t)rows * K * (bf16 ? 2 : 4) >= (size_t)32 << 20;
-#define ROWS_AS(BF, V, TPR, KEEP, O)                                                                         \
-    hipLaunchKernelGGL((k_rows_int8<BF, V, TPR, KEEP, O>), dim3((unsigned)(((size_t)some * TPR + 255) / (TPR < 256 ? 256 : TPR))), \
+    const bool once = (size_t)rows * K * (bf16 ? 2 : 4) >= (size_t)32 << 20;
+#define ROWS_AS(BF, TPR, KEEP, O)                                                                            \
+    hipLaunchKernelGGL((k_rows_int8<BF, TPR, KEEP, O>), dim3((unsigned)(((size_t)some * TPR + 255) / (TPR < 256 ? 256 : TPR))), \
                        dim3(TPR < 256 ? 256 : TPR), 0, g_stream, q, ldq, scale, x, ldx, K, some)
-#define ROWS(BF, V, O)                                     \
+#define ROWS(BF, O)                                        \
     do {                                                   \
-        if (K <= 256) ROWS_AS(BF, V, 16, 2, O);            \
-        else if (K <= 1024) ROWS_AS(BF, V, 64, 2, O);      \
-        else if (K <= 4096) ROWS_AS(BF, V, 256, 2, O);     \
-        else if (K <= 8192) ROWS_AS(BF, V, 256, 4, O);     \
-        else ROWS_AS(BF, V, 1024, 2, O);                   \
+        if (K <= 256) ROWS_AS(BF, 16, 2, O);            \
+        else if (K <= 1024) ROWS_AS(BF, 64, 2, O);      \
+        else if (K <= 4096) ROWS_AS(BF, 256, 2, O);     \
+        else if (K <= 8192) ROWS_AS(BF, 256, 4, O);     \
+        else ROWS_AS(BF, 1024, 2, O);                   \
     } while (0)
     // 2^31 threads a launch at most
     for (int done = 0;;) {
         const int some = rows - done < 1 << 21 ? rows - done : 1 << 21;
         if (bf16) {
-            if (once) ROWS(true, true, true);
-            else if (vec) ROWS(true, true, false);
-            else ROWS(true, false, false);
+            if (once) ROWS(true, true);
+            else ROWS(true, false);
         } else {
-            if (once) ROWS(false, true, true);
-            else if (vec) ROWS(false, true, false);
-            else ROWS(false, false, false);
+            if (once) ROWS(false, true);
+            else ROWS(false, false);
         }
         HCHECK(hipGetLastError(), QH_ELAUNCH);
         if ((done += some) >= rows) return QH_OK;
@@ -684,7 +688,7 @@ extern "C" const char *qh_int8_plan(int M, int K, int N, int gated) {
                                         "tile192x256", "tile256"};
     if (M <= 0 || N <= 0 || K < 0 || K > I8_MAX_K) return "none";
     const size_t ld = ((size_t)K + 15) / 16 * 16;
-    return names[i8_plan_of(I8Args{nullptr, (size_t)N, nullptr, ld, nullptr, nullptr, nullptr, ld, nullptr, nullptr, M, K, N}, gated)];
+    return names[i8_plan_of(I8Args{nullptr, (size_t)N, nullptr, ld, nullptr, nullptr, nullptr, ld, nullptr, nullptr, M, K, N, 0}, gated)];
 }
 
 // a launch has fewer than 2^32 threads along x
@@ -730,7 +734,7 @@ static int i8_launch(const I8Args &p) {
     }
 }
 
-static int i8_common(const I8Args &p, bool gated, int bf16) {
+static int i8_common(I8Args p, bool gated, int bf16) {
     if (p.M < 0 || p.N < 0 || p.K < 0) return QH_EINVAL;
     if (p.lda < (size_t)p.K || p.ldb < (size_t)p.K || p.ldc < (size_t)p.N) return QH_EINVAL;
     if (p.M == 0 || p.N == 0) return QH_OK;
@@ -738,19 +742,20 @@ static int i8_common(const I8Args &p, bool gated, int bf16) {
     if (p.K > 0 && (!p.a || !p.b || (gated && !p.b2))) return QH_EINVAL;
     if (!aligned(p.c, bf16 ? 2 : 4) || !aligned(p.as, 4) || !aligned(p.bs, 4) || !aligned(p.bs2, 4)) return QH_EINVAL;
     if (p.K > I8_MAX_K || p.lda > I8_MAX_LD || p.ldb > I8_MAX_LD || p.ldc > I8_MAX_LD) return QH_ETOOBIG;
+    p.whole = p.ldc % 32 == 0 && aligned(p.c, bf16 ? 64 : 128);
     if (gated) return bf16 ? i8_launch<true, true>(p) : i8_launch<true, false>(p);
     return bf16 ? i8_launch<false, true>(p) : i8_launch<false, false>(p);
 }
 
 extern "C" int qh_gemm_int8(void *c, size_t ldc, int bf16, const int8_t *a, size_t lda, const float *as, const int8_t *b,
                             size_t ldb, const float *bs, int M, int K, int N) {
-    return i8_common(I8Args{c, ldc, a, lda, as, b, nullptr, ldb, bs, nullptr, M, K, N}, false, bf16);
+    return i8_common(I8Args{c, ldc, a, lda, as, b, nullptr, ldb, bs, nullptr, M, K, N, 0}, false, bf16);
 }
 
 extern "C" int qh_gemm_int8_gate_up_silu(void *h, size_t ldh, int bf16, const int8_t *x, size_t ldx, const float *xs,
                                          const int8_t *wg, const float *gs, const int8_t *wu, const float *us, size_t ldw,
                                          int M, int K, int N) {
-    return i8_common(I8Args{h, ldh, x, ldx, xs, wg, wu, ldw, gs, us, M, K, N}, true, bf16);
+    return i8_common(I8Args{h, ldh, x, ldx, xs, wg, wu, ldw, gs, us, M, K, N, 0}, true, bf16);
 }
 
 #endif  // QH_INT8_KERNELS_H

@@ -30,23 +30,25 @@ __device__ __forceinline__ float rules_penalised(float x, uint32_t e, float r, f
     return x;
 }
 
-// four tokens from x on, `left` of them there.  ONCE: past the caches, for rows that
+// four tokens from x on, `left` of them there, wherever they begin.  ONCE: past the caches, for rows that
 // are copied (64 rows of 151,936 that are in no cache 23.9 -> 20.5 us, 128 of 32,000
 // 10.8 -> 7.8; in a cache the same)
-template <bool VEC, bool ONCE>
+typedef float rules_f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned int rules_u32x4 __attribute__((ext_vector_type(4), aligned(4)));
+template <bool ONCE>
 __device__ __forceinline__ f32x4 rules_load(const float *x, int left) {
-    if (VEC && left >= 4) return ONCE ? __builtin_nontemporal_load((const f32x4 *)x) : *(const f32x4 *)x;
+    if (left >= 4) return ONCE ? __builtin_nontemporal_load((const rules_f32x4 *)x) : *(const rules_f32x4 *)x;
     f32x4 v = {};
 #pragma unroll
     for (int e = 0; e < 4; e++)
         if (e < left) v[e] = x[e];
     return v;
 }
-template <bool VEC, bool ONCE>
+template <bool ONCE>
 __device__ __forceinline__ void rules_store(float *x, f32x4 v, int left) {
-    if (VEC && left >= 4) {
-        if constexpr (ONCE) __builtin_nontemporal_store(v, (f32x4 *)x);
-        else *(f32x4 *)x = v;
+    if (left >= 4) {
+        if constexpr (ONCE) __builtin_nontemporal_store((rules_f32x4)v, (rules_f32x4 *)x);
+        else *(rules_f32x4 *)x = v;
         return;
     }
 #pragma unroll
@@ -55,8 +57,11 @@ __device__ __forceinline__ void rules_store(float *x, f32x4 v, int left) {
 }
 
 // four tokens of the history from j on, below n
-__device__ __forceinline__ uint4 rules_tokens(const int *h, int j, int n, bool vec) {
-    if (vec && j + 4 <= n) return *(const uint4 *)(h + j);
+__device__ __forceinline__ uint4 rules_tokens(const int *h, int j, int n) {
+    if (j + 4 <= n) {
+        const rules_u32x4 v = *(const rules_u32x4 *)(h + j);
+        return make_uint4(v[0], v[1], v[2], v[3]);
+    }
     uint4 v = make_uint4(~0u, ~0u, ~0u, ~0u);
     if (j < n) v.x = h[j];
     if (j + 1 < n) v.y = h[j + 1];
@@ -69,9 +74,9 @@ __device__ __forceinline__ uint4 rules_tokens(const int *h, int j, int n, bool v
 // Every load that does not wait for another one goes out first: the logits, the
 // first tokens of the history (whose number is then not known yet), the row's
 // numbers.  The biases take the table's place once the penalties are done with it.
-template <bool VEC, bool INPLACE>
+template <bool INPLACE>
 __global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ldo, const float *in, size_t ldx, int vocab,
-                                                          qm_rules_t t, bool hvec) {
+                                                          qm_rules_t t) {
     constexpr int NT = RULES_NT;
     __shared__ __align__(16) uint32_t tab[RULES_PIECE];   // occurrences behind the prompt, RULES_SEEN; then 1 + a bias entry
     const int i = blockIdx.y, tid = threadIdx.x;
@@ -81,10 +86,10 @@ __global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ld
     f32x4 y[RULES_GROUPS];
     if constexpr (!INPLACE) {
 #pragma unroll
-        for (int u = 0; u < RULES_GROUPS; u++) y[u] = rules_load<VEC, !INPLACE>(x + 4 * (tid + u * NT), nv - 4 * (tid + u * NT));
+        for (int u = 0; u < RULES_GROUPS; u++) y[u] = rules_load<!INPLACE>(x + 4 * (tid + u * NT), nv - 4 * (tid + u * NT));
     }
     const int *h = t.token + (size_t)i * t.ld_token;
-    const uint4 early = rules_tokens(h, 4 * tid, t.token ? t.ld_token : 0, hvec);
+    const uint4 early = rules_tokens(h, 4 * tid, t.token ? t.ld_token : 0);
     int len = t.token ? t.n_token[i] : 0;
     if (len > t.ld_token) len = 0;
     const int prompt = t.n_prompt ? t.n_prompt[i] : 0;
@@ -123,7 +128,7 @@ __global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ld
     };
     count4(early, 4 * tid);
     for (int j = 4 * (tid + NT); j < len; j += 8 * NT) {
-        const uint4 one = rules_tokens(h, j, len, hvec), two = rules_tokens(h, j + 4 * NT, len, hvec);
+        const uint4 one = rules_tokens(h, j, len), two = rules_tokens(h, j + 4 * NT, len);
         count4(one, j);
         count4(two, j + 4 * NT);
     }
@@ -134,7 +139,7 @@ __global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ld
         const int g = tid + u * NT, left = nv - 4 * g;
         const uint4 e = ((const uint4 *)tab)[g];
         if ((e.x | e.y | e.z | e.w) == 0) continue;
-        if constexpr (INPLACE) y[u] = rules_load<VEC, !INPLACE>(x + 4 * g, left);
+        if constexpr (INPLACE) y[u] = rules_load<!INPLACE>(x + 4 * g, left);
         have |= 1u << u;
         const uint32_t ee[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
@@ -154,7 +159,7 @@ __global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ld
             const int g = tid + u * NT, left = nv - 4 * g;
             const uint4 e = ((const uint4 *)tab)[g];
             if ((e.x | e.y | e.z | e.w) == 0) continue;
-            if (INPLACE && !(have >> u & 1)) y[u] = rules_load<VEC, !INPLACE>(x + 4 * g, left);
+            if (INPLACE && !(have >> u & 1)) y[u] = rules_load<!INPLACE>(x + 4 * g, left);
             have |= 1u << u;
             const uint32_t ee[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
@@ -168,12 +173,12 @@ __global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ld
         if (left <= 0) continue;
         if constexpr (INPLACE) {
             if (!(have >> u & 1) && words[u] == 15) continue;
-            if (!(have >> u & 1) && words[u]) y[u] = rules_load<VEC, !INPLACE>(x + 4 * g, left);
+            if (!(have >> u & 1) && words[u]) y[u] = rules_load<!INPLACE>(x + 4 * g, left);
         }
 #pragma unroll
         for (int k = 0; k < 4; k++)
             if (!(words[u] >> k & 1)) y[u][k] = -INFINITY;
-        rules_store<VEC, !INPLACE>(o + 4 * g, y[u], left);
+        rules_store<!INPLACE>(o + 4 * g, y[u], left);
     }
 }
 
@@ -216,17 +221,9 @@ extern "C" int qm_logits_rules(float *out, size_t ldo, const float *logits, size
     if (t->mask_of && !t->mask) return QH_EINVAL;
     if (!stream()) return QH_ESTATE;
     const dim3 grid((vocab + RULES_PIECE - 1) / RULES_PIECE, n);
-    const bool vec = aligned16(out) && aligned16(logits) && ldo % 4 == 0 && ld % 4 == 0;
-    const bool hvec = t->token && aligned16(t->token) && t->ld_token % 4 == 0;
-#define RULES(V, I) \
-    hipLaunchKernelGGL((k_logits_rules<V, I>), grid, dim3(RULES_NT), 0, stream(), out, ldo, logits, ld, vocab, *t, hvec)
-    if (out == logits) {
-        if (vec) RULES(true, true);
-        else RULES(false, true);
-    } else {
-        if (vec) RULES(true, false);
-        else RULES(false, false);
-    }
-#undef RULES
+    if (out == logits)
+        hipLaunchKernelGGL(k_logits_rules<true>, grid, dim3(RULES_NT), 0, stream(), out, ldo, logits, ld, vocab, *t);
+    else
+        hipLaunchKernelGGL(k_logits_rules<false>, grid, dim3(RULES_NT), 0, stream(), out, ldo, logits, ld, vocab, *t);
     return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
 }

@@ -192,8 +192,8 @@ __device__ __forceinline__ float i8_silu_mul(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
-// Any K, strides and addresses: 64 x 64 outputs a block, 64 bytes of K a step
-// through LDS, read byte by byte, 4 x 4 outputs a thread by v_dot4.
+// Any strides and addresses: 64 x 64 outputs a block, 64 codes of K a step through
+// LDS, four a load wherever they begin, 4 x 4 outputs a thread by v_dot4.
 #define I8_ANY 64
 template <bool GATED, bool CBF>
 __global__ __launch_bounds__(NTHREADS) void k_i8_any(I8Args p, unsigned nt) {
@@ -201,9 +201,12 @@ __global__ __launch_bounds__(NTHREADS) void k_i8_any(I8Args p, unsigned nt) {
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const size_t m0 = (size_t)(blockIdx.x / nt) * I8_ANY, n0 = (size_t)(blockIdx.x % nt) * I8_ANY;
     auto four = [&](const int8_t *x, size_t ld, size_t row, int rows, int k) {
+        typedef int any_i32 __attribute__((aligned(1)));
+        if (row >= (size_t)rows) return 0;
+        if (k + 4 <= p.K) return *(const any_i32 *)(x + row * ld + k);
         int w = 0;
-        for (int j = 0; j < 4; j++)
-            if (row < (size_t)rows && k + j < p.K) w |= (int)(uint8_t)x[row * ld + k + j] << (8 * j);
+        for (int j = 0; j < 3; j++)
+            if (k + j < p.K) w |= (int)(uint8_t)x[row * ld + k + j] << (8 * j);
         return w;
     };
     int acc[GATED ? 2 : 1][4][4] = {};
@@ -264,6 +267,10 @@ __device__ __forceinline__ i32x4 i8_load(const int8_t *p) { return *(const i32x4
 // and gets rows 4 g + i (columns of C) of column r (a row of C).  Operands come
 // straight from memory, a wave's pieces of 128 bytes of each row.  Sums are
 // integers, so the waves' may be added in any order.
+// Bound by the launch, two latencies and the waves' exchange: 16 x 1024 x 4096 2.9
+// us (operands in no cache 3.6), 64 x 2048 x 1024 3.9, where an empty launch takes
+// 2.3; for one row by memory, 1 x 1024 x 151936 30.1 us (5.2 TB/s).  4 or 16 waves
+// are as fast at K = 1,024 to 8,192.
 template <int MT, int W, bool GATED, bool CBF>
 __global__ __launch_bounds__(WAVE *W) void k_i8_narrow(I8Args p) {
     constexpr int G = GATED ? 2 : 1;
@@ -353,7 +360,7 @@ __global__ __launch_bounds__(WAVE *W) void k_i8_narrow(I8Args p) {
 // place and the first fragments of stage kt + 1 be read while the matrix cores
 // still have work (4096 x 4096 x 8192 132 us with the barrier between stages, 124
 // so).
-// What bounds it: 4096 x 4096 x 8192, bf16 results, 124 us on 256 x 256 tiles, 2.2
+// What bounds it: 4096 x 4096 x 8192, bf16 results, 121 us on 256 x 256 tiles, 2.3
 // POP/s; without the copies 109, the copies alone 75 to 105.  The matrix cores
 // alone reach 3.3 POP/s on such data (the clock falls to two thirds under it; on
 // zeros 4.9).  64 x 64 tiles take in 16 KB a stage and are bound by that: 2048 x

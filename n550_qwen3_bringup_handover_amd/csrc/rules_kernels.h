@@ -12,6 +12,11 @@
 // which integer atomics fill in any order with the same result.  So there is
 // no bound on the history's length, no table of n x vocab counts in memory and
 // nothing to clear between calls.
+// Copied rows are bound by memory, 64 of 151,936 under penalties, biases and masks
+// 18.9 us (20.4 from no cache; a copy of as much 15.0); rows in place by the scans of
+// the histories, 64 behind 2,048 tokens 11.2, and one row by its chain of latencies,
+// 4.9.  Pieces of 4,096 on 256 threads scan them twice as often: behind 8,000
+// tokens 26.1 us against 22.7, in place 26.0 against 18.1.
 
 #define RULES_NT 512
 #define RULES_PIECE 8192

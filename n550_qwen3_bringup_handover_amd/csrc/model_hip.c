@@ -737,6 +737,7 @@ struct qwen3_hip_batch {
     int *h_out;                        /* host staging of out */
     int use_graph;
     int graph_id[3];                   /* the greedy step, the beams' forward, the step under rules; -1 until captured */
+    int ruled;                         /* a step under rules has run eagerly since the graphs went */
     int have_logits;
     int head8;                         /* the head's product in 8-bit integers */
     double t_decode_ms;
@@ -767,6 +768,7 @@ static void drop_graphs(qwen3_hip_batch *b) {
         if (b->graph_id[g] >= 0) (void)qh_graph_destroy(b->graph_id[g]);
         b->graph_id[g] = -1;
     }
+    b->ruled = 0;
 }
 
 static void detach_batches(qwen3_hip_model *m) {
@@ -1182,10 +1184,14 @@ static int batch_step(qwen3_hip_batch *b, int which) {
 
 /* step i of a call: with graphs on, a first step runs eagerly (any workspace
  * its GEMM plans need is allocated then, outside capture); later steps replay
- * the one captured step */
+ * the one captured step.  Steps under rules are called for one by one where a
+ * mask follows each: their first call's stays the only eager one */
 static int batch_run(qwen3_hip_batch *b, int i, int which) {
     int *id = &b->graph_id[which];
-    if (!b->use_graph || (*id < 0 && i == 0)) return batch_step(b, which);
+    if (!b->use_graph || (*id < 0 && i == 0 && !(which == 2 && b->ruled))) {
+        if (which == 2) b->ruled = 1;
+        return batch_step(b, which);
+    }
     if (*id < 0) {
         int rc = qh_capture_begin();
         if (rc) return rc;

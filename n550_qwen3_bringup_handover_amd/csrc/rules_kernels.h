@@ -7,20 +7,23 @@
 //   mask bit 0:                             y = -inf
 // each step rounded to fp32, without fused multiply-adds.
 //
-// A block takes RULES_PIECE tokens of a row and reads the row's whole history
-// for those that lie there: a count and a "seen" bit for each token in LDS,
-// which integer atomics fill in any order with the same result.  So there is
-// no bound on the history's length, no table of n x vocab counts in memory and
-// nothing to clear between calls.
-// Copied rows are bound by memory, 64 of 151,936 under penalties, biases and masks
-// 18.9 us (20.4 from no cache; a copy of as much 15.0); rows in place by the scans of
-// the histories, 64 behind 2,048 tokens 11.2, and one row by its chain of latencies,
-// 4.9.  Pieces of 4,096 on 256 threads scan them twice as often: behind 8,000
-// tokens 26.1 us against 22.7, in place 26.0 against 18.1.
+// A block takes PIECE tokens of a row and reads the row's whole history for
+// those that lie there: a count and a "seen" bit for each token in LDS, which
+// integer atomics fill in any order with the same result.  So there is no bound
+// on the history's length, no table of n x vocab counts in memory and nothing to
+// clear between calls.
+// Many copied rows are bound by memory, 64 of 151,936 under penalties, biases and
+// masks 18.9 us (20.4 from no cache; a copy of as much 15.0); many in place by the
+// scans of the histories, 64 behind 2,048 tokens 11.3; few by a block's chain of
+// latencies, which is shorter the fewer tokens a thread has: one row behind 700
+// tokens 3.3 us in pieces of 2,048, 3.8 of 4,096 and 4.9 of 8,192, in place 3.5, 4.3
+// and 6.1; 16 rows 5.9, 5.6 and 6.5.  Small pieces scan the histories more often, and
+// more of them than the CUs hold at once (four on each) take turns: 34 rows 10.0 us
+// in pieces of 4,096 and 8.6 of 8,192, 24 behind 8,000 tokens 10.8 in pieces of 2,048
+// and 8.1 of 4,096.
 
 #define RULES_NT 512
-#define RULES_PIECE 8192
-#define RULES_GROUPS (RULES_PIECE / 4 / RULES_NT)  // of four tokens a thread: tid, tid + NT, ...
+#define RULES_AT_ONCE 1024
 #define RULES_SEEN 0x80000000u
 
 // e: a token's word of the table
@@ -79,19 +82,19 @@ __device__ __forceinline__ uint4 rules_tokens(const int *h, int j, int n) {
 // Every load that does not wait for another one goes out first: the logits, the
 // first tokens of the history (whose number is then not known yet), the row's
 // numbers.  The biases take the table's place once the penalties are done with it.
-template <bool INPLACE>
+template <bool INPLACE, int PIECE>
 __global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ldo, const float *in, size_t ldx, int vocab,
                                                           qm_rules_t t) {
-    constexpr int NT = RULES_NT;
-    __shared__ __align__(16) uint32_t tab[RULES_PIECE];   // occurrences behind the prompt, RULES_SEEN; then 1 + a bias entry
+    constexpr int NT = RULES_NT, GROUPS = PIECE / 4 / NT;    // of four tokens a thread: tid, tid + NT, ...
+    __shared__ __align__(16) uint32_t tab[PIECE];   // occurrences behind the prompt, RULES_SEEN; then 1 + a bias entry
     const int i = blockIdx.y, tid = threadIdx.x;
-    const int v0 = blockIdx.x * RULES_PIECE, nv = min(vocab - v0, RULES_PIECE);
+    const int v0 = blockIdx.x * PIECE, nv = min(vocab - v0, PIECE);
     const float *x = in + (size_t)i * ldx + v0;
     float *o = out + (size_t)i * ldo + v0;
-    f32x4 y[RULES_GROUPS];
+    f32x4 y[GROUPS];
     if constexpr (!INPLACE) {
 #pragma unroll
-        for (int u = 0; u < RULES_GROUPS; u++) y[u] = rules_load<!INPLACE>(x + 4 * (tid + u * NT), nv - 4 * (tid + u * NT));
+        for (int u = 0; u < GROUPS; u++) y[u] = rules_load<!INPLACE>(x + 4 * (tid + u * NT), nv - 4 * (tid + u * NT));
     }
     const int *h = t.token + (size_t)i * t.ld_token;
     const uint4 early = rules_tokens(h, 4 * tid, t.token ? t.ld_token : 0);
@@ -111,12 +114,12 @@ __global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ld
 
     auto clear = [&] {
 #pragma unroll
-        for (int u = 0; u < RULES_GROUPS; u++) ((uint4 *)tab)[tid + u * NT] = make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < GROUPS; u++) ((uint4 *)tab)[tid + u * NT] = make_uint4(0, 0, 0, 0);
     };
     clear();
-    uint32_t words[RULES_GROUPS];
+    uint32_t words[GROUPS];
 #pragma unroll
-    for (int u = 0; u < RULES_GROUPS; u++)
+    for (int u = 0; u < GROUPS; u++)
         words[u] = mask && 4 * (tid + u * NT) < nv ? mask[(tid + u * NT) / 8] >> (tid % 8 * 4) & 15 : 15;
     __syncthreads();
     auto count = [&](uint32_t token, int j) {
@@ -140,7 +143,7 @@ __global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ld
     __syncthreads();
     uint32_t have = 0;                                    // groups whose values are in y
 #pragma unroll
-    for (int u = 0; u < RULES_GROUPS; u++) {
+    for (int u = 0; u < GROUPS; u++) {
         const int g = tid + u * NT, left = nv - 4 * g;
         const uint4 e = ((const uint4 *)tab)[g];
         if ((e.x | e.y | e.z | e.w) == 0) continue;
@@ -160,7 +163,7 @@ __global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ld
         }
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < RULES_GROUPS; u++) {
+        for (int u = 0; u < GROUPS; u++) {
             const int g = tid + u * NT, left = nv - 4 * g;
             const uint4 e = ((const uint4 *)tab)[g];
             if ((e.x | e.y | e.z | e.w) == 0) continue;
@@ -173,7 +176,7 @@ __global__ __launch_bounds__(RULES_NT) void k_logits_rules(float *out, size_t ld
         }
     }
 #pragma unroll
-    for (int u = 0; u < RULES_GROUPS; u++) {
+    for (int u = 0; u < GROUPS; u++) {
         const int g = tid + u * NT, left = nv - 4 * g;
         if (left <= 0) continue;
         if constexpr (INPLACE) {
@@ -225,10 +228,20 @@ extern "C" int qm_logits_rules(float *out, size_t ldo, const float *logits, size
     if (t->mask && !t->mask_of && t->n_mask < n) return QH_EINVAL;
     if (t->mask_of && !t->mask) return QH_EINVAL;
     if (!stream()) return QH_ESTATE;
-    const dim3 grid((vocab + RULES_PIECE - 1) / RULES_PIECE, n);
-    if (out == logits)
-        hipLaunchKernelGGL(k_logits_rules<true>, grid, dim3(RULES_NT), 0, stream(), out, ldo, logits, ld, vocab, *t);
-    else
-        hipLaunchKernelGGL(k_logits_rules<false>, grid, dim3(RULES_NT), 0, stream(), out, ldo, logits, ld, vocab, *t);
+    // the smallest piece that takes a row, or whose blocks all run at once
+    auto fits = [&](int piece) { return vocab <= piece || (size_t)((vocab + piece - 1) / piece) * n <= RULES_AT_ONCE; };
+#define RULES(INPLACE, PIECE)                                                                                     \
+    hipLaunchKernelGGL((k_logits_rules<INPLACE, PIECE>), dim3((vocab + PIECE - 1) / PIECE, n), dim3(RULES_NT), 0, \
+                       stream(), out, ldo, logits, ld, vocab, *t)
+#define RULES_OF(PIECE)                         \
+    do {                                        \
+        if (out == logits) RULES(true, PIECE);  \
+        else RULES(false, PIECE);               \
+    } while (0)
+    if (fits(2048)) RULES_OF(2048);
+    else if (fits(4096)) RULES_OF(4096);
+    else RULES_OF(8192);
+#undef RULES_OF
+#undef RULES
     return hipGetLastError() == hipSuccess ? QH_OK : QH_ELAUNCH;
 }

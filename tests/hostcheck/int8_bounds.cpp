@@ -203,6 +203,15 @@ template <bool G, bool CB> static void products() {
 #undef TILE
 }
 
+// PIECE: of a row, for those that the launcher keeps for many rows; 0: its choice
+template <int PIECE>
+static void rules_launch(float *o, size_t ld, const float *x, int vocab, int n, const qm_rules_t &t) {
+    const dim3 grid((vocab + PIECE - 1) / PIECE, n);
+    if (o == x) hipLaunchKernelGGL((k_logits_rules<true, PIECE>), grid, dim3(RULES_NT), 0, stream(), o, ld, x, ld, vocab, t);
+    else hipLaunchKernelGGL((k_logits_rules<false, PIECE>), grid, dim3(RULES_NT), 0, stream(), o, ld, x, ld, vocab, t);
+}
+
+template <int PIECE = 0>
 static void rules_case(int n, int vocab, int pad, int history, int shift, bool masks, bool in_place) {
     printf("rules %d x %d + %d, %d tokens + %d, %d %d\n", n, vocab, pad, history, shift, masks, in_place);
     const size_t ld = vocab + pad, words = (vocab + 31) / 32;
@@ -245,7 +254,8 @@ static void rules_case(int n, int vocab, int pad, int history, int shift, bool m
         }
     const qm_rules_t t = {tok, history, from, len, pen, pen + n, pen + 2 * n, row, btok, bias, 3 * n,
                           masks ? mask : nullptr, words, masks ? n : 0, masks ? of : nullptr};
-    want(qm_logits_rules(o, ld, x, ld, vocab, n, &t) == QH_OK, "refused");
+    if constexpr (PIECE > 0) rules_launch<PIECE>(o, ld, x, vocab, n, t);
+    else want(qm_logits_rules(o, ld, x, ld, vocab, n, &t) == QH_OK, "refused");
     for (int i = 0; i < n; i++)
         for (size_t v = 0; v < (i + 1 < n ? ld : vocab); v++)
             want(o[i * ld + v] == (v < (size_t)vocab ? y[i * (size_t)vocab + v] : mark), "a logit");
@@ -278,6 +288,9 @@ int main(int argc, char **argv) {
                 rules_case(5, 8190, 2, 70, 0, masks, in_place);
                 rules_case(2, 8193, 3, 2600, 0, masks, in_place);
                 rules_case(1, 9000, 0, 5003, 0, masks, in_place);
+                rules_case<4096>(3, 4099, 1, 4100, 0, masks, in_place);
+                rules_case<8192>(3, 8190, 2, 70, 0, masks, in_place);
+                rules_case<8192>(2, 8195, 3, 2600, 0, masks, in_place);
             }
         break;
     }

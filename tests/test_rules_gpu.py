@@ -90,7 +90,12 @@ CASES = [(1, 1, dict(history=1)), (1, 31, dict(masks=1)), (2, 33, dict(history=5
          (2, 8192, dict(history=9000, biases=500, masks=2)), (3, 12001, dict(history=70, prompt=False)),
          (1, 151936, dict(history=700, biases=10)), (64, 151936, dict(history=600, biases=30, masks=8, allowed=0.3)),
          (9, 151936, dict(masks=9, allowed=0.001, mask_of=False)), (128, 2000, dict(history=200, masks=5, allowed=0.99)),
-         (2, 300001, dict(history=20000, biases=7)), (3, 500, dict())]
+         (2, 300001, dict(history=20000, biases=7)), (3, 500, dict()),
+         # a row in one piece of each size, and in more: what the blocks of many rows change
+         (16, 151936, dict(history=2000, biases=40, masks=3)), (1500, 2048, dict(history=50, masks=2)),
+         (400, 4095, dict(history=300, biases=9, masks=4)), (400, 4097, dict(history=300, biases=9, masks=4)),
+         (350, 8191, dict(history=300, biases=9, masks=4)), (350, 8193, dict(history=300, biases=9, masks=4)),
+         (1024, 2049, dict(history=20, masks=1)), (27, 151936, dict(history=5000))]
 
 
 @pytest.mark.parametrize("in_place", [False, True])

@@ -76,10 +76,13 @@ __device__ __forceinline__ void i8_eight(float *v, const void *x, size_t i, int 
 // TPR threads a row, in turns of 8 values each.  The first KEEP turns' values stay
 // in registers between the maximum and the codes; a longer row's others are read
 // again.  Bound by memory: 65,536 x 1,024 fp32 57.4 us (5.8 TB/s; 60.9 through the
-// caches), 4,096 x 4,096 16.8 (18.3), bf16 12.8 (15.2); below some MB by the launch and two latencies: one row 2.9, 1,999 x 2,048
-// bf16 6.3.  As few threads a row as hold it in registers: 30,000 x 64 5.6 us on 16
-// threads and 13.8 on 64, 8,000 x 5,000 39 on 256 with four turns and 52 on 1,024;
-// four turns where two do (64 x 1,024) 3.7 and 3.2.
+// caches), 4,096 x 4,096 16.8 (18.3), bf16 12.8 (15.2); below some MB by the launch
+// and two latencies: one row 2.4, 1,999 x 2,048 bf16 6.3.  Many rows: as few threads
+// a row as hold it in registers, 30,000 x 64 5.6 us on 16 threads and 13.8 on 64, 30,000
+// x 1,500 bf16 36 on 64 with four turns and 60 on 256, 8,000 x 5,000 39 on 256 and 52
+// on 1,024.  Few: one turn a thread, a shorter chain, 64 x 1,024 bf16 2.8 us on 256
+// threads and 3.3 on 64 (2,000 rows 4.9 and 3.9), 64 x 256 2.7 on 64 and 3.2 on 16, 64 x
+// 8,192 4.1 on 1,024 and 4.9 on 256 (1,024 rows 9.9 and 7.2).
 template <bool BF, int TPR, int KEEP, bool ONCE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rows_int8(int8_t *__restrict__ q, size_t ldq, float *__restrict__ scale,
                                                                    const void *__restrict__ x, size_t ldx, int K, int rows) {
@@ -607,6 +610,7 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
     if (!scale || !aligned(scale, 4) || (K > 0 && (!q || !x)) || !aligned(x, bf16 ? 2 : 4)) return QH_EINVAL;
     if (K > I8_MAX_K || ldq > I8_MAX_LD || ldx > I8_MAX_LD) return QH_ETOOBIG;
     if (!g_inited) return QH_ESTATE;
+    const bool few = rows <= 1024;
     // more than the L2s hold is read and written past them
     const bool once = (size_t)rows * K * (bf16 ? 2 : 4) >= (size_t)32 << 20;
 #define ROWS_AS(BF, TPR, KEEP, O)                                                                            \
@@ -614,9 +618,13 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
                        dim3(TPR < 256 ? 256 : TPR), 0, g_stream, q, ldq, scale, x, ldx, K, some)
 #define ROWS(BF, O)                                        \
     do {                                                   \
-        if (K <= 256) ROWS_AS(BF, 16, 2, O);            \
-        else if (K <= 1024) ROWS_AS(BF, 64, 2, O);      \
+        if (K <= 256 && !few) ROWS_AS(BF, 16, 2, O);    \
+        else if (K <= 512) ROWS_AS(BF, 64, 1, O);       \
+        else if (K <= 1024 && !few) ROWS_AS(BF, 64, 2, O); \
+        else if (K <= 2048 && few) ROWS_AS(BF, 256, 1, O); \
+        else if (K <= 2048 && rows >= 4096) ROWS_AS(BF, 64, 4, O); \
         else if (K <= 4096) ROWS_AS(BF, 256, 2, O);     \
+        else if (K <= 8192 && rows <= 256) ROWS_AS(BF, 1024, 1, O); \
         else if (K <= 8192) ROWS_AS(BF, 256, 4, O);     \
         else ROWS_AS(BF, 1024, 2, O);                   \
     } while (0)

@@ -275,6 +275,8 @@ int main(int argc, char **argv) {
                     rows_case(rows, K, bf, K + 1, K);
                 }
         rows_case(2100, 4000, false, 4000, 4000);         // past the caches
+        for (auto [rows, K] : {std::pair{1030, 200}, {1030, 1001}, {1030, 2047}, {4100, 1500}, {260, 8190}})
+            rows_case(rows, K, rows & 2, K, K);           // enough rows for other kernels
         break;
     case 1: products<false, false>(); break;
     case 2: products<true, false>(); break;

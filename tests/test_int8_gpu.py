@@ -49,7 +49,8 @@ def quantise(x, bf16=False, ldx=None, ldq=None, shift_x=0, shift_q=0):
 
 
 ROWS = [(1, 1024), (3, 1), (1, 5), (7, 64), (5, 100), (2, 255), (9, 1001), (64, 2048), (2, 4096), (3, 5000), (2, 8192), (1, 12289),
-        (2, 20000), (1, 131071), (1500, 640)]
+        (2, 20000), (1, 131071), (1500, 640), (1025, 256), (1030, 77), (4, 512), (1026, 1024), (1027, 2048), (4096, 1025), (4097, 2047),
+        (256, 8192), (257, 8191), (300, 4097)]
 
 
 @pytest.mark.parametrize("bf16", [False, True])

@@ -165,7 +165,9 @@ int qwen3_hip_rows_int8_dev(int8_t *q_d, size_t ldq, float *scale_d, const void 
  * 16 bytes are read many times faster, and then all of a row's lda (ldb) bytes
  * may be read, the last row's too: what lies behind K does not matter.  c_d must
  * not overlap what the call reads.  QWEN3_HIP_ETOOBIG where a launch would have
- * 2^32 threads: from 2^27 columns with up to four rows, from 2^36 results. */
+ * 2^32 threads: from 2^27 columns with up to four rows of codes that are read
+ * fast; otherwise never up to 2^24 - 8 blocks of 64 x 64 results (of 64 rows or
+ * columns begun each), and beyond as the sizes' kernel has it. */
 int qwen3_hip_gemm_int8_dev(void *c_d, size_t ldc, int bf16, const int8_t *a_d, size_t lda, const float *a_scale_d,
                             const int8_t *b_d, size_t ldb, const float *b_scale_d, int M, int K, int N);
 /* h = silu(g) * u with g and u such products of the same rows x_d, in fp32 up to
@@ -173,8 +175,9 @@ int qwen3_hip_gemm_int8_dev(void *c_d, size_t ldc, int bf16, const int8_t *a_d, 
 int qwen3_hip_gemm_int8_gate_up_silu_dev(void *h_d, size_t ldh, int bf16, const int8_t *x_d, size_t ldx,
                                          const float *x_scale_d, const int8_t *wg_d, const float *g_scale_d,
                                          const int8_t *wu_d, const float *u_scale_d, size_t ldw, int M, int K, int N);
-/* which kernel an 8-bit product of aligned codes and adjoining rows of C goes to
- * ("narrow16", "tile64", ..., "any" for K = 0, "none" for what is refused) */
+/* which kernel an 8-bit product of aligned codes and adjoining rows of C goes to:
+ * "narrow16", "tile64", ..., "any" for K = 0, "none" where M or N is not above 0
+ * or K not in 0 .. 131,071.  Sizes whose launch would be too large have a name. */
 const char *qwen3_hip_int8_plan(int M, int K, int N, int gated);
 /* qwen3_hip_gemm_dev that allocates nothing: no counterpart in the
  * reference ABI; for callers that cannot allocate device memory (code under

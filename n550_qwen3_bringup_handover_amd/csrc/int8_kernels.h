@@ -675,7 +675,10 @@ static int i8_plan_of(const I8Args &p, bool gated) {
     const long cols = ((long)p.N + 15) / 16;
     if (p.M <= 4 || cols * ((p.M + 15l) / 16) <= (p.M <= 16 ? 512 : 256)) return I8_NARROW1;
     if (cols * ((p.M + 31l) / 32) <= 256) return I8_NARROW2;
-    if (p.ldc > I8_MAX_NEAR / 4) return p.M <= 65535 * 32 ? I8_NARROW2 : I8_ANY_PLAN;   // tiles' stores have 32-bit offsets
+    // tiles' stores have 32-bit offsets: a tile's rows of C, as fp32, within 2^31 bytes.  Rows further apart
+    // than the lowest tile takes go to the narrow kernel, whose addresses have 64 bits
+    const auto near = [&](int bm) { return (size_t)bm * p.ldc <= (size_t)1 << 29; };
+    if (!near(64)) return p.M <= 65535 * 32 ? I8_NARROW2 : I8_ANY_PLAN;
     static const struct { int plan, bm, bn; float fixed, tile, stage, shared; } T[] = {
         {I8_TILE64, 64, 64, 2.41f, 0.67f, 0.201f, 0.012f},      {I8_TILE64X128, 64, 128, 2.59f, 0.79f, 0.300f, 0.062f},
         {I8_TILE128, 128, 128, 0.72f, 1.88f, 0.345f, 0.190f},   {I8_TILE128_ALONE, 128, 128, 4.0f, 0.0f, 0.404f, 0.210f},
@@ -685,7 +688,7 @@ static int i8_plan_of(const I8Args &p, bool gated) {
     int plan = I8_TILE64;
     for (const auto &t : T) {
         const double tiles = ceil(p.M / (double)t.bm) * ceil(p.N * (gated ? 2.0 : 1.0) / t.bn);
-        if (t.plan == (tiles > 256 ? I8_TILE128_ALONE : I8_TILE128)) continue;
+        if (t.plan == (tiles > 256 ? I8_TILE128_ALONE : I8_TILE128) || !near(t.bm)) continue;
         const double rounds = ceil(tiles / 256);
         const double us = t.fixed + rounds * t.tile + stages * (rounds * t.stage + tiles / 256 * t.shared);
         if (us < best) {
@@ -721,6 +724,23 @@ template <int MT, int W, bool GATED, bool CBF>
 static int i8_narrow(const I8Args &p) {
     I8_GO((k_i8_narrow<MT, W, GATED, CBF>), (p.N + 15l) / 16, (unsigned)((p.M + 16 * MT - 1l) / (16 * MT)), WAVE *W, p);
 }
+// any number of columns, 2^26 a launch
+template <bool GATED, bool CBF>
+static int i8_narrow_any(I8Args p) {
+    const int most = 1 << 26, N = p.N;
+    for (int n = 0;; n += most) {
+        p.N = N - n < most ? N - n : most;
+        const int rc = i8_narrow<2, 8, GATED, CBF>(p);
+        if (rc != QH_OK || N - n <= most) return rc;
+        p.b += (size_t)most * p.ldb;
+        p.bs += most;
+        if (GATED) {
+            p.b2 += (size_t)most * p.ldb;
+            p.bs2 += most;
+        }
+        p.c = (char *)p.c + (size_t)most * (CBF ? 2 : 4);
+    }
+}
 template <typename T, bool GATED, bool CBF>
 static int i8_tile(const I8Args &p) {
     const long bno = GATED ? T::BN / 2 : T::BN, mt = (p.M + T::BM - 1l) / T::BM, nt = (p.N + bno - 1) / bno;
@@ -737,7 +757,7 @@ template <bool GATED, bool CBF>
 static int i8_launch(const I8Args &p) {
     switch (i8_plan_of(p, GATED)) {
     case I8_NARROW1: return i8_narrow<1, 8, GATED, CBF>(p);
-    case I8_NARROW2: return i8_narrow<2, 8, GATED, CBF>(p);
+    case I8_NARROW2: return i8_narrow_any<GATED, CBF>(p);
     case I8_TILE64: return i8_tile<I8Tile<64, 64, 2, 2 - GATED, 4>, GATED, CBF>(p);
     case I8_TILE64X128: return i8_tile<I8Tile<64, 128, 2, 2, 3>, GATED, CBF>(p);
     case I8_TILE64X128_ONCE: return i8_tile<I8Tile<64, 128, 2, 2, 2, 2>, GATED, CBF>(p);

@@ -171,7 +171,11 @@ int qwen3_hip_rows_int8_dev(int8_t *q_d, size_t ldq, float *scale_d, const void 
 int qwen3_hip_gemm_int8_dev(void *c_d, size_t ldc, int bf16, const int8_t *a_d, size_t lda, const float *a_scale_d,
                             const int8_t *b_d, size_t ldb, const float *b_scale_d, int M, int K, int N);
 /* h = silu(g) * u with g and u such products of the same rows x_d, in fp32 up to
- * the store (silu as in qwen3_gemm_gate_up_silu); both weights ldw bytes a row. */
+ * the store, silu(g) = g / (1 + exp(-g)); both weights ldw bytes a row.  From g and
+ * u on fp32 results are off by at most 7 half steps of theirs (2^-24), bf16 ones by
+ * their own rounding and 2^-17; beside that by 2^-244 |u| where g < -174, by 2^-149
+ * |u| where g is subnormal, and by the last place of subnormal results.  An
+ * infinite u may give NaN where silu(g) is below fp32's range. */
 int qwen3_hip_gemm_int8_gate_up_silu_dev(void *h_d, size_t ldh, int bf16, const int8_t *x_d, size_t ldx,
                                          const float *x_scale_d, const int8_t *wg_d, const float *g_scale_d,
                                          const int8_t *wu_d, const float *u_scale_d, size_t ldw, int M, int K, int N);

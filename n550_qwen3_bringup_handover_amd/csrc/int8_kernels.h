@@ -177,22 +177,37 @@ __device__ __forceinline__ void i8_store(void *c, size_t i, float v) {
     else ((float *)c)[i] = v;
 }
 
-// silu(g) u = g / (1 + exp(-g)) u in a third of the instructions that the library's
-// exponential and division take, of which a block has as much as of a product of
-// K = 1,024: a power of two of -g log2 e, and a reciprocal.  That product's
-// remainder is put back for fp32 results, which are then within 9 half steps; bf16
-// ones are off by up to |g| 2^-24 more, at most 2^-17.5, where a half step is 2^-9.
+// silu(g) u = g / (1 + exp(-g)) u, for |g| < I8_SILU_FAR by the hardware's power of two
+// of -g log2 e and its reciprocal, in a third of the instructions that the library's
+// exponential and division take (1,999 x 1,024 x 2,816 15.4 us, with those 17.4; in bf16
+// 14.1 and 16.8).
+// For fp32 results the power's remainder is put back and the quotient corrected by its
+// own: e is off by 3 half steps of 2^-24, sum, quotient and product by one each, 6 in
+// all.  bf16 results go without, which adds 1.23 |g| 2^-24, at most 2^-17.2 where a half
+// step of theirs is 2^-8.
+#define I8_SILU_FAR 87.0f
+template <bool CBF>
+__device__ __forceinline__ float i8_silu_near(float g, float u) {
+    if constexpr (CBF) return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504e+00f)) * u;
+    const float hi = g * -1.44269504e+00f, lo = fmaf(g, -1.92596299e-08f, fmaf(g, -1.44269504e+00f, -hi));
+    float e = __builtin_amdgcn_exp2f(hi);
+    e = fmaf(e, lo * 6.93147182e-01f, e);
+    const float d = 1.0f + e, r = __builtin_amdgcn_rcpf(d), q = g * r;
+    return fmaf(fmaf(-d, q, g), r, q) * u;
+}
+// For |g| from there on, where exp(-g) or the reciprocal leaves fp32's range: g u, or,
+// 1 + exp(g) being 1, g exp(g) u with half of the exponent on either side of u, so that
+// only a result that is subnormal itself passes through subnormal values: 7 half steps.
+// exp(g / 2) is subnormal for g < -174, 0 to the hardware; that loses less than 2^-244 |u|.
+__device__ __forceinline__ float i8_silu_far(float g, float u) {
+    const float x = fminf(g, 0.0f), hi = x * 7.21347511e-01f, lo = fmaf(x, 9.62981495e-09f, fmaf(x, 7.21347511e-01f, -hi));
+    float h = __builtin_amdgcn_exp2f(hi);
+    h = fmaf(h, lo * 6.93147182e-01f, h);
+    return g * h * u * h;
+}
 template <bool CBF>
 __device__ __forceinline__ float i8_silu_mul(float g, float u) {
-    float e;
-    if constexpr (CBF) {
-        e = __builtin_amdgcn_exp2f(g * -1.44269504e+00f);
-    } else {
-        const float x = -fminf(fmaxf(g, -104.0f), 104.0f);
-        const float hi = x * 1.44269504e+00f, lo = fmaf(x, 1.92596299e-08f, fmaf(x, 1.44269504e+00f, -hi));
-        e = __builtin_amdgcn_exp2f(hi) * fmaf(lo, 6.93147182e-01f, 1.0f);
-    }
-    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+    return fabsf(g) >= I8_SILU_FAR ? i8_silu_far(g, u) : i8_silu_near<CBF>(g, u);
 }
 
 // Any strides and addresses: 64 x 64 outputs a block, 64 codes of K a step through
@@ -564,7 +579,8 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW / 4) void k_i8_tile(I8Args p, in
         s2[j] = GATED ? su[n] : 0.0f;
         at[j] = (n < cols ? n * ES : BUF_OOB) + 4 * fh * ldc;
     }
-    auto finish = [&](auto AUX) {
+    float far = 0.0f;                                     // the largest |g| of the wave's gated results
+    auto finish = [&](auto AUX, auto FAR) {
 #pragma unroll
         for (int i = 0; i < T::TM; i++)
 #pragma unroll
@@ -575,10 +591,17 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW / 4) void k_i8_tile(I8Args p, in
 #pragma unroll
                 for (int j = 0; j < TNO; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        y[j][e] = (float)acc[i][j][4 * e4 + e] * (r[e] * s[j]);
-                        if constexpr (GATED) y[j][e] = i8_silu_mul<CBF>(y[j][e], (float)acc[i][j + TNO][4 * e4 + e] * (r[e] * s2[j]));
-                    }
+                    for (int e = 0; e < 4; e++) y[j][e] = (float)acc[i][j][4 * e4 + e] * (r[e] * s[j]);
+                if constexpr (GATED) {
+#pragma unroll
+                    for (int j = 0; j < TNO; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float u = (float)acc[i][j + TNO][4 * e4 + e] * (r[e] * s2[j]);
+                            if constexpr (!decltype(FAR)::value) far = fmaxf(far, fabsf(y[j][e]));
+                            y[j][e] = decltype(FAR)::value ? i8_silu_mul<CBF>(y[j][e], u) : i8_silu_near<CBF>(y[j][e], u);
+                        }
+                }
 #pragma unroll
                 for (int e = 0; e < 4; e++)
 #pragma unroll
@@ -593,8 +616,15 @@ __global__ __launch_bounds__(WAVE *T::NW, T::NW / 4) void k_i8_tile(I8Args p, in
                     }
             }
     };
-    if (p.whole) finish(IC<AUX_SC1>{});
-    else finish(IC<0>{});
+    auto finish_all = [&](auto FAR) {
+        if (p.whole) finish(IC<AUX_SC1>{}, FAR);
+        else finish(IC<0>{}, FAR);
+    };
+    finish_all(IC<0>{});
+    // rare, so out of the way: all of the lane's results again (a look at each step's in its
+    // place, with these instructions among the others, cost 2 to 4% of a call)
+    if constexpr (GATED)
+        if (far >= I8_SILU_FAR) finish_all(IC<1>{});
 }
 
 // ---------------------------------------------------------------------------

@@ -198,11 +198,9 @@ __device__ __forceinline__ float i8_silu_near(float g, float u) {
 // For |g| from there on, where exp(-g) or the reciprocal leaves fp32's range: g u, or,
 // 1 + exp(g) being 1, g exp(g) u with half of the exponent on either side of u, so that
 // only a result that is subnormal itself passes through subnormal values: 7 half steps.
-// exp(g / 2) is subnormal for g < -174, 0 to the hardware; that loses less than 2^-244 |u|.
+// exp(g / 2), off by 2 of them, is subnormal for g < -174; that loses less than 2^-244 |u|.
 __device__ __forceinline__ float i8_silu_far(float g, float u) {
-    const float x = fminf(g, 0.0f), hi = x * 7.21347511e-01f, lo = fmaf(x, 9.62981495e-09f, fmaf(x, 7.21347511e-01f, -hi));
-    float h = __builtin_amdgcn_exp2f(hi);
-    h = fmaf(h, lo * 6.93147182e-01f, h);
+    const float h = expf(0.5f * fminf(g, 0.0f));
     return g * h * u * h;
 }
 template <bool CBF>

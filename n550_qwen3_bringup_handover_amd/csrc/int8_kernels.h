@@ -639,7 +639,7 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
     if (K > I8_MAX_K || ldq > I8_MAX_LD || ldx > I8_MAX_LD) return QH_ETOOBIG;
     if (!g_inited) return QH_ESTATE;
     const bool few = rows <= 1024;
-    // more than the L2s hold is read and written past them
+    // more than the L2s hold is read and written past them; few rows' kernels never have as much
     const bool once = (size_t)rows * K * (bf16 ? 2 : 4) >= (size_t)32 << 20;
 #define ROWS_AS(BF, TPR, KEEP, O)                                                                            \
     hipLaunchKernelGGL((k_rows_int8<BF, TPR, KEEP, O>), dim3((unsigned)(((size_t)some * TPR + 255) / (TPR < 256 ? 256 : TPR))), \
@@ -649,10 +649,10 @@ extern "C" int qh_rows_int8(int8_t *q, size_t ldq, float *scale, const void *x, 
         if (K <= 256 && !few) ROWS_AS(BF, 16, 2, O);    \
         else if (K <= 512) ROWS_AS(BF, 64, 1, O);       \
         else if (K <= 1024 && !few) ROWS_AS(BF, 64, 2, O); \
-        else if (K <= 2048 && few) ROWS_AS(BF, 256, 1, O); \
+        else if (K <= 2048 && few) ROWS_AS(BF, 256, 1, false); \
         else if (K <= 2048 && rows >= 4096) ROWS_AS(BF, 64, 4, O); \
         else if (K <= 4096) ROWS_AS(BF, 256, 2, O);     \
-        else if (K <= 8192 && rows <= 256) ROWS_AS(BF, 1024, 1, O); \
+        else if (K <= 8192 && rows <= 256) ROWS_AS(BF, 1024, 1, false); \
         else if (K <= 8192) ROWS_AS(BF, 256, 4, O);     \
         else ROWS_AS(BF, 1024, 2, O);                   \
     } while (0)

@@ -119,8 +119,8 @@ static int upload(const uint8_t *blob, const qw3m_info_t *info, int t, uint16_t 
         int rc = qh_h2d(stage, src, bytes);
         if (!rc) rc = qh_tile_to_row(dst, stage, rows, cols, info->tile_n, info->tile_k);
         /* the next upload overwrites stage: wait here (pageable source too) */
-        if (!rc) rc = qh_sync();
-        return rc;
+        const int rc2 = qh_sync();
+        return rc ? rc : rc2;
     }
     int rc = qh_h2d(dst, src, bytes);
     if (!rc) rc = qh_sync();
@@ -264,7 +264,8 @@ int qwen3_hip_model_open(qwen3_hip_model **out, const void *blob, size_t size, i
         rope_tables(c, s, max_seq);
         rc = qh_h2d(m->rcos, c, rope_bytes);
         if (!rc) rc = qh_h2d(m->rsin, s, rope_bytes);
-        if (!rc) rc = qh_sync();
+        const int rc2 = qh_sync();     /* copies read these tables, whatever happened */
+        if (!rc) rc = rc2;
         free(c);
         free(s);
         if (rc) goto fail;
@@ -587,8 +588,8 @@ static int load_chunk(qwen3_hip_model *m, const int *tokens, int nt, int pos0) {
     if (nt <= QM_MAX_CHUNK) return qm_set_tokens(m->tok_in, tokens, nt, m->state + 1, pos0);
     int rc = qh_h2d(m->tok_in, tokens, (size_t)nt * sizeof(int));
     if (!rc) rc = qm_set_i32(m->state + 1, pos0);
-    if (!rc) rc = qh_sync();
-    return rc;
+    const int rc2 = qh_sync();         /* the copy reads the caller's tokens, whatever happened */
+    return rc ? rc : rc2;
 }
 
 /* a whole prompt at positions 0 .. n - 1 into the sequence whose cache is kv,
@@ -939,10 +940,10 @@ static qm_rules_t rules_from(const qwen3_hip_batch *b, int seq) {
  * have put out: kept up by the steps from here on while there are rules */
 static int rules_texts(qwen3_hip_batch *b) {
     const size_t all = (size_t)b->n_seq * b->out_ld;
-    int rc = qh_d2h(b->h_out, b->out, all * sizeof(int));
-    if (!rc) rc = qh_sync();
     int *n = (int *)malloc((size_t)b->n_seq * sizeof(int));
     if (!n) return QWEN3_HIP_ENOMEM;
+    int rc = qh_d2h(b->h_out, b->out, all * sizeof(int));
+    if (!rc) rc = qh_sync();
     for (int s = 0; s < b->n_seq && !rc; s++) {
         const size_t row = (size_t)s * b->out_ld;
         n[s] = b->h_next[s] < 0 ? 0 : b->h_next[s] + 1;       /* the token that is fed next is the last */
@@ -950,9 +951,9 @@ static int rules_texts(qwen3_hip_batch *b) {
     }
     if (!rc) rc = qh_h2d(b->text, b->h_text, all * sizeof(int));
     if (!rc) rc = qh_h2d(b->n_text, n, (size_t)b->n_seq * sizeof(int));
-    if (!rc) rc = qh_sync();
+    const int rc2 = qh_sync();         /* copies read n, whatever happened */
     free(n);
-    return rc;
+    return rc ? rc : rc2;
 }
 
 /* device room for the rules, `biases` in all */
@@ -1015,8 +1016,9 @@ static int rules_upload(qwen3_hip_batch *b, int biases) {
         if (!rc) rc = qh_h2d(b->mask_of, of, (size_t)n * sizeof(int));
         if (!rc && biases) rc = qh_h2d(b->bias_token, tok, (size_t)biases * sizeof(int));
         if (!rc && biases) rc = qh_h2d(b->bias, val, (size_t)biases * sizeof(float));
-        if (!rc) rc = qh_sync();
     }
+    const int rc2 = qh_sync();         /* copies read these arrays and the caller's mask, whatever happened */
+    if (!rc) rc = rc2;
     free(pen);
     free(row);
     free(of);
@@ -1060,6 +1062,7 @@ int qwen3_hip_batch_set_rules(qwen3_hip_batch *b, int seq, const qwen3_hip_batch
         if (!rc && r->mask) rc = qh_h2d(b->mask + (size_t)seq * MASK_WORDS, r->mask, MASK_WORDS * sizeof(uint32_t));
     }
     if (rc) {                          /* the rules stay as they were, but a mask may be half of each */
+        (void)qh_sync();
         free(next.bias_token);
         free(next.bias);
         return rc;
@@ -1108,9 +1111,9 @@ int qwen3_hip_batch_prefill(qwen3_hip_batch *b, int seq, const int *prompt, int 
     if (rc) return rc;
     qwen3_hip_model *m = b->m;
     b->h_next[seq] = -1;
-    rc = batch_prompt(b, seq, prompt, n_prompt);
+    if ((rc = batch_prompt(b, seq, prompt, n_prompt)) != 0) return rc;
     /* first token: out[seq][0] at pos - plen + 1 = 0, then pos = n_prompt */
-    if (!rc) rc = qm_set_i32(b->pos + seq, n_prompt - 1);
+    rc = qm_set_i32(b->pos + seq, n_prompt - 1);
     if (!rc) rc = qm_set_i32(b->plen + seq, n_prompt);
     int *text = b->h_text + (size_t)seq * b->out_ld;
     memcpy(text, prompt, (size_t)n_prompt * sizeof(int));
@@ -1124,7 +1127,8 @@ int qwen3_hip_batch_prefill(qwen3_hip_batch *b, int seq, const int *prompt, int 
                                  b->out + (size_t)seq * b->out_ld, b->out_ld);
     if (!rc && b->n_rules)
         rc = qm_rules_note(b->text + (size_t)seq * b->out_ld, b->out_ld, b->n_text + seq, b->tok + seq, b->pos + seq, 1);
-    if (!rc) rc = qh_sync();
+    const int rc2 = qh_sync();         /* the text's copy reads h_text, whatever happened */
+    if (!rc) rc = rc2;
     if (!rc) {
         b->h_next[seq] = n_prompt;
         b->h_plen[seq] = n_prompt;
@@ -1327,7 +1331,8 @@ int qwen3_hip_batch_beam(qwen3_hip_batch *b, int width, const int *prompts, cons
     }
     if (!rc) rc = qh_d2h(hist, b->hist, (size_t)n_tokens * n * 2 * sizeof(int));
     if (!rc) rc = qh_d2h(scores, b->score, (size_t)n * sizeof(float));
-    if (!rc) rc = qh_sync();
+    const int rc3 = qh_sync();         /* copies write hist and the caller's scores, whatever happened */
+    if (!rc) rc = rc3;
     for (int s = 0; s < n && !rc; s++)
         for (int t = n_tokens - 1, at = s; t >= 0; t--) {
             const int *h = hist + ((size_t)t * n + at) * 2;

@@ -226,7 +226,9 @@ int qwen3_hip_batch_beam(qwen3_hip_batch *batch, int width, const int *prompts, 
  * Rules stay through prefills.  QWEN3_HIP_EINVAL for a repetition that is not
  * above 0, numbers that are not finite (a bias may be infinite) and tokens
  * outside the vocabulary.  While a sequence has rules qwen3_hip_batch_beam
- * returns QWEN3_HIP_ESTATE. */
+ * returns QWEN3_HIP_ESTATE.  A call that fails leaves every sequence's rules as
+ * they were; where it failed over copies to the device, prefills and decodes of a
+ * batch under rules return QWEN3_HIP_ESTATE until a call succeeds. */
 #define QWEN3_HIP_BATCH_MAX_BIAS 151936
 typedef struct {
     float repetition;            /* 1: none */

@@ -714,9 +714,10 @@ int qwen3_hip_model_timing(const qwen3_hip_model *m, double *prefill_ms, double 
 /* ---- multi-sequence batched decode ------------------------------------------ */
 
 #define MASK_WORDS ((V + 31) / 32)
-/* what is asked of a sequence's tokens */
+/* what is asked of a sequence's tokens; of the batch's masks two are a sequence's, so
+ * that a new one leaves the one in use whole */
 typedef struct {
-    int on, masked, n_bias;
+    int on, mask, n_bias;              /* mask: its place, 2 seq or 2 seq + 1; -1: none */
     float repetition, presence, frequency;
     int *bias_token;
     float *bias;
@@ -744,14 +745,15 @@ struct qwen3_hip_batch {
     double t_decode_ms;
     /* rules on logits, allocated by the first: the texts [n_seq][out_ld] and their
      * lengths, kept up while a sequence is under rules; penalties [3][n_seq]; the
-     * sequences' biases one after another, room for bias_room; a mask each */
+     * sequences' biases one after another, room for bias_room; two masks each.
+     * torn: an upload failed, and what is here is no one's until the next succeeds */
     int *h_text;                       /* host: every prefilled sequence's prompt */
     seq_rules_t *h_rules;
     int n_rules;                       /* sequences under rules */
     int *text, *n_text, *bias_row, *bias_token, *mask_of;
     float *penalty, *bias;
     uint32_t *mask;
-    int bias_room;
+    int bias_room, torn;
     /* beam search, allocated by the first: per sequence score, finished, parent;
      * {token, parent} of every step; the choice's workspace */
     float *score;
@@ -932,16 +934,15 @@ static qm_rules_t rules_from(const qwen3_hip_batch *b, int seq) {
     const int n = b->n_seq;
     const qm_rules_t r = {b->text + (size_t)seq * b->out_ld, b->out_ld, b->plen + seq, b->n_text + seq, b->penalty + seq,
                           b->penalty + n + seq, b->penalty + 2 * n + seq, b->bias_row + seq, b->bias_token, b->bias,
-                          b->bias_room, b->mask, MASK_WORDS, n, b->mask_of + seq};
+                          b->bias_room, b->mask, MASK_WORDS, 2 * n, b->mask_of + seq};
     return r;
 }
 
 /* the texts of all sequences as they stand, from the prompts and what the steps
- * have put out: kept up by the steps from here on while there are rules */
-static int rules_texts(qwen3_hip_batch *b) {
+ * have put out: kept up by the steps from here on while there are rules.  n [n_seq]
+ * is read until the stream is waited for */
+static int rules_texts(qwen3_hip_batch *b, int *n) {
     const size_t all = (size_t)b->n_seq * b->out_ld;
-    int *n = (int *)malloc((size_t)b->n_seq * sizeof(int));
-    if (!n) return QWEN3_HIP_ENOMEM;
     int rc = qh_d2h(b->h_out, b->out, all * sizeof(int));
     if (!rc) rc = qh_sync();
     for (int s = 0; s < b->n_seq && !rc; s++) {
@@ -951,9 +952,7 @@ static int rules_texts(qwen3_hip_batch *b) {
     }
     if (!rc) rc = qh_h2d(b->text, b->h_text, all * sizeof(int));
     if (!rc) rc = qh_h2d(b->n_text, n, (size_t)b->n_seq * sizeof(int));
-    const int rc2 = qh_sync();         /* copies read n, whatever happened */
-    free(n);
-    return rc ? rc : rc2;
+    return rc;
 }
 
 /* device room for the rules, `biases` in all */
@@ -965,7 +964,7 @@ static int rules_room(qwen3_hip_batch *b, int biases) {
     if (!rc && !b->penalty) rc = qh_malloc((void **)&b->penalty, 3 * n * sizeof(float));
     if (!rc && !b->bias_row) rc = qh_malloc((void **)&b->bias_row, (n + 1) * sizeof(int));
     if (!rc && !b->mask_of) rc = qh_malloc((void **)&b->mask_of, n * sizeof(int));
-    if (!rc && !b->mask) rc = qh_malloc((void **)&b->mask, n * MASK_WORDS * sizeof(uint32_t));
+    if (!rc && !b->mask) rc = qh_malloc((void **)&b->mask, 2 * n * MASK_WORDS * sizeof(uint32_t));
     if (rc || (b->bias_room && biases <= b->bias_room)) return rc;
     const int room = biases < 512 ? 1024 : 2 * biases;
     int *tok = NULL;
@@ -980,6 +979,7 @@ static int rules_room(qwen3_hip_batch *b, int biases) {
     }
     if (b->graph_id[2] >= 0) (void)qh_graph_destroy(b->graph_id[2]);
     b->graph_id[2] = -1;
+    b->torn = 1;                       /* the biases are in neither until they are uploaded */
     (void)qh_free(b->bias_token);
     (void)qh_free(b->bias);
     b->bias_token = tok;
@@ -988,42 +988,32 @@ static int rules_room(qwen3_hip_batch *b, int biases) {
     return rc;
 }
 
-/* penalties, biases and which sequences have masks, from the host's copies */
-static int rules_upload(qwen3_hip_batch *b, int biases) {
+/* penalties, biases and which sequences have masks, with `next` in the place of sequence
+ * seq's rules.  stage: 5 n_seq + 1 + 2 biases words, read until the stream is waited for */
+static int rules_upload(qwen3_hip_batch *b, int seq, const seq_rules_t *next, int biases, int *stage) {
     const int n = b->n_seq;
-    float *pen = (float *)malloc(3 * (size_t)n * sizeof(float));
-    int *row = (int *)malloc(((size_t)n + 1) * sizeof(int)), *of = (int *)malloc((size_t)n * sizeof(int));
-    int *tok = (int *)malloc(((size_t)biases + 1) * sizeof(int));
-    float *val = (float *)malloc(((size_t)biases + 1) * sizeof(float));
-    int rc = QWEN3_HIP_ENOMEM;
-    if (pen && row && of && tok && val) {
-        row[0] = 0;
-        for (int s = 0; s < n; s++) {
-            const seq_rules_t *r = &b->h_rules[s];
-            pen[s] = r->on ? r->repetition : 1.0f;
-            pen[n + s] = r->on ? r->presence : 0.0f;
-            pen[2 * n + s] = r->on ? r->frequency : 0.0f;
-            of[s] = r->on && r->masked ? s : -1;
-            const int k = r->on ? r->n_bias : 0;
-            if (k) {
-                memcpy(tok + row[s], r->bias_token, (size_t)k * sizeof(int));
-                memcpy(val + row[s], r->bias, (size_t)k * sizeof(float));
-            }
-            row[s + 1] = row[s] + k;
+    float *pen = (float *)stage, *val = (float *)(stage + 5 * n + 1 + biases);
+    int *of = stage + 3 * n, *row = of + n, *tok = row + n + 1;
+    row[0] = 0;
+    for (int s = 0; s < n; s++) {
+        const seq_rules_t *r = s == seq ? next : &b->h_rules[s];
+        pen[s] = r->on ? r->repetition : 1.0f;
+        pen[n + s] = r->on ? r->presence : 0.0f;
+        pen[2 * n + s] = r->on ? r->frequency : 0.0f;
+        of[s] = r->on ? r->mask : -1;
+        const int k = r->on ? r->n_bias : 0;
+        if (k) {
+            memcpy(tok + row[s], r->bias_token, (size_t)k * sizeof(int));
+            memcpy(val + row[s], r->bias, (size_t)k * sizeof(float));
         }
-        rc = qh_h2d(b->penalty, pen, 3 * (size_t)n * sizeof(float));
-        if (!rc) rc = qh_h2d(b->bias_row, row, ((size_t)n + 1) * sizeof(int));
-        if (!rc) rc = qh_h2d(b->mask_of, of, (size_t)n * sizeof(int));
-        if (!rc && biases) rc = qh_h2d(b->bias_token, tok, (size_t)biases * sizeof(int));
-        if (!rc && biases) rc = qh_h2d(b->bias, val, (size_t)biases * sizeof(float));
+        row[s + 1] = row[s] + k;
     }
-    const int rc2 = qh_sync();         /* copies read these arrays and the caller's mask, whatever happened */
-    if (!rc) rc = rc2;
-    free(pen);
-    free(row);
-    free(of);
-    free(tok);
-    free(val);
+    b->torn = 1;
+    int rc = qh_h2d(b->penalty, pen, 3 * (size_t)n * sizeof(float));
+    if (!rc) rc = qh_h2d(b->mask_of, of, (size_t)n * sizeof(int));
+    if (!rc) rc = qh_h2d(b->bias_row, row, ((size_t)n + 1) * sizeof(int));
+    if (!rc && biases) rc = qh_h2d(b->bias_token, tok, (size_t)biases * sizeof(int));
+    if (!rc && biases) rc = qh_h2d(b->bias, val, (size_t)biases * sizeof(float));
     return rc;
 }
 
@@ -1031,7 +1021,7 @@ int qwen3_hip_batch_set_rules(qwen3_hip_batch *b, int seq, const qwen3_hip_batch
     if (!b || seq < 0 || seq >= b->n_seq) return QWEN3_HIP_EINVAL;
     if (!b->m) return QWEN3_HIP_ESTATE;
     seq_rules_t *now = &b->h_rules[seq];
-    if (!r && !now->on) return QWEN3_HIP_OK;
+    if (!r && !now->on && !(b->torn && b->n_rules)) return QWEN3_HIP_OK;
     if (r) {
         if (!(r->repetition > 0.0f) || !isfinite(r->repetition) || !isfinite(r->presence) || !isfinite(r->frequency))
             return QWEN3_HIP_EINVAL;
@@ -1042,13 +1032,17 @@ int qwen3_hip_batch_set_rules(qwen3_hip_batch *b, int seq, const qwen3_hip_batch
     }
     if (qh_capturing()) return QWEN3_HIP_ERUNTIME;   /* rules come from the host */
 
-    seq_rules_t next = {0};
+    const int n = b->n_seq;
     int biases = r ? r->n_bias : 0, rc = QWEN3_HIP_OK;
-    for (int s = 0; s < b->n_seq; s++)
+    for (int s = 0; s < n; s++)
         if (s != seq && b->h_rules[s].on) biases += b->h_rules[s].n_bias;
+    seq_rules_t next = {0};
+    int *stage = (int *)malloc((6 * (size_t)n + 1 + 2 * (size_t)biases) * sizeof(int));
+    if (!stage) rc = QWEN3_HIP_ENOMEM;
     if (r) {
-        next = (seq_rules_t){1, r->mask != NULL, r->n_bias, r->repetition, r->presence, r->frequency, NULL, NULL};
-        if (r->n_bias) {
+        const int place = now->on && now->mask == 2 * seq ? 2 * seq + 1 : 2 * seq;
+        next = (seq_rules_t){1, r->mask ? place : -1, r->n_bias, r->repetition, r->presence, r->frequency, NULL, NULL};
+        if (!rc && r->n_bias) {
             next.bias_token = (int *)malloc((size_t)r->n_bias * sizeof(int));
             next.bias = (float *)malloc((size_t)r->n_bias * sizeof(float));
             if (!next.bias_token || !next.bias) rc = QWEN3_HIP_ENOMEM;
@@ -1058,20 +1052,26 @@ int qwen3_hip_batch_set_rules(qwen3_hip_batch *b, int seq, const qwen3_hip_batch
             }
         }
         if (!rc) rc = rules_room(b, biases);
-        if (!rc && b->n_rules == 0) rc = rules_texts(b);
-        if (!rc && r->mask) rc = qh_h2d(b->mask + (size_t)seq * MASK_WORDS, r->mask, MASK_WORDS * sizeof(uint32_t));
+        if (!rc && b->n_rules == 0) rc = rules_texts(b, stage + 5 * n + 1 + 2 * biases);
+        if (!rc && r->mask) rc = qh_h2d(b->mask + (size_t)place * MASK_WORDS, r->mask, MASK_WORDS * sizeof(uint32_t));
     }
-    if (rc) {                          /* the rules stay as they were, but a mask may be half of each */
-        (void)qh_sync();
+    if (!rc) rc = rules_upload(b, seq, &next, biases, stage);
+    if (stage) {
+        const int rc2 = qh_sync();     /* copies read the staging and the caller's mask, whatever happened */
+        if (!rc) rc = rc2;
+    }
+    free(stage);
+    if (rc) {                          /* the rules stay as they were, torn or whole */
         free(next.bias_token);
         free(next.bias);
         return rc;
     }
+    b->torn = 0;
     b->n_rules += next.on - now->on;
     free(now->bias_token);
     free(now->bias);
     *now = next;
-    return rules_upload(b, biases);
+    return rc;
 }
 
 int qwen3_hip_batch_set_int8_head(qwen3_hip_batch *b, int on) {
@@ -1106,7 +1106,7 @@ int qwen3_hip_batch_set_int8_head(qwen3_hip_batch *b, int on) {
 int qwen3_hip_batch_prefill(qwen3_hip_batch *b, int seq, const int *prompt, int n_prompt) {
     if (!b || !prompt || seq < 0 || seq >= b->n_seq || n_prompt < 1 || n_prompt >= b->max_ctx)
         return QWEN3_HIP_EINVAL;
-    if (!b->m) return QWEN3_HIP_ESTATE;
+    if (!b->m || (b->n_rules && b->torn)) return QWEN3_HIP_ESTATE;
     int rc = check_tokens(prompt, n_prompt);
     if (rc) return rc;
     qwen3_hip_model *m = b->m;
@@ -1214,7 +1214,7 @@ static int batch_run(qwen3_hip_batch *b, int i, int which) {
 
 int qwen3_hip_batch_decode(qwen3_hip_batch *b, int n_decode, int *out) {
     if (!b || !out || n_decode < 0) return QWEN3_HIP_EINVAL;
-    if (!b->m) return QWEN3_HIP_ESTATE;
+    if (!b->m || (b->n_rules && b->torn)) return QWEN3_HIP_ESTATE;
     for (int s = 0; s < b->n_seq; s++)
         if (b->h_next[s] < 0 || (long)b->h_next[s] + n_decode > b->max_ctx) return QWEN3_HIP_EINVAL;
     int rc = QWEN3_HIP_OK;

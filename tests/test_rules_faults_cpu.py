@@ -13,7 +13,7 @@ CSRC = os.path.join(ROOT, "n550_qwen3_bringup_handover_amd", "csrc")
 
 
 @pytest.mark.skipif(not shutil.which("gcc") or not shutil.which("nm") or not os.path.isdir(HC), reason="no host compiler")
-@pytest.mark.parametrize("what", ["copies"])
+@pytest.mark.parametrize("what", ["copies", "rules"])
 def test_calls_that_fail(tmp_path, what):
     flags = ["-O1", "-g", "-std=c11", "-w", "-fsanitize=address", "-fno-omit-frame-pointer",
              "-I", os.path.join(ROOT, "include"), "-I", CSRC]

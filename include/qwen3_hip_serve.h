@@ -174,9 +174,10 @@ typedef struct {
  * So a row whose mask allows nothing is -inf throughout (qwen3_hip_argmax_dev
  * gives 0 for it), and a NaN stays one where it is allowed.  out_d may be
  * logits_d, with ldo = ld: then only what changes is written, and without a mask
- * only that is read.  Otherwise the two must not overlap.  Rows ld and ldo
- * values apart, what lies behind vocab is left as it was; vocab <= 2^24, n <=
- * 65,535.  The structure is read before the call returns; no workspace. */
+ * only that is read.  Otherwise no row may overlap one of the other's; rows of
+ * different strides: nor the memory that they span.  Rows ld and ldo values
+ * apart, what lies behind vocab is left as it was; vocab <= 2^24, n <= 65,535.
+ * The structure is read before the call returns; no workspace. */
 int qwen3_hip_logits_rules_dev(float *out_d, size_t ldo, const float *logits_d, size_t ld, int vocab, int n,
                                const qwen3_hip_rules *rules);
 

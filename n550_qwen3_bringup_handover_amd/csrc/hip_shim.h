@@ -26,6 +26,17 @@ enum {
     QH_ETOOBIG = 8      /* size beyond a documented maximum */
 };
 
+/* whether n rows of wide_a bytes every pitch_a bytes from a on and n of wide_b every
+ * pitch_b from b on share memory; rows of different pitches: whether what they span does */
+static inline int qh_rows_meet(const void *a, size_t pitch_a, size_t wide_a, const void *b, size_t pitch_b, size_t wide_b,
+                               size_t n) {
+    const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
+    if (!n || !wide_a || !wide_b || pa >= pb + (n - 1) * pitch_b + wide_b || pb >= pa + (n - 1) * pitch_a + wide_a) return 0;
+    if (pitch_a != pitch_b || n == 1) return 1;
+    const size_t behind = pb >= pa ? (pb - pa) % pitch_a : (pitch_a - (pa - pb) % pitch_a) % pitch_a;   /* b in a's pitch */
+    return behind < wide_a || behind + wide_b > pitch_a;
+}
+
 int         qh_init(int device);        /* idempotent; creates the stream */
 void        qh_shutdown(void);
 int         qh_device(void);

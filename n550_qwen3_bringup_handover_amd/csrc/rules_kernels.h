@@ -214,10 +214,8 @@ extern "C" int qm_logits_rules(float *out, size_t ldo, const float *logits, size
     if (n == 0) return QH_OK;
     if (!out || !logits || (out == logits && ldo != ld) || (((uintptr_t)out | (uintptr_t)logits) & 3)) return QH_EINVAL;
     if (n > QM_RULES_MAX_ROWS || vocab > QM_RULES_MAX_VOCAB || ldo > (size_t)1 << 40 || ld > (size_t)1 << 40) return QH_ETOOBIG;
-    // rows must not reach into other rows of the other buffer
-    const uintptr_t o = (uintptr_t)out, x = (uintptr_t)logits;
-    const uintptr_t oe = o + ((size_t)(n - 1) * ldo + vocab) * sizeof(float), xe = x + ((size_t)(n - 1) * ld + vocab) * sizeof(float);
-    if (o != x && o < xe && x < oe) return QH_EINVAL;
+    const size_t es = sizeof(float);
+    if (out != logits && qh_rows_meet(out, ldo * es, vocab * es, logits, ld * es, vocab * es, n)) return QH_EINVAL;
     if (t->ld_token < 0 || t->n_bias < 0 || t->n_mask < 0) return QH_EINVAL;
     if (t->token && !t->n_token) return QH_EINVAL;
     if (!t->token && (t->repetition || t->presence || t->frequency)) return QH_EINVAL;

@@ -152,8 +152,8 @@ int qwen3_hip_gemm_gate_up_silu_bf16a_dev(float *h_d, const uint16_t *x_d,
  *   code = x / scale (fp32) rounded to the nearest integer, ties to even
  * and scale = 0 and codes of 0 where a < 2^-100 (or K = 0).  x_d: rows ldx >= K
  * values apart; q_d: ldq >= K bytes apart, what lies between K and ldq is left
- * as it was.  Any strides and addresses aligned to the values' own size.  K <=
- * 131,071. */
+ * as it was.  Any strides and addresses aligned to the values' own size.  The rows
+ * of q_d, the scales and the rows of x_d must not overlap.  K <= 131,071. */
 int qwen3_hip_rows_int8_dev(int8_t *q_d, size_t ldq, float *scale_d, const void *x_d, size_t ldx, int bf16, int rows,
                             int K);
 /* C[m][n] = a_scale[m] b_scale[n] sum_k A[m][k] B[n][k]: A [M] and B [N] rows of

@@ -704,7 +704,8 @@ static int i8_plan_of(const I8Args &p, bool gated) {
     if (p.M <= 4 || cols * ((p.M + 15l) / 16) <= (p.M <= 16 ? 512 : 256)) return I8_NARROW1;
     if (cols * ((p.M + 31l) / 32) <= 256) return I8_NARROW2;
     // tiles' stores have 32-bit offsets: a tile's rows of C, as fp32, within 2^31 bytes.  Rows further apart
-    // than the lowest tile takes go to the narrow kernel, whose addresses have 64 bits
+    // than the lowest tile takes go to the narrow kernel, whose addresses have 64 bits (4096 x 1024 x (2^20 + 16)
+    // 7.1 ms on tiles, 60.7 there)
     const auto near = [&](int bm) { return (size_t)bm * p.ldc <= (size_t)1 << 29; };
     if (!near(64)) return p.M <= 65535 * 32 ? I8_NARROW2 : I8_ANY_PLAN;
     static const struct { int plan, bm, bn; float fixed, tile, stage, shared; } T[] = {

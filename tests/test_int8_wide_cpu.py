@@ -57,3 +57,17 @@ def test_results_in_far_rows_land_in_their_places(tmp_path):
     with concurrent.futures.ThreadPoolExecutor(4) as pool:
         for p in pool.map(one, range(n)):
             assert p.returncode == 0 and p.stdout.endswith("every result in its place\n"), f"exit {p.returncode}: {p.stdout[-400:]}"
+
+
+@pytest.mark.skipif(not os.path.exists(CLANG) or not os.path.isdir(os.path.join(HERE, "hostcheck")),
+                    reason="no host compiler that knows the kernels' vector types")
+def test_launches_of_many_columns_cover_them_once(tmp_path):
+    # behind the harness' own macro, before the kernels
+    (tmp_path / "hip_shim.h").write_text('#include_next "hip_shim.h"\n#undef hipLaunchKernelGGL\n'
+                                         '#define hipLaunchKernelGGL(K, GRID, BLOCK, SHM, STREAM, ...) launched(GRID, __VA_ARGS__)\n')
+    exe = str(tmp_path / "int8_split")
+    subprocess.run([CLANG, "-x", "c++", "-std=c++17", "-O0", "-w", "-I", str(tmp_path), "-I",
+                    os.path.join(ROOT, "n550_qwen3_bringup_handover_amd", "csrc"),
+                    os.path.join(HERE, "hostcheck", "int8_split.cpp"), "-o", exe, "-lpthread"], check=True)
+    p = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert p.returncode == 0 and p.stdout.endswith("every column once\n"), p.stdout

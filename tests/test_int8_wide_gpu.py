@@ -3,7 +3,7 @@ definition (tests/int8_oracle.py)."""
 import pytest
 
 from n550_qwen3_bringup_handover_amd import abi, runtime
-from tests.test_int8_gpu import Product
+from tests.test_int8_gpu import At, Product
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +29,14 @@ def test_columns_behind_2_20(gated):
     for n in (1 << 20, (1 << 20) + 16):
         assert abi.int8_plan(40, 64, n, gated).startswith("tile")
         Product(40, 64, n, gated=gated, seed=7).run()
+
+
+# a size of every kernel
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,n", [(3, 1001), (60, 1400), (60, 4010), (130, 5603), (700, 3301), (1001, 4301), (1905, 7001)])
+def test_results_at_any_address_of_their_own_size(m, n, gated, bf16):
+    p = Product(m, 200, n // (1 + gated), gated=gated, bf16=bf16, ldc=-(-n // 32) * 32, seed=8)
+    for shift in (2, 6) if bf16 else (4, 12):
+        p.cd = At(p.mark, shift)
+        p.run()
